@@ -164,6 +164,16 @@ class ScalingUpdate(ctypes.Structure):
 
 MAX_SCALING_UPDATES = 4
 
+TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2   # element types of the operators around the layers
+
+
+class NormTensor(ctypes.Structure):
+    """struct fp8gmm_norm_tensor"""
+
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("count", ctypes.c_int64), ("type", ctypes.c_int32),
+                ("out_type", ctypes.c_int32)]
+
+
 
 class PassLaunch(ctypes.Structure):
     """struct fp8gmm_pass_launch"""
@@ -243,6 +253,15 @@ EXPORTS = (
     "fp8gmm_moe_gather",
     "fp8gmm_moe_scatter",
     "fp8gmm_moe_scatter_wgrad",
+    "fp8gmm_layer_norm",
+    "fp8gmm_layer_norm_workspace_bytes",
+    "fp8gmm_layer_norm_backward",
+    "fp8gmm_embedding",
+    "fp8gmm_embedding_workspace_bytes",
+    "fp8gmm_embedding_backward",
+    "fp8gmm_multi_norm_workspace_bytes",
+    "fp8gmm_multi_norm",
+    "fp8gmm_multi_clip",
     "fp8gmm_gemm_schedule",
     "fp8gmm_gemm_fixup",
 )
@@ -375,6 +394,25 @@ def load():
     L.fp8gmm_moe_scatter.argtypes = [vp, vp, vp, vp, ci, ci, ci, vp]
     L.fp8gmm_moe_scatter_wgrad.restype = ci
     L.fp8gmm_moe_scatter_wgrad.argtypes = [vp, vp, vp, vp, ci, ci, ci, vp]
+    cl, sz, cf = ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
+    L.fp8gmm_layer_norm.restype = ci
+    L.fp8gmm_layer_norm.argtypes = [vp, cl, vp, vp, vp, vp, vp, cl, ci, cf, ci, ci, vp]
+    L.fp8gmm_layer_norm_workspace_bytes.restype = sz
+    L.fp8gmm_layer_norm_workspace_bytes.argtypes = [cl, ci, ci]
+    L.fp8gmm_layer_norm_backward.restype = ci
+    L.fp8gmm_layer_norm_backward.argtypes = [vp, cl, vp, cl, vp, vp, vp, vp, vp, vp, cl, ci, ci, ci, vp, sz, vp]
+    L.fp8gmm_embedding.restype = ci
+    L.fp8gmm_embedding.argtypes = [vp, ci, cl, vp, cl, ci, cf, ci, vp, vp]
+    L.fp8gmm_embedding_workspace_bytes.restype = sz
+    L.fp8gmm_embedding_workspace_bytes.argtypes = [cl, cl, ci, ci]
+    L.fp8gmm_embedding_backward.restype = ci
+    L.fp8gmm_embedding_backward.argtypes = [vp, ci, cl, vp, vp, cl, ci, cf, cl, ci, vp, sz, vp]
+    L.fp8gmm_multi_norm_workspace_bytes.restype = sz
+    L.fp8gmm_multi_norm_workspace_bytes.argtypes = [ci]
+    L.fp8gmm_multi_norm.restype = ci
+    L.fp8gmm_multi_norm.argtypes = [vp, ci, vp, vp, sz, vp]
+    L.fp8gmm_multi_clip.restype = ci
+    L.fp8gmm_multi_clip.argtypes = [vp, ci, ctypes.c_double, vp, vp, sz, vp]
     L.fp8gmm_gemm_schedule.restype = ci
     L.fp8gmm_gemm_schedule.argtypes = [vp, ci, ci, ci, ci, ci, vp, ci]
     L.fp8gmm_gemm_fixup.restype = ci

@@ -20,6 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import GEMM_PROBLEM, TENSOR_DESC
+from . import native
 from .native import set_kernel_timing
 import os
 
@@ -680,6 +681,21 @@ def multi_scale_mul(inputs, scales_1, scales_2):
     table["scale"] = _scalar_ptrs(scales_1, n, "scales_1")
     table["in2"] = _scalar_ptrs(scales_2, n, "scales_2")
     _launch_multi(_lib.OP_SCALE_MUL, table, _lib.E4M3, dev, (x, scales_1, scales_2))
+
+
+def multi_norm(tensors):
+    """The 2-norm of all elements of all ``tensors`` together, a float32 scalar on their device: bfloat16, float16 and float32 in
+    any mixture and of any shapes and strides, squared and added up in float64.  The same bits from call to call."""
+    flush_uploads()   # a queued launch may write what is read here
+    return native.multi_norm(list(tensors))
+
+
+def multi_clip(tensors, outs, max_norm):
+    """``outs[i] = tensors[i] * min(1, max_norm / (norm + 1e-6))`` with the norm of ``multi_norm``, which is returned.  A result has
+    its tensor's shape, and its type or float32.  It may be its tensor itself (in place: not written again where the factor is
+    1), but may share memory with nothing else of the call.  No gradients are taken."""
+    flush_uploads()
+    return native.multi_clip(list(tensors), list(outs), max_norm)
 
 
 def _fill_transpose_shapes(table, x, t):

@@ -9,40 +9,17 @@
 // What a pass computes is stated in fp8gmm.h and grouped_linear.py / grouped_mlp.py (reference fp8_gmm/grouped_linear.py:11-183,
 // fp8_gmm/grouped_mlp.py:18-325); the Python functions there launch the same kernels with the same tables and serve
 // the layouts and options that this file leaves to them.
-#include <torch/csrc/autograd/VariableTypeUtils.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/utils/pybind.h>
+#include "host_common.h"
 
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/Event.h>
-#include <c10/core/impl/VirtualGuardImpl.h>
-#include <c10/hip/HIPStream.h>
+namespace fp8gmm_host {
 
-#include <atomic>
+std::atomic<bool> kernel_timing{false};
 
-#include "fp8gmm.h"
+}  // namespace fp8gmm_host
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::Node;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-void check(int status) { TORCH_CHECK(status == FP8GMM_OK, "fp8gmm error ", status, ": ", fp8gmm_status_string(status)); }
-
-void* current_stream(const at::Device& device) {
-  return c10::hip::getCurrentHIPStream(device.index()).stream();
-}
-
-template <class T>
-T* ptr(const Tensor& t) {
-  return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
-}
+using namespace fp8gmm_host;
 
 // Rows per expert, from a CPU tensor or anything that iterates over numbers.
 std::vector<int64_t> sizes_of(const py::object& group_sizes) {
@@ -55,18 +32,6 @@ std::vector<int64_t> sizes_of(const py::object& group_sizes) {
   std::vector<int64_t> sizes;
   for (const py::handle n : py::iter(group_sizes)) sizes.push_back(py::cast<int64_t>(py::int_(py::reinterpret_borrow<py::object>(n))));
   return sizes;
-}
-
-// An exception of Python code that a pass calls - saved-tensor hooks; activation checkpointing ends its recomputation
-// with one - reaches the caller as it is.
-template <class F>
-Tensor with_python_errors(F&& pass) {
-  try {
-    return pass();
-  } catch (python_error& e) {
-    e.restore();
-    throw py::error_already_set();
-  }
 }
 
 // How the launches of a module are planned, and its scaling state of both directions.
@@ -86,26 +51,6 @@ struct Due {
   int margin = 0;
   bool most_recent = false, keep_weights = false;
 };
-
-// Whether a block of backend.kernel_timing is open (set_kernel_timing).
-std::atomic<bool> kernel_timing{false};
-
-// Enqueues what `launch` does; inside a block of kernel_timing between two events, under what `block` makes of the module
-// `backend`: a bracket of that block.  On the current device and stream, as the launch.
-template <class Block, class Launch>
-void timed(Block&& block, Launch&& launch) {
-  if (!kernel_timing.load(std::memory_order_relaxed)) return launch();
-  py::gil_scoped_acquire gil;
-  const py::object bracket = block(py::module_::import("fp8_gmm_amd.backend"));
-  bracket.attr("__enter__")();
-  launch();
-  bracket.attr("__exit__")(py::none(), py::none(), py::none());
-}
-// ... that moves `bytes` bytes under a name of its own.
-template <class Launch>
-void timed(const char* name, int64_t bytes, Launch&& launch) {
-  timed([&](const py::module_& backend) { return backend.attr("_timed")(name, py::cpp_function([bytes] { return bytes; })); }, launch);
-}
 
 // Builds the tables of a pass and enqueues its launches on the current stream.
 void run_pass(int which, const void* desc, const at::Device& device, const Setup* update, Due* due, const Tensor& snapshot_of,
@@ -281,20 +226,6 @@ void check_shapes(const std::vector<int64_t>& sizes, const Tensor& x, const Tens
   TORCH_CHECK(s.fwd_scale.numel() >= 3 * n && s.fwd_scale_inv.numel() >= 3 * n && s.fwd_amax.size(-1) >= 3 * n &&
                   s.bwd_scale.numel() >= 2 * n && s.bwd_scale_inv.numel() >= 2 * n && s.bwd_amax.size(-1) >= 2 * n,
               "fp8_gmm_amd: the scaling state has too few slots");
-}
-
-// Forward-mode differentiation has no rule here and is refused, as the Python functions refuse it: a tangent that is
-// silently dropped would be a wrong derivative.
-void check_no_tangent(at::TensorList inputs) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor& t : inputs)
-    TORCH_CHECK(!torch::autograd::isFwGradDefined(t), "fp8_gmm_amd: the grouped modules do not support forward-mode AD");
-}
-
-// What a backward pass starts from.  A node behind the pass that returned no gradient stands for zeros, as it does for a
-// Python autograd function.
-Tensor gradient_of_result(const Node& node, const variable_list& grads) {
-  return grads[0].defined() ? grads[0].contiguous() : node.input_metadata(0).zeros_like();
 }
 
 // ---- GroupedLinear ------------------------------------------------------------------------------------------------
@@ -846,4 +777,5 @@ PYBIND11_MODULE(_host, m) {
   m.def("gating", &gating);
   m.def("route", &route);
   m.def("set_kernel_timing", [](bool on) { kernel_timing.store(on, std::memory_order_relaxed); });
+  define_layers(m);
 }

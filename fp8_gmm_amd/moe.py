@@ -13,6 +13,7 @@ import torch
 from . import moe_ops
 from .grouped_linear import GroupedLinear
 from .grouped_mlp import GroupedMlp
+from .layers import LayerNorm
 from .native import Route, route
 
 
@@ -22,7 +23,9 @@ def _own(module, cls):
 
 
 class _RoutedModule(torch.nn.Module):
-    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype, device):
+    """``layer_norm``: the layer norms its rows (layers.LayerNorm) in front of the router and the experts."""
+
+    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm=False):
         super().__init__()
         self.n_embd = n_embd
         self.n_inner = n_inner
@@ -30,6 +33,7 @@ class _RoutedModule(torch.nn.Module):
         self.top_k = top_k
         self.sort_end_bit = max(int(np.ceil(np.log2(n_experts))), 1)
         self.gating_network = torch.nn.Linear(n_embd, n_experts, bias=False).to(dtype).to(device)
+        self.layer_norm = LayerNorm(n_embd, dtype=dtype, device=device) if layer_norm else None
         self._counts_host = None    # page-locked landing place of the per-expert counts, and the event of its copy
         self._counts_ready = None
 
@@ -82,6 +86,8 @@ class _RoutedModule(torch.nn.Module):
 
     def forward(self, input):
         input = input.view(-1, input.size(-1))
+        if self.layer_norm is not None:
+            input = self.layer_norm(input)
         # Another compute, of a subclass or set on the module, is called as ever: on the rows themselves, which it may change in
         # place where nothing else needs them, and without the inverse.
         own = getattr(self.compute, "__func__", None) is _RoutedModule.compute
@@ -103,8 +109,9 @@ class _RoutedModule(torch.nn.Module):
 class Fp8LinearModule(_RoutedModule):
     """Two ``GroupedLinear`` layers with an (erf) GELU between them (fp8_gmm/example.py:72-103)."""
 
-    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype=torch.bfloat16, cutlass=False, device="cuda"):
-        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device)
+    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype=torch.bfloat16, cutlass=False, device="cuda",
+                 layer_norm=False):
+        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm)
         self.grouped_linear1 = GroupedLinear(n_embd, n_inner, n_experts, dtype=dtype, cutlass=cutlass, device=device)
         self.grouped_linear2 = GroupedLinear(n_inner, n_embd, n_experts, dtype=dtype, cutlass=cutlass, device=device)
         self.act = torch.nn.GELU()
@@ -132,8 +139,8 @@ class Fp8LinearModule(_RoutedModule):
 class Fp8MlpModule(_RoutedModule):
     """One ``GroupedMlp`` (tanh-GELU fused into the first GEMM) as the experts (fp8_gmm/example.py:106-130)."""
 
-    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype=torch.bfloat16, device="cuda"):
-        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device)
+    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype=torch.bfloat16, device="cuda", layer_norm=False):
+        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm)
         self.grouped_mlp = GroupedMlp(n_embd, n_inner, n_experts, dtype=dtype, device=device)
 
     def start_experts(self):

@@ -43,6 +43,10 @@ extern "C" {
 #define FP8GMM_E5M2 1
 /* output kind of the GEMM epilogue */
 #define FP8GMM_OUT_BF16 2
+/* element types of the operators around the layers (layer norm, embedding, norm of many tensors) */
+#define FP8GMM_TYPE_BF16 0
+#define FP8GMM_TYPE_FP16 1
+#define FP8GMM_TYPE_FP32 2
 
 typedef enum fp8gmm_status {
   FP8GMM_OK = 0,
@@ -673,6 +677,59 @@ int fp8gmm_moe_scatter_wgrad(const void* x, const void* grad_out, const int32_t*
  * calls.  grad_x: bf16 [rows, hidden]. */
 int fp8gmm_moe_scatter_backward(const void* x, const void* grad_out, const int32_t* indices, const float* weights,
                                 void* grad_x, float* grad_w, int rows, int hidden, int top_k, void* stream);
+
+/* ---- around the routed layers of a training step ------------------------------------------ */
+/*
+ * No counterparts in the reference, whose users take these from torch.  Types: FP8GMM_TYPE_*.  Pointers need the alignment of
+ * an element unless stated otherwise; sums, statistics and norms are kept in fp32 or fp64, a result is rounded once.
+ *
+ * fp8gmm_layer_norm: y[r, :] = (x[r, :] - m) / sqrt(mean((x[r, :] - m)^2) + eps) * weight + bias, m the mean of x[r, :].
+ * x: [rows, cols] of `type` with a pitch of ldx >= cols elements; y: the same without a pitch; weight and bias (may be NULL):
+ * [cols] of `param_type`, which is `type` or fp32.  mean, rstd: fp32 [rows] for the backward pass, or both NULL.
+ * 1 <= cols <= 2^30, rows < 2^31.
+ */
+int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                      int64_t rows, int cols, float eps, int type, int param_type, void* stream);
+/*
+ * Its gradients.  With z the normed rows before the weight and g = dy * weight: dx[r, :] = rstd (g - mean(g) - z mean(g z)),
+ * dweight = sum over the rows of dy z, dbias = sum over the rows of dy; each of the three may be NULL and is then not computed.
+ * dx: [rows, cols] without a pitch.  workspace: fp8gmm_layer_norm_workspace_bytes bytes on 16 bytes where dweight or dbias is
+ * asked for and there are rows; without rows they are zeros.  The same bits from call to call.
+ */
+size_t fp8gmm_layer_norm_workspace_bytes(int64_t rows, int cols, int type);
+int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* weight, const float* mean,
+                               const float* rstd, void* dx, void* dweight, void* dbias, int64_t rows, int cols, int type,
+                               int param_type, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * fp8gmm_embedding: y[t, :] = scale * weight[ids[t], :] for t in [0, n), a row of zeros where ids[t] is outside [0, table).
+ * ids: int64 (ids64 != 0) or int32; weight: [table, cols] of `type`; n <= 2^28, table < 2^31 - 1, cols <= 2^24.
+ * fp8gmm_embedding_backward: dweight[v, :] = scale * sum of dy[t, :] over the t with ids[t] == v, in the order of t, the whole
+ * table, zeros where there are none; `padding` (-1: none) is an id whose tokens are left out.  dweight and workspace
+ * (fp8gmm_embedding_workspace_bytes) on 16 bytes.  The same bits from call to call.
+ */
+int fp8gmm_embedding(const void* ids, int ids64, int64_t n, const void* weight, int64_t table, int cols, float scale, int type,
+                     void* y, void* stream);
+size_t fp8gmm_embedding_workspace_bytes(int64_t n, int64_t table, int cols, int type);
+int fp8gmm_embedding_backward(const void* ids, int ids64, int64_t n, const void* dy, void* dweight, int64_t table, int cols,
+                              float scale, int64_t padding, int type, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * fp8gmm_multi_norm: *norm = sqrt of the sum of the squares of all elements of all tensors, added up in fp64.
+ * fp8gmm_multi_clip: the same, and out = in * min(1, max_norm / (norm + 1e-6)) for every tensor, out_type its type or fp32.
+ * A result may stand in the place of its own tensor (in == out, the same type); it may overlap nothing else of the call
+ * (FP8GMM_ERR_BAD_ARGUMENT).  Gradients in place are not written again where the factor is 1.  A norm that is infinite or a
+ * NaN makes a factor of 0 or a NaN.  `tensors` is HOST memory and is read during the call only: the table travels in the
+ * launches' arguments.  norm: device fp32.  workspace: fp8gmm_multi_norm_workspace_bytes(n) bytes on 16 bytes.
+ */
+typedef struct fp8gmm_norm_tensor {
+  const void* in;
+  void* out;              /* fp8gmm_multi_clip */
+  int64_t count;          /* elements */
+  int32_t type, out_type;
+} fp8gmm_norm_tensor;     /* 32 bytes */
+size_t fp8gmm_multi_norm_workspace_bytes(int n);
+int fp8gmm_multi_norm(const fp8gmm_norm_tensor* tensors, int n, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+int fp8gmm_multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float* norm, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* ---- schedule introspection (host only, no GPU needed) ------------------------------------ */
 /*
