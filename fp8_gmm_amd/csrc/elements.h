@@ -61,18 +61,25 @@ struct Elements {
     else if constexpr (TYPE == FP8GMM_TYPE_FP16) return __builtin_bit_cast(uint16_t, (_Float16)v);
     else return __float_as_uint(v);
   }
-  // the piece at `p`, of which the first `n` elements are the row's: zeros behind them
+  // the piece at `p`, of which the first `n` elements are the row's: zeros behind them.  STREAM: with the streaming hint.
+  template <bool STREAM = false>
   static __device__ __forceinline__ u32x4 load(const bits* p, int n) {
-    if (n >= kVec) return *reinterpret_cast<const piece*>(p);
+    if (n >= kVec) {
+      const piece* const at = reinterpret_cast<const piece*>(p);
+      if constexpr (STREAM) return __builtin_nontemporal_load(at);
+      return *at;
+    }
     u32x4 raw = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < kVec - 1; ++i)
       if (i < n) raw[i * kBytes / 4] |= (uint32_t)p[i] << (i * kBytes % 4 * 8);
     return raw;
   }
+  template <bool STREAM = false>   // (chosen at run time, the two stores are made one by the compiler, without the hint)
   static __device__ __forceinline__ void store(bits* p, int n, u32x4 raw) {
     if (n >= kVec) {
-      *reinterpret_cast<piece*>(p) = raw;
+      if constexpr (STREAM) __builtin_nontemporal_store((piece)raw, reinterpret_cast<piece*>(p));
+      else *reinterpret_cast<piece*>(p) = raw;
       return;
     }
 #pragma unroll
@@ -104,10 +111,24 @@ struct Parameters {
   }
 };
 
-template <int WIDTH>   // lanes, a power of two up to 64
+// The sum over groups of 16 lanes, or over all 64, the same bits in every lane of a group: lanes exchange their values inside the
+// vector unit (data-parallel primitives), which takes a tenth of the time of an exchange through LDS.
+template <int CONTROL>
+__device__ __forceinline__ float lanes_step(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CONTROL, 0xf, 0xf, true));
+}
+template <int WIDTH>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int off = WIDTH / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  static_assert(WIDTH == 16 || WIDTH == 64, "a row of the data-parallel primitives, or a wavefront");
+  v = lanes_step<0xb1>(v);    // quad_perm: the neighbour
+  v = lanes_step<0x4e>(v);    // quad_perm: the other pair
+  v = lanes_step<0x141>(v);   // row_half_mirror: the other four
+  v = lanes_step<0x140>(v);   // row_mirror: the other eight
+  if constexpr (WIDTH == 64) {
+    const int bits = __float_as_int(v);
+    v = (__int_as_float(__builtin_amdgcn_readlane(bits, 0)) + __int_as_float(__builtin_amdgcn_readlane(bits, 16))) +
+        (__int_as_float(__builtin_amdgcn_readlane(bits, 32)) + __int_as_float(__builtin_amdgcn_readlane(bits, 48)));
+  }
   return v;
 }
 

@@ -16,93 +16,175 @@
 namespace fp8gmm {
 namespace {
 
-constexpr int kNormMaxBlocks = 512;   // workgroups of a backward pass, each with one partial sum of the parameters' gradients
+constexpr int kBackwardThreads = 1024;   // of a workgroup of the backward pass: as many rows at a time as fit, since every workgroup
+constexpr int kBackwardBlocks = 256;     // leaves one partial sum of the parameters' gradients in memory; one per compute unit
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormSlab = 1 << 21;   // rows of a launch with a workgroup to a row: a grid has fewer than 2^32 threads
+
+constexpr int kNormWaves = 16;           // the most wavefronts that share a row
+constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, where a row needs no more
+constexpr int kForwardAll = 256 * 2048;  // of its launch: what the compute units hold
 
 // The sum over the THREADS threads of a row, the same in all of them.  `slot`: THREADS / 64 floats of LDS per row that nobody
 // uses before the next barrier but one.
 template <int THREADS>
 __device__ __forceinline__ float row_sum(float v, float* slot) {
-  if constexpr (THREADS <= 64) {
-    return lanes_sum<THREADS>(v);
-  } else {
-    v = lanes_sum<64>(v);
-    if (threadIdx.x % 64 == 0) slot[threadIdx.x % THREADS / 64] = v;
-    __syncthreads();
-    float sum = 0.f;
+  v = lanes_sum<64>(v);
+  if (threadIdx.x % 64 == 0) slot[threadIdx.x / 64] = v;
+  __syncthreads();
+  float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) sum += slot[i];
-    return sum;
-  }
+  for (int i = 0; i < THREADS / 64; ++i) sum += slot[i];
+  return sum;
 }
 
-// THREADS threads share a row, C pieces each; a workgroup of 256 at least.
-template <int TYPE, int PTYPE, int THREADS, int C>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void layer_norm_kernel(
-    const void* __restrict__ x_, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* __restrict__ y_,
-    float* __restrict__ mean_out, float* __restrict__ rstd_out, int rows, int cols, float eps) {
+// How the pieces of a row are reached, without a branch where that can be: the compiler then knows how many accesses are under
+// way, and waits for the loads of the next row alone and not for the stores behind them.
+//   kWhole  rows of whole pieces on 16 bytes: through a buffer descriptor of the row.  What lies behind its end, or belongs to no
+//           row, reads as zeros and is not stored.
+//   kEdge   other rows of at least one piece, at any element: the last piece ends where the row ends and begins inside the piece
+//           before it, and threads behind the end have the last piece too.  What a thread has twice it leaves out of the sums and
+//           stores all the same: the same bits to the same place.
+//   kShort  shorter rows, element by element.
+//   kEdgeStream  kEdge with its results written with the streaming hint: the compiler makes one store, without it, of two that are
+//           chosen from at run time
+enum { kWhole, kEdge, kEdgeStream, kShort };
+constexpr bool is_edge(int mode) { return mode == kEdge || mode == kEdgeStream; }
+
+// Where a thread's piece begins that begins at `at`, and how many of its elements are not its own
+template <int MODE, int V>
+__device__ __forceinline__ int piece_begin(int at, int cols) { return is_edge(MODE) ? min(at, cols - V) : at; }
+template <int MODE, int V>
+__device__ __forceinline__ int piece_skip(int at, int cols) {
+  return is_edge(MODE) ? min(at - piece_begin<MODE, V>(at, cols), V) : at < cols ? 0 : V;
+}
+// Whether element i counts: of kShort, the row's first piece only
+template <int MODE>
+__device__ __forceinline__ bool own(int i, int skip, int cols) { return i >= skip && (MODE != kShort || i < cols); }
+
+template <int TYPE, int MODE>
+struct RowAccess {
   typedef Elements<TYPE> E;
   typedef typename E::bits bits;
-  constexpr int V = E::kVec, ROWS = THREADS < 256 ? 256 / THREADS : 1;
-  __shared__ float slots[2][THREADS > 64 ? THREADS / 64 : 1];
-  const int t = threadIdx.x % THREADS;
-  int64_t row = (int64_t)blockIdx.x * ROWS;
-  if constexpr (THREADS == 64) row += __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  else if constexpr (THREADS < 64) row += threadIdx.x / THREADS;
-  if (row >= rows) return;   // never with more than a wavefront to a row
-  const bits* const x = static_cast<const bits*>(x_) + row * ldx;
-  u32x4 raw[C];
+  bits* p;
+  __amdgpu_buffer_rsrc_t r;
+  int cols;
+  __device__ __forceinline__ RowAccess(const void* base, int64_t row, int64_t rows, int64_t pitch, int n) {
+    const bool live = row < rows;
+    cols = live || is_edge(MODE) ? n : 0;
+    p = const_cast<bits*>(static_cast<const bits*>(base)) + (live ? row : rows - 1) * pitch;   // kEdge: the last row once more
+    if constexpr (MODE == kWhole) r = make_rsrc(p, (uint32_t)cols * E::kBytes);
+  }
+  template <bool STREAM>
+  __device__ __forceinline__ u32x4 load(int at) const {
+    if constexpr (MODE == kWhole) return STREAM ? buf_load16_stream(r, (uint32_t)at * E::kBytes) : buf_load16(r, (uint32_t)at * E::kBytes);
+    else return E::template load<STREAM>(p + at, is_edge(MODE) ? E::kVec : cols - at);
+  }
+  __device__ __forceinline__ void store(int at, u32x4 v, bool stream) const {
+    if constexpr (MODE == kWhole) stream ? buf_store16_stream(v, r, (uint32_t)at * E::kBytes) : buf_store16(v, r, (uint32_t)at * E::kBytes);
+    else E::template store<MODE == kEdgeStream>(p + at, is_edge(MODE) ? E::kVec : cols - at, v);
+  }
+};
+
+// A workgroup takes ROWS rows at a time, THREADS threads to a row and C pieces to a thread, and goes on to other rows by the grid:
+// the next rows are loaded before the statistics of the present ones are shared, and the parameters stay in registers.
+// The wavefronts of a row meet once: each brings its sum and the squares around its own mean, which combine to those around the
+// row's, sum (M2_w + n_w (m_w - m)^2).
+template <int TYPE, int PTYPE, int LANES, int C, int MODE, int MOST>
+__global__ __launch_bounds__(MOST) void layer_norm_kernel(
+    const void* __restrict__ x_, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, void* __restrict__ y_,
+    float* __restrict__ mean_out, float* __restrict__ rstd_out, int rows, int cols, float eps, int waves, bool stream) {
+  typedef Elements<TYPE> E;
+  constexpr int V = E::kVec;
+  __shared__ float slots[2][2][kNormWaves][kNormWaves];
+  const int THREADS = LANES * waves, ROWS = blockDim.x / THREADS;
+  int group = threadIdx.x / THREADS;
+  if constexpr (LANES == 64) group = __builtin_amdgcn_readfirstlane(group);
+  const int t = threadIdx.x - group * THREADS;
+  int at[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) at[c] = (c * THREADS + t) * V;
+  const int skip = piece_skip<MODE, V>(at[C - 1], cols);   // the pieces before the last one are there in whole
+  at[C - 1] = piece_begin<MODE, V>(at[C - 1], cols);
+  u32x4 next[C];
+  const auto load = [&](int64_t row) {
+    const RowAccess<TYPE, MODE> from(x_, row, rows, ldx, cols);
+#pragma unroll
+    for (int c = 0; c < C; ++c) next[c] = from.template load<false>(at[c]);
+  };
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + group;
+  load(row);
   Parameters<TYPE, PTYPE> pw[C], pb[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int at = (c * THREADS + t) * V;
-    raw[c] = E::load(x + at, cols - at);
+    pw[c].load(w, at[c], cols - at[c]);
+    if (b != nullptr) pb[c].load(b, at[c], cols - at[c]);
   }
+  // elements of a row's wavefront (group of 16 lanes): its piece c covers columns from (c THREADS + first lane) V on
+  const auto held = [&](int wave) {
+    int n = 0;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int at = (c * THREADS + t) * V;
-    pw[c].load(w, at, cols - at);
-    if (b != nullptr) pb[c].load(b, at, cols - at);
-  }
-  const float count = (float)cols;
-  float sum = 0.f;
+    for (int c = 0; c < C; ++c) n += min(max(cols - (c * THREADS + wave * LANES) * V, 0), LANES * V);
+    return (float)n;
+  };
+  const int wave = LANES == 64 ? __builtin_amdgcn_readfirstlane(t / 64) : 0;
+  const float count = (float)cols, mine = held(wave);
+  const int peer = threadIdx.x % 16;   // the wavefront whose share this lane takes up where they meet
+  const float peer_count = peer < waves ? held(peer) : 0.f;
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * ROWS; first < rows; first += stride, row += stride, turn ^= 1) {
+    u32x4 x[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    float f[V];
-    E::unpack(raw[c], f);
+    for (int c = 0; c < C; ++c) x[c] = next[c];
+    if (first + stride < rows) load(row + stride);
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum += f[i];
-  }
-  const float mean = row_sum<THREADS>(sum, slots[0]) / count;
-  float squares = 0.f;
+    for (int c = 0; c < C; ++c) {
+      float f[V];
+      E::unpack(x[c], f);
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int n = cols - (c * THREADS + t) * V;
-    float f[V];
-    E::unpack(raw[c], f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float d = i < n ? f[i] - mean : 0.f;
-      squares = __builtin_fmaf(d, d, squares);
+      for (int i = 0; i < V; ++i) sum += !is_edge(MODE) || c < C - 1 || i >= skip ? f[i] : 0.f;
     }
-  }
-  const float rstd = 1.0f / sqrtf(row_sum<THREADS>(squares, slots[1]) / count + eps);
-  if (mean_out != nullptr && t == 0) {
-    mean_out[row] = mean;
-    rstd_out[row] = rstd;
-  }
-  bits* const y = static_cast<bits*>(y_) + row * cols;
+    sum = lanes_sum<LANES>(sum);
+    float mean = sum / mine, squares = 0.f;   // every wavefront of a row has some of it
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int at = (c * THREADS + t) * V;
-    float f[V], fw[V], fb[V];
-    E::unpack(raw[c], f);
-    pw[c].get(fw);
-    if (b != nullptr) pb[c].get(fb);
+    for (int c = 0; c < C; ++c) {
+      float f[V];
+      E::unpack(x[c], f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = __builtin_fmaf((f[i] - mean) * rstd, fw[i], b != nullptr ? fb[i] : 0.f);
-    E::store(y + at, cols - at, E::pack(f));
+      for (int i = 0; i < V; ++i) {
+        const float d = c < C - 1 || own<MODE>(i, skip, cols) ? f[i] - mean : 0.f;
+        squares = __builtin_fmaf(d, d, squares);
+      }
+    }
+    squares = lanes_sum<LANES>(squares);
+    if (LANES == 64 && waves > 1) {   // the other turn's slots are read before the next barrier
+      if (threadIdx.x % 64 == 0) {
+        slots[turn][0][group][wave] = mean;
+        slots[turn][1][group][wave] = squares;
+      }
+      __syncthreads();
+      const float m = peer < waves ? slots[turn][0][group][peer] : 0.f, q = peer < waves ? slots[turn][1][group][peer] : 0.f;
+      mean = lanes_sum<16>(peer_count * m) / count;
+      squares = lanes_sum<16>(__builtin_fmaf(peer_count * (m - mean), m - mean, q));
+    }
+    const float rstd = 1.0f / sqrtf(squares / count + eps);
+    if (mean_out != nullptr && t == 0 && row < rows) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    const RowAccess<TYPE, MODE> y(y_, row, rows, cols, cols);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float f[V], fw[V], fb[V];
+      E::unpack(x[c], f);
+      pw[c].get(fw);
+      if (b != nullptr) pb[c].get(fb);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = __builtin_fmaf((f[i] - mean) * rstd, fw[i], b != nullptr ? fb[i] : 0.f);
+      y.store(at[c], E::pack(f), stream);
+    }
   }
 }
 
@@ -159,46 +241,43 @@ __global__ __launch_bounds__(kNormLongThreads) void layer_norm_long_kernel(
   }
 }
 
-// Threads of a workgroup of the backward pass whose threads hold C pieces of a row each: as many rows at a time as their
-// registers allow, since every workgroup leaves one partial sum of the parameters' gradients in memory.
-constexpr int backward_threads(int c) { return c >= 4 ? 512 : 1024; }
-
-// A workgroup takes ROWS rows at a time, THREADS threads and C pieces each, and keeps the sums of dy z and dy for its
-// columns; the rows' next ones are loaded before the sums of the present ones are shared.  `part`: [workgroup][2][cols], the
+// The backward pass in the same way, with the sums of dy z and dy for the columns of its threads.  `part`: [workgroup][2][cols], the
 // second without a bias left out; NULL where the parameters take no gradients.  dx may be NULL.
-template <int TYPE, int PTYPE, int THREADS, int C>
-__global__ __launch_bounds__(THREADS > backward_threads(C) ? THREADS : backward_threads(C)) void layer_norm_backward_kernel(
+template <int TYPE, int PTYPE, int LANES, int C, int MODE>
+__global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
     const void* __restrict__ dy_, int64_t ldy, const void* __restrict__ x_, int64_t ldx, const void* __restrict__ w,
     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, void* __restrict__ dx_, float* __restrict__ part,
-    int bias, int rows, int cols) {
+    int bias, int rows, int cols, int waves, bool stream) {
   typedef Elements<TYPE> E;
-  typedef typename E::bits bits;
-  constexpr int BLOCK = THREADS > backward_threads(C) ? THREADS : backward_threads(C);
-  constexpr int V = E::kVec, ROWS = BLOCK / THREADS, WAVES = THREADS > 64 ? THREADS / 64 : 1;
-  __shared__ float slots[2][2][ROWS][WAVES];
-  __shared__ float sums[BLOCK * V];
-  const int t = threadIdx.x % THREADS;
+  constexpr int V = E::kVec;
+  __shared__ float slots[2][2][kNormWaves][kNormWaves];
+  __shared__ float sums[kBackwardThreads * V];
+  const int THREADS = LANES * waves, ROWS = blockDim.x / THREADS;
   int group = threadIdx.x / THREADS;
-  if constexpr (THREADS >= 64) group = __builtin_amdgcn_readfirstlane(group);
+  if constexpr (LANES == 64) group = __builtin_amdgcn_readfirstlane(group);
+  const int t = threadIdx.x - group * THREADS;
+  const int wave = LANES == 64 ? __builtin_amdgcn_readfirstlane(t / 64) : 0, peer = threadIdx.x % 16;
+  int at[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) at[c] = (c * THREADS + t) * V;
+  const int skip = piece_skip<MODE, V>(at[C - 1], cols);   // the pieces before the last one are there in whole
+  at[C - 1] = piece_begin<MODE, V>(at[C - 1], cols);
   Parameters<TYPE, PTYPE> pw[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int at = (c * THREADS + t) * V;
-    pw[c].load(w, at, cols - at);
-  }
+  for (int c = 0; c < C; ++c) pw[c].load(w, at[c], cols - at[c]);
   float dw[C][V] = {}, db[C][V] = {};
   u32x4 nx[C], ny[C];
-  float nm = 0.f, nr = 0.f;
+  float nm, nr;
   const auto load = [&](int64_t row) {
-    const bool live = row < rows;
+    const RowAccess<TYPE, MODE> x(x_, row, rows, ldx, cols), y(dy_, row, rows, ldy, cols);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int at = (c * THREADS + t) * V;
-      nx[c] = E::load(static_cast<const bits*>(x_) + row * ldx + at, live ? cols - at : 0);
-      ny[c] = E::load(static_cast<const bits*>(dy_) + row * ldy + at, live ? cols - at : 0);
+      nx[c] = x.template load<true>(at[c]);
+      ny[c] = y.template load<true>(at[c]);
     }
-    nm = live ? mean_in[row] : 0.f;
-    nr = live ? rstd_in[row] : 0.f;
+    const int64_t live = row < rows ? row : rows - 1;
+    nm = mean_in[live];
+    nr = rstd_in[live];
   };
   const int64_t stride = (int64_t)gridDim.x * ROWS;
   int64_t row = (int64_t)blockIdx.x * ROWS + group;
@@ -211,9 +290,10 @@ __global__ __launch_bounds__(THREADS > backward_threads(C) ? THREADS : backward_
       x[c] = nx[c];
       y[c] = ny[c];
     }
-    const float mean = nm, rstd = nr;
-    load(row + stride);
+    const float rstd = nr, shift = -nm * nr;
+    if (first + stride < rows) load(row + stride);
     float s1 = 0.f, s2 = 0.f;
+    if (!is_edge(MODE) || row < rows) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       float fx[V], fy[V], fw[V];
@@ -222,48 +302,42 @@ __global__ __launch_bounds__(THREADS > backward_threads(C) ? THREADS : backward_
       pw[c].get(fw);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float z = (fx[i] - mean) * rstd, g = fy[i] * fw[i];
+        if (is_edge(MODE) && c == C - 1 && i < skip) fy[i] = 0.f;   // elsewhere they are zeros
+        const float z = __builtin_fmaf(fx[i], rstd, shift), g = fy[i] * fw[i];
         s1 += g;
         s2 = __builtin_fmaf(g, z, s2);
         dw[c][i] = __builtin_fmaf(fy[i], z, dw[c][i]);
         db[c][i] += fy[i];
       }
     }
+    }
     if (dx_ == nullptr) continue;
-    if constexpr (THREADS <= 64) {
-      s1 = lanes_sum<THREADS>(s1);
-      s2 = lanes_sum<THREADS>(s2);
-    } else {   // both with one barrier; the other turn's slots are read before the next one
-      s1 = lanes_sum<64>(s1);
-      s2 = lanes_sum<64>(s2);
+    s1 = lanes_sum<LANES>(s1);
+    s2 = lanes_sum<LANES>(s2);
+    if (LANES == 64 && waves > 1) {   // the other turn's slots are read before the next barrier
       if (threadIdx.x % 64 == 0) {
-        slots[turn][0][group][t / 64] = s1;
-        slots[turn][1][group][t / 64] = s2;
+        slots[turn][0][group][wave] = s1;
+        slots[turn][1][group][wave] = s2;
       }
       __syncthreads();
-      s1 = s2 = 0.f;
-#pragma unroll
-      for (int i = 0; i < WAVES; ++i) {
-        s1 += slots[turn][0][group][i];
-        s2 += slots[turn][1][group][i];
-      }
+      s1 = lanes_sum<16>(peer < waves ? slots[turn][0][group][peer] : 0.f);
+      s2 = lanes_sum<16>(peer < waves ? slots[turn][1][group][peer] : 0.f);
     }
-    if (row >= rows) continue;
-    const float m1 = s1 / (float)cols, m2 = s2 / (float)cols;
-    bits* const dx = static_cast<bits*>(dx_) + row * cols;
+    if (is_edge(MODE) && row >= rows) continue;   // its sums leave no row out
+    const float c1 = -rstd * (s1 / (float)cols), c2 = -rstd * (s2 / (float)cols);
+    const RowAccess<TYPE, MODE> dx(dx_, row, rows, cols, cols);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int at = (c * THREADS + t) * V;
       float fx[V], fy[V], fw[V];
       E::unpack(x[c], fx);
       E::unpack(y[c], fy);
       pw[c].get(fw);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float z = (fx[i] - mean) * rstd;
-        fx[i] = rstd * (__builtin_fmaf(fy[i], fw[i], -m1) - z * m2);
+        const float z = __builtin_fmaf(fx[i], rstd, shift);
+        fx[i] = __builtin_fmaf(fy[i], fw[i] * rstd, __builtin_fmaf(z, c2, c1));
       }
-      E::store(dx + at, cols - at, E::pack(fx));
+      dx.store(at[c], E::pack(fx), stream);
     }
   }
   if (part == nullptr) return;
@@ -274,23 +348,22 @@ __global__ __launch_bounds__(THREADS > backward_threads(C) ? THREADS : backward_
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       if (which == 1 && !bias) continue;
-      if constexpr (ROWS > 1) {
+      if (ROWS > 1) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < V; ++i) sums[(group * THREADS + t) * V + i] = which == 0 ? dw[c][i] : db[c][i];
+        for (int i = 0; i < V; ++i) sums[threadIdx.x * V + i] = which == 0 ? dw[c][i] : db[c][i];
         __syncthreads();
-        for (int col = threadIdx.x; col < THREADS * V; col += BLOCK) {
+        for (int k = threadIdx.x; k < THREADS * V; k += blockDim.x) {
           float sum = 0.f;
-#pragma unroll
-          for (int r = 0; r < ROWS; ++r) sum += sums[r * THREADS * V + col];
-          const int64_t at = (int64_t)c * THREADS * V + col;
-          if (at < cols) out[(int64_t)which * cols + at] = sum;
+          for (int r = 0; r < ROWS; ++r) sum += sums[r * THREADS * V + k];
+          const int piece = (c * THREADS + k / V) * V;
+          if (own<MODE>(k % V, piece_skip<MODE, V>(piece, cols), cols))
+            out[(int64_t)which * cols + piece_begin<MODE, V>(piece, cols) + k % V] = sum;
         }
       } else {
-        const int at = (c * THREADS + t) * V;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          if (at + i < cols) out[(int64_t)which * cols + at + i] = which == 0 ? dw[c][i] : db[c][i];
+          if (c < C - 1 || own<MODE>(i, skip, cols)) out[(int64_t)which * cols + at[c] + i] = which == 0 ? dw[c][i] : db[c][i];
       }
     }
 }
@@ -397,32 +470,55 @@ __global__ __launch_bounds__(1024) void layer_norm_params_kernel(const float* __
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// How a row's pieces are shared out: threads to a row and pieces to a thread, by the number of pieces.  Zero threads: longer
-// than the registers of a workgroup hold.
+// How a row is shared out: `lanes` * `waves` threads, `pieces` 16-byte pieces to each.  No lanes: longer than the registers of a
+// workgroup hold.
 struct Shape {
-  int threads, pieces;
+  int lanes, waves, pieces;
+  int threads() const { return lanes * waves; }
 };
-Shape norm_shape(int cols, int type) {
-  const int pieces = ceil_div(cols, type == FP8GMM_TYPE_FP32 ? 4 : 8);
-  if (pieces <= 16) return {16, 1};
-  if (pieces <= 64) return {64, 1};
-  if (pieces <= 128) return {64, 2};
-  if (pieces <= 256) return {64, 4};
-  if (pieces <= 512) return {256, 2};
-  if (pieces <= 1024) return {256, 4};
-  if (pieces <= 2048) return {1024, 2};
-  if (pieces <= 4096) return {1024, 4};
-  return {0, 0};
+int pieces_of(int cols, int type) { return ceil_div(cols, 16 / type_bytes(type)); }
+// Up to `most` pieces to a thread, as few threads as that allows, and then as few pieces: a thread behind the row's end works for
+// nothing.  `waves`: the most of them.  A row's first 64 * waves pieces are there, so that every wavefront has some of the row.
+Shape shape_of(int pieces, int most, int waves) {
+  if (pieces <= 16) return {16, 1, 1};
+  const int w = ceil_div(pieces, 64 * most);
+  return w <= waves ? Shape{64, w, ceil_div(pieces, 64 * w)} : Shape{0, 0, 0};
+}
+// The longest rows that stay in registers have 4 pieces in each of 1024 threads, which fits fp32 alone: a 16-bit type has twice
+// the elements and spills (4096 x 32768, bf16: 190 and 638 us forward and backward, by the kernels for longer rows 148 and
+// 302; 4096 x 16384, fp32: 99 and 186, by those 143 and 294).
+Shape widest(int cols, int type) {
+  const int w = ceil_div(pieces_of(cols, type), 64 * 4);
+  return type == FP8GMM_TYPE_FP32 && w <= kNormWaves ? Shape{64, w, 4} : Shape{0, 0, 0};
+}
+// Forward, 4 pieces to a thread: few barriers and many loads under way.
+Shape forward_shape(int cols, int type) {
+  const Shape s = shape_of(pieces_of(cols, type), 4, 8);
+  return s.lanes != 0 ? s : widest(cols, type);
+}
+// Backward, 2: the sums of the parameters' gradients take registers as well.
+Shape backward_shape(int cols, int type) {
+  const int pieces = pieces_of(cols, type);
+  if (pieces > 128 && pieces <= 192) return {64, 3, 1};   // not 2 x 2, of which these leave a quarter idle or more
+  const Shape s = shape_of(pieces, 2, kNormWaves);
+  return s.lanes != 0 ? s : widest(cols, type);
+}
+// Rows of whole pieces on 16 bytes
+bool whole(const void* p, int64_t pitch, int cols, int type) {
+  const int pieces = 16 / type_bytes(type);
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch % pieces == 0 && cols % pieces == 0;
+}
+// Whether a result is written with the streaming hint: one that outgrows the cache is not found there by whoever reads it.
+bool streams(int64_t rows, int cols, int type) { return rows * cols * type_bytes(type) > (int64_t)64 << 20; }
+int mode_of(int cols, int type, bool aligned, bool stream_edges) {
+  return cols < 16 / type_bytes(type) ? kShort : aligned ? kWhole : stream_edges ? kEdgeStream : kEdge;
 }
 // Workgroups of a backward pass: partial sums that its parameters' gradients have.
 int backward_blocks(int rows, int cols, int type) {
-  const Shape s = norm_shape(cols, type);
-  if (s.threads == 0) return std::min(rows, 64);
-  const int block = std::max(s.threads, backward_threads(s.pieces));
-  return std::min(ceil_div(rows, block / s.threads), kNormMaxBlocks * 512 / block);
+  const Shape s = backward_shape(cols, type);
+  if (s.lanes == 0) return std::min(rows, 64);
+  return std::min(ceil_div(rows, kBackwardThreads / s.threads()), kBackwardBlocks);
 }
-
-#define FP8GMM_NORM_SHAPES(X) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(256, 4) X(1024, 2) X(1024, 4)
 
 // calls f(TYPE, PTYPE) with the two as integral constants
 template <class F>
@@ -456,7 +552,10 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
   if (rows == 0) return FP8GMM_OK;
   if (x == nullptr || weight == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr)) return FP8GMM_ERR_NULL_POINTER;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const Shape shape = norm_shape(cols, type);
+  const Shape shape = forward_shape(cols, type);
+  const int threads = shape.lanes == 0 ? 0 : std::max(shape.threads(), kForwardThreads / shape.threads() * shape.threads());
+  const bool streaming = streams(rows, cols, type);
+  const int mode = mode_of(cols, type, whole(x, ldx, cols, type) && whole(y, cols, cols, type), streaming);
   for (int64_t r0 = 0; r0 < rows; r0 += kNormSlab) {
     const int n = (int)std::min<int64_t>(kNormSlab, rows - r0), size = type_bytes(type);
     const void* const xs = static_cast<const char*>(x) + r0 * ldx * size;
@@ -464,14 +563,25 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
     float* const ms = mean != nullptr ? mean + r0 : nullptr;
     float* const rs = rstd != nullptr ? rstd + r0 : nullptr;
     with_types(type, param_type, [&](auto tc, auto pc) {
-      constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
-#define FP8GMM_LAUNCH(THREADS, C)                                                                                       \
-  if (shape.threads == THREADS && shape.pieces == C)                                                                    \
-    hipLaunchKernelGGL((layer_norm_kernel<T, P, THREADS, C>), dim3(ceil_div(n, THREADS < 256 ? 256 / THREADS : 1)),     \
-                       dim3(THREADS < 256 ? 256 : THREADS), 0, s, xs, ldx, weight, bias, ys, ms, rs, n, cols, eps);
-      FP8GMM_NORM_SHAPES(FP8GMM_LAUNCH)
+      constexpr int T = decltype(tc)::value, P = decltype(pc)::value; 
+#define FP8GMM_LAUNCH(LANES, C, MOST)                                                                                         \
+  if (shape.lanes == LANES && shape.pieces == C && threads <= MOST) {                                                         \
+    auto* kernel = mode == kEdge         ? &layer_norm_kernel<T, P, LANES, C, kEdge, MOST>                                    \
+                   : mode == kEdgeStream ? &layer_norm_kernel<T, P, LANES, C, kEdgeStream, MOST>                              \
+                                         : &layer_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : kShort, MOST>;           \
+    hipLaunchKernelGGL(kernel, dim3(std::min(ceil_div(n, threads / shape.threads()), kForwardAll / threads)), dim3(threads), 0, s, \
+                       xs, ldx, weight, bias, ys, ms, rs, n, cols, eps, shape.waves, streaming);                              \
+  } else
+      FP8GMM_LAUNCH(16, 1, 256)
+      FP8GMM_LAUNCH(64, 1, 256)
+      FP8GMM_LAUNCH(64, 2, 512)
+      FP8GMM_LAUNCH(64, 3, 512)
+      FP8GMM_LAUNCH(64, 4, 512)
+      if constexpr (T == FP8GMM_TYPE_FP32) {
+        FP8GMM_LAUNCH(64, 4, 1024) {}
+      }
 #undef FP8GMM_LAUNCH
-      if (shape.threads == 0)
+      if (shape.lanes == 0)
         hipLaunchKernelGGL((layer_norm_long_kernel<T, P>), dim3(n), dim3(kNormLongThreads), 0, s, xs, ldx, weight, bias, ys, ms,
                            rs, cols, eps);
     });
@@ -503,18 +613,30 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
   hipStream_t s = static_cast<hipStream_t>(stream);
   float* const part = params ? static_cast<float*>(workspace) : nullptr;
   const int blocks = backward_blocks((int)rows, cols, type), bias = dbias != nullptr;
-  const Shape shape = norm_shape(cols, type);
+  const Shape shape = backward_shape(cols, type);
+  const bool streaming = streams(rows, cols, type);
+  // of a 16-bit type, edges are written without the hint (16384 x 4093, bf16: 76 us, with it 80; 60001 x 2047, fp32: 286 and 267)
+  const int mode = mode_of(cols, type, whole(x, ldx, cols, type) && whole(dy, ldy, cols, type) && (dx == nullptr || whole(dx, cols, cols, type)),
+                           streaming && type == FP8GMM_TYPE_FP32);
   with_types(type, param_type, [&](auto tc, auto pc) {
-    constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
+    constexpr int T = decltype(tc)::value, P = decltype(pc)::value; 
     if (rows > 0) {
-#define FP8GMM_LAUNCH(THREADS, C)                                                                                       \
-  if (shape.threads == THREADS && shape.pieces == C)                                                                    \
-    hipLaunchKernelGGL((layer_norm_backward_kernel<T, P, THREADS, C>), dim3(blocks),                                    \
-                       dim3(THREADS > backward_threads(C) ? THREADS : backward_threads(C)), 0, s, dy, ldy, x, ldx, weight, \
-                       mean, rstd, dx, part, bias, (int)rows, cols);
-      FP8GMM_NORM_SHAPES(FP8GMM_LAUNCH)
+#define FP8GMM_LAUNCH(LANES, C)                                                                                               \
+  if (shape.lanes == LANES && shape.pieces == C) {                                                                            \
+    auto* kernel = mode == kEdge         ? &layer_norm_backward_kernel<T, P, LANES, C, kEdge>                                 \
+                   : mode == kEdgeStream ? &layer_norm_backward_kernel<T, P, LANES, C, kEdgeStream>                           \
+                                         : &layer_norm_backward_kernel<T, P, LANES, C, LANES == 64 ? kWhole : kShort>;        \
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBackwardThreads / shape.threads() * shape.threads()), 0, s, dy, ldy, x, ldx, \
+                       weight, mean, rstd, dx, part, bias, (int)rows, cols, shape.waves, streaming);                          \
+  } else
+      FP8GMM_LAUNCH(16, 1)
+      FP8GMM_LAUNCH(64, 1)
+      FP8GMM_LAUNCH(64, 2)
+      if constexpr (T == FP8GMM_TYPE_FP32) {
+        FP8GMM_LAUNCH(64, 4) {}
+      }
 #undef FP8GMM_LAUNCH
-      if (shape.threads == 0) {
+      if (shape.lanes == 0) {
         for (int64_t r0 = 0; dx != nullptr && r0 < rows; r0 += kNormSlab) {
           const int size = type_bytes(type);
           hipLaunchKernelGGL((layer_norm_long_dx_kernel<T, P>), dim3((unsigned)std::min<int64_t>(kNormSlab, rows - r0)),

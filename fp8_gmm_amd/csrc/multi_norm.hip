@@ -7,10 +7,11 @@
 // bits, which the memory hides (two conversions and a multiply-add per value, a third of the time that its bytes take): no
 // magnitude that a gradient can have overflows or vanishes, and the order of the sums does not show in 32 bits.
 //
-// The tensors travel as the launch's own arguments, 128 of them at a time, so nothing is uploaded, and a captured launch holds
-// its table.  Every tensor is cut into chunks; a workgroup takes a contiguous range of all chunks of its launch.  The partial
-// sums, one per workgroup, are added up by every workgroup of the scaling for itself, in the same order.  The scaling goes
-// backwards through the launches and chunks, from what the norm has read last and the caches still hold.
+// Every tensor is cut into chunks of 16 KB, and a workgroup takes a contiguous range of all chunks.  The table of the tensors of a
+// short list travels in the launches' arguments; that of a longer one is written to the workspace first, 112 tensors to a launch,
+// by their arguments too - so nothing is uploaded, and a captured call holds its table.  The partial sums, one per workgroup of the
+// norm, are added up by every workgroup of the scaling for itself, in the same order.  The scaling goes backwards, from what the
+// norm has read last and the caches still hold.
 #include <algorithm>
 #include <vector>
 
@@ -19,33 +20,54 @@
 namespace fp8gmm {
 namespace {
 
-constexpr int kTensors = 128;        // of a launch
+constexpr int kTensors = 112;        // of a launch's arguments
 constexpr int kThreads = 256;
 constexpr int kPieces = 4;           // of 16 bytes per thread and chunk
-constexpr int kNormBlocks = 1024;    // workgroups of a launch: four per compute unit
-constexpr int kManyPartials = 4096;  // more than these are added up by a launch of their own
+constexpr int kChunkBytes = kThreads * kPieces * 16;
+constexpr int kRun = 4;              // chunks of a workgroup, and more of very long lists
+constexpr int kNormBlocks = 8192;    // the most workgroups of a launch
+constexpr int kFewPartials = 512;    // partial sums that every workgroup of the scaling adds up for itself
+constexpr int kClipBlocks = 1 << 20; // of the scaling, a chunk to each but for lists of 16 GB and more
+// Gradients are read with the streaming hint where nothing of them would be found in the caches by a second pass, 512 MB on,
+// or where there is none; results are written with it where whoever reads them does not find them there.
+constexpr int64_t kStreamTwice = (int64_t)512 << 20, kStreamOnce = (int64_t)32 << 20, kStreamOut = (int64_t)64 << 20;
 
-struct NormTable {
-  const void* in[kTensors];
-  int64_t count[kTensors];
-  uint32_t begin[kTensors + 1];   // first chunk of every tensor; behind the last one, the launch's chunks
-  int n;
+struct Entry {
+  const void* in;
+  void* out;
+  int64_t count;
+  uint32_t begin;   // first chunk
+  uint16_t type, out_type;
 };
-struct ClipTable {
-  const void* in[kTensors];
-  void* out[kTensors];
-  int64_t count[kTensors];
-  uint32_t begin[kTensors + 1];
-  int n;
+static_assert(sizeof(Entry) == 32, "two to a cache line's half");
+struct Part {
+  Entry e[kTensors];
 };
-static_assert(sizeof(NormTable) <= 4000 && sizeof(ClipTable) <= 4000, "the arguments of a launch");
+static_assert(sizeof(Part) <= 3600, "the arguments of a launch");
 
-template <int TYPE>
-constexpr int chunk_elements() { return kThreads * kPieces * Elements<TYPE>::kVec; }
+// The tensors of a call: in the arguments, or in memory.
+template <bool DIRECT>
+struct Table {
+  const Part& part;
+  const Entry* memory;
+  int n;
+  uint32_t chunks;
+  __device__ __forceinline__ const Entry& operator[](int i) const { return DIRECT ? part.e[i] : memory[i]; }
+  __device__ __forceinline__ uint32_t end(int i) const { return i + 1 < n ? (*this)[i + 1].begin : chunks; }
+  // The tensor that a chunk is of: every thread looks at tensors of its own
+  __device__ __forceinline__ int of(uint32_t chunk) const {
+    __shared__ int found;
+    for (int i = threadIdx.x; i < n; i += kThreads)
+      if ((*this)[i].begin <= chunk && chunk < end(i)) found = i;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(found);
+  }
+};
 
-template <class Table>
-__device__ __forceinline__ int tensor_of(const Table& t, uint32_t chunk) {
-  return upper_slot(t.n, (int)chunk, [&](int i) { return (int)t.begin[i]; });
+__global__ __launch_bounds__(kTensors * 2) void multi_norm_table_kernel(const Part part, int n, Entry* __restrict__ table) {
+  // half an entry a thread
+  if ((int)threadIdx.x < 2 * n)
+    reinterpret_cast<u32x4*>(table)[threadIdx.x] = reinterpret_cast<const u32x4*>(&part)[threadIdx.x];
 }
 
 __device__ __forceinline__ double lanes_sum64(double v) {
@@ -65,114 +87,179 @@ __device__ __forceinline__ double block_sum(double v, double* slots) {
   return sum;
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void multi_norm_kernel(const NormTable t, double* __restrict__ partials) {
+// f(TYPE, elements of a chunk) for a tensor's type
+template <class F>
+__device__ __forceinline__ void with_type(int type, F&& f) {
+  if (type == FP8GMM_TYPE_BF16) f(std::integral_constant<int, FP8GMM_TYPE_BF16>{});
+  else if (type == FP8GMM_TYPE_FP16) f(std::integral_constant<int, FP8GMM_TYPE_FP16>{});
+  else f(std::integral_constant<int, FP8GMM_TYPE_FP32>{});
+}
+
+// The pieces of a thread of the chunk at `p`, of which `n` elements are the tensor's
+template <int TYPE, bool STREAM>
+__device__ __forceinline__ void load_chunk(const typename Elements<TYPE>::bits* p, int n, u32x4 (&raw)[kPieces]) {
   typedef Elements<TYPE> E;
-  typedef typename E::bits bits;
-  constexpr int V = E::kVec, CHUNK = chunk_elements<TYPE>();
+  constexpr int V = E::kVec;
+  if (n == kThreads * kPieces * V) {
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u) raw[u] = E::template load<STREAM>(p + (u * kThreads + threadIdx.x) * V, V);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u) raw[u] = E::load(p + (u * kThreads + threadIdx.x) * V, n - (int)(u * kThreads + threadIdx.x) * V);
+  }
+}
+
+template <bool DIRECT, bool STREAM>
+__global__ __launch_bounds__(kThreads) void multi_norm_kernel(const Part part, const Entry* __restrict__ memory, int n, uint32_t chunks,
+                                                              double* __restrict__ partials) {
   __shared__ double slots[kThreads / 64];
-  const uint32_t chunks = t.begin[t.n];
+  const Table<DIRECT> table = {part, memory, n, chunks};
   const uint32_t lo = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x), hi = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
   double sum[2] = {0., 0.};
-  int i = tensor_of(t, lo);
-  for (uint32_t c = lo; c < hi; ++c) {
-    while (c >= t.begin[i + 1]) ++i;
-    const int64_t first = (int64_t)(c - t.begin[i]) * CHUNK, left = t.count[i] - first;
-    const int n = (int)(left < CHUNK ? left : CHUNK);
-    const bits* const p = static_cast<const bits*>(t.in[i]) + first;
-    u32x4 raw[kPieces];
+  int i = table.of(lo);
+  for (uint32_t c = lo; c < hi; ++i) {
+    const Entry e = table[i];
+    const uint32_t last = min(table.end(i), hi);
+    with_type(e.type, [&](auto type) {
+      typedef Elements<decltype(type)::value> E;
+      constexpr int V = E::kVec, CHUNK = kThreads * kPieces * V;
+      for (; c < last; ++c) {
+        const int64_t first = (int64_t)(c - e.begin) * CHUNK, left = e.count - first;
+        u32x4 raw[kPieces];
+        load_chunk<decltype(type)::value, STREAM>(static_cast<const typename E::bits*>(e.in) + first, (int)(left < CHUNK ? left : CHUNK), raw);
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) {
-      const int at = (u * kThreads + threadIdx.x) * V;
-      raw[u] = E::load(p + at, n - at);
-    }
+        for (int u = 0; u < kPieces; ++u) {
+          float f[V];
+          E::unpack(raw[u], f);
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) {
-      float f[V];
-      E::unpack(raw[u], f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) sum[j & 1] = __builtin_fma((double)f[j], (double)f[j], sum[j & 1]);
-    }
+          for (int j = 0; j < V; ++j) sum[j & 1] = __builtin_fma((double)f[j], (double)f[j], sum[j & 1]);
+        }
+      }
+    });
   }
   const double total = block_sum<kThreads / 64>(sum[0] + sum[1], slots);
   if (threadIdx.x == 0) partials[blockIdx.x] = total;
 }
 
-// norm = sqrt of the sum; `sum` (may be NULL, may be partials): the sum itself
-__global__ __launch_bounds__(1024) void multi_norm_finish_kernel(const double* __restrict__ partials, int n,
-                                                                 float* __restrict__ norm, double* __restrict__ sum) {
-  __shared__ double slots[16];
-  double v = 0.;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += 1024) v += partials[i];
-  v = block_sum<16>(v, slots);
-  if (threadIdx.x != 0) return;
-  if (norm != nullptr) *norm = (float)sqrt(v);
-  if (sum != nullptr) *sum = v;
+// The factor of the scaling: 1 within the bound; a norm that is a NaN stays one, an infinite one makes it 0.
+__device__ __forceinline__ float factor_of(double norm, double max_norm) {
+  const double ratio = max_norm / (norm + 1e-6);
+  return ratio > 1. ? 1.f : (float)ratio;
 }
 
-template <int TYPE, int OUT>
-__global__ __launch_bounds__(kThreads) void multi_clip_kernel(const ClipTable t, const double* __restrict__ partials, int n_partials,
-                                                              double max_norm, float* __restrict__ norm) {
+// The norm, and the factor behind it where a scaling follows.
+__global__ __launch_bounds__(1024) void multi_norm_finish_kernel(const double* __restrict__ partials, int n, double max_norm,
+                                                                 float* __restrict__ norm, float* __restrict__ factor) {
+  __shared__ double slots[16];
+  double v = 0.;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += 1024) v += partials[i];
+  v = sqrt(block_sum<16>(v, slots));
+  if (threadIdx.x != 0) return;
+  *norm = (float)v;
+  if (factor != nullptr) *factor = factor_of(v, max_norm);
+}
+
+// A chunk's pieces times the factor.  fp32 results of a 16-bit type: pieces of four elements, 8 bytes read and 16 written, so
+// that a store instruction writes whole lines (with 8 elements a thread, whose two stores share lines, the streaming hint made
+// 1.9 GB to 3.8 take 2440 us; without it 1544).
+template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT>
+__device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits* p, typename Elements<OUT>::bits* out, int n, float factor) {
   typedef Elements<TYPE> E;
   typedef Elements<OUT> O;
-  typedef typename E::bits bits;
-  constexpr int V = E::kVec, CHUNK = chunk_elements<TYPE>();
-  __shared__ double slots[kThreads / 64];
-  double v = 0.;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n_partials; i += kThreads) v += partials[i];
-  const double total = sqrt(block_sum<kThreads / 64>(v, slots));
-  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
-  const double ratio = max_norm / (total + 1e-6);
-  const float factor = ratio > 1. ? 1.f : (float)ratio;   // a NaN stays one
-  const uint32_t chunks = t.begin[t.n], block = gridDim.x - 1 - blockIdx.x;   // backwards
-  const uint32_t lo = (uint32_t)((uint64_t)chunks * block / gridDim.x), hi = (uint32_t)((uint64_t)chunks * (block + 1) / gridDim.x);
-  if (lo == hi) return;
-  int i = tensor_of(t, hi - 1);
-  for (uint32_t c = hi; c-- > lo;) {
-    while (c < t.begin[i]) --i;
-    if (factor == 1.f && t.in[i] == t.out[i]) {   // gradients within the bound stay as they are, in place
-      if (t.begin[i] <= lo) return;
-      c = t.begin[i];
-      continue;
-    }
-    const int64_t first = (int64_t)(c - t.begin[i]) * CHUNK, left = t.count[i] - first;
-    const int n = (int)(left < CHUNK ? left : CHUNK);
-    const bits* const p = static_cast<const bits*>(t.in[i]) + first;
-    typename O::bits* const out = static_cast<typename O::bits*>(t.out[i]) + first;
+  if constexpr (TYPE == OUT) {
+    constexpr int V = E::kVec;
+    const bool all = n == kThreads * kPieces * V;
     u32x4 raw[kPieces];
+    load_chunk<TYPE, STREAM>(p, n, raw);
 #pragma unroll
     for (int u = 0; u < kPieces; ++u) {
-      const int at = (u * kThreads + threadIdx.x) * V;
-      raw[u] = E::load(p + at, n - at);
-    }
-#pragma unroll
-    for (int u = 0; u < kPieces; ++u) {
-      const int at = (u * kThreads + threadIdx.x) * V;
       float f[V];
       E::unpack(raw[u], f);
 #pragma unroll
       for (int j = 0; j < V; ++j) f[j] *= factor;
-      if constexpr (O::kVec >= V) {   // fp32 gradients stay in fp32
-        O::store(out + at, n - at, O::pack(f));
-      } else {
+      raw[u] = E::pack(f);
+    }
+    if (all) {
 #pragma unroll
-        for (int q = 0; q < V / O::kVec; ++q) {
-          float part[O::kVec];
+      for (int u = 0; u < kPieces; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + threadIdx.x) * V, V, raw[u]);
+    } else {
 #pragma unroll
-          for (int j = 0; j < O::kVec; ++j) part[j] = f[q * O::kVec + j];
-          O::store(out + at + q * O::kVec, n - at - q * O::kVec, O::pack(part));
-        }
+      for (int u = 0; u < kPieces; ++u)
+        O::store(out + (u * kThreads + threadIdx.x) * V, n - (int)(u * kThreads + threadIdx.x) * V, raw[u]);
+    }
+  } else {
+    constexpr int V = 4, COUNT = kPieces * E::kVec / V;
+    typedef uint32_t half_piece __attribute__((ext_vector_type(2), aligned(2)));
+    const auto scaled = [&](u32x2 raw) {
+      float f[E::kVec];
+      E::unpack(u32x4{raw.x, raw.y, 0u, 0u}, f);
+      return u32x4{__float_as_uint(f[0] * factor), __float_as_uint(f[1] * factor), __float_as_uint(f[2] * factor), __float_as_uint(f[3] * factor)};
+    };
+    if (n == kThreads * COUNT * V) {
+      u32x2 raw[COUNT];
+#pragma unroll
+      for (int u = 0; u < COUNT; ++u) {
+        const half_piece* const at = reinterpret_cast<const half_piece*>(p + (u * kThreads + threadIdx.x) * V);
+        raw[u] = STREAM ? __builtin_nontemporal_load(at) : *at;
+      }
+#pragma unroll
+      for (int u = 0; u < COUNT; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + threadIdx.x) * V, V, scaled(raw[u]));
+    } else {
+      for (int at = threadIdx.x * V; at < n; at += kThreads * V) {
+        const u32x4 raw = E::load(p + at, min(n - at, V));
+        O::store(out + at, n - at, scaled(u32x2{raw.x, raw.y}));
       }
     }
   }
 }
 
-uint32_t chunks_of(int64_t count, int type) {
-  const int64_t chunk = (int64_t)kThreads * kPieces * 16 / type_bytes(type);
-  return (uint32_t)((count + chunk - 1) / chunk);
+template <bool DIRECT, bool STREAM, bool STREAM_OUT>
+__global__ __launch_bounds__(kThreads) void multi_clip_kernel(const Part part, const Entry* __restrict__ memory, int n, uint32_t chunks,
+                                                              const double* __restrict__ partials, int n_partials, double max_norm,
+                                                              const float* __restrict__ finished, float* __restrict__ norm) {
+  __shared__ double slots[kThreads / 64];
+  float factor;
+  if (finished != nullptr) {
+    factor = *finished;
+  } else {
+    double v = 0.;
+    for (int i = threadIdx.x; i < n_partials; i += kThreads) v += partials[i];
+    const double total = sqrt(block_sum<kThreads / 64>(v, slots));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
+    factor = factor_of(total, max_norm);
+  }
+  const Table<DIRECT> table = {part, memory, n, chunks};
+  const uint32_t block = gridDim.x - 1 - blockIdx.x;      // backwards
+  const uint32_t lo = (uint32_t)((uint64_t)chunks * block / gridDim.x), hi = (uint32_t)((uint64_t)chunks * (block + 1) / gridDim.x);
+  if (lo == hi) return;
+  int i = table.of(hi - 1);
+  for (uint32_t c = hi; c > lo; --i) {
+    const Entry e = table[i];
+    const uint32_t first = max(e.begin, lo);
+    if (factor == 1.f && e.in == e.out) {   // gradients within the bound stay as they are, in place
+      c = first;
+      continue;
+    }
+    with_type(e.type, [&](auto type) {
+      constexpr int TYPE = decltype(type)::value;
+      typedef Elements<TYPE> E;
+      constexpr int CHUNK = kThreads * kPieces * E::kVec;
+      while (c > first) {
+        --c;
+        const int64_t at = (int64_t)(c - e.begin) * CHUNK, left = e.count - at;
+        const typename E::bits* const p = static_cast<const typename E::bits*>(e.in) + at;
+        const int here = (int)(left < CHUNK ? left : CHUNK);
+        if (TYPE != FP8GMM_TYPE_FP32 && e.out_type == FP8GMM_TYPE_FP32)
+          scale_chunk<TYPE, FP8GMM_TYPE_FP32, STREAM, STREAM_OUT>(p, static_cast<uint32_t*>(e.out) + at, here, factor);
+        else
+          scale_chunk<TYPE, TYPE, STREAM, STREAM_OUT>(p, static_cast<typename E::bits*>(e.out) + at, here, factor);
+      }
+    });
+  }
 }
+
+uint32_t chunks_of(int64_t count, int type) { return (uint32_t)((count * type_bytes(type) + kChunkBytes - 1) / kChunkBytes); }
 
 int check_tensors(const fp8gmm_norm_tensor* tensors, int n, bool out) {
   if (n < 0) return FP8GMM_ERR_BAD_ARGUMENT;
@@ -215,72 +302,54 @@ int check_apart(const fp8gmm_norm_tensor* tensors, int n) {
   return FP8GMM_OK;
 }
 
-struct Part {   // of a list: up to kTensors tensors of one type (of one pair of types)
-  std::vector<int> which;
+// The tensors with elements, as the launches take them.
+struct List {
+  std::vector<Entry> entries;
   uint32_t chunks = 0;
+  int64_t bytes_in = 0, bytes_out = 0;
+  List(const fp8gmm_norm_tensor* tensors, int n) {
+    entries.reserve((size_t)n);
+    for (int i = 0; i < n; ++i) {
+      const fp8gmm_norm_tensor& t = tensors[i];
+      if (t.count == 0) continue;
+      entries.push_back({t.in, t.out, t.count, chunks, (uint16_t)t.type, (uint16_t)t.out_type});
+      chunks += chunks_of(t.count, t.type);
+      bytes_in += t.count * type_bytes(t.type);
+      bytes_out += t.count * type_bytes(t.out_type);
+    }
+  }
+  int n() const { return (int)entries.size(); }
+  bool direct() const { return n() <= kTensors; }
+  int blocks() const { return (int)std::min<uint32_t>(kNormBlocks, (chunks + kRun - 1) / kRun); }
+  Part part(int first) const {
+    Part p = {};
+    std::copy(entries.begin() + first, entries.begin() + std::min(n(), first + kTensors), p.e);
+    return p;
+  }
 };
-std::vector<Part> parts_of(const fp8gmm_norm_tensor* tensors, int n, int type, int out_type) {
-  std::vector<Part> parts;
-  for (int i = 0; i < n; ++i) {
-    const fp8gmm_norm_tensor& t = tensors[i];
-    if (t.count == 0 || t.type != type || (out_type >= 0 && t.out_type != out_type)) continue;
-    const uint32_t chunks = chunks_of(t.count, type);
-    if (parts.empty() || parts.back().which.size() == kTensors) parts.emplace_back();
-    parts.back().which.push_back(i);
-    parts.back().chunks += chunks;
-  }
-  return parts;
+
+// The workspace: the partial sums, the factor, and the table behind them.
+double* partials_of(void* workspace) { return static_cast<double*>(workspace); }
+float* factor_at(void* workspace) { return reinterpret_cast<float*>(partials_of(workspace) + kNormBlocks); }
+Entry* table_of(void* workspace) { return reinterpret_cast<Entry*>(partials_of(workspace) + kNormBlocks + 2); }
+
+// Enqueues the partial sums of a list that is not empty; the list's first tensors, for the scaling.
+Part launch_norm(const List& list, bool stream, void* workspace, hipStream_t s) {
+  if (!list.direct())
+    for (int first = 0; first < list.n(); first += kTensors)
+      hipLaunchKernelGGL(multi_norm_table_kernel, dim3(1), dim3(kTensors * 2), 0, s, list.part(first), std::min(kTensors, list.n() - first),
+                         table_of(workspace) + first);
+  const Part part = list.part(0);
+  auto* kernel = list.direct() ? stream ? &multi_norm_kernel<true, true> : &multi_norm_kernel<true, false>
+                 : stream      ? &multi_norm_kernel<false, true>
+                               : &multi_norm_kernel<false, false>;
+  hipLaunchKernelGGL(kernel, dim3(list.blocks()), dim3(kThreads), 0, s, part, table_of(workspace), list.n(), list.chunks,
+                     partials_of(workspace));
+  return part;
 }
 
-constexpr int kAllTypes[] = {FP8GMM_TYPE_BF16, FP8GMM_TYPE_FP16, FP8GMM_TYPE_FP32};
-
-// Enqueues the partial sums; how many there are.
-int launch_norms(const fp8gmm_norm_tensor* tensors, int n, double* partials, hipStream_t s) {
-  int total = 0;
-  for (const int type : kAllTypes)
-    for (const Part& part : parts_of(tensors, n, type, -1)) {
-      NormTable t;
-      t.n = (int)part.which.size();
-      uint32_t at = 0;
-      for (int i = 0; i < t.n; ++i) {
-        const fp8gmm_norm_tensor& from = tensors[part.which[i]];
-        t.in[i] = from.in;
-        t.count[i] = from.count;
-        t.begin[i] = at;
-        at += chunks_of(from.count, type);
-      }
-      t.begin[t.n] = at;
-      const int blocks = (int)std::min<uint32_t>(kNormBlocks, part.chunks);
-      auto* kernel = type == FP8GMM_TYPE_BF16   ? &multi_norm_kernel<FP8GMM_TYPE_BF16>
-                     : type == FP8GMM_TYPE_FP16 ? &multi_norm_kernel<FP8GMM_TYPE_FP16>
-                                                : &multi_norm_kernel<FP8GMM_TYPE_FP32>;
-      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, s, t, partials + total);
-      total += blocks;
-    }
-  return total;
-}
-
-template <int TYPE, int OUT>
-void launch_clips(const fp8gmm_norm_tensor* tensors, int n, const double* partials, int n_partials, double max_norm, float** norm,
-                  hipStream_t s) {
-  const std::vector<Part> parts = parts_of(tensors, n, TYPE, OUT);
-  for (auto part = parts.rbegin(); part != parts.rend(); ++part) {
-    ClipTable t;
-    t.n = (int)part->which.size();
-    uint32_t at = 0;
-    for (int i = 0; i < t.n; ++i) {
-      const fp8gmm_norm_tensor& from = tensors[part->which[i]];
-      t.in[i] = from.in;
-      t.out[i] = from.out;
-      t.count[i] = from.count;
-      t.begin[i] = at;
-      at += chunks_of(from.count, TYPE);
-    }
-    t.begin[t.n] = at;
-    hipLaunchKernelGGL((multi_clip_kernel<TYPE, OUT>), dim3(std::min<uint32_t>(2 * kNormBlocks, part->chunks)), dim3(kThreads), 0,
-                       s, t, partials, n_partials, max_norm, *norm);
-    *norm = nullptr;   // by the first launch
-  }
+void launch_finish(const List& list, double max_norm, float* norm, float* factor, void* workspace, hipStream_t s) {
+  hipLaunchKernelGGL(multi_norm_finish_kernel, dim3(1), dim3(1024), 0, s, partials_of(workspace), list.blocks(), max_norm, norm, factor);
 }
 
 int check_workspace(int n, void* workspace, size_t bytes) {
@@ -293,9 +362,9 @@ int multi_norm(const fp8gmm_norm_tensor* tensors, int n, float* norm, void* work
   int rc = check_tensors(tensors, n, false);
   if (rc == FP8GMM_OK) rc = norm == nullptr ? FP8GMM_ERR_NULL_POINTER : check_workspace(n, workspace, bytes);
   if (rc != FP8GMM_OK) return rc;
-  double* const partials = static_cast<double*>(workspace);
-  const int total = launch_norms(tensors, n, partials, s);
-  hipLaunchKernelGGL(multi_norm_finish_kernel, dim3(1), dim3(1024), 0, s, partials, total, norm, static_cast<double*>(nullptr));
+  const List list(tensors, n);
+  if (list.n() > 0) launch_norm(list, list.bytes_in > kStreamOnce, workspace, s);
+  launch_finish(list, 0., norm, nullptr, workspace, s);
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
@@ -306,20 +375,23 @@ int multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float*
   if (rc == FP8GMM_OK && !(max_norm >= 0.)) rc = FP8GMM_ERR_BAD_ARGUMENT;
   if (rc == FP8GMM_OK) rc = check_apart(tensors, n);
   if (rc != FP8GMM_OK) return rc;
-  double* partials = static_cast<double*>(workspace);
-  int total = launch_norms(tensors, n, partials, s);
-  if (total == 0 || total > kManyPartials) {
-    double* const sum = partials + total;
-    hipLaunchKernelGGL(multi_norm_finish_kernel, dim3(1), dim3(1024), 0, s, partials, total, norm, sum);
-    partials = sum;
-    total = 1;
-    norm = nullptr;   // written
+  const List list(tensors, n);
+  if (list.n() == 0) {
+    launch_finish(list, max_norm, norm, nullptr, workspace, s);
+  } else {
+    const bool in = list.bytes_in > kStreamTwice, out = list.bytes_out > kStreamOut;
+    const Part part = launch_norm(list, in, workspace, s);
+    float* const finished = list.blocks() > kFewPartials ? factor_at(workspace) : nullptr;
+    if (finished != nullptr) launch_finish(list, max_norm, norm, finished, workspace, s);
+    auto* kernel = list.direct() ? in ? out ? &multi_clip_kernel<true, true, true> : &multi_clip_kernel<true, true, false>
+                                   : out ? &multi_clip_kernel<true, false, true>
+                                         : &multi_clip_kernel<true, false, false>
+                   : in ? out ? &multi_clip_kernel<false, true, true> : &multi_clip_kernel<false, true, false>
+                   : out ? &multi_clip_kernel<false, false, true>
+                         : &multi_clip_kernel<false, false, false>;
+    hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks)), dim3(kThreads), 0, s, part, table_of(workspace), list.n(), list.chunks,
+                       partials_of(workspace), list.blocks(), max_norm, finished, norm);
   }
-  launch_clips<FP8GMM_TYPE_FP32, FP8GMM_TYPE_FP32>(tensors, n, partials, total, max_norm, &norm, s);
-  launch_clips<FP8GMM_TYPE_FP16, FP8GMM_TYPE_FP32>(tensors, n, partials, total, max_norm, &norm, s);
-  launch_clips<FP8GMM_TYPE_FP16, FP8GMM_TYPE_FP16>(tensors, n, partials, total, max_norm, &norm, s);
-  launch_clips<FP8GMM_TYPE_BF16, FP8GMM_TYPE_FP32>(tensors, n, partials, total, max_norm, &norm, s);
-  launch_clips<FP8GMM_TYPE_BF16, FP8GMM_TYPE_BF16>(tensors, n, partials, total, max_norm, &norm, s);
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
@@ -340,8 +412,7 @@ extern "C" {
 
 size_t fp8gmm_multi_norm_workspace_bytes(int n) {
   using namespace fp8gmm;
-  // a launch per kTensors tensors and one more that is not full for every type, and the sum
-  return n < 0 ? 0 : ((size_t)(n / kTensors + 4) * kNormBlocks + 2) * sizeof(double);
+  return n < 0 ? 0 : (kNormBlocks + 2) * sizeof(double) + (n > kTensors ? (size_t)n * sizeof(Entry) : 0);
 }
 
 int fp8gmm_multi_norm(const fp8gmm_norm_tensor* tensors, int n, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
