@@ -86,6 +86,8 @@ def check_norm(x, w, b, dy, eps=1e-5, what=""):
 
 SHAPES = [(1, 1), (3, 7), (5, 64), (40, 127), (17, 129), (33, 512), (7, 1000), (129, 1411), (65, 2048), (1531, 1024), (9, 4097),
           (300, 4096), (3, 8191), (5, 16384), (700, 768), (5000, 24)]
+# columns on both sides of where a row takes another number of threads, of pieces per thread, or another kernel
+SHAPES += [(37, c + d) for c in (4, 8, 64, 128, 256, 512, 768, 1024, 1536, 2048, 6144, 8192, 16384) for d in (-1, 0, 1, 8)]
 
 
 @pytest.mark.parametrize("rows, cols", SHAPES)
@@ -224,7 +226,7 @@ def check_embedding(dev, ids, table, cols, t, scale=1.0, padding=None, seed=0, i
 
 @pytest.mark.parametrize("tokens, table, cols", [(1, 1, 1), (1, 5, 64), (7, 300, 33), (64, 4001, 256), (513, 17, 100), (1000, 4001, 250),
                                                  (1024, 1024, 512), (4096, 100, 1030), (5000, 70000, 24), (16384, 2000, 64),
-                                                 (16385, 2000, 64), (20000, 3, 40), (3000, 262143, 8), (3000, 262144, 8), (40000, 300000, 16)])
+                                                 (16385, 2000, 64), (20000, 3, 40), (3000, 262143, 8), (3000, 262144, 8), (40000, 300000, 16), (131072, 600, 8), (131073, 60000, 9)])
 @pytest.mark.parametrize("t", ["bf16", "fp16", "fp32"])
 def test_embedding_against_64_bits(dev, tokens, table, cols, t):
     """The sort in one workgroup and in many, of one to three digits; runs that end inside, at and beyond a chunk's end."""
@@ -240,7 +242,7 @@ def test_embedding_of_one_id_and_of_runs(dev, tokens, cols):
     check_embedding(dev, one, 9, cols, "fp32", 0.5)
     check_embedding(dev, one, 9, cols, "bf16", padding=5)
     check_embedding(dev, torch.arange(tokens).flip(0), tokens, cols, "bf16", 2.0)
-    for run in (8, 31, 32, 33, 64):
+    for run in (8, 31, 32, 33, 64, 65, 127, 129, 300):
         check_embedding(dev, torch.arange(tokens) // run, tokens, cols, "fp16", seed=run)
 
 
