@@ -502,7 +502,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int check_embedding(int64_t n, int64_t table, int cols, int type) {
   if (!known_type(type)) return FP8GMM_ERR_BAD_FORMAT;
   // keys below 2^31, offsets of a row in 32 bits, a grid of fewer than 2^32 threads
-  if (n < 0 || n > (1 << 28) || table < 0 || table >= INT32_MAX || cols < 0 || cols > (1 << 24)) return FP8GMM_ERR_BAD_SHAPE;
+  if (n < 0 || n > (1 << 28) || table < 0 || table >= INT32_MAX || cols < 0 || cols > (1 << 23)) return FP8GMM_ERR_BAD_SHAPE;
   return FP8GMM_OK;
 }
 

@@ -209,8 +209,8 @@ Tensor embedding(const Tensor& ids_, const Tensor& weight, double scale, std::op
     TORCH_CHECK(weight.device() == ids_.device(), "fp8_gmm_amd: all tensors of one call must live on the same device");
     TORCH_CHECK(std::isfinite((float)scale), "fp8_gmm_amd: scale must be a finite number");
     const int64_t table = weight.size(0), cols = weight.size(1), tokens = ids_.numel();
-    TORCH_CHECK(cols <= 1 << 24 && table < INT32_MAX && tokens <= 1 << 28,
-                "fp8_gmm_amd: at most 2^24 columns, 2^31 - 2 rows and 2^28 ids are supported");
+    TORCH_CHECK(cols <= 1 << 23 && table < INT32_MAX && tokens <= 1 << 28,
+                "fp8_gmm_amd: at most 2^23 columns, 2^31 - 2 rows and 2^28 ids are supported");
     int64_t padding = -1;
     if (padding_idx.has_value()) {
       TORCH_CHECK(*padding_idx >= -table && *padding_idx < table, "fp8_gmm_amd: padding_idx must be a row of the table");

@@ -275,9 +275,8 @@ __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
       nx[c] = x.template load<true>(at[c]);
       ny[c] = y.template load<true>(at[c]);
     }
-    const int64_t live = row < rows ? row : rows - 1;
-    nm = mean_in[live];
-    nr = rstd_in[live];
+    nm = row < rows ? mean_in[row] : 0.f;
+    nr = row < rows ? rstd_in[row] : 0.f;
   };
   const int64_t stride = (int64_t)gridDim.x * ROWS;
   int64_t row = (int64_t)blockIdx.x * ROWS + group;
@@ -290,7 +289,8 @@ __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
       x[c] = nx[c];
       y[c] = ny[c];
     }
-    const float rstd = nr, shift = -nm * nr;
+    const float mean = nm, rstd = nr;
+    const float last_rstd = skip < V ? rstd : 0.f;   // a piece behind the end has z = 0, whatever the mean times rstd is
     if (first + stride < rows) load(row + stride);
     float s1 = 0.f, s2 = 0.f;
     if (!is_edge(MODE) || row < rows) {
@@ -303,7 +303,8 @@ __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         if (is_edge(MODE) && c == C - 1 && i < skip) fy[i] = 0.f;   // elsewhere they are zeros
-        const float z = __builtin_fmaf(fx[i], rstd, shift), g = fy[i] * fw[i];
+        const bool mine = MODE != kShort || i < cols;
+        const float z = mine ? (fx[i] - mean) * (c < C - 1 ? rstd : last_rstd) : 0.f, g = fy[i] * fw[i];
         s1 += g;
         s2 = __builtin_fmaf(g, z, s2);
         dw[c][i] = __builtin_fmaf(fy[i], z, dw[c][i]);
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
       pw[c].get(fw);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float z = __builtin_fmaf(fx[i], rstd, shift);
+        const float z = (fx[i] - mean) * rstd;
         fx[i] = __builtin_fmaf(fy[i], fw[i] * rstd, __builtin_fmaf(z, c2, c1));
       }
       dx.store(at[c], E::pack(fx), stream);
@@ -556,36 +557,33 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
   const int threads = shape.lanes == 0 ? 0 : std::max(shape.threads(), kForwardThreads / shape.threads() * shape.threads());
   const bool streaming = streams(rows, cols, type);
   const int mode = mode_of(cols, type, whole(x, ldx, cols, type) && whole(y, cols, cols, type), streaming);
-  for (int64_t r0 = 0; r0 < rows; r0 += kNormSlab) {
-    const int n = (int)std::min<int64_t>(kNormSlab, rows - r0), size = type_bytes(type);
-    const void* const xs = static_cast<const char*>(x) + r0 * ldx * size;
-    void* const ys = static_cast<char*>(y) + r0 * cols * size;
-    float* const ms = mean != nullptr ? mean + r0 : nullptr;
-    float* const rs = rstd != nullptr ? rstd + r0 : nullptr;
-    with_types(type, param_type, [&](auto tc, auto pc) {
-      constexpr int T = decltype(tc)::value, P = decltype(pc)::value; 
+  with_types(type, param_type, [&](auto tc, auto pc) {
+    constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
 #define FP8GMM_LAUNCH(LANES, C, MOST)                                                                                         \
   if (shape.lanes == LANES && shape.pieces == C && threads <= MOST) {                                                         \
     auto* kernel = mode == kEdge         ? &layer_norm_kernel<T, P, LANES, C, kEdge, MOST>                                    \
                    : mode == kEdgeStream ? &layer_norm_kernel<T, P, LANES, C, kEdgeStream, MOST>                              \
                                          : &layer_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : kShort, MOST>;           \
-    hipLaunchKernelGGL(kernel, dim3(std::min(ceil_div(n, threads / shape.threads()), kForwardAll / threads)), dim3(threads), 0, s, \
-                       xs, ldx, weight, bias, ys, ms, rs, n, cols, eps, shape.waves, streaming);                              \
+    hipLaunchKernelGGL(kernel, dim3(std::min(ceil_div(rows, threads / shape.threads()), kForwardAll / threads)), dim3(threads), \
+                       0, s, x, ldx, weight, bias, y, mean, rstd, (int)rows, cols, eps, shape.waves, streaming);              \
   } else
-      FP8GMM_LAUNCH(16, 1, 256)
-      FP8GMM_LAUNCH(64, 1, 256)
-      FP8GMM_LAUNCH(64, 2, 512)
-      FP8GMM_LAUNCH(64, 3, 512)
-      FP8GMM_LAUNCH(64, 4, 512)
-      if constexpr (T == FP8GMM_TYPE_FP32) {
-        FP8GMM_LAUNCH(64, 4, 1024) {}
-      }
+    FP8GMM_LAUNCH(16, 1, 256)
+    FP8GMM_LAUNCH(64, 1, 256)
+    FP8GMM_LAUNCH(64, 2, 512)
+    FP8GMM_LAUNCH(64, 3, 512)
+    FP8GMM_LAUNCH(64, 4, 512)
+    if constexpr (T == FP8GMM_TYPE_FP32) {
+      FP8GMM_LAUNCH(64, 4, 1024) {}
+    }
 #undef FP8GMM_LAUNCH
-      if (shape.lanes == 0)
-        hipLaunchKernelGGL((layer_norm_long_kernel<T, P>), dim3(n), dim3(kNormLongThreads), 0, s, xs, ldx, weight, bias, ys, ms,
-                           rs, cols, eps);
-    });
-  }
+    for (int64_t r0 = 0; shape.lanes == 0 && r0 < rows; r0 += kNormSlab) {
+      const int size = type_bytes(type);
+      hipLaunchKernelGGL((layer_norm_long_kernel<T, P>), dim3((unsigned)std::min<int64_t>(kNormSlab, rows - r0)),
+                         dim3(kNormLongThreads), 0, s, static_cast<const char*>(x) + r0 * ldx * size, ldx, weight, bias,
+                         static_cast<char*>(y) + r0 * cols * size, mean != nullptr ? mean + r0 : nullptr,
+                         rstd != nullptr ? rstd + r0 : nullptr, cols, eps);
+    }
+  });
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 

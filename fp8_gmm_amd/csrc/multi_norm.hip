@@ -217,7 +217,7 @@ __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits*
 template <bool DIRECT, bool STREAM, bool STREAM_OUT>
 __global__ __launch_bounds__(kThreads) void multi_clip_kernel(const Part part, const Entry* __restrict__ memory, int n, uint32_t chunks,
                                                               const double* __restrict__ partials, int n_partials, double max_norm,
-                                                              const float* __restrict__ finished, float* __restrict__ norm) {
+                                                              const float* __restrict__ finished, bool in_place, float* __restrict__ norm) {
   __shared__ double slots[kThreads / 64];
   float factor;
   if (finished != nullptr) {
@@ -229,6 +229,7 @@ __global__ __launch_bounds__(kThreads) void multi_clip_kernel(const Part part, c
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
     factor = factor_of(total, max_norm);
   }
+  if (in_place && factor == 1.f) return;   // all of them
   const Table<DIRECT> table = {part, memory, n, chunks};
   const uint32_t block = gridDim.x - 1 - blockIdx.x;      // backwards
   const uint32_t lo = (uint32_t)((uint64_t)chunks * block / gridDim.x), hi = (uint32_t)((uint64_t)chunks * (block + 1) / gridDim.x);
@@ -307,6 +308,7 @@ struct List {
   std::vector<Entry> entries;
   uint32_t chunks = 0;
   int64_t bytes_in = 0, bytes_out = 0;
+  bool in_place = true;   // all of them
   List(const fp8gmm_norm_tensor* tensors, int n) {
     entries.reserve((size_t)n);
     for (int i = 0; i < n; ++i) {
@@ -316,6 +318,7 @@ struct List {
       chunks += chunks_of(t.count, t.type);
       bytes_in += t.count * type_bytes(t.type);
       bytes_out += t.count * type_bytes(t.out_type);
+      in_place = in_place && t.in == t.out;
     }
   }
   int n() const { return (int)entries.size(); }
@@ -390,7 +393,7 @@ int multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float*
                    : out ? &multi_clip_kernel<false, false, true>
                          : &multi_clip_kernel<false, false, false>;
     hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks)), dim3(kThreads), 0, s, part, table_of(workspace), list.n(), list.chunks,
-                       partials_of(workspace), list.blocks(), max_norm, finished, norm);
+                       partials_of(workspace), list.blocks(), max_norm, finished, list.in_place, norm);
   }
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }

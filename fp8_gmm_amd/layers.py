@@ -28,7 +28,8 @@ def layer_norm(x, weight, bias=None, eps=1e-5):
     """Layer norm of ``x [..., columns]`` over its last dimension.  ``weight`` and ``bias`` (may be None) ``[columns]``, of the
     type of ``x`` or float32; the result has the type of ``x`` and is contiguous.  Rows may be strided as long as the columns
     are neighbours; others are copied first.  Differentiable in all three; a row whose variance is zero has ``rstd = 1 /
-    sqrt(eps)``, and the rows of an empty ``x`` leave gradients of zeros."""
+    sqrt(eps)``, one whose sum or squares pass float32's range is no number or its bias, and the rows of an empty ``x`` leave
+    gradients of zeros."""
     _check_unwrapped("layer_norm")
     return native.layer_norm(x, weight, bias, eps)
 

@@ -686,7 +686,7 @@ int fp8gmm_moe_scatter_backward(const void* x, const void* grad_out, const int32
  * fp8gmm_layer_norm: y[r, :] = (x[r, :] - m) / sqrt(mean((x[r, :] - m)^2) + eps) * weight + bias, m the mean of x[r, :].
  * x: [rows, cols] of `type` with a pitch of ldx >= cols elements; y: the same without a pitch; weight and bias (may be NULL):
  * [cols] of `param_type`, which is `type` or fp32.  mean, rstd: fp32 [rows] for the backward pass, or both NULL.
- * 1 <= cols <= 2^30, rows < 2^31.
+ * 1 <= cols <= 2^30, rows < 2^31.  y (and dx below) lies apart from what is read.
  */
 int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void* bias, void* y, float* mean, float* rstd,
                       int64_t rows, int cols, float eps, int type, int param_type, void* stream);
@@ -702,7 +702,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
                                int param_type, void* workspace, size_t workspace_bytes, void* stream);
 /*
  * fp8gmm_embedding: y[t, :] = scale * weight[ids[t], :] for t in [0, n), a row of zeros where ids[t] is outside [0, table).
- * ids: int64 (ids64 != 0) or int32; weight: [table, cols] of `type`; n <= 2^28, table < 2^31 - 1, cols <= 2^24.
+ * ids: int64 (ids64 != 0) or int32; weight: [table, cols] of `type`; n <= 2^28, table < 2^31 - 1, cols <= 2^23.
  * fp8gmm_embedding_backward: dweight[v, :] = scale * sum of dy[t, :] over the t with ids[t] == v, in the order of t, the whole
  * table, zeros where there are none; `padding` (-1: none) is an id whose tokens are left out.  dweight and workspace
  * (fp8gmm_embedding_workspace_bytes) on 16 bytes.  The same bits from call to call.

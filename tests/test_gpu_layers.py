@@ -170,6 +170,27 @@ def test_layer_norm_keeps_what_is_no_number_in_its_row(dev):
     assert torch.isnan(pkg.layer_norm(flat, w, b, 0.0)).all()
 
 
+@pytest.mark.parametrize("t, cols", [("fp32", 128), ("fp32", 4), ("fp32", 2), ("bf16", 64), ("bf16", 256), ("bf16", 4)])
+def test_layer_norm_of_equal_values_next_to_infinity(dev, t, cols):
+    """The mean of rows of one value is that value, and z is 0 although the mean times rstd is infinite: threads without columns
+    and rows that are none leave nothing behind."""
+    x = torch.full((5, cols), 2.0 ** 120, dtype=TYPES[t], device=dev)
+    g = gen(cols)
+    w, b = (torch.randn(cols, generator=g).to(TYPES[t]).to(dev) for _ in range(2))
+    dy = torch.randn(5, cols, generator=g).to(TYPES[t]).to(dev)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    y = pkg.layer_norm(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    if cols * 2.0 ** 120 > torch.finfo(torch.float32).max:   # 256 * 2^120 = 2^128: the sum of a row is kept in fp32
+        assert y.isnan().all() and dx.isnan().all()
+        return
+    assert torch.equal(y, b.expand(5, -1)) and not dw.any()
+    h = dy.double() * w.double()
+    want = (h - h.mean(1, keepdim=True)) / math.sqrt(1e-5)
+    assert_within(dx, want, half_step(dx.dtype) * want.abs() + 70 * U * (h.abs() + h.abs().mean(1, keepdim=True)) / math.sqrt(1e-5), "dx")
+    assert_within(db, dy.double().sum(0), half_step(db.dtype) * dy.double().sum(0).abs() + 8 * U * dy.double().abs().sum(0), "db")
+
+
 def test_layer_norm_past_32_bits(dev):
     """More rows than one launch takes, and more elements than 32 bits count."""
     rows, cols = (1 << 21) + 37, 1040

@@ -82,7 +82,7 @@ def test_embedding_status():
 
     for call in (lookup, backward):
         for bad, status in ((dict(t=3), FORMAT), (dict(n=-1), SHAPE), (dict(n=(1 << 28) + 1), SHAPE), (dict(table=-1), SHAPE),
-                            (dict(table=(1 << 31) - 1), SHAPE), (dict(cols=-1), SHAPE), (dict(cols=(1 << 24) + 1), SHAPE), (dict(ids=None), NULL)):
+                            (dict(table=(1 << 31) - 1), SHAPE), (dict(cols=-1), SHAPE), (dict(cols=(1 << 23) + 1), SHAPE), (dict(ids=None), NULL)):
             assert call(**bad) == status, bad
     assert lookup(w=None) == NULL and lookup(y=None) == NULL and lookup(n=0, ids=None, w=None, y=None) == OK and lookup(cols=0) == OK
     assert backward(dw=None) == NULL and backward(dy=None) == NULL and backward(work=None) == NULL
