@@ -21,6 +21,7 @@ constexpr int kBackwardBlocks = 256;     // leaves one partial sum of the parame
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormSlab = 1 << 21;   // rows of a launch with a workgroup to a row: a grid has fewer than 2^32 threads
 
+constexpr int kBackwardAlone = 4;        // so many turns of one workgroup take less than a second launch for the sums of several
 constexpr int kNormWaves = 16;           // the most wavefronts that share a row
 constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, where a row needs no more
 constexpr int kForwardAll = 256 * 2048;  // of its launch: what the compute units hold
@@ -242,12 +243,13 @@ __global__ __launch_bounds__(kNormLongThreads) void layer_norm_long_kernel(
 }
 
 // The backward pass in the same way, with the sums of dy z and dy for the columns of its threads.  `part`: [workgroup][2][cols], the
-// second without a bias left out; NULL where the parameters take no gradients.  dx may be NULL.
+// second without a bias left out; NULL where the parameters take no gradients.  dx may be NULL.  A single workgroup writes the
+// gradients themselves.
 template <int TYPE, int PTYPE, int LANES, int C, int MODE>
 __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
     const void* __restrict__ dy_, int64_t ldy, const void* __restrict__ x_, int64_t ldx, const void* __restrict__ w,
     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, void* __restrict__ dx_, float* __restrict__ part,
-    int bias, int rows, int cols, int waves, bool stream) {
+    void* __restrict__ dweight, void* __restrict__ dbias, int rows, int cols, int waves, bool stream) {
   typedef Elements<TYPE> E;
   constexpr int V = E::kVec;
   __shared__ float slots[2][2][kNormWaves][kNormWaves];
@@ -290,27 +292,29 @@ __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
       y[c] = ny[c];
     }
     const float mean = nm, rstd = nr;
-    const float last_rstd = skip < V ? rstd : 0.f;   // a piece behind the end has z = 0, whatever the mean times rstd is
     if (first + stride < rows) load(row + stride);
     float s1 = 0.f, s2 = 0.f;
     if (!is_edge(MODE) || row < rows) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float fx[V], fy[V], fw[V];
-      E::unpack(x[c], fx);
-      E::unpack(y[c], fy);
-      pw[c].get(fw);
+      for (int c = 0; c < C; ++c) {
+        float fx[V], fy[V], fw[V];
+        E::unpack(x[c], fx);
+        E::unpack(y[c], fy);
+        pw[c].get(fw);
+        float u1 = 0.f, u2 = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (is_edge(MODE) && c == C - 1 && i < skip) fy[i] = 0.f;   // elsewhere they are zeros
-        const bool mine = MODE != kShort || i < cols;
-        const float z = mine ? (fx[i] - mean) * (c < C - 1 ? rstd : last_rstd) : 0.f, g = fy[i] * fw[i];
-        s1 += g;
-        s2 = __builtin_fmaf(g, z, s2);
-        dw[c][i] = __builtin_fmaf(fy[i], z, dw[c][i]);
-        db[c][i] += fy[i];
+        for (int i = 0; i < V; ++i) {
+          if (is_edge(MODE) && c == C - 1 && i < skip) fy[i] = 0.f;   // elsewhere they are zeros
+          const float z = MODE != kShort || i < cols ? (fx[i] - mean) * rstd : 0.f, g = fy[i] * fw[i];
+          u1 += g;
+          u2 = __builtin_fmaf(g, z, u2);
+          dw[c][i] = __builtin_fmaf(fy[i], z, dw[c][i]);
+          db[c][i] += fy[i];
+        }
+        // nothing of a piece behind the end, whose zeros have a z of minus the mean times rstd, be that infinite
+        s1 += c < C - 1 || skip < V ? u1 : 0.f;
+        s2 += c < C - 1 || skip < V ? u2 : 0.f;
       }
-    }
     }
     if (dx_ == nullptr) continue;
     s1 = lanes_sum<LANES>(s1);
@@ -344,11 +348,17 @@ __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
   if (part == nullptr) return;
   // the workgroup's rows together, in their order: THREADS * V columns at a time
   float* const out = part + (int64_t)blockIdx.x * 2 * cols;
+  const auto write = [&](int which, int64_t col, float sum) {
+    typedef Elements<PTYPE> P;
+    void* const to = which == 0 ? dweight : dbias;
+    if (gridDim.x > 1) out[(int64_t)which * cols + col] = sum;
+    else if (to != nullptr) static_cast<typename P::bits*>(to)[col] = P::pack1(sum);
+  };
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      if (which == 1 && !bias) continue;
+      if (which == 1 && dbias == nullptr) continue;
       if (ROWS > 1) {
         __syncthreads();
 #pragma unroll
@@ -359,12 +369,12 @@ __global__ __launch_bounds__(kBackwardThreads) void layer_norm_backward_kernel(
           for (int r = 0; r < ROWS; ++r) sum += sums[r * THREADS * V + k];
           const int piece = (c * THREADS + k / V) * V;
           if (own<MODE>(k % V, piece_skip<MODE, V>(piece, cols), cols))
-            out[(int64_t)which * cols + piece_begin<MODE, V>(piece, cols) + k % V] = sum;
+            write(which, piece_begin<MODE, V>(piece, cols) + k % V, sum);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          if (c < C - 1 || own<MODE>(i, skip, cols)) out[(int64_t)which * cols + at[c] + i] = which == 0 ? dw[c][i] : db[c][i];
+          if (c < C - 1 || own<MODE>(i, skip, cols)) write(which, at[c] + i, which == 0 ? dw[c][i] : db[c][i]);
       }
     }
 }
@@ -518,7 +528,8 @@ int mode_of(int cols, int type, bool aligned, bool stream_edges) {
 int backward_blocks(int rows, int cols, int type) {
   const Shape s = backward_shape(cols, type);
   if (s.lanes == 0) return std::min(rows, 64);
-  return std::min(ceil_div(rows, kBackwardThreads / s.threads()), kBackwardBlocks);
+  const int blocks = ceil_div(rows, kBackwardThreads / s.threads());
+  return blocks <= kBackwardAlone ? std::min(blocks, 1) : std::min(blocks, kBackwardBlocks);
 }
 
 // calls f(TYPE, PTYPE) with the two as integral constants
@@ -625,7 +636,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
                    : mode == kEdgeStream ? &layer_norm_backward_kernel<T, P, LANES, C, kEdgeStream>                           \
                                          : &layer_norm_backward_kernel<T, P, LANES, C, LANES == 64 ? kWhole : kShort>;        \
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBackwardThreads / shape.threads() * shape.threads()), 0, s, dy, ldy, x, ldx, \
-                       weight, mean, rstd, dx, part, bias, (int)rows, cols, shape.waves, streaming);                          \
+                       weight, mean, rstd, dx, part, dweight, dbias, (int)rows, cols, shape.waves, streaming);                          \
   } else
       FP8GMM_LAUNCH(16, 1)
       FP8GMM_LAUNCH(64, 1)
@@ -647,7 +658,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
                              0, s, dy, ldy, x, ldx, mean, rstd, part, bias, (int)rows, cols);
       }
     }
-    if (params)
+    if (params && (blocks != 1 || shape.lanes == 0))
       hipLaunchKernelGGL((layer_norm_params_kernel<P>), dim3(ceil_div(cols, 64), dbias != nullptr ? 2 : 1), dim3(1024), 0, s,
                          part, blocks, cols, dweight, dbias);
   });

@@ -97,15 +97,32 @@ __device__ __forceinline__ void with_type(int type, F&& f) {
 
 // The pieces of a thread of the chunk at `p`, of which `n` elements are the tensor's
 template <int TYPE, bool STREAM>
-__device__ __forceinline__ void load_chunk(const typename Elements<TYPE>::bits* p, int n, u32x4 (&raw)[kPieces]) {
+__device__ __forceinline__ void load_chunk(const typename Elements<TYPE>::bits* p, int n, int t, u32x4 (&raw)[kPieces]) {
   typedef Elements<TYPE> E;
   constexpr int V = E::kVec;
   if (n == kThreads * kPieces * V) {
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) raw[u] = E::template load<STREAM>(p + (u * kThreads + threadIdx.x) * V, V);
+    for (int u = 0; u < kPieces; ++u) raw[u] = E::template load<STREAM>(p + (u * kThreads + t) * V, V);
   } else {
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) raw[u] = E::load(p + (u * kThreads + threadIdx.x) * V, n - (int)(u * kThreads + threadIdx.x) * V);
+    for (int u = 0; u < kPieces; ++u) raw[u] = E::load(p + (u * kThreads + t) * V, n - (u * kThreads + t) * V);
+  }
+}
+
+// The squares of thread t's share of chunk c, added to `sum`
+template <int TYPE, bool STREAM>
+__device__ __forceinline__ void add_squares(const Entry& e, uint32_t c, int t, double (&sum)[2]) {
+  typedef Elements<TYPE> E;
+  constexpr int V = E::kVec, CHUNK = kThreads * kPieces * V;
+  const int64_t first = (int64_t)(c - e.begin) * CHUNK, left = e.count - first;
+  u32x4 raw[kPieces];
+  load_chunk<TYPE, STREAM>(static_cast<const typename E::bits*>(e.in) + first, (int)(left < CHUNK ? left : CHUNK), t, raw);
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) {
+    float f[V];
+    E::unpack(raw[u], f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j & 1] = __builtin_fma((double)f[j], (double)f[j], sum[j & 1]);
   }
 }
 
@@ -121,20 +138,7 @@ __global__ __launch_bounds__(kThreads) void multi_norm_kernel(const Part part, c
     const Entry e = table[i];
     const uint32_t last = min(table.end(i), hi);
     with_type(e.type, [&](auto type) {
-      typedef Elements<decltype(type)::value> E;
-      constexpr int V = E::kVec, CHUNK = kThreads * kPieces * V;
-      for (; c < last; ++c) {
-        const int64_t first = (int64_t)(c - e.begin) * CHUNK, left = e.count - first;
-        u32x4 raw[kPieces];
-        load_chunk<decltype(type)::value, STREAM>(static_cast<const typename E::bits*>(e.in) + first, (int)(left < CHUNK ? left : CHUNK), raw);
-#pragma unroll
-        for (int u = 0; u < kPieces; ++u) {
-          float f[V];
-          E::unpack(raw[u], f);
-#pragma unroll
-          for (int j = 0; j < V; ++j) sum[j & 1] = __builtin_fma((double)f[j], (double)f[j], sum[j & 1]);
-        }
-      }
+      for (; c < last; ++c) add_squares<decltype(type)::value, STREAM>(e, c, threadIdx.x, sum);
     });
   }
   const double total = block_sum<kThreads / 64>(sum[0] + sum[1], slots);
@@ -164,14 +168,14 @@ __global__ __launch_bounds__(1024) void multi_norm_finish_kernel(const double* _
 // that a store instruction writes whole lines (with 8 elements a thread, whose two stores share lines, the streaming hint made
 // 1.9 GB to 3.8 take 2440 us; without it 1544).
 template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT>
-__device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits* p, typename Elements<OUT>::bits* out, int n, float factor) {
+__device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits* p, typename Elements<OUT>::bits* out, int n, int t, float factor) {
   typedef Elements<TYPE> E;
   typedef Elements<OUT> O;
   if constexpr (TYPE == OUT) {
     constexpr int V = E::kVec;
     const bool all = n == kThreads * kPieces * V;
     u32x4 raw[kPieces];
-    load_chunk<TYPE, STREAM>(p, n, raw);
+    load_chunk<TYPE, STREAM>(p, n, t, raw);
 #pragma unroll
     for (int u = 0; u < kPieces; ++u) {
       float f[V];
@@ -182,11 +186,11 @@ __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits*
     }
     if (all) {
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + threadIdx.x) * V, V, raw[u]);
+      for (int u = 0; u < kPieces; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + t) * V, V, raw[u]);
     } else {
 #pragma unroll
       for (int u = 0; u < kPieces; ++u)
-        O::store(out + (u * kThreads + threadIdx.x) * V, n - (int)(u * kThreads + threadIdx.x) * V, raw[u]);
+        O::store(out + (u * kThreads + t) * V, n - (u * kThreads + t) * V, raw[u]);
     }
   } else {
     constexpr int V = 4, COUNT = kPieces * E::kVec / V;
@@ -200,18 +204,32 @@ __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits*
       u32x2 raw[COUNT];
 #pragma unroll
       for (int u = 0; u < COUNT; ++u) {
-        const half_piece* const at = reinterpret_cast<const half_piece*>(p + (u * kThreads + threadIdx.x) * V);
+        const half_piece* const at = reinterpret_cast<const half_piece*>(p + (u * kThreads + t) * V);
         raw[u] = STREAM ? __builtin_nontemporal_load(at) : *at;
       }
 #pragma unroll
-      for (int u = 0; u < COUNT; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + threadIdx.x) * V, V, scaled(raw[u]));
+      for (int u = 0; u < COUNT; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + t) * V, V, scaled(raw[u]));
     } else {
-      for (int at = threadIdx.x * V; at < n; at += kThreads * V) {
+      for (int at = t * V; at < n; at += kThreads * V) {
         const u32x4 raw = E::load(p + at, min(n - at, V));
         O::store(out + at, n - at, scaled(u32x2{raw.x, raw.y}));
       }
     }
   }
+}
+
+// Thread t's share of chunk c of a tensor, scaled
+template <int TYPE, bool STREAM, bool STREAM_OUT>
+__device__ __forceinline__ void scale(const Entry& e, uint32_t c, int t, float factor) {
+  typedef Elements<TYPE> E;
+  constexpr int CHUNK = kThreads * kPieces * E::kVec;
+  const int64_t at = (int64_t)(c - e.begin) * CHUNK, left = e.count - at;
+  const typename E::bits* const p = static_cast<const typename E::bits*>(e.in) + at;
+  const int here = (int)(left < CHUNK ? left : CHUNK);
+  if (TYPE != FP8GMM_TYPE_FP32 && e.out_type == FP8GMM_TYPE_FP32)
+    scale_chunk<TYPE, FP8GMM_TYPE_FP32, STREAM, STREAM_OUT>(p, static_cast<uint32_t*>(e.out) + at, here, t, factor);
+  else
+    scale_chunk<TYPE, TYPE, STREAM, STREAM_OUT>(p, static_cast<typename E::bits*>(e.out) + at, here, t, factor);
 }
 
 template <bool DIRECT, bool STREAM, bool STREAM_OUT>
@@ -243,18 +261,96 @@ __global__ __launch_bounds__(kThreads) void multi_clip_kernel(const Part part, c
       continue;
     }
     with_type(e.type, [&](auto type) {
-      constexpr int TYPE = decltype(type)::value;
-      typedef Elements<TYPE> E;
-      constexpr int CHUNK = kThreads * kPieces * E::kVec;
-      while (c > first) {
-        --c;
-        const int64_t at = (int64_t)(c - e.begin) * CHUNK, left = e.count - at;
-        const typename E::bits* const p = static_cast<const typename E::bits*>(e.in) + at;
-        const int here = (int)(left < CHUNK ? left : CHUNK);
-        if (TYPE != FP8GMM_TYPE_FP32 && e.out_type == FP8GMM_TYPE_FP32)
-          scale_chunk<TYPE, FP8GMM_TYPE_FP32, STREAM, STREAM_OUT>(p, static_cast<uint32_t*>(e.out) + at, here, factor);
-        else
-          scale_chunk<TYPE, TYPE, STREAM, STREAM_OUT>(p, static_cast<typename E::bits*>(e.out) + at, here, factor);
+      while (c > first) scale<decltype(type)::value, STREAM, STREAM_OUT>(e, --c, threadIdx.x, factor);
+    });
+  }
+}
+
+// A short list in one launch of one workgroup, and one pass over memory: cut into units of 4 KB, up to four of them to a wavefront,
+// which stay in its registers while the workgroup shares the norm.  Bound by the latency of a launch and of one access: 24 tensors
+// of 1300 fp32 take 8.3 us from call to call, by two launches over chunks 12.6; 64 units 8.4, and 13.
+constexpr int kUnitWaves = 16, kUnitsEach = 4, kUnits = kUnitWaves * kUnitsEach;
+struct Unit {
+  const void* in;
+  void* out;
+  int32_t count;   // elements, at most kPieces 16-byte pieces of every lane
+  uint16_t type, out_type;
+};
+struct Units {
+  Unit u[kUnits];
+};
+static_assert(sizeof(Units) <= 1600, "the arguments of a launch");
+
+__global__ __launch_bounds__(kUnitWaves * 64) void multi_small_kernel(const Units units, int n, bool clip, double max_norm,
+                                                                      float* __restrict__ norm) {
+  __shared__ double slots[kUnitWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  u32x4 raw[kUnitsEach][kPieces];
+#pragma unroll
+  for (int r = 0; r < kUnitsEach; ++r) {
+    const int k = wave + r * kUnitWaves;
+    if (k >= n) continue;
+    const Unit& u = units.u[k];
+    if (u.type == FP8GMM_TYPE_FP32) {
+      typedef Elements<FP8GMM_TYPE_FP32> E;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int at = (i * 64 + lane) * E::kVec;
+        raw[r][i] = E::load(static_cast<const uint32_t*>(u.in) + at, u.count - at);
+      }
+    } else {   // the bits of either 16-bit type
+      typedef Elements<FP8GMM_TYPE_BF16> E;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int at = (i * 64 + lane) * E::kVec;
+        raw[r][i] = E::load(static_cast<const uint16_t*>(u.in) + at, u.count - at);
+      }
+    }
+  }
+  double sum = 0.;
+#pragma unroll
+  for (int r = 0; r < kUnitsEach; ++r) {
+    const int k = wave + r * kUnitWaves;
+    if (k >= n) continue;
+    with_type(units.u[k].type, [&](auto type) {
+      typedef Elements<decltype(type)::value> E;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        float f[E::kVec];
+        E::unpack(raw[r][i], f);
+#pragma unroll
+        for (int j = 0; j < E::kVec; ++j) sum = __builtin_fma((double)f[j], (double)f[j], sum);
+      }
+    });
+  }
+  const double total = sqrt(block_sum<kUnitWaves>(sum, slots));
+  if (threadIdx.x == 0) *norm = (float)total;
+  if (!clip) return;
+  const float factor = factor_of(total, max_norm);
+#pragma unroll
+  for (int r = 0; r < kUnitsEach; ++r) {
+    const int k = wave + r * kUnitWaves;
+    if (k >= n) continue;
+    const Unit& u = units.u[k];
+    if (factor == 1.f && u.in == u.out) continue;   // gradients within the bound stay as they are, in place
+    with_type(u.type, [&](auto type) {
+      typedef Elements<decltype(type)::value> E;
+      typedef Elements<FP8GMM_TYPE_FP32> F;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int at = (i * 64 + lane) * E::kVec;
+        float f[E::kVec];
+        E::unpack(raw[r][i], f);
+#pragma unroll
+        for (int j = 0; j < E::kVec; ++j) f[j] *= factor;
+        if (u.out_type == u.type) {
+          E::store(static_cast<typename E::bits*>(u.out) + at, u.count - at, E::pack(f));
+        } else {
+#pragma unroll
+          for (int q = 0; q < E::kVec; q += 4)
+            F::store(static_cast<uint32_t*>(u.out) + at + q, u.count - at - q,
+                     u32x4{__float_as_uint(f[q]), __float_as_uint(f[q + 1]), __float_as_uint(f[q + 2]), __float_as_uint(f[q + 3])});
+        }
       }
     });
   }
@@ -294,7 +390,8 @@ int check_apart(const fp8gmm_norm_tensor* tensors, int n) {
     ranges.push_back({out, out + (uintptr_t)t.count * type_bytes(t.out_type), i, 1});
     if (in != out || t.type != t.out_type) ranges.push_back({in, in + (uintptr_t)t.count * type_bytes(t.type), i, 0});
   }
-  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+  if (!std::is_sorted(ranges.begin(), ranges.end(), before)) std::sort(ranges.begin(), ranges.end(), before);   // buckets are
   uintptr_t written = 0, read = 0;   // ends of what the ranges so far write and read
   for (const Range& r : ranges) {
     if (r.begin < written || (r.writes && r.begin < read)) return FP8GMM_ERR_BAD_ARGUMENT;
@@ -323,6 +420,18 @@ struct List {
   }
   int n() const { return (int)entries.size(); }
   bool direct() const { return n() <= kTensors; }
+  // The list in units, where there are no more than one workgroup takes: their number, or -1.
+  int small(Units* units) const {
+    int k = 0;
+    for (const Entry& e : entries) {
+      const int size = type_bytes(e.type), most = 64 * kPieces * 16 / size;
+      if (e.count > (int64_t)(kUnits - k) * most) return -1;
+      for (int64_t at = 0; at < e.count; at += most)
+        units->u[k++] = {static_cast<const char*>(e.in) + at * size, static_cast<char*>(e.out) + at * type_bytes(e.out_type),
+                         (int32_t)std::min<int64_t>(most, e.count - at), e.type, e.out_type};
+    }
+    return k;
+  }
   int blocks() const { return (int)std::min<uint32_t>(kNormBlocks, (chunks + kRun - 1) / kRun); }
   Part part(int first) const {
     Part p = {};
@@ -355,6 +464,14 @@ void launch_finish(const List& list, double max_norm, float* norm, float* factor
   hipLaunchKernelGGL(multi_norm_finish_kernel, dim3(1), dim3(1024), 0, s, partials_of(workspace), list.blocks(), max_norm, norm, factor);
 }
 
+// Whether the list was a short one, which is enqueued then
+bool launch_small(const List& list, bool clip, double max_norm, float* norm, hipStream_t s) {
+  Units units = {};
+  const int n = list.small(&units);
+  if (n >= 0) hipLaunchKernelGGL(multi_small_kernel, dim3(1), dim3(kUnitWaves * 64), 0, s, units, n, clip, max_norm, norm);
+  return n >= 0;
+}
+
 int check_workspace(int n, void* workspace, size_t bytes) {
   if (workspace == nullptr) return FP8GMM_ERR_NULL_POINTER;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return FP8GMM_ERR_ALIGNMENT;
@@ -366,8 +483,10 @@ int multi_norm(const fp8gmm_norm_tensor* tensors, int n, float* norm, void* work
   if (rc == FP8GMM_OK) rc = norm == nullptr ? FP8GMM_ERR_NULL_POINTER : check_workspace(n, workspace, bytes);
   if (rc != FP8GMM_OK) return rc;
   const List list(tensors, n);
-  if (list.n() > 0) launch_norm(list, list.bytes_in > kStreamOnce, workspace, s);
-  launch_finish(list, 0., norm, nullptr, workspace, s);
+  if (!launch_small(list, false, 0., norm, s)) {
+    launch_norm(list, list.bytes_in > kStreamOnce, workspace, s);
+    launch_finish(list, 0., norm, nullptr, workspace, s);
+  }
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
@@ -379,22 +498,19 @@ int multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float*
   if (rc == FP8GMM_OK) rc = check_apart(tensors, n);
   if (rc != FP8GMM_OK) return rc;
   const List list(tensors, n);
-  if (list.n() == 0) {
-    launch_finish(list, max_norm, norm, nullptr, workspace, s);
-  } else {
-    const bool in = list.bytes_in > kStreamTwice, out = list.bytes_out > kStreamOut;
-    const Part part = launch_norm(list, in, workspace, s);
-    float* const finished = list.blocks() > kFewPartials ? factor_at(workspace) : nullptr;
-    if (finished != nullptr) launch_finish(list, max_norm, norm, finished, workspace, s);
-    auto* kernel = list.direct() ? in ? out ? &multi_clip_kernel<true, true, true> : &multi_clip_kernel<true, true, false>
-                                   : out ? &multi_clip_kernel<true, false, true>
-                                         : &multi_clip_kernel<true, false, false>
-                   : in ? out ? &multi_clip_kernel<false, true, true> : &multi_clip_kernel<false, true, false>
-                   : out ? &multi_clip_kernel<false, false, true>
-                         : &multi_clip_kernel<false, false, false>;
-    hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks)), dim3(kThreads), 0, s, part, table_of(workspace), list.n(), list.chunks,
-                       partials_of(workspace), list.blocks(), max_norm, finished, list.in_place, norm);
-  }
+  if (launch_small(list, true, max_norm, norm, s)) return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
+  const bool in = list.bytes_in > kStreamTwice, out = list.bytes_out > kStreamOut;
+  const Part part = launch_norm(list, in, workspace, s);
+  float* const finished = list.blocks() > kFewPartials ? factor_at(workspace) : nullptr;
+  if (finished != nullptr) launch_finish(list, max_norm, norm, finished, workspace, s);
+  auto* kernel = list.direct() ? in ? out ? &multi_clip_kernel<true, true, true> : &multi_clip_kernel<true, true, false>
+                                 : out ? &multi_clip_kernel<true, false, true>
+                                       : &multi_clip_kernel<true, false, false>
+                 : in ? out ? &multi_clip_kernel<false, true, true> : &multi_clip_kernel<false, true, false>
+                 : out ? &multi_clip_kernel<false, false, true>
+                       : &multi_clip_kernel<false, false, false>;
+  hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks)), dim3(kThreads), 0, s, part, table_of(workspace), list.n(), list.chunks,
+                     partials_of(workspace), list.blocks(), max_norm, finished, list.in_place, norm);
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
@@ -402,9 +518,9 @@ int multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float*
 template <class F>
 int without_exceptions(F&& f) noexcept {
   try {
-    return f();
+  return f();
   } catch (...) {
-    return FP8GMM_ERR_BAD_ARGUMENT;
+  return FP8GMM_ERR_BAD_ARGUMENT;
   }
 }
 
@@ -420,13 +536,13 @@ size_t fp8gmm_multi_norm_workspace_bytes(int n) {
 
 int fp8gmm_multi_norm(const fp8gmm_norm_tensor* tensors, int n, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   return fp8gmm::without_exceptions(
-      [&] { return fp8gmm::multi_norm(tensors, n, norm, workspace, workspace_bytes, static_cast<hipStream_t>(stream)); });
+    [&] { return fp8gmm::multi_norm(tensors, n, norm, workspace, workspace_bytes, static_cast<hipStream_t>(stream)); });
 }
 
 int fp8gmm_multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float* norm, void* workspace,
-                      size_t workspace_bytes, void* stream) {
+                    size_t workspace_bytes, void* stream) {
   return fp8gmm::without_exceptions([&] {
-    return fp8gmm::multi_clip(tensors, n, max_norm, norm, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+  return fp8gmm::multi_clip(tensors, n, max_norm, norm, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
   });
 }
 
