@@ -186,7 +186,8 @@ struct EmbeddingBackward : public Node {
       const int type = type_of(dy, "gradient");
       result[0] = at::empty({table, cols}, dy.options());
       const size_t bytes = fp8gmm_embedding_workspace_bytes(tokens, table, (int)cols, type);
-      const Tensor work = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
+      Tensor work;   // short batches need none
+      if (bytes > 0) work = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
       timed("embedding_backward", (dy.numel() + result[0].numel()) * (int64_t)dy.element_size(), [&] {
         check(fp8gmm_embedding_backward(ptr<void>(list), id_type == at::kLong, tokens, ptr<void>(dy), ptr<void>(result[0]), table,
                                         (int)cols, (float)scale, padding, type, ptr<void>(work), bytes, current_stream(grad.device())));

@@ -77,7 +77,7 @@ def test_embedding_status():
     def lookup(ids=P, ids64=1, n=4, w=P, table=10, cols=8, scale=1.0, t=0, y=P):
         return L.fp8gmm_embedding(ids, ids64, n, w, table, cols, scale, t, y, None)
 
-    def backward(ids=P, ids64=1, n=4, dy=P, dw=P, table=10, cols=8, scale=1.0, padding=-1, t=0, work=P, size=1 << 30):
+    def backward(ids=P, ids64=1, n=4000, dy=P, dw=P, table=10, cols=8, scale=1.0, padding=-1, t=0, work=P, size=1 << 30):
         return L.fp8gmm_embedding_backward(ids, ids64, n, dy, dw, table, cols, scale, padding, t, work, size, None)
 
     for call in (lookup, backward):
@@ -88,8 +88,8 @@ def test_embedding_status():
     assert backward(dw=None) == NULL and backward(dy=None) == NULL and backward(work=None) == NULL
     assert backward(dw=P + 8) == ALIGN and backward(work=P + 4) == ALIGN
     assert backward(table=0) == OK and backward(cols=0) == OK
-    need = L.fp8gmm_embedding_workspace_bytes(4, 10, 8, 0)
-    assert need > 0 and backward(size=need - 1) == WORKSPACE
+    need = L.fp8gmm_embedding_workspace_bytes(4000, 10, 8, 0)
+    assert L.fp8gmm_embedding_workspace_bytes(4, 10, 8, 0) == 0 and need > 0 and backward(size=need - 1) == WORKSPACE
     assert L.fp8gmm_embedding_workspace_bytes(0, 10, 8, 0) == 0 and L.fp8gmm_embedding_workspace_bytes(4, 0, 8, 0) == 0
 
 
