@@ -290,30 +290,57 @@ Tensor multi_norm(const std::vector<Tensor>& tensors) {
   return norm;
 }
 
-// The addresses from a tensor's first element to behind its last one
-std::pair<uintptr_t, uintptr_t> extent(const Tensor& t) {
-  int64_t last = 0;
-  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-  const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data_ptr());
-  return {begin, begin + (uintptr_t)(last + 1) * t.element_size()};
+// The order of the elements in memory, which strides of a dimension of size 1 say nothing of
+bool same_order(const Tensor& a, const Tensor& b) {
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+bool pass_as_they_are(const Tensor& in, const Tensor& out) { return dense(in) && dense(out) && same_order(in, out); }
+
+// Where a tensor lies, in bytes: from its first element to behind its last one, and the rows in that where it consists of rows of
+// one pitch (0: of none, or of one).
+struct Place {
+  uintptr_t begin, end;
+  uintptr_t width, pitch;
+};
+Place place_of(const Tensor& t) {
+  int64_t last = 0, width = 1, pitch = 0, span = 0;
+  bool rows = true;
+  for (int64_t d = t.dim() - 1; d >= 0; --d) {
+    const int64_t size = t.size(d), stride = t.stride(d);
+    if (size == 1) continue;
+    last += (size - 1) * stride;
+    if (pitch == 0 && stride == width) width *= size;
+    else if (pitch == 0 || stride == span) span = stride * size, pitch = pitch == 0 ? stride : pitch;
+    else rows = false;
+  }
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data_ptr()), size = t.element_size();
+  return {begin, begin + (uintptr_t)(last + 1) * size, (uintptr_t)width * size, rows ? (uintptr_t)pitch * size : 0};
+}
+// Whether they lie apart: by their ends, or as slices of the columns of one buffer.  What cannot be told apart so counts as shared.
+bool apart(const Place& a, const Place& b) {
+  if (a.end <= b.begin || b.end <= a.begin) return true;
+  if (a.begin > b.begin) return apart(b, a);
+  const uintptr_t from = a.pitch != 0 && a.pitch == b.pitch ? (b.begin - a.begin) % a.pitch : 0;
+  return from >= a.width && from + b.width <= a.pitch;
 }
 
-// A copy stands in for a result with gaps, so the library does not see where that result lies.
-void check_gaps(const std::vector<Tensor>& tensors, const std::vector<Tensor>& outs) {
+// A copy stands in for a tensor or its result where their elements do not pass as they are, so the library does not see where
+// those lie.
+void check_copied(const std::vector<Tensor>& tensors, const std::vector<Tensor>& outs) {
   for (size_t i = 0; i < outs.size(); ++i) {
-    if (outs[i].numel() == 0 || dense(outs[i])) continue;
-    const auto a = extent(outs[i]);
+    const Tensor &in = tensors[i], &out = outs[i];
+    if (out.numel() == 0 || pass_as_they_are(in, out)) continue;
+    const Place read = place_of(in), written = place_of(out);
+    const bool in_place = in.data_ptr() == out.data_ptr() && in.scalar_type() == out.scalar_type() && same_order(in, out);
+    bool shared = !in_place && !apart(read, written);
     for (size_t j = 0; j < outs.size(); ++j) {
-      for (const Tensor* other : {&tensors[j], &outs[j]}) {
-        if (i == j && (other == &outs[j] || other->is_same(outs[i]) ||
-                       (other->data_ptr() == outs[i].data_ptr() && other->strides() == outs[i].strides() &&
-                        other->scalar_type() == outs[i].scalar_type())))
-          continue;
-        if (other->numel() == 0) continue;
-        const auto b = extent(*other);
-        TORCH_CHECK(a.second <= b.first || b.second <= a.first, "fp8_gmm_amd: a result of multi_clip overlaps another tensor of the call");
-      }
+      if (j == i || outs[j].numel() == 0) continue;
+      const Place other = place_of(outs[j]);
+      shared = shared || !apart(written, other) || !apart(read, other) || !apart(written, place_of(tensors[j]));
     }
+    TORCH_CHECK(!shared, "fp8_gmm_amd: a result of multi_clip overlaps another tensor of the call");
   }
 }
 
@@ -324,16 +351,14 @@ Tensor multi_clip(const std::vector<Tensor>& tensors, const std::vector<Tensor>&
   check_list(outs, "multi_clip");
   TORCH_CHECK(outs[0].device() == tensors[0].device(), "fp8_gmm_amd: all tensors of one call must live on the same device");
   TORCH_CHECK(max_norm >= 0, "fp8_gmm_amd: max_norm must be a number, not negative");
-  bool gaps = false;
   for (size_t i = 0; i < tensors.size(); ++i) {
     TORCH_CHECK(outs[i].sizes() == tensors[i].sizes() &&
                     (outs[i].scalar_type() == tensors[i].scalar_type() || outs[i].scalar_type() == at::kFloat),
                 "fp8_gmm_amd: results of multi_clip have their tensors' shapes, and their types or float32");
     TORCH_CHECK(!(at::GradMode::is_enabled() && outs[i].requires_grad()), "fp8_gmm_amd: a result of multi_clip requires a gradient");
     at::assert_no_internal_overlap(outs[i]);
-    gaps = gaps || !dense(outs[i]);
   }
-  if (gaps) check_gaps(tensors, outs);
+  check_copied(tensors, outs);
   at::AutoGradMode no_grad(false);
   const at::Device device = tensors[0].device();
   const c10::OptionalDeviceGuard guard(device);
@@ -342,7 +367,7 @@ Tensor multi_clip(const std::vector<Tensor>& tensors, const std::vector<Tensor>&
   std::vector<std::pair<Tensor, Tensor>> copies;   // results that are copied to where they belong
   for (size_t i = 0; i < tensors.size(); ++i) {
     Tensor in = tensors[i], out = outs[i];
-    if (!dense(in) || !dense(out) || in.strides() != out.strides()) {   // element by element, in one order
+    if (!pass_as_they_are(in, out)) {   // element by element, in one order
       in = in.contiguous();
       kept.push_back(in);
       if (!out.is_contiguous()) {

@@ -230,16 +230,42 @@ def test_clip_grad_norm(dev):
         pkg.clip_grad_norm_(params, 1.0)
 
 
+@pytest.mark.parametrize("slices", [lambda g: (g[:, :37], g[:, 37:100]), lambda g: (g[:, ::2], g[:, 1::2]), lambda g: (g[0::2], g[1::2], g[:0]),
+                                    lambda g: (g.view(5, 10, 10, 10)[:, :, :3], g.view(5, 10, 10, 10)[:, :, 3:]), lambda g: (g[7:8, 3:], g[7, :3])],
+                         ids=["columns", "every other column", "every other row", "inner", "a row"])
+def test_slices_of_one_buffer_are_clipped_in_place(dev, slices):
+    g = torch.Generator(device=dev).manual_seed(11)
+    buffer = torch.randn(50, 100, generator=g, device=dev)
+    parts, before = slices(buffer), buffer.clone()
+    copies = [p.clone() for p in slices(before)]
+    norm = norm_of(copies)
+    got = backend.multi_clip(parts, parts, 0.5 * norm)
+    assert abs(got.item() - norm) <= 1.01 * U * norm
+    check_scaled(parts, copies, 0.5 * norm / (norm + 1e-6))
+    assert sum(p.numel() for p in parts) == (buffer != before).sum().item()   # (half of no value is the value)
+
+
+def test_strides_of_a_single_element_say_nothing(dev):
+    flat = torch.ones(5, device=dev)
+    norm = backend.multi_clip([flat.as_strided((1, 5), (7, 1))], [flat.as_strided((1, 5), (1, 1))], 1.0)
+    assert abs(norm.item() - math.sqrt(5)) <= 1.01 * U * math.sqrt(5) and abs(flat[0].item() - 1 / math.sqrt(5)) < 1e-6
+
+
 def test_refusals(dev):
     a, b = torch.ones(16, device=dev), torch.ones(16, device=dev)
     flat = torch.ones(40, device=dev)
     grid = torch.ones(6, 10, device=dev)
+    wide = torch.ones(1, 4, 4, device=dev).expand(2, 4, 4)
+    square = wide[1]
     leaf = torch.ones(16, device=dev, requires_grad=True)
     for ins, outs, what in (([a], [], "a result for every"), ([], [], "at least one"), ([a, b], [a, a], "overlaps"), ([a, b], [b, a], "overlaps"),
                             ([flat[:20], a], [flat[5:25], a], "overlaps"), ([flat[:20], flat[30:]], [b.new_empty(20), flat[10:20]], "overlaps"),
                             ([a], [a.half()], "shapes"), ([a], [torch.ones(4, 4, device=dev)], "shapes"), ([a.double()], [a], "bfloat16, float16 or float32"),
                             ([a], [a.cpu()], "GPU tensors"), ([a.cpu()], [a.cpu()], "GPU tensors"), ([a], [leaf], "requires a gradient"),
-                            ([grid[:, ::2], grid[:, 1::2]], [grid[:, ::2], grid[:, 1::2]], "overlaps"),
+                            ([grid[:, :6], grid[:, 5:]], [grid[:, :6], grid[:, 5:]], "overlaps"),
+                            ([grid[:4, :4]], [grid[:4, :4].t()], "overlaps"), ([grid[:4, :4], a], [grid[2:, 2:6], b], "overlaps"),
+                            ([square.t(), a], [square, b], "overlaps"), ([a.view(4, 4).t(), b], [square, a], "overlaps"),
+                            ([square, square], [square.new_empty(4, 4).t(), wide[0]], "overlaps"),
                             ([a.to_sparse()], [a], "dense")):
         with pytest.raises(RuntimeError, match=what):
             backend.multi_clip(ins, outs, 1.0)
