@@ -33,7 +33,7 @@ class _RoutedModule(torch.nn.Module):
         self.top_k = top_k
         self.sort_end_bit = max(int(np.ceil(np.log2(n_experts))), 1)
         self.gating_network = torch.nn.Linear(n_embd, n_experts, bias=False).to(dtype).to(device)
-        self.layer_norm = LayerNorm(n_embd, dtype=dtype, device=device) if layer_norm else None
+        self.row_norm = LayerNorm(n_embd, dtype=dtype, device=device) if layer_norm else None
         self._counts_host = None    # page-locked landing place of the per-expert counts, and the event of its copy
         self._counts_ready = None
 
@@ -86,8 +86,8 @@ class _RoutedModule(torch.nn.Module):
 
     def forward(self, input):
         input = input.view(-1, input.size(-1))
-        if self.layer_norm is not None:
-            input = self.layer_norm(input)
+        if (norm := getattr(self, "row_norm", None)) is not None:   # (modules pickled ahead of the option have none)
+            input = norm(input)
         # Another compute, of a subclass or set on the module, is called as ever: on the rows themselves, which it may change in
         # place where nothing else needs them, and without the inverse.
         own = getattr(self.compute, "__func__", None) is _RoutedModule.compute

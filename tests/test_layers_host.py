@@ -28,8 +28,8 @@ def test_modules_hold_their_parameters():
     assert table.weight.shape == (10, 4) and not table.weight[9].any() and table.weight[8].any() and "scale=2.0" in repr(table)
     plain = moe.Fp8MlpModule(32, 64, 2, 1, device="cpu")
     normed = moe.Fp8LinearModule(32, 64, 2, 1, device="cpu", layer_norm=True)
-    assert plain.layer_norm is None and not any("layer_norm" in k for k in plain.state_dict())
-    assert {"layer_norm.weight", "layer_norm.bias"} <= set(normed.state_dict())
+    assert plain.row_norm is None and not any("norm" in k for k in plain.state_dict())
+    assert {"row_norm.weight", "row_norm.bias"} <= set(normed.state_dict())
 
 
 def test_clipping_without_gradients():
