@@ -5,9 +5,19 @@
 //   g = dy w, dx = r (g - mean(g) - z mean(g z)), dw = sum over rows of dy z, db = sum over rows of dy
 //
 // Bound by memory: x and y pass once, and in the backward pass x, dy and dx.  A row stays in the registers of the threads
-// that share it, so the squares are taken around the mean that is already known (no cancellation where a row lies far off
-// zero) and nothing is read twice.  The statistics are kept in fp32 for the backward pass, m and r of every row; every
-// sum is taken in fp32, and a result is rounded once.
+// that share it, so nothing is read twice, and the squares are taken around a mean that is already known (no cancellation where
+// a row lies far off zero).  The statistics are kept in fp32 for the backward pass, m and r of every row; every sum is taken in
+// fp32, and a result is rounded once.
+//
+// From call to call, with buffers that the caches do not hold, in us and TB/s of what has to pass:
+//                          forward        backward
+//   1 x 4096, bf16         8.0            8.4            one or two launches
+//   1024 x 4096, bf16      7.9            17             out of the caches
+//   16384 x 4096, bf16     43.7   6.1     73.4   5.5
+//   16384 x 4093, bf16     44     6.1     77     5.2     rows that begin at any element
+//   65536 x 2048, fp32     192    5.6     264    6.1
+//   8192 x 16384, bf16     94     5.7     164    4.9     long rows, read twice, the second time from the cache
+// A large copy reaches 5.3 here.
 #include <algorithm>
 #include <type_traits>
 
@@ -21,7 +31,9 @@ constexpr int kBackwardBlocks = 256;     // leaves one partial sum of the parame
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormSlab = 1 << 21;   // rows of a launch with a workgroup to a row: a grid has fewer than 2^32 threads
 
-constexpr int kBackwardAlone = 4;        // so many turns of one workgroup take less than a second launch for the sums of several
+// So many turns of one workgroup take less than a second launch for the sums of several: 32 x 1024, bf16, 2 turns: 8.6 us, by two
+// workgroups 10.9; 64 x 1024, 4 turns: 12.0 and 11.0; 16 x 4096, 4 turns: 14.5 and 11.3.
+constexpr int kBackwardAlone = 2;
 constexpr int kNormWaves = 16;           // the most wavefronts that share a row
 constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, where a row needs no more
 constexpr int kForwardAll = 256 * 2048;  // of its launch: what the compute units hold
@@ -502,15 +514,19 @@ Shape widest(int cols, int type) {
   const int w = ceil_div(pieces_of(cols, type), 64 * 4);
   return type == FP8GMM_TYPE_FP32 && w <= kNormWaves ? Shape{64, w, 4} : Shape{0, 0, 0};
 }
-// Forward, 4 pieces to a thread: few barriers and many loads under way.
+// Forward, 4 pieces to a thread: few barriers and many loads under way (16384 x 4096, bf16: 43.5 us, with 2 pieces 45.6; 65536 x
+// 2048, fp32: 194 and 206; 16384 x 1536, bf16: 21.6 and 24.6).
 Shape forward_shape(int cols, int type) {
   const Shape s = shape_of(pieces_of(cols, type), 4, 8);
   return s.lanes != 0 ? s : widest(cols, type);
 }
-// Backward, 2: the sums of the parameters' gradients take registers as well.
-Shape backward_shape(int cols, int type) {
+// Backward, 2: the sums of the parameters' gradients take registers as well.  Of fp32 rows of whole pieces 1, where that fills the
+// workgroup (65536 x 2048: 263 us, with 2 pieces 272; 32768 x 4096: 265 and 281; but 32768 x 3000, in 12 wavefronts, 224 and 210,
+// and 60001 x 2047, with edges, 281 and 264; 16384 x 4096, bf16: 75 and 73).
+Shape backward_shape(int cols, int type, bool aligned) {
   const int pieces = pieces_of(cols, type);
-  if (pieces > 128 && pieces <= 192) return {64, 3, 1};   // not 2 x 2, of which these leave a quarter idle or more
+  const Shape one = shape_of(pieces, 1, kNormWaves);
+  if (type == FP8GMM_TYPE_FP32 && aligned && one.lanes == 64 && kBackwardThreads % one.threads() == 0) return one;
   const Shape s = shape_of(pieces, 2, kNormWaves);
   return s.lanes != 0 ? s : widest(cols, type);
 }
@@ -519,14 +535,16 @@ bool whole(const void* p, int64_t pitch, int cols, int type) {
   const int pieces = 16 / type_bytes(type);
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch % pieces == 0 && cols % pieces == 0;
 }
-// Whether a result is written with the streaming hint: one that outgrows the cache is not found there by whoever reads it.
+// Whether a result is written with the streaming hint: one that outgrows the cache is not found there by whoever reads it.  With it
+// and without: 16384 x 4096, bf16, forward 43.7 and 50.9 us, backward 73.4 and 71.5; 65536 x 2048, fp32, 194 and 197, 279 and 305;
+// 24576 x 2048, bf16, 37.0 and 38.6, 55.9 and 58.4.
 bool streams(int64_t rows, int cols, int type) { return rows * cols * type_bytes(type) > (int64_t)64 << 20; }
 int mode_of(int cols, int type, bool aligned, bool stream_edges) {
   return cols < 16 / type_bytes(type) ? kShort : aligned ? kWhole : stream_edges ? kEdgeStream : kEdge;
 }
-// Workgroups of a backward pass: partial sums that its parameters' gradients have.
-int backward_blocks(int rows, int cols, int type) {
-  const Shape s = backward_shape(cols, type);
+// Workgroups of a backward pass: partial sums that its parameters' gradients have.  Of aligned rows no fewer than of others.
+int backward_blocks(int rows, int cols, int type, bool aligned) {
+  const Shape s = backward_shape(cols, type, aligned);
   if (s.lanes == 0) return std::min(rows, 64);
   const int blocks = ceil_div(rows, kBackwardThreads / s.threads());
   return blocks <= kBackwardAlone ? std::min(blocks, 1) : std::min(blocks, kBackwardBlocks);
@@ -601,7 +619,7 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
 size_t fp8gmm_layer_norm_workspace_bytes(int64_t rows, int cols, int type) {
   using namespace fp8gmm;
   if (check_norm(rows, cols, cols, type, type) != FP8GMM_OK) return 0;
-  return (size_t)backward_blocks((int)rows, cols, type) * 2 * cols * sizeof(float);
+  return (size_t)backward_blocks((int)rows, cols, type, true) * 2 * cols * sizeof(float);
 }
 
 int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* weight, const float* mean,
@@ -621,14 +639,14 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
   if (!params && (dx == nullptr || rows == 0)) return FP8GMM_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   float* const part = params ? static_cast<float*>(workspace) : nullptr;
-  const int blocks = backward_blocks((int)rows, cols, type), bias = dbias != nullptr;
-  const Shape shape = backward_shape(cols, type);
+  const bool aligned = whole(x, ldx, cols, type) && whole(dy, ldy, cols, type) && (dx == nullptr || whole(dx, cols, cols, type));
+  const int blocks = backward_blocks((int)rows, cols, type, aligned), bias = dbias != nullptr;
+  const Shape shape = backward_shape(cols, type, aligned);
   const bool streaming = streams(rows, cols, type);
   // of a 16-bit type, edges are written without the hint (16384 x 4093, bf16: 76 us, with it 80; 60001 x 2047, fp32: 286 and 267)
-  const int mode = mode_of(cols, type, whole(x, ldx, cols, type) && whole(dy, ldy, cols, type) && (dx == nullptr || whole(dx, cols, cols, type)),
-                           streaming && type == FP8GMM_TYPE_FP32);
+  const int mode = mode_of(cols, type, aligned, streaming && type == FP8GMM_TYPE_FP32);
   with_types(type, param_type, [&](auto tc, auto pc) {
-    constexpr int T = decltype(tc)::value, P = decltype(pc)::value; 
+    constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
     if (rows > 0) {
 #define FP8GMM_LAUNCH(LANES, C)                                                                                               \
   if (shape.lanes == LANES && shape.pieces == C) {                                                                            \
@@ -636,7 +654,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
                    : mode == kEdgeStream ? &layer_norm_backward_kernel<T, P, LANES, C, kEdgeStream>                           \
                                          : &layer_norm_backward_kernel<T, P, LANES, C, LANES == 64 ? kWhole : kShort>;        \
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBackwardThreads / shape.threads() * shape.threads()), 0, s, dy, ldy, x, ldx, \
-                       weight, mean, rstd, dx, part, dweight, dbias, (int)rows, cols, shape.waves, streaming);                          \
+                       weight, mean, rstd, dx, part, dweight, dbias, (int)rows, cols, shape.waves, streaming);                 \
   } else
       FP8GMM_LAUNCH(16, 1)
       FP8GMM_LAUNCH(64, 1)

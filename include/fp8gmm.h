@@ -703,7 +703,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
 /*
  * fp8gmm_embedding: y[t, :] = scale * weight[ids[t], :] for t in [0, n), a row of zeros where ids[t] is outside [0, table).
  * ids: int64 (ids64 != 0) or int32; weight: [table, cols] of `type`; n <= 2^28, table < 2^31 - 1, cols <= 2^23.
- * fp8gmm_embedding_backward: dweight[v, :] = scale * sum of dy[t, :] over the t with ids[t] == v, in the order of t, the whole
+ * fp8gmm_embedding_backward: dweight[v, :] = scale * sum of dy[t, :] over the t with ids[t] == v, in a fixed order, the whole
  * table, zeros where there are none; `padding` (-1: none) is an id whose tokens are left out.  dweight and workspace
  * (fp8gmm_embedding_workspace_bytes, none for short batches) on 16 bytes.  The same bits from call to call.
  */

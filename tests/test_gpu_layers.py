@@ -108,6 +108,15 @@ def test_layer_norm_of_rows_far_off_zero(dev, t, offset):
     check_norm(*norm_inputs(dev, 37, 1030, t, "fp32", True, 5, offset), what=f"offset {offset}")
 
 
+@pytest.mark.parametrize("t, cols", [("fp32", 512), ("fp32", 768), ("fp32", 2048), ("fp32", 4096), ("bf16", 2048)])
+def test_layer_norm_of_whole_pieces_off_their_alignment(dev, t, cols):
+    """Rows that share their threads another way when they, or their gradients, begin between two pieces."""
+    x, w, b, dy = norm_inputs(dev, 130, cols, t, t, True, cols)
+    off = torch.empty(130 * cols + 1, dtype=x.dtype, device=dev)
+    for xv, dv in ((x, dy), (off[1:].view(130, cols).copy_(x), dy), (x, off[1:].view(130, cols).copy_(dy))):
+        check_norm(xv, w, b, dv, what=f"{xv.data_ptr() % 16} {dv.data_ptr() % 16}")
+
+
 def test_layer_norm_takes_views(dev):
     """Rows with a pitch, at any element, of more dimensions; columns that are no neighbours; gradients that are expanded."""
     x, w, b, dy = norm_inputs(dev, 24, 650, "bf16", "bf16", True, 7)
@@ -247,7 +256,9 @@ def check_embedding(dev, ids, table, cols, t, scale=1.0, padding=None, seed=0, i
 
 @pytest.mark.parametrize("tokens, table, cols", [(1, 1, 1), (1, 5, 64), (7, 300, 33), (64, 4001, 256), (513, 17, 100), (1000, 4001, 250),
                                                  (1024, 1024, 512), (4096, 100, 1030), (5000, 70000, 24), (16384, 2000, 64),
-                                                 (16385, 2000, 64), (20000, 3, 40), (3000, 262143, 8), (3000, 262144, 8), (40000, 300000, 16), (131072, 600, 8), (131073, 60000, 9)])
+                                                 (16385, 2000, 64), (20000, 3, 40), (3000, 262143, 8), (3000, 262144, 8), (40000, 300000, 16),
+                                                 (131072, 600, 8), (131073, 60000, 9),
+                                                 (768 * 2048, 900, 8), (768 * 2048 + 1, 60000, 9)])
 @pytest.mark.parametrize("t", ["bf16", "fp16", "fp32"])
 def test_embedding_against_64_bits(dev, tokens, table, cols, t):
     """The sort in one workgroup and in many, of one to three digits; runs that end inside, at and beyond a chunk's end."""
@@ -410,15 +421,16 @@ def test_other_streams(dev):
             assert torch.equal(a, c)
 
 
-def test_captured_passes_replay(dev):
+@pytest.mark.parametrize("tokens, rows", [(700, 500), (3000, 70000), (20000, 500)])
+def test_captured_passes_replay(dev, tokens, rows):
     """Both operators, forward and backward, in one graph: four replays with new inputs and eager work in between."""
     g = torch.Generator(device=dev).manual_seed(3)
 
     def inputs():
-        return (torch.randint(0, 500, (700,), generator=g, device=dev),
-                torch.randn(700, 264, generator=g, device=dev).to(torch.bfloat16))
+        return (torch.randint(0, rows, (tokens,), generator=g, device=dev),
+                torch.randn(tokens, 264, generator=g, device=dev).to(torch.bfloat16))
 
-    table = torch.randn(500, 264, generator=g, device=dev).to(torch.bfloat16).requires_grad_()
+    table = torch.randn(rows, 264, generator=g, device=dev).to(torch.bfloat16).requires_grad_()
     w, b = torch.rand(264, device=dev).requires_grad_(), torch.rand(264, device=dev).requires_grad_()
 
     def step(ids, dy):
@@ -452,18 +464,18 @@ def test_routed_layer_norms_its_rows(dev, kind):
     """``layer_norm=True`` is the layer on normed rows, bit for bit, and its gradients go back through the norm."""
     make = moe.Fp8LinearModule if kind == "linear" else moe.Fp8MlpModule
     with_norm, without = (make(256, 512, 4, 2, device=dev, layer_norm=f) for f in (True, False))
-    assert "layer_norm.weight" in with_norm.state_dict() and without.layer_norm is None
+    assert "row_norm.weight" in with_norm.state_dict() and without.row_norm is None
     with torch.no_grad():
-        with_norm.layer_norm.weight.normal_(1, 0.1)
-        with_norm.layer_norm.bias.normal_(0, 0.1)
-    without.load_state_dict({k: v for k, v in with_norm.state_dict().items() if not k.startswith("layer_norm")})
+        with_norm.row_norm.weight.normal_(1, 0.1)
+        with_norm.row_norm.bias.normal_(0, 0.1)
+    without.load_state_dict({k: v for k, v in with_norm.state_dict().items() if not k.startswith("row_norm")})
     g = torch.Generator(device=dev).manual_seed(5)
     x = torch.randn(300, 256, generator=g, device=dev).to(torch.bfloat16)
     dy = (torch.randn(300, 256, generator=g, device=dev) * 1e-2).to(torch.bfloat16)
     grads = []
     for module in (with_norm, without):
         xs = x.clone().requires_grad_()
-        norm = with_norm.layer_norm
+        norm = with_norm.row_norm
         norm.zero_grad()
         with pkg.fp8_autocast(fp8_recipe=pkg.DelayedScaling(amax_history_len=1)):
             out = module(xs) if module is with_norm else module(pkg.layer_norm(xs, norm.weight, norm.bias, norm.eps))
@@ -471,6 +483,24 @@ def test_routed_layer_norms_its_rows(dev, kind):
         grads.append([out.detach(), xs.grad, norm.weight.grad.clone(), norm.bias.grad.clone(), module.gating_network.weight.grad])
     for a, c in zip(*grads):
         assert torch.equal(a, c) and torch.isfinite(a.float()).all() and a.any()
+
+
+def test_routed_layers_of_before_run_as_they_did(dev):
+    """A layer without the option's attribute (pickled ahead of it), and a subclass that has a norm of its own by the usual name."""
+    class Own(moe.Fp8MlpModule):
+        def __init__(self, *args, **kwargs):
+            super().__init__(*args, **kwargs)
+            self.layer_norm = torch.nn.LayerNorm(256, dtype=torch.bfloat16, device=dev)
+
+    plain, own = moe.Fp8MlpModule(256, 512, 4, 2, device=dev), Own(256, 512, 4, 2, device=dev)
+    own.load_state_dict(plain.state_dict(), strict=False)
+    old = moe.Fp8MlpModule(256, 512, 4, 2, device=dev)
+    old.load_state_dict(plain.state_dict())
+    del old.row_norm
+    x = torch.randn(300, 256, generator=torch.Generator(device=dev).manual_seed(6), device=dev).to(torch.bfloat16)
+    with torch.no_grad(), pkg.fp8_autocast(fp8_recipe=pkg.DelayedScaling(amax_history_len=1)):
+        want, *got = [module(x) for module in (plain, own, old)]
+    assert all(torch.equal(g, want) for g in got)
 
 
 def test_a_training_step_of_a_small_model(dev):
