@@ -718,7 +718,8 @@ int fp8gmm_embedding_backward(const void* ids, int ids64, int64_t n, const void*
  * A result may stand in the place of its own tensor (in == out, the same type); it may overlap nothing else of the call
  * (FP8GMM_ERR_BAD_ARGUMENT).  Gradients in place are not written again where the factor is 1.  A norm that is infinite or a
  * NaN makes a factor of 0 or a NaN.  `tensors` is HOST memory and is read during the call only: the table travels in the
- * launches' arguments.  norm: device fp32.  workspace: fp8gmm_multi_norm_workspace_bytes(n) bytes on 16 bytes.
+ * launches' arguments.  Fewer than 2^40 elements in all, addresses below 2^48.  norm: device fp32.  workspace:
+ * fp8gmm_multi_norm_workspace_bytes(n) bytes on 16 bytes.
  */
 typedef struct fp8gmm_norm_tensor {
   const void* in;

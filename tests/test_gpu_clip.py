@@ -58,6 +58,8 @@ SIZES = {
     "one": [1], "one value each": [1] * 7, "odd": [3, 1, 4097, 129, 65535, 17], "none among them": [0, 5, 0, 8192, 8193, 0],
     "chunks": [8192, 4096, 16384, 8191, 8193], "all empty": [0, 0], "more than a launch": [50 + 37 * i % 900 for i in range(300)],
     "many partial sums": [20000 + i for i in range(900)],
+    **{f"{n} tensors": [1 + 41 * i % 300 for i in range(n)] for n in (64, 65, 112, 113, 200, 201, 400, 401)},
+    "a long one among short ones": [10] * 150 + [3000001] + [20] * 150,
 }
 
 

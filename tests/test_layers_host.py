@@ -108,12 +108,12 @@ def test_multi_norm_status():
     for clip in (False, True):
         assert call([good], clip, n=-1) == ARGUMENT and call([good], clip, norm=None) == NULL and call([good], clip, work=None) == NULL
         assert call([good], clip, work=P + 8) == ALIGN and call([good], clip, size=L.fp8gmm_multi_norm_workspace_bytes(1) - 1) == WORKSPACE
-        for bad, status in (((P, P, 10, 3, 0), FORMAT), ((P, P, -1, 0, 0), SHAPE), ((P, P, (1 << 40) + 1, 0, 0), SHAPE), ((None, P, 10, 0, 0), NULL),
+        for bad, status in (((P, P, 10, 3, 0), FORMAT), ((P, P, -1, 0, 0), SHAPE), ((P, P, 1 << 40, 0, 0), SHAPE), (((1 << 48) + P, P, 10, 0, 0), ARGUMENT), ((None, P, 10, 0, 0), NULL),
                             ((P + 1, P, 10, 0, 0), ALIGN), ((P + 2, P, 10, 2, 2), ALIGN)):
             assert call([good, bad], clip) == status, bad
-        assert call([(P, P, 1 << 39, 0, 0), (P, P, (1 << 39) + 1, 0, 0)], clip) == SHAPE
+        assert call([(P, P, 1 << 39, 0, 0), (P, P, 1 << 39, 0, 0)], clip) == SHAPE
     assert L.fp8gmm_multi_norm(None, 1, P, P, 1 << 20, None) == NULL
-    for bad, status in (((P, None, 10, 0, 0), NULL), ((P, P, 10, 0, 1), FORMAT), ((P, P, 10, 2, 0), FORMAT), ((P, P + 2, 10, 0, 2), ALIGN),
+    for bad, status in (((P, None, 10, 0, 0), NULL), ((P, P, 10, 0, 1), FORMAT), ((P, P, 10, 2, 0), FORMAT), ((P, P + 2, 10, 0, 2), ALIGN), ((P, (1 << 48) + P, 10, 0, 0), ARGUMENT),
                         ((P, P, 10, 0, 2), ARGUMENT), ((P, P + 18, 10, 0, 0), ARGUMENT), ((P + 18, P, 10, 0, 0), ARGUMENT)):
         assert call([bad], True) == status, bad
     assert call([good, good], True) == ARGUMENT                                         # the same one twice
