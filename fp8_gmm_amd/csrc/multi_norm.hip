@@ -8,7 +8,7 @@
 // magnitude that a gradient can have overflows or vanishes, and the order of the sums does not show in 32 bits.
 //
 // Every tensor is cut into chunks of 16 KB, and a workgroup takes a contiguous range of all chunks.  The table of the tensors of a
-// short list travels in the launches' arguments (96 tensors to fp32, 290 MB of bf16: 218 us, through memory 234); that of a longer
+// short list travels in the launches' arguments (96 tensors, 290 MB of bf16, clipped: 150.8 us, through memory 152.6; of 112 short ones 14.7, of 113 19.6); that of a longer
 // one is written to the workspace first, 200 tensors to a launch, by their arguments too - so nothing is uploaded, and a captured
 // call holds its table.  The partial sums, one per workgroup of the
 // norm, are added up by every workgroup of the scaling for itself, in the same order.  The scaling goes backwards, from what the
@@ -25,18 +25,18 @@ constexpr int kTensors = 112;        // of a launch's arguments
 constexpr int kThreads = 256;
 constexpr int kPieces = 4;           // of 16 bytes per thread and chunk
 constexpr int kChunkBytes = kThreads * kPieces * 16;
-// Chunks of a workgroup of the norm, and more of very long lists.  Norms of 96 tensors, 290 MB of bf16, by 1, 4 and 16 chunks: 59,
-// 60 and 71 us; of 24 tensors, 67 MB of fp32, 17.4 and 15.9 by 1 and 4: more workgroups, more partial sums.
+// Chunks of a workgroup of the norm, and more of very long lists.  Norms of 96 tensors, 290 MB of bf16, by 1, 4 and 16 chunks:
+// 50.6, 51.8 and 53.5 us; of 24 tensors, 67 MB of fp32, by 1 and 4: 17.4 and 15.9 (more workgroups, more partial sums).
 constexpr int kRun = 4;
 constexpr int kNormBlocks = 8192;    // the most workgroups of a launch
 // Partial sums that every workgroup of the scaling adds up for itself; more have a launch for that.  Clipping of 24 tensors of
-// 87381 fp32 elements (129 sums) 13.0 us, with the launch 15.7; of 349525 (516) 22.0 without it and 23.1; of 300 MB (4600) 195
-// and 163.
+// 87381 fp32 elements (129 sums) 13.0 us, with the launch 15.7; of 349525 (516) 22.0 without it and 23.1; of 300 MB (4600) 182
+// and 151.
 constexpr int kFewPartials = 512;
 constexpr int kClipBlocks = 1 << 20; // of the scaling, a chunk to each but for lists of 16 GB and more
 // Gradients are read with the streaming hint where nothing of them would be found in the caches by a second pass, 512 MB on (1.9
-// GB to 3.8: 1332 us, without the hint 1346; 270 MB: 172, with it 186), or where there is none (norm of 290 MB: 52 us, without 58).
-// Results are written with it where whoever reads them does not find them there (290 MB clipped: 163 us, without 190).
+// GB to 3.8: 1332 us, without the hint 1346; 270 MB: 159, with it 163), or where there is none (norm of 290 MB: 52 us, without 58).
+// Results are written with it where whoever reads them does not find them there (290 MB clipped: 151 us, without 182).
 constexpr int64_t kStreamTwice = (int64_t)512 << 20, kStreamOnce = (int64_t)32 << 20, kStreamOut = (int64_t)64 << 20;
 
 struct Entry {
@@ -156,14 +156,35 @@ __device__ __forceinline__ void load_chunk(const typename Elements<TYPE>::bits* 
   }
 }
 
+// The elements of a tensor in front of the first 16 bytes that are aligned.  They belong to its first chunk, and the chunks' pieces
+// are aligned (270 MB in tensors at any element: norm 65 us with chunks from the first element on, 58 with these; clipped 169 and
+// 161).  A tensor's last chunk may be left without elements.
+template <int SIZE>
+__device__ __forceinline__ int head_of(const void* p, int64_t count) {
+  const int head = (int)(-reinterpret_cast<uintptr_t>(p) & 15) / SIZE;
+  return count < head ? (int)count : head;
+}
+template <int TYPE>
+__device__ __forceinline__ float element(const typename Elements<TYPE>::bits* p) {
+  float f[Elements<TYPE>::kVec];
+  Elements<TYPE>::unpack(Elements<TYPE>::load(p, 1), f);
+  return f[0];
+}
+
 // The squares of thread t's share of chunk c, added to `sum`
 template <int TYPE, bool STREAM>
 __device__ __forceinline__ void add_squares(const Entry& e, uint32_t c, int t, double (&sum)[2]) {
   typedef Elements<TYPE> E;
   constexpr int V = E::kVec, CHUNK = kThreads * kPieces * V;
-  const int64_t first = (int64_t)(c - e.begin) * CHUNK, left = e.count - first;
+  const typename E::bits* const p = static_cast<const typename E::bits*>(e.in);
+  const int head = head_of<E::kBytes>(p, e.count);
+  const int64_t first = head + (int64_t)(c - e.begin) * CHUNK, left = e.count - first;
   u32x4 raw[kPieces];
-  load_chunk<TYPE, STREAM>(static_cast<const typename E::bits*>(e.in) + first, (int)(left < CHUNK ? left : CHUNK), t, raw);
+  load_chunk<TYPE, STREAM>(p + first, (int)(left < CHUNK ? left : CHUNK), t, raw);
+  if (c == e.begin && t < head) {
+    const float f = element<TYPE>(p + t);
+    sum[0] = __builtin_fma((double)f, (double)f, sum[0]);
+  }
 #pragma unroll
   for (int u = 0; u < kPieces; ++u) {
     float f[V];
@@ -265,18 +286,23 @@ __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits*
   }
 }
 
-// Thread t's share of chunk c of a tensor, scaled
+// Thread t's share of chunk c of a tensor, scaled; the chunks as the result is aligned
+template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT>
+__device__ __forceinline__ void scale_as(const Entry& e, uint32_t c, int t, float factor) {
+  typedef Elements<TYPE> E;
+  typedef Elements<OUT> O;
+  constexpr int CHUNK = kThreads * kPieces * E::kVec;
+  const typename E::bits* const p = static_cast<const typename E::bits*>(e.in);
+  typename O::bits* const out = static_cast<typename O::bits*>(e.out);
+  const int head = head_of<O::kBytes>(out, e.count);
+  const int64_t at = head + (int64_t)(c - e.begin) * CHUNK, left = e.count - at;
+  scale_chunk<TYPE, OUT, STREAM, STREAM_OUT>(p + at, out + at, (int)(left < CHUNK ? left : CHUNK), t, factor);
+  if (c == e.begin && t < head) out[t] = O::pack1(element<TYPE>(p + t) * factor);
+}
 template <int TYPE, bool STREAM, bool STREAM_OUT>
 __device__ __forceinline__ void scale(const Entry& e, uint32_t c, int t, float factor) {
-  typedef Elements<TYPE> E;
-  constexpr int CHUNK = kThreads * kPieces * E::kVec;
-  const int64_t at = (int64_t)(c - e.begin) * CHUNK, left = e.count - at;
-  const typename E::bits* const p = static_cast<const typename E::bits*>(e.in) + at;
-  const int here = (int)(left < CHUNK ? left : CHUNK);
-  if (TYPE != FP8GMM_TYPE_FP32 && e.out_type == FP8GMM_TYPE_FP32)
-    scale_chunk<TYPE, FP8GMM_TYPE_FP32, STREAM, STREAM_OUT>(p, static_cast<uint32_t*>(e.out) + at, here, t, factor);
-  else
-    scale_chunk<TYPE, TYPE, STREAM, STREAM_OUT>(p, static_cast<typename E::bits*>(e.out) + at, here, t, factor);
+  if (TYPE != FP8GMM_TYPE_FP32 && e.out_type == FP8GMM_TYPE_FP32) scale_as<TYPE, FP8GMM_TYPE_FP32, STREAM, STREAM_OUT>(e, c, t, factor);
+  else scale_as<TYPE, TYPE, STREAM, STREAM_OUT>(e, c, t, factor);
 }
 
 template <bool DIRECT, bool STREAM, bool STREAM_OUT>
