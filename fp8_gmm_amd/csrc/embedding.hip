@@ -520,7 +520,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embedding_join_kernel(const i
 // the columns a wavefront, over the row's tokens in their order; a row of more than 64 tokens is shared out by 64 entries of the
 // list to a wavefront.  Bound by latency, its own and the host's, which has three launches fewer.  Short batches, call to call, by
 // this launch and by the sort: 1000 tokens of 4001 x 256, fp32, 8.6 and 18.4 us; 500 of 50000 x 65, bf16, 7.0 and 18.3; 1000 of a
-// million rows of 64, bf16, 21 and 43; but all of 1024 tokens of 512 columns the same, 25 and 15.  A table of 262 MB is written faster beside the sort (41 us, 49).
+// million rows of 64, bf16, 21 and 43; but all of 1024 tokens of 512 columns the same, 25 and 15.  A table of 262 MB is written
+// faster beside the sort (41 us, 49).
 template <int V>
 struct RowSum {
   float f[V];

@@ -24,7 +24,7 @@ int type_of(const Tensor& t, const char* what) {
 
 void check_plain(const Tensor& t, const char* what) {
   TORCH_CHECK(t.is_cuda(), "fp8_gmm_amd: expected GPU tensors (the HIP path has no CPU fallback)");
-  TORCH_CHECK(t.layout() == at::kStrided, "fp8_gmm_amd: ", what, " must be a dense tensor");
+  TORCH_CHECK(t.layout() == at::kStrided && !t.is_neg(), "fp8_gmm_amd: ", what, " must be a dense tensor");
 }
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -356,6 +356,8 @@ Tensor multi_clip(const std::vector<Tensor>& tensors, const std::vector<Tensor>&
                     (outs[i].scalar_type() == tensors[i].scalar_type() || outs[i].scalar_type() == at::kFloat),
                 "fp8_gmm_amd: results of multi_clip have their tensors' shapes, and their types or float32");
     TORCH_CHECK(!(at::GradMode::is_enabled() && outs[i].requires_grad()), "fp8_gmm_amd: a result of multi_clip requires a gradient");
+    TORCH_CHECK(!outs[i].is_inference() || c10::InferenceMode::is_enabled(),
+                "fp8_gmm_amd: a result of multi_clip is an inference tensor, which is written in inference mode only");
     at::assert_no_internal_overlap(outs[i]);
   }
   check_copied(tensors, outs);

@@ -8,11 +8,11 @@
 // magnitude that a gradient can have overflows or vanishes, and the order of the sums does not show in 32 bits.
 //
 // Every tensor is cut into chunks of 16 KB, and a workgroup takes a contiguous range of all chunks.  The table of the tensors of a
-// short list travels in the launches' arguments (96 tensors, 290 MB of bf16, clipped: 150.8 us, through memory 152.6; of 112 short ones 14.7, of 113 19.6); that of a longer
-// one is written to the workspace first, 200 tensors to a launch, by their arguments too - so nothing is uploaded, and a captured
-// call holds its table.  The partial sums, one per workgroup of the
-// norm, are added up by every workgroup of the scaling for itself, in the same order.  The scaling goes backwards, from what the
-// norm has read last and the caches still hold.
+// short list travels in the launches' arguments (96 tensors, 290 MB of bf16, clipped: 150.8 us, through memory 152.6; 112 short ones
+// 14.7, 113 of them 19.6); that of a longer one is written to the workspace first, 200 tensors to a launch, by their arguments too -
+// so nothing is uploaded, and a captured call holds its table.  The partial sums, one per workgroup of the norm, are added up by every
+// workgroup of the scaling for itself, in the same order, or in a launch of their own where they are many.  The scaling goes
+// backwards, from what the norm has read last and the caches still hold.
 #include <algorithm>
 #include <vector>
 
@@ -86,7 +86,8 @@ __host__ __device__ inline uint32_t chunks_of(int64_t count, int type) {
   return (uint32_t)((count * (type == FP8GMM_TYPE_FP32 ? 4 : 2) + kChunkBytes - 1) / kChunkBytes);
 }
 
-__global__ __launch_bounds__(kPackedThreads) void multi_norm_table_kernel(const PackedPart part, int n, uint32_t begin, Entry* __restrict__ table) {
+__global__ __launch_bounds__(kPackedThreads) void multi_norm_table_kernel(const PackedPart part, int n, uint32_t begin,
+                                                                          Entry* __restrict__ table) {
   __shared__ uint32_t sums[kPackedThreads / 64];
   const int i = threadIdx.x, lane = i % 64, wave = i / 64;
   Entry e = {};
@@ -236,7 +237,8 @@ __global__ __launch_bounds__(1024) void multi_norm_finish_kernel(const double* _
 // that a store instruction writes whole lines (with 8 elements a thread, whose two stores share lines, the streaming hint made
 // 1.9 GB to 3.8 take 2440 us; without it 1544).
 template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT>
-__device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits* p, typename Elements<OUT>::bits* out, int n, int t, float factor) {
+__device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits* p, typename Elements<OUT>::bits* out, int n, int t,
+                                            float factor) {
   typedef Elements<TYPE> E;
   typedef Elements<OUT> O;
   if constexpr (TYPE == OUT) {
@@ -266,7 +268,8 @@ __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits*
     const auto scaled = [&](u32x2 raw) {
       float f[E::kVec];
       E::unpack(u32x4{raw.x, raw.y, 0u, 0u}, f);
-      return u32x4{__float_as_uint(f[0] * factor), __float_as_uint(f[1] * factor), __float_as_uint(f[2] * factor), __float_as_uint(f[3] * factor)};
+      return u32x4{__float_as_uint(f[0] * factor), __float_as_uint(f[1] * factor), __float_as_uint(f[2] * factor),
+                   __float_as_uint(f[3] * factor)};
     };
     if (n == kThreads * COUNT * V) {
       u32x2 raw[COUNT];
@@ -447,7 +450,8 @@ int check_tensors(const fp8gmm_norm_tensor* tensors, int n, bool out) {
   return FP8GMM_OK;
 }
 
-// Nothing is written that another tensor of the call reads or writes: a result lies apart from all else, or in the place of its own tensor.
+// Nothing is written that another tensor of the call reads or writes: a result lies apart from all else, or in the place of its own
+// tensor.
 int check_apart(const fp8gmm_norm_tensor* tensors, int n) {
   struct Range {
     uintptr_t begin, end;
@@ -595,8 +599,8 @@ int multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float*
                  : in ? out ? &multi_clip_kernel<false, true, true> : &multi_clip_kernel<false, true, false>
                  : out ? &multi_clip_kernel<false, false, true>
                        : &multi_clip_kernel<false, false, false>;
-  hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks)), dim3(kThreads), 0, s, part, table_of(workspace), list.n(), list.chunks,
-                     partials_of(workspace), list.blocks(), max_norm, finished, list.in_place, norm);
+  hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks)), dim3(kThreads), 0, s, part, table_of(workspace),
+                     list.n(), list.chunks, partials_of(workspace), list.blocks(), max_norm, finished, list.in_place, norm);
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 

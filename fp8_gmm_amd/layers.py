@@ -35,8 +35,8 @@ def layer_norm(x, weight, bias=None, eps=1e-5):
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None):
-    """Rows of the table ``weight [rows, columns]`` by token id, times ``scale``: ``[*ids.shape, columns]`` in the table's type.
-    ``ids``: int64 or int32.  An id outside the table gives a row of zeros and takes no gradient (a table that is sharded by
+    """Rows of the table ``weight [rows, columns]`` (contiguous) by token id, times ``scale``: ``[*ids.shape, columns]`` in the
+    table's type.  ``ids``: int64 or int32.  An id outside the table gives a row of zeros and takes no gradient (a table that is sharded by
     rows is looked up with ``ids - first_row`` and its results added up); the row ``padding_idx`` is read like any other and
     takes no gradient.  The table's gradient is dense, summed in float32 over every row's tokens in a fixed order."""
     _check_unwrapped("embedding")

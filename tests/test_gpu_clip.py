@@ -211,7 +211,7 @@ def test_clip_grad_norm(dev):
     before = [p.grad.clone() for p in params[:3]]
     norm = norm_of(before)
     versions = [p.grad._version for p in params[:3]]
-    got = pkg.clip_grad_norm_(iter(params), 0.3 * norm)   # a generator is walked through once
+    got = pkg.clip_grad_norm_(iter(params), 0.3 * norm, foreach=True)   # a generator is walked through once
     assert abs(got.item() - norm) <= 1.01 * U * norm and not got.requires_grad
     check_scaled([p.grad for p in params[:3]], before, 0.3 * norm / (norm + 1e-6))
     assert all(p.grad._version > v for p, v in zip(params, versions)), "autograd does not see the change"
@@ -271,6 +271,15 @@ def test_refusals(dev):
                             ([a.to_sparse()], [a], "dense")):
         with pytest.raises(RuntimeError, match=what):
             backend.multi_clip(ins, outs, 1.0)
+    with torch.inference_mode():
+        frozen = torch.ones(16, device=dev)
+        backend.multi_clip([frozen], [frozen], 2.0)
+    before = frozen.clone()
+    with pytest.raises(RuntimeError, match="inference"):
+        backend.multi_clip([frozen], [frozen], 1.0)
+    with pytest.raises(RuntimeError, match="dense"):
+        backend.multi_norm([torch._neg_view(a)])
+    assert torch.equal(frozen, before) and (before == torch.tensor(2 / (4 + 1e-6), device=dev)).all()   # 16 ones have norm 4
     for bad in (-1.0, math.nan):
         with pytest.raises(RuntimeError, match="max_norm"):
             backend.multi_clip([a], [a], bad)
