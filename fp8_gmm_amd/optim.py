@@ -1,7 +1,7 @@
 """Between the backward pass and the optimizer: clipping of the gradients by their global norm.
 
-The operand-level calls are ``backend.multi_norm`` and ``backend.multi_clip``; this is the one on parameters, with the
-arguments of ``torch.nn.utils.clip_grad_norm_``.
+The operand-level calls are ``backend.multi_norm`` and ``backend.multi_clip``; this is the one on parameters, with the name and
+the arguments that torch's users know.
 """
 import torch
 
