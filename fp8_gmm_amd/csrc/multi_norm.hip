@@ -33,10 +33,14 @@ constexpr int kNormBlocks = 8192;    // the most workgroups of a launch
 // 87381 fp32 elements (129 sums) 13.0 us, with the launch 15.7; of 349525 (516) 22.0 without it and 23.1; of 300 MB (4600) 182
 // and 151.
 constexpr int kFewPartials = 512;
-constexpr int kClipBlocks = 1 << 20; // of the scaling, a chunk to each but for lists of 16 GB and more
+constexpr int kClipBlocks = 1 << 20; // of the scaling, a chunk or half of one to each but for lists of 8 GB and more
+// Halves of a chunk to a workgroup of the scaling where some results are fp32 of 16 bits, twice what is read: 1.9 GB to 3.8 1224 us, by
+// whole chunks 1331; 305 MB to 610, 400 tensors, 215.5 and 217.  Results of the same type by halves: 160 us, and 171.
+constexpr int kWiderParts = 2;
 // Gradients are read with the streaming hint where nothing of them would be found in the caches by a second pass, 512 MB on (1.9
-// GB to 3.8: 1332 us, without the hint 1346; 270 MB: 159, with it 163), or where there is none (norm of 290 MB: 52 us, without 58).
-// Results are written with it where whoever reads them does not find them there (290 MB clipped: 151 us, without 182).
+// GB to 3.8 by whole chunks: 1332 us, without the hint 1346; 270 MB: 159, with it 163), or where there is none (norm of 290 MB:
+// 52 us, without 58).  Results are written with it where whoever reads them does not find them there (290 MB clipped: 151 us,
+// without 182).
 constexpr int64_t kStreamTwice = (int64_t)512 << 20, kStreamOnce = (int64_t)32 << 20, kStreamOut = (int64_t)64 << 20;
 
 struct Entry {
@@ -143,17 +147,17 @@ __device__ __forceinline__ void with_type(int type, F&& f) {
   else f(std::integral_constant<int, FP8GMM_TYPE_FP32>{});
 }
 
-// The pieces of a thread of the chunk at `p`, of which `n` elements are the tensor's
-template <int TYPE, bool STREAM>
-__device__ __forceinline__ void load_chunk(const typename Elements<TYPE>::bits* p, int n, int t, u32x4 (&raw)[kPieces]) {
+// The pieces of a thread of the chunk, or share of one, at `p`, of which `n` elements are the tensor's
+template <int TYPE, bool STREAM, int PIECES>
+__device__ __forceinline__ void load_chunk(const typename Elements<TYPE>::bits* p, int n, int t, u32x4 (&raw)[PIECES]) {
   typedef Elements<TYPE> E;
   constexpr int V = E::kVec;
-  if (n == kThreads * kPieces * V) {
+  if (n == kThreads * PIECES * V) {
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) raw[u] = E::template load<STREAM>(p + (u * kThreads + t) * V, V);
+    for (int u = 0; u < PIECES; ++u) raw[u] = E::template load<STREAM>(p + (u * kThreads + t) * V, V);
   } else {
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) raw[u] = E::load(p + (u * kThreads + t) * V, n - (u * kThreads + t) * V);
+    for (int u = 0; u < PIECES; ++u) raw[u] = E::load(p + (u * kThreads + t) * V, n - (u * kThreads + t) * V);
   }
 }
 
@@ -236,18 +240,18 @@ __global__ __launch_bounds__(1024) void multi_norm_finish_kernel(const double* _
 // A chunk's pieces times the factor.  fp32 results of a 16-bit type: pieces of four elements, 8 bytes read and 16 written, so
 // that a store instruction writes whole lines (with 8 elements a thread, whose two stores share lines, the streaming hint made
 // 1.9 GB to 3.8 take 2440 us; without it 1544).
-template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT>
+template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT, int PIECES>
 __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits* p, typename Elements<OUT>::bits* out, int n, int t,
                                             float factor) {
   typedef Elements<TYPE> E;
   typedef Elements<OUT> O;
   if constexpr (TYPE == OUT) {
     constexpr int V = E::kVec;
-    const bool all = n == kThreads * kPieces * V;
-    u32x4 raw[kPieces];
+    const bool all = n == kThreads * PIECES * V;
+    u32x4 raw[PIECES];
     load_chunk<TYPE, STREAM>(p, n, t, raw);
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) {
+    for (int u = 0; u < PIECES; ++u) {
       float f[V];
       E::unpack(raw[u], f);
 #pragma unroll
@@ -256,14 +260,14 @@ __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits*
     }
     if (all) {
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + t) * V, V, raw[u]);
+      for (int u = 0; u < PIECES; ++u) O::template store<STREAM_OUT>(out + (u * kThreads + t) * V, V, raw[u]);
     } else {
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u)
+      for (int u = 0; u < PIECES; ++u)
         O::store(out + (u * kThreads + t) * V, n - (u * kThreads + t) * V, raw[u]);
     }
   } else {
-    constexpr int V = 4, COUNT = kPieces * E::kVec / V;
+    constexpr int V = 4, COUNT = PIECES * E::kVec / V;
     typedef uint32_t half_piece __attribute__((ext_vector_type(2), aligned(2)));
     const auto scaled = [&](u32x2 raw) {
       float f[E::kVec];
@@ -289,26 +293,28 @@ __device__ __forceinline__ void scale_chunk(const typename Elements<TYPE>::bits*
   }
 }
 
-// Thread t's share of chunk c of a tensor, scaled; the chunks as the result is aligned
-template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT>
-__device__ __forceinline__ void scale_as(const Entry& e, uint32_t c, int t, float factor) {
+// Thread t's share of a part of chunk c of a tensor, scaled; the chunks as the result is aligned
+template <int TYPE, int OUT, bool STREAM, bool STREAM_OUT, int PARTS>
+__device__ __forceinline__ void scale_as(const Entry& e, uint32_t c, int part, int t, float factor) {
   typedef Elements<TYPE> E;
   typedef Elements<OUT> O;
-  constexpr int CHUNK = kThreads * kPieces * E::kVec;
+  constexpr int CHUNK = kThreads * kPieces * E::kVec, SHARE = CHUNK / PARTS;
   const typename E::bits* const p = static_cast<const typename E::bits*>(e.in);
   typename O::bits* const out = static_cast<typename O::bits*>(e.out);
   const int head = head_of<O::kBytes>(out, e.count);
-  const int64_t at = head + (int64_t)(c - e.begin) * CHUNK, left = e.count - at;
-  scale_chunk<TYPE, OUT, STREAM, STREAM_OUT>(p + at, out + at, (int)(left < CHUNK ? left : CHUNK), t, factor);
-  if (c == e.begin && t < head) out[t] = O::pack1(element<TYPE>(p + t) * factor);
+  const int64_t at = head + (int64_t)(c - e.begin) * CHUNK + part * SHARE, left = e.count - at;
+  scale_chunk<TYPE, OUT, STREAM, STREAM_OUT, kPieces / PARTS>(p + at, out + at, (int)(left < SHARE ? left : SHARE), t, factor);
+  if (c == e.begin && part == 0 && t < head) out[t] = O::pack1(element<TYPE>(p + t) * factor);
 }
-template <int TYPE, bool STREAM, bool STREAM_OUT>
-__device__ __forceinline__ void scale(const Entry& e, uint32_t c, int t, float factor) {
-  if (TYPE != FP8GMM_TYPE_FP32 && e.out_type == FP8GMM_TYPE_FP32) scale_as<TYPE, FP8GMM_TYPE_FP32, STREAM, STREAM_OUT>(e, c, t, factor);
-  else scale_as<TYPE, TYPE, STREAM, STREAM_OUT>(e, c, t, factor);
+template <int TYPE, bool STREAM, bool STREAM_OUT, int PARTS>
+__device__ __forceinline__ void scale(const Entry& e, uint32_t c, int part, int t, float factor) {
+  if (TYPE != FP8GMM_TYPE_FP32 && e.out_type == FP8GMM_TYPE_FP32)
+    scale_as<TYPE, FP8GMM_TYPE_FP32, STREAM, STREAM_OUT, PARTS>(e, c, part, t, factor);
+  else
+    scale_as<TYPE, TYPE, STREAM, STREAM_OUT, PARTS>(e, c, part, t, factor);
 }
 
-template <bool DIRECT, bool STREAM, bool STREAM_OUT>
+template <bool DIRECT, bool STREAM, bool STREAM_OUT, int PARTS>
 __global__ __launch_bounds__(kThreads) void multi_clip_kernel(const Part part, const Entry* __restrict__ memory, int n, uint32_t chunks,
                                                               const double* __restrict__ partials, int n_partials, double max_norm,
                                                               const float* __restrict__ finished, bool in_place, float* __restrict__ norm) {
@@ -326,18 +332,20 @@ __global__ __launch_bounds__(kThreads) void multi_clip_kernel(const Part part, c
   if (in_place && factor == 1.f) return;   // all of them
   const Table<DIRECT> table = {part, memory, n, chunks};
   const uint32_t block = gridDim.x - 1 - blockIdx.x;      // backwards
-  const uint32_t lo = (uint32_t)((uint64_t)chunks * block / gridDim.x), hi = (uint32_t)((uint64_t)chunks * (block + 1) / gridDim.x);
+  const uint64_t parts = (uint64_t)chunks * PARTS;
+  const uint32_t lo = (uint32_t)(parts * block / gridDim.x), hi = (uint32_t)(parts * (block + 1) / gridDim.x);
   if (lo == hi) return;
-  int i = table.of(hi - 1);
+  int i = table.of((hi - 1) / PARTS);
   for (uint32_t c = hi; c > lo; --i) {
     const Entry e = table[i];
-    const uint32_t first = max(e.begin, lo);
+    const uint32_t first = max(e.begin * PARTS, lo);
     if (factor == 1.f && e.in == e.out) {   // gradients within the bound stay as they are, in place
       c = first;
       continue;
     }
     with_type(e.type, [&](auto type) {
-      while (c > first) scale<decltype(type)::value, STREAM, STREAM_OUT>(e, --c, threadIdx.x, factor);
+      for (; c > first; --c)
+        scale<decltype(type)::value, STREAM, STREAM_OUT, PARTS>(e, (c - 1) / PARTS, (c - 1) % PARTS, threadIdx.x, factor);
     });
   }
 }
@@ -482,6 +490,7 @@ struct List {
   uint32_t chunks = 0;
   int64_t bytes_in = 0, bytes_out = 0;
   bool in_place = true;   // all of them
+  bool wider = false;     // some in fp32 of 16 bits
   List(const fp8gmm_norm_tensor* tensors, int n) {
     entries.reserve((size_t)n);
     for (int i = 0; i < n; ++i) {
@@ -492,6 +501,7 @@ struct List {
       bytes_in += t.count * type_bytes(t.type);
       bytes_out += t.count * type_bytes(t.out_type);
       in_place = in_place && t.in == t.out;
+      wider = wider || t.out_type != t.type;
     }
   }
   int n() const { return (int)entries.size(); }
@@ -593,14 +603,19 @@ int multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float*
   const Part part = launch_norm(list, in, workspace, s);
   float* const finished = list.blocks() > kFewPartials ? factor_at(workspace) : nullptr;
   if (finished != nullptr) launch_finish(list, max_norm, norm, finished, workspace, s);
-  auto* kernel = list.direct() ? in ? out ? &multi_clip_kernel<true, true, true> : &multi_clip_kernel<true, true, false>
-                                 : out ? &multi_clip_kernel<true, false, true>
-                                       : &multi_clip_kernel<true, false, false>
-                 : in ? out ? &multi_clip_kernel<false, true, true> : &multi_clip_kernel<false, true, false>
-                 : out ? &multi_clip_kernel<false, false, true>
-                       : &multi_clip_kernel<false, false, false>;
-  hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks)), dim3(kThreads), 0, s, part, table_of(workspace),
-                     list.n(), list.chunks, partials_of(workspace), list.blocks(), max_norm, finished, list.in_place, norm);
+  const auto launch = [&](auto parts) {
+    constexpr int PARTS = decltype(parts)::value;
+    auto* kernel = list.direct() ? in ? out ? &multi_clip_kernel<true, true, true, PARTS> : &multi_clip_kernel<true, true, false, PARTS>
+                                   : out ? &multi_clip_kernel<true, false, true, PARTS>
+                                         : &multi_clip_kernel<true, false, false, PARTS>
+                   : in ? out ? &multi_clip_kernel<false, true, true, PARTS> : &multi_clip_kernel<false, true, false, PARTS>
+                   : out ? &multi_clip_kernel<false, false, true, PARTS>
+                         : &multi_clip_kernel<false, false, false, PARTS>;
+    hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks / PARTS) * PARTS), dim3(kThreads), 0, s, part,
+                       table_of(workspace), list.n(), list.chunks, partials_of(workspace), list.blocks(), max_norm, finished,
+                       list.in_place, norm);
+  };
+  list.wider ? launch(std::integral_constant<int, kWiderParts>{}) : launch(std::integral_constant<int, 1>{});
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
