@@ -16,7 +16,8 @@
 //   16384 x 4096, bf16     43.7   6.1     73.4   5.5
 //   16384 x 4093, bf16     44     6.1     77     5.2     rows that begin at any element
 //   65536 x 2048, fp32     192    5.6     264    6.1
-//   8192 x 16384, bf16     94     5.7     164    4.9     long rows, read twice, the second time from the cache
+//   8192 x 16384, bf16     94     5.7     164    4.9     the longest rows that stay in registers
+//   262144 x 256, bf16     44     6.1     72     5.6     four rows to a wavefront
 // A large copy reaches 5.3 here.
 #include <algorithm>
 #include <type_traits>
@@ -502,8 +503,10 @@ struct Shape {
 int pieces_of(int cols, int type) { return ceil_div(cols, 16 / type_bytes(type)); }
 // Up to `most` pieces to a thread, as few threads as that allows, and then as few pieces: a thread behind the row's end works for
 // nothing.  `waves`: the most of them.  A row's first 64 * waves pieces are there, so that every wavefront has some of the row.
-Shape shape_of(int pieces, int most, int waves) {
-  if (pieces <= 16) return {16, 1, 1};
+// `narrow`: the most pieces of a thread where 16 lanes have a row.  4 forward (262144 x 256, bf16, 75 us by 64 lanes, 44 so; 131072 x
+// 384, 44 and 35; 131072 x 512, 49 and 42), 2 backward (262144 x 256, 85 and 72; with 3, 131072 x 384, 55 and 161: spills).
+Shape shape_of(int pieces, int most, int waves, int narrow) {
+  if (pieces <= 16 * narrow) return {16, 1, ceil_div(pieces, 16)};
   const int w = ceil_div(pieces, 64 * most);
   return w <= waves ? Shape{64, w, ceil_div(pieces, 64 * w)} : Shape{0, 0, 0};
 }
@@ -517,7 +520,7 @@ Shape widest(int cols, int type) {
 // Forward, 4 pieces to a thread: few barriers and many loads under way (16384 x 4096, bf16: 43.5 us, with 2 pieces 45.6; 65536 x
 // 2048, fp32: 194 and 206; 16384 x 1536, bf16: 21.6 and 24.6).
 Shape forward_shape(int cols, int type) {
-  const Shape s = shape_of(pieces_of(cols, type), 4, 8);
+  const Shape s = shape_of(pieces_of(cols, type), 4, 8, 4);
   return s.lanes != 0 ? s : widest(cols, type);
 }
 // Backward, 2: the sums of the parameters' gradients take registers as well.  Of fp32 rows of whole pieces 1, where that fills the
@@ -525,9 +528,8 @@ Shape forward_shape(int cols, int type) {
 // and 60001 x 2047, with edges, 281 and 264; 16384 x 4096, bf16: 75 and 73).
 Shape backward_shape(int cols, int type, bool aligned) {
   const int pieces = pieces_of(cols, type);
-  const Shape one = shape_of(pieces, 1, kNormWaves);
-  if (type == FP8GMM_TYPE_FP32 && aligned && one.lanes == 64 && kBackwardThreads % one.threads() == 0) return one;
-  const Shape s = shape_of(pieces, 2, kNormWaves);
+  const Shape one = shape_of(pieces, 1, kNormWaves, 1), s = shape_of(pieces, 2, kNormWaves, 2);
+  if (type == FP8GMM_TYPE_FP32 && aligned && s.lanes != 16 && one.lanes != 0 && kBackwardThreads % one.threads() == 0) return one;
   return s.lanes != 0 ? s : widest(cols, type);
 }
 // Rows of whole pieces on 16 bytes
@@ -539,8 +541,9 @@ bool whole(const void* p, int64_t pitch, int cols, int type) {
 // and without: 16384 x 4096, bf16, forward 43.7 and 50.9 us, backward 73.4 and 71.5; 65536 x 2048, fp32, 194 and 197, 279 and 305;
 // 24576 x 2048, bf16, 37.0 and 38.6, 55.9 and 58.4.
 bool streams(int64_t rows, int cols, int type) { return rows * cols * type_bytes(type) > (int64_t)64 << 20; }
-int mode_of(int cols, int type, bool aligned, bool stream_edges) {
-  return cols < 16 / type_bytes(type) ? kShort : aligned ? kWhole : stream_edges ? kEdgeStream : kEdge;
+// A descriptor is a wavefront's, which has four rows where 16 lanes have one: these have edges, if empty ones.
+int mode_of(int cols, int type, int lanes, bool aligned, bool stream_edges) {
+  return cols < 16 / type_bytes(type) ? kShort : aligned && lanes == 64 ? kWhole : stream_edges ? kEdgeStream : kEdge;
 }
 // Workgroups of a backward pass: partial sums that its parameters' gradients have.  Of aligned rows no fewer than of others.
 int backward_blocks(int rows, int cols, int type, bool aligned) {
@@ -585,18 +588,21 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
   const Shape shape = forward_shape(cols, type);
   const int threads = shape.lanes == 0 ? 0 : std::max(shape.threads(), kForwardThreads / shape.threads() * shape.threads());
   const bool streaming = streams(rows, cols, type);
-  const int mode = mode_of(cols, type, whole(x, ldx, cols, type) && whole(y, cols, cols, type), streaming);
+  const int mode = mode_of(cols, type, shape.lanes, whole(x, ldx, cols, type) && whole(y, cols, cols, type), streaming);
   with_types(type, param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
 #define FP8GMM_LAUNCH(LANES, C, MOST)                                                                                         \
   if (shape.lanes == LANES && shape.pieces == C && threads <= MOST) {                                                         \
     auto* kernel = mode == kEdge         ? &layer_norm_kernel<T, P, LANES, C, kEdge, MOST>                                    \
                    : mode == kEdgeStream ? &layer_norm_kernel<T, P, LANES, C, kEdgeStream, MOST>                              \
-                                         : &layer_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : kShort, MOST>;           \
+                                         : &layer_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge, MOST>; \
     hipLaunchKernelGGL(kernel, dim3(std::min(ceil_div(rows, threads / shape.threads()), kForwardAll / threads)), dim3(threads), \
                        0, s, x, ldx, weight, bias, y, mean, rstd, (int)rows, cols, eps, shape.waves, streaming);              \
   } else
     FP8GMM_LAUNCH(16, 1, 256)
+    FP8GMM_LAUNCH(16, 2, 256)
+    FP8GMM_LAUNCH(16, 3, 256)
+    FP8GMM_LAUNCH(16, 4, 256)
     FP8GMM_LAUNCH(64, 1, 256)
     FP8GMM_LAUNCH(64, 2, 512)
     FP8GMM_LAUNCH(64, 3, 512)
@@ -644,7 +650,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
   const Shape shape = backward_shape(cols, type, aligned);
   const bool streaming = streams(rows, cols, type);
   // of a 16-bit type, edges are written without the hint (16384 x 4093, bf16: 76 us, with it 80; 60001 x 2047, fp32: 286 and 267)
-  const int mode = mode_of(cols, type, aligned, streaming && type == FP8GMM_TYPE_FP32);
+  const int mode = mode_of(cols, type, shape.lanes, aligned, streaming && type == FP8GMM_TYPE_FP32);
   with_types(type, param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
     if (rows > 0) {
@@ -652,11 +658,12 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
   if (shape.lanes == LANES && shape.pieces == C) {                                                                            \
     auto* kernel = mode == kEdge         ? &layer_norm_backward_kernel<T, P, LANES, C, kEdge>                                 \
                    : mode == kEdgeStream ? &layer_norm_backward_kernel<T, P, LANES, C, kEdgeStream>                           \
-                                         : &layer_norm_backward_kernel<T, P, LANES, C, LANES == 64 ? kWhole : kShort>;        \
+                                         : &layer_norm_backward_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge>; \
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBackwardThreads / shape.threads() * shape.threads()), 0, s, dy, ldy, x, ldx, \
                        weight, mean, rstd, dx, part, dweight, dbias, (int)rows, cols, shape.waves, streaming);                 \
   } else
       FP8GMM_LAUNCH(16, 1)
+      FP8GMM_LAUNCH(16, 2)
       FP8GMM_LAUNCH(64, 1)
       FP8GMM_LAUNCH(64, 2)
       if constexpr (T == FP8GMM_TYPE_FP32) {

@@ -88,6 +88,7 @@ SHAPES = [(1, 1), (3, 7), (5, 64), (40, 127), (17, 129), (33, 512), (7, 1000), (
           (300, 4096), (3, 8191), (5, 16384), (700, 768), (5000, 24)]
 # columns on both sides of where a row takes another number of threads, of pieces per thread, or another kernel
 SHAPES += [(37, c + d) for c in (4, 8, 64, 128, 256, 512, 768, 1024, 1536, 2048, 6144, 8192, 16384) for d in (-1, 0, 1, 8)]
+SHAPES += [(1001, c) for c in (192, 193, 384, 385)] + [(70000, 129)]
 
 
 @pytest.mark.parametrize("rows, cols", SHAPES)
