@@ -69,41 +69,53 @@ __device__ __forceinline__ int piece_at(int at, int cols) { return SHORT ? at : 
 template <int V, bool SHORT>
 __device__ __forceinline__ int piece_size(int at, int cols) { return SHORT ? cols - at : V; }
 
-template <int TYPE, typename Id, int LANES, bool SHORT, bool STREAM>   // lanes to a row
+// LANES lanes to a row, PIECES of a row's pieces to each, of as many rows as make kLookupPieces together (2^20 rows of 64 columns,
+// bf16: 50 us, with 4 pieces of one row, most of them the last one again, 93; 2^19 of 256 columns 43 and 55).  A row behind the last
+// one is the last one once more.
+template <int TYPE, typename Id, int LANES, int PIECES, bool SHORT, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_kernel(const Id* __restrict__ ids, int64_t n, const void* __restrict__ weight,
                                                         int64_t table, int cols, float scale, void* __restrict__ y) {
   typedef Elements<TYPE> E;
   typedef typename E::bits bits;
-  constexpr int V = E::kVec, ROWS = 256 / LANES;
+  constexpr int V = E::kVec, ROWS = 256 / LANES, TURNS = kLookupPieces / PIECES;
   const int lane = threadIdx.x % LANES;
-  const int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
-  if (t >= n) return;
-  const int64_t id = ids[t];
-  const bool in = id >= 0 && id < table;
-  const bits* const w = static_cast<const bits*>(weight) + (in ? id : 0) * cols;
-  bits* const out = static_cast<bits*>(y) + t * cols;
-  const int first = blockIdx.y * LANES * kLookupPieces;
-  u32x4 raw[kLookupPieces];
-  if (in) {
+  const int first = blockIdx.y * LANES * PIECES;
+  int64_t row[TURNS], id[TURNS];
 #pragma unroll
-    for (int u = 0; u < kLookupPieces; ++u) {
+  for (int k = 0; k < TURNS; ++k) {
+    row[k] = min((int64_t)blockIdx.x * ROWS * TURNS + k * ROWS + threadIdx.x / LANES, n - 1);
+    id[k] = ids[row[k]];
+  }
+  u32x4 raw[TURNS][PIECES];
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) {
+    const bool in = id[k] >= 0 && id[k] < table;
+    const bits* const w = static_cast<const bits*>(weight) + (in ? id[k] : 0) * cols;
+    if (in) {
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u) {
+        const int at = piece_at<V, SHORT>((first + u * LANES + lane) * V, cols);
+        raw[k][u] = E::load(w + at, piece_size<V, SHORT>(at, cols));
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u) raw[k][u] = u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k)
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) {
       const int at = piece_at<V, SHORT>((first + u * LANES + lane) * V, cols);
-      raw[u] = E::load(w + at, piece_size<V, SHORT>(at, cols));
-    }
-  }
+      if (scale != 1.f) {
+        float f[V];
+        E::unpack(raw[k][u], f);
 #pragma unroll
-  for (int u = 0; u < kLookupPieces; ++u) {
-    const int at = piece_at<V, SHORT>((first + u * LANES + lane) * V, cols);
-    if (!in) raw[u] = u32x4{0u, 0u, 0u, 0u};
-    if (scale != 1.f) {
-      float f[V];
-      E::unpack(raw[u], f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] *= scale;
-      raw[u] = E::pack(f);
+        for (int i = 0; i < V; ++i) f[i] *= scale;
+        raw[k][u] = E::pack(f);
+      }
+      E::template store<STREAM>(static_cast<bits*>(y) + row[k] * cols + at, piece_size<V, SHORT>(at, cols), raw[k][u]);
     }
-    E::template store<STREAM>(out + at, piece_size<V, SHORT>(at, cols), raw[u]);
-  }
 }
 
 // ---- zeros -----------------------------------------------------------------------------------------------------------
@@ -711,22 +723,25 @@ int fp8gmm_embedding(const void* ids, int ids64_, int64_t n, const void* weight,
   if (ids == nullptr || y == nullptr || (weight == nullptr && table > 0)) return FP8GMM_ERR_NULL_POINTER;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t pieces = ceil_div(cols, 16 / type_bytes(type));
-  const int lanes = pieces <= 16 * kLookupPieces ? 16 : 64;
-  const unsigned segments = (unsigned)ceil_div(pieces, lanes * kLookupPieces);
+  const int lanes = pieces <= 16 * kLookupPieces ? 16 : 64, each = pieces <= 16 ? 1 : pieces <= 32 ? 2 : kLookupPieces;
+  const int rows = 256 / lanes * (kLookupPieces / each);   // of a workgroup
+  const unsigned segments = (unsigned)ceil_div(pieces, lanes * each);
   const int64_t slab = 1 << 22;   // tokens of a launch: a grid has fewer than 2^32 threads
   for (int64_t t0 = 0; t0 < n; t0 += slab) {
     const int64_t m = std::min(slab, n - t0);
-    const dim3 grid((unsigned)ceil_div(m, 256 / lanes), segments);
+    const dim3 grid((unsigned)ceil_div(m, rows), segments);
     const void* const from = static_cast<const char*>(ids) + t0 * (ids64 ? 8 : 4);
     void* const to = static_cast<char*>(y) + t0 * cols * type_bytes(type);
-#define FP8GMM_LOOKUP_OF(TYPE, ID)                                                                                          \
-  if (type == TYPE && ids64 == (sizeof(ID) == 8)) {                                                                         \
-    auto* kernel = cols < Elements<TYPE>::kVec ? &embedding_kernel<TYPE, ID, 16, true, false>                               \
-                   : lanes == 16 && stream_out ? &embedding_kernel<TYPE, ID, 16, false, true>                               \
-                   : lanes == 16               ? &embedding_kernel<TYPE, ID, 16, false, false>                              \
-                   : stream_out                ? &embedding_kernel<TYPE, ID, 64, false, true>                               \
-                                               : &embedding_kernel<TYPE, ID, 64, false, false>;                             \
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, static_cast<const ID*>(from), m, weight, table, cols, scale, to);     \
+#define FP8GMM_LOOKUP_AS(TYPE, ID, STREAM)                                                                                 \
+  (cols < Elements<TYPE>::kVec ? &embedding_kernel<TYPE, ID, 16, 1, true, STREAM>                                          \
+   : each == 1                 ? &embedding_kernel<TYPE, ID, 16, 1, false, STREAM>                                         \
+   : each == 2                 ? &embedding_kernel<TYPE, ID, 16, 2, false, STREAM>                                         \
+   : lanes == 16               ? &embedding_kernel<TYPE, ID, 16, kLookupPieces, false, STREAM>                             \
+                               : &embedding_kernel<TYPE, ID, 64, kLookupPieces, false, STREAM>)
+#define FP8GMM_LOOKUP_OF(TYPE, ID)                                                                                         \
+  if (type == TYPE && ids64 == (sizeof(ID) == 8)) {                                                                        \
+    auto* kernel = stream_out ? FP8GMM_LOOKUP_AS(TYPE, ID, true) : FP8GMM_LOOKUP_AS(TYPE, ID, false);                      \
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, static_cast<const ID*>(from), m, weight, table, cols, scale, to);    \
   }
     FP8GMM_LOOKUP_OF(FP8GMM_TYPE_BF16, int64_t)
     FP8GMM_LOOKUP_OF(FP8GMM_TYPE_FP16, int64_t)
@@ -735,6 +750,7 @@ int fp8gmm_embedding(const void* ids, int ids64_, int64_t n, const void* weight,
     FP8GMM_LOOKUP_OF(FP8GMM_TYPE_FP16, int32_t)
     FP8GMM_LOOKUP_OF(FP8GMM_TYPE_FP32, int32_t)
 #undef FP8GMM_LOOKUP_OF
+#undef FP8GMM_LOOKUP_AS
   }
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
