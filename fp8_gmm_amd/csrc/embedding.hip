@@ -31,6 +31,7 @@ constexpr int kSortSteps = 16;                      // .. that hold so many toke
 constexpr int kSortMax = kSortWaves * kSortSteps * 64;
 constexpr int kSortPlaceBits = 14;                  // of a token's place there, packed with its id into 32 bits
 static_assert(kSortMax == 1 << kSortPlaceBits, "a place of the list in its bits");
+constexpr int64_t kSortZeros = 128 << 20;           // the least bytes of a table whose zeros outlast the sort of more than half of those
 constexpr int kPlaceWaves = 16;                     // longer lists: wavefronts of a workgroup, and their tokens per lane
 constexpr int kPlaceSteps = 2;
 constexpr int kPlaceChunk = kPlaceWaves * kPlaceSteps * 64;
@@ -189,8 +190,9 @@ __device__ __forceinline__ int bins_before(int count, int* wave_sums) {
 
 // A list of at most kSortMax tokens and 18 bits of id, by the first workgroup: the entries stay in registers, (id, place)
 // packed into a word, and go through LDS once a pass.  The other workgroups write zeros.  Gradients by this sort and by the next
-// one, whose passes are two launches each: 2048 tokens, table 8000 x 1024, bf16, 21.6 and 28.3 us; 4096, 128000 x 1024, 47.6 and
-// 57.7; 16384, 32000 x 4096, 86 to 103 and 96; 16384, 8000 x 128, 41 and 35, which has few zeros to write meanwhile.
+// one, whose passes are two launches each: 2048 tokens, table 8000 x 1024, bf16, 21.6 and 28.3 us; 4096, 50000 x 1024, 28.6 and 36.9;
+// 8192, 38 and 41; 10000, 42.6 and 43.9; 12000, 8000 x 512, 36.7 and 32.4; 16384, 44 and 35 - but where there are zeros enough to
+// write meanwhile, 32000 x 4096, 90.5 and 102.
 template <typename Id>
 __global__ __launch_bounds__(kSortWaves * 64) void embedding_sort_kernel(const Id* __restrict__ ids, int n, int64_t table,
                                                                          int64_t padding, int passes, int digit_bits,
@@ -694,7 +696,8 @@ struct Layout {   // of the workspace
 Layout layout_of(int64_t n, int64_t table, int cols, int type) {
   Layout l{};
   while (l.key_bits < 31 && (table >> l.key_bits) != 0) ++l.key_bits;   // keys of 0 .. table
-  l.one = n <= kSortMax && l.key_bits + kSortPlaceBits <= 32;
+  l.one = n <= kSortMax && l.key_bits + kSortPlaceBits <= 32 &&
+          (n <= kSortMax / 2 || table * cols * type_bytes(type) >= kSortZeros);
   l.passes = (int)ceil_div(l.key_bits, kMaxDigit);
   l.digit_bits = (int)ceil_div(l.key_bits, std::max(l.passes, 1));
   l.chunk = chunk_of(n, cols, type);

@@ -268,6 +268,13 @@ def test_embedding_against_64_bits(dev, tokens, table, cols, t):
     check_embedding(dev, ids, table, cols, t, scale=(1.0, math.sqrt(cols))[tokens % 2], padding=(None, 0, -1)[tokens % 3], seed=tokens)
 
 
+@pytest.mark.parametrize("tokens, rows", [(9001, 131072), (16383, 200000), (16384, 262143), (16385, 131072)])
+def test_embedding_gradient_of_a_large_table(dev, tokens, rows):
+    """Zeros that outlast the sort beside them."""
+    ids = (torch.rand(tokens, generator=gen(tokens), dtype=torch.float64) ** 2 * rows).long().clamp_(max=rows - 1)
+    check_embedding(dev, ids, rows, 520, "bf16", seed=tokens)
+
+
 @pytest.mark.parametrize("tokens, cols", [(300, 65), (1024, 515), (9000, 700), (30000, 130)])
 def test_embedding_of_one_id_and_of_runs(dev, tokens, cols):
     """All tokens the same, as many runs as tokens, runs of 8, 31, 32 and 33, and ids in falling order."""
