@@ -682,9 +682,9 @@ int few_rows(int64_t n, int64_t table, int cols, int type) {
 }
 
 // Sorted tokens of a wavefront: few where longer chunks would leave the chip short of wavefronts (2048 tokens of 1024 columns, bf16,
-// by 8 tokens 21.6 us, by 32 25; 65536 tokens 75 and 62).
+// by 8 tokens 21.6 us, by 32 25; 32768 tokens 51.5 and 44; 65536 of 256 columns 47 and 41.5; 65536 of 1024 75 and 62).
 int chunk_of(int64_t n, int cols, int type) {
-  return ceil_div(n, kSumMaxChunk) * slices_of(cols, type) >= 4096 ? kSumMaxChunk : kSumMinChunk;
+  return ceil_div(n, kSumMaxChunk) * slices_of(cols, type) >= 1024 ? kSumMaxChunk : kSumMinChunk;
 }
 
 struct Layout {   // of the workspace
