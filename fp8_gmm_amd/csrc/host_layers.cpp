@@ -48,6 +48,7 @@ struct Rows {
   int64_t pitch;
 };
 Rows rows_of(const Tensor& t, int64_t rows, int64_t cols) {
+  if (t.is_contiguous()) return {t, cols};
   Tensor flat = t.reshape({rows, cols});
   if ((cols > 1 && flat.stride(1) != 1) || (rows > 1 && flat.stride(0) < cols)) flat = flat.contiguous();
   return {flat, rows > 1 ? flat.stride(0) : cols};
@@ -55,7 +56,7 @@ Rows rows_of(const Tensor& t, int64_t rows, int64_t cols) {
 
 struct LayerNormBackward : public Node {
   SavedVariable x, weight;
-  Tensor mean, rstd;
+  Tensor stats;   // mean and rstd of every row
   int64_t rows = 0, cols = 0;
   int type = 0, param_type = 0;
   bool bias = false;
@@ -65,8 +66,7 @@ struct LayerNormBackward : public Node {
     const std::lock_guard<std::mutex> lock(mutex_);
     x.reset_data();
     weight.reset_data();
-    mean.reset();
-    rstd.reset();
+    stats.reset();
   }
   variable_list apply(variable_list&& grads) override {
     const std::lock_guard<std::mutex> lock(mutex_);
@@ -92,8 +92,8 @@ struct LayerNormBackward : public Node {
         work = at::empty({(int64_t)bytes}, xs.options().dtype(at::kByte));
       }
       timed("layer_norm_backward", (2 + result[0].defined()) * xs.numel() * (int64_t)xs.element_size(), [&] {
-        check(fp8gmm_layer_norm_backward(ptr<void>(dy.t), dy.pitch, ptr<void>(from.t), from.pitch, ptr<void>(w), ptr<float>(mean),
-                                         ptr<float>(rstd), ptr<void>(result[0]), ptr<void>(result[1]),
+        check(fp8gmm_layer_norm_backward(ptr<void>(dy.t), dy.pitch, ptr<void>(from.t), from.pitch, ptr<void>(w), ptr<float>(stats),
+                                         ptr<float>(stats) + rows, ptr<void>(result[0]), ptr<void>(result[1]),
                                          bias ? ptr<void>(result[2]) : nullptr, rows, (int)cols, type, param_type, ptr<void>(work),
                                          bytes, current_stream(grad.device())));
       });
@@ -124,20 +124,18 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const std::optional<Ten
     const c10::OptionalDeviceGuard guard(x.device());
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias));
     const int64_t cols = x.size(-1), rows = x.numel() / cols;
-    Tensor y, mean, rstd, w;
+    Tensor y, stats, w;
     {
       at::AutoGradMode no_grad(false);
       const Rows from = rows_of(x, rows, cols);
       w = weight.contiguous();
       const Tensor b = bias.defined() ? bias.contiguous() : Tensor();
       y = at::empty(x.sizes(), x.options());
-      if (grad) {
-        mean = at::empty({rows}, x.options().dtype(at::kFloat));
-        rstd = at::empty({rows}, mean.options());
-      }
+      if (grad) stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+      float* const mean = ptr<float>(stats);
       timed("layer_norm", 2 * x.numel() * (int64_t)x.element_size(), [&] {
-        check(fp8gmm_layer_norm(ptr<void>(from.t), from.pitch, ptr<void>(w), ptr<void>(b), ptr<void>(y), ptr<float>(mean),
-                                ptr<float>(rstd), rows, (int)cols, (float)eps, type, param_type, current_stream(x.device())));
+        check(fp8gmm_layer_norm(ptr<void>(from.t), from.pitch, ptr<void>(w), ptr<void>(b), ptr<void>(y), mean,
+                                mean != nullptr ? mean + rows : nullptr, rows, (int)cols, (float)eps, type, param_type, current_stream(x.device())));
       });
     }
     if (grad) {
@@ -147,8 +145,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const std::optional<Ten
       else node->set_next_edges(torch::autograd::collect_next_edges(x, weight));
       node->x = SavedVariable(x, false);
       node->weight = SavedVariable(weight.is_contiguous() ? weight : w, false);
-      node->mean = mean;
-      node->rstd = rstd;
+      node->stats = stats;
       node->rows = rows;
       node->cols = cols;
       node->type = type;
