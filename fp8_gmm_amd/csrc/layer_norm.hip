@@ -15,7 +15,7 @@
 //   1024 x 4096, bf16      7.9            17             out of the caches
 //   16384 x 4096, bf16     43.7   6.1     73.4   5.5
 //   16384 x 4093, bf16     44     6.1     77     5.2     rows that begin at any element
-//   65536 x 2048, fp32     192    5.6     264    6.1
+//   65536 x 2048, fp32     189    5.7     264    6.1
 //   8192 x 16384, bf16     94     5.7     164    4.9     the longest rows that stay in registers
 //   262144 x 256, bf16     44     6.1     72     5.6     four rows to a wavefront
 // A large copy reaches 5.3 here.
@@ -37,7 +37,10 @@ constexpr int kNormSlab = 1 << 21;   // rows of a launch with a workgroup to a r
 constexpr int kBackwardAlone = 2;
 constexpr int kNormWaves = 16;           // the most wavefronts that share a row
 constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, where a row needs no more
-constexpr int kForwardAll = 256 * 2048;  // of its launch: what the compute units hold
+// Threads of its launch: what the compute units hold at a time, which go on to other rows; three times that where they would go on
+// more than five times (16384 x 4096, bf16, 4 turns: 43 us, with twice as many 45, with all rows at once 49; 24576 x 4096, 6 turns: 74,
+// with three times as many 69; 65536 x 2048, 8 turns, 97.5 and 89.6, all at once 101; fp32, 16 turns, 194 and 189).
+constexpr int kForwardAll = 256 * 2048, kForwardTurns = 5, kForwardMore = 3;
 
 // The sum over the THREADS threads of a row, the same in all of them.  `slot`: THREADS / 64 floats of LDS per row that nobody
 // uses before the next barrier but one.
@@ -588,6 +591,10 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
   const Shape shape = forward_shape(cols, type);
   const int threads = shape.lanes == 0 ? 0 : std::max(shape.threads(), kForwardThreads / shape.threads() * shape.threads());
   const bool streaming = streams(rows, cols, type);
+  const auto blocks = [&] {
+    const int groups = ceil_div(rows, threads / shape.threads()), all = kForwardAll / threads;   // rows that a workgroup takes at a time
+    return std::min(groups, groups > kForwardTurns * all ? kForwardMore * all : all);
+  };
   const int mode = mode_of(cols, type, shape.lanes, whole(x, ldx, cols, type) && whole(y, cols, cols, type), streaming);
   with_types(type, param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
@@ -596,8 +603,8 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
     auto* kernel = mode == kEdge         ? &layer_norm_kernel<T, P, LANES, C, kEdge, MOST>                                    \
                    : mode == kEdgeStream ? &layer_norm_kernel<T, P, LANES, C, kEdgeStream, MOST>                              \
                                          : &layer_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge, MOST>; \
-    hipLaunchKernelGGL(kernel, dim3(std::min(ceil_div(rows, threads / shape.threads()), kForwardAll / threads)), dim3(threads), \
-                       0, s, x, ldx, weight, bias, y, mean, rstd, (int)rows, cols, eps, shape.waves, streaming);              \
+    hipLaunchKernelGGL(kernel, dim3(blocks()), dim3(threads), 0, s, x, ldx, weight, bias, y, mean, rstd, (int)rows, cols, eps, \
+                       shape.waves, streaming);                                                                               \
   } else
     FP8GMM_LAUNCH(16, 1, 256)
     FP8GMM_LAUNCH(16, 2, 256)
