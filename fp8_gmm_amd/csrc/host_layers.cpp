@@ -121,9 +121,10 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const std::optional<Ten
     }
     TORCH_CHECK(eps >= 0 && std::isfinite(eps), "fp8_gmm_amd: eps must be a number, not negative");
     check_no_tangent({x, weight, bias}, "layer_norm does");
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    TORCH_CHECK(cols <= 1 << 30 && rows <= INT32_MAX, "fp8_gmm_amd: at most 2^30 columns and 2^31 - 1 rows are supported");
     const c10::OptionalDeviceGuard guard(x.device());
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias));
-    const int64_t cols = x.size(-1), rows = x.numel() / cols;
     Tensor y, stats, w;
     {
       at::AutoGradMode no_grad(false);

@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+from torch._subclasses import FakeTensorMode
 
 import fp8_gmm_amd as pkg
 from fp8_gmm_amd import _lib, backend, moe
@@ -121,3 +122,16 @@ def test_multi_norm_status():
     assert call([(P, P + 4096, 10, 0, 0), (P + 64, P + 4100, 10, 0, 0)], True) == ARGUMENT
     assert call([good], True, max_norm=-1.0) == ARGUMENT and call([good], True, max_norm=float("nan")) == ARGUMENT
     assert L.fp8gmm_multi_norm_workspace_bytes(-1) == 0 and L.fp8gmm_multi_norm_workspace_bytes(0) > 0
+
+
+# Tensors without memory that say they are on a GPU: a refusal ahead of any launch needs no more.
+def fake_gpu(*shape, dtype=torch.bfloat16):
+    return torch.empty(1, dtype=dtype, device="cuda").expand(*shape)
+
+
+@pytest.mark.parametrize("rows, cols", [(1, (1 << 30) + 1), (1, (1 << 32) + 64), (3, 1 << 32), (1 << 31, 8), ((1 << 32) + 1, 8)])
+def test_layer_norm_refuses_sizes_before_they_are_cut_to_32_bits(rows, cols):
+    with FakeTensorMode():
+        x, w = fake_gpu(rows, cols), fake_gpu(cols)
+        with pytest.raises(RuntimeError, match=r"2\^30 columns"):
+            pkg.layer_norm(x, w)
