@@ -72,9 +72,9 @@ void timed(const char* name, int64_t bytes, Launch&& launch) {
 }
 
 // Forward-mode differentiation has no rule here and is refused, as the Python functions refuse it: a tangent that is
-// silently dropped would be a wrong derivative.
+// silently dropped would be a wrong derivative.  Under no_grad too, where torch keeps tangents; where it drops them (inference mode)
+// none is seen here.
 inline void check_no_tangent(at::TensorList inputs, const char* what = "the grouped modules do") {
-  if (!at::GradMode::is_enabled()) return;
   for (const Tensor& t : inputs)
     TORCH_CHECK(!t.defined() || !torch::autograd::isFwGradDefined(t), "fp8_gmm_amd: ", what, " not support forward-mode AD");
 }

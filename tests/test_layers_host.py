@@ -4,10 +4,11 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 from torch._subclasses import FakeTensorMode
 
 import fp8_gmm_amd as pkg
-from fp8_gmm_amd import _lib, backend, moe
+from fp8_gmm_amd import _lib, backend, moe, native
 
 OK, NULL, SHAPE, FORMAT, ALIGN, ARGUMENT, WORKSPACE = 0, -1, -2, -3, -4, -6, -9
 P = 0x10000   # an address that nothing follows
@@ -135,3 +136,27 @@ def test_layer_norm_refuses_sizes_before_they_are_cut_to_32_bits(rows, cols):
         x, w = fake_gpu(rows, cols), fake_gpu(cols)
         with pytest.raises(RuntimeError, match=r"2\^30 columns"):
             pkg.layer_norm(x, w)
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["with gradients", "without"])
+def test_tangents_are_refused_whatever_the_gradient_mode(grad):
+    """torch keeps tangents under ``no_grad``, so a result without one would be a wrong derivative; it drops them in inference mode."""
+    with FakeTensorMode(), fw.dual_level():
+        x, table, ids = torch.empty(3, 16, device="cuda"), torch.empty(5, 16, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+        w = torch.empty(16, device="cuda")
+        dx, dw, dt = (fw.make_dual(t, torch.empty_like(t)) for t in (x, w, table))
+        calls = [lambda: pkg.layer_norm(dx, w), lambda: pkg.layer_norm(x, dw), lambda: pkg.layer_norm(x, w, dw), lambda: pkg.embedding(ids, dt)]
+        for call in calls:
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.inference_mode(), pytest.raises(Exception) as e:   # goes on as far as the missing GPU
+                call()
+            assert "forward-mode" not in str(e.value)
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["with gradients", "without"])
+def test_grouped_modules_refuse_tangents_whatever_the_gradient_mode(grad):
+    with FakeTensorMode(), fw.dual_level():
+        scores = fw.make_dual(torch.empty(3, 8, device="cuda"), torch.empty(3, 8, device="cuda"))
+        with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+            native.route(scores, 2)
