@@ -80,9 +80,9 @@ inline void check_no_tangent(at::TensorList inputs, const char* what = "the grou
 }
 
 // What a backward pass starts from.  A node behind the pass that returned no gradient stands for zeros, as it does for a
-// Python autograd function.
+// Python autograd function.  torch hands gradients on whose sign is a bit beside their memory, of which the kernels see the memory alone.
 inline Tensor gradient_of_result(const Node& node, const variable_list& grads) {
-  return grads[0].defined() ? grads[0].contiguous() : node.input_metadata(0).zeros_like();
+  return grads[0].defined() ? grads[0].resolve_neg() : node.input_metadata(0).zeros_like();
 }
 
 void define_layers(py::module_& m);   // host_layers.cpp

@@ -73,7 +73,7 @@ struct LayerNormBackward : public Node {
     const bool graph = at::GradMode::is_enabled();
     variable_list result(bias ? 3 : 2);
     const Tensor xs = x.unpack(), w = weight.unpack();
-    const Tensor grad = grads[0].defined() ? grads[0] : input_metadata(0).zeros_like();
+    const Tensor grad = gradient_of_result(*this, grads);
     const c10::OptionalDeviceGuard guard(grad.device());
     {
       at::AutoGradMode no_grad(false);
@@ -81,7 +81,8 @@ struct LayerNormBackward : public Node {
                       w.device() == grad.device() && w.numel() == cols && w.is_contiguous() && type_of(w, "weight") == param_type &&
                       type_of(xs, "input") == type,
                   "fp8_gmm_amd: a saved-tensor hook returned another tensor than was saved");
-      const Rows from = rows_of(xs, rows, cols), dy = rows_of(grad, rows, cols);
+      const Rows from = rows_of(xs.resolve_neg(), rows, cols), dy = rows_of(grad, rows, cols);
+      const Tensor params = w.resolve_neg();
       if (task_should_compute_output(0)) result[0] = at::empty(xs.sizes(), xs.options());
       if (task_should_compute_output(1)) result[1] = at::empty({cols}, w.options());
       if (bias && task_should_compute_output(2)) result[2] = at::empty({cols}, w.options());
@@ -92,7 +93,7 @@ struct LayerNormBackward : public Node {
         work = at::empty({(int64_t)bytes}, xs.options().dtype(at::kByte));
       }
       timed("layer_norm_backward", (2 + result[0].defined()) * xs.numel() * (int64_t)xs.element_size(), [&] {
-        check(fp8gmm_layer_norm_backward(ptr<void>(dy.t), dy.pitch, ptr<void>(from.t), from.pitch, ptr<void>(w), ptr<float>(stats),
+        check(fp8gmm_layer_norm_backward(ptr<void>(dy.t), dy.pitch, ptr<void>(from.t), from.pitch, ptr<void>(params), ptr<float>(stats),
                                          ptr<float>(stats) + rows, ptr<void>(result[0]), ptr<void>(result[1]),
                                          bias ? ptr<void>(result[2]) : nullptr, rows, (int)cols, type, param_type, ptr<void>(work),
                                          bytes, current_stream(grad.device())));
@@ -172,9 +173,9 @@ struct EmbeddingBackward : public Node {
   variable_list apply(variable_list&& grads) override {
     const std::lock_guard<std::mutex> lock(mutex_);
     const bool graph = at::GradMode::is_enabled();
-    const Tensor list = ids.unpack();
+    const Tensor list = ids.unpack().resolve_neg();
     variable_list result(1);
-    const Tensor grad = grads[0].defined() ? grads[0] : input_metadata(0).zeros_like();
+    const Tensor grad = gradient_of_result(*this, grads);
     const c10::OptionalDeviceGuard guard(grad.device());
     {
       at::AutoGradMode no_grad(false);

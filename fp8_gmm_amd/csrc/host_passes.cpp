@@ -124,9 +124,9 @@ void check_route(const Route& r, int64_t rows, const Tensor& x) {
   TORCH_CHECK(!r.scatters || list(r.weights, at::kFloat), "fp8_gmm_amd: expected ", rows, " fp32 scatter weights");
 }
 
-// What a row mover takes: contiguous, on 16 bytes.
+// What a row mover takes: contiguous, on 16 bytes, with its sign in its elements.
 Tensor aligned(const Tensor& t) {
-  const Tensor c = t.contiguous();
+  const Tensor c = t.resolve_neg().contiguous();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -170,7 +170,7 @@ struct SavedRoute {
   }
   // The kernels follow addresses, and a saved-tensor hook may return anything.
   Tensor list(SavedVariable& v, at::ScalarType type, const at::Device& device) const {
-    const Tensor t = v.unpack();
+    const Tensor t = v.unpack().resolve_neg();
     TORCH_CHECK(t.scalar_type() == type && t.numel() == rows && t.is_contiguous() && t.device() == device,
                 "fp8_gmm_amd: a saved-tensor hook returned another tensor than was saved");
     return t;
@@ -266,7 +266,7 @@ struct GroupedLinearBackward : public Node {
     variable_list result(route.scatters ? 3 : 2);
     const bool dgrad = task_should_compute_output(0), wgrad = task_should_compute_output(1);
     const bool rgrad = route.want_weights && task_should_compute_output(2);
-    const Tensor grad = gradient_of_result(*this, grads);
+    const Tensor grad = gradient_of_result(*this, grads).contiguous();
     const c10::OptionalDeviceGuard guard(grad.device());
     const RoutedGradient from(route, grad, rgrad);
     const Tensor& dy = from.dy;
@@ -399,7 +399,7 @@ struct GroupedMlpBackward : public Node {
     const bool want_x = dgrad && task_should_compute_output(0);
     const bool want_w = wgrad && (task_should_compute_output(1) || task_should_compute_output(2));
     const bool rgrad = route.want_weights && task_should_compute_output(3);
-    const Tensor grad = gradient_of_result(*this, grads);
+    const Tensor grad = gradient_of_result(*this, grads).contiguous();
     const c10::OptionalDeviceGuard guard(grad.device());
     const RoutedGradient from(route, grad, rgrad);
     const Tensor& dy = from.dy;
@@ -605,7 +605,7 @@ struct GatingBackward : public Node {
       return result;
     }
     const Tensor g = aligned(grad), in = grad_in.defined() ? aligned(grad_in) : Tensor();
-    const Tensor xs = want_weight ? aligned(rows) : Tensor(), ws = want_x ? w.contiguous() : Tensor();
+    const Tensor xs = want_weight ? aligned(rows) : Tensor(), ws = want_x ? w.resolve_neg().contiguous() : Tensor();
     if (want_x) result[0] = at::empty({tokens, hidden}, g.options());
     Tensor work;
     if (want_weight) {
@@ -658,7 +658,7 @@ struct RouteTopKBackward : public Node {
   variable_list apply(variable_list&& grads) override {
     const std::lock_guard<std::mutex> lock(mutex_);
     at::AutoGradMode no_grad(false);
-    const Tensor grad = gradient_of_result(*this, grads), p = probs.unpack(), s = selected.unpack();
+    const Tensor grad = gradient_of_result(*this, grads).contiguous(), p = probs.unpack().resolve_neg(), s = selected.unpack().resolve_neg();
     TORCH_CHECK(p.scalar_type() == at::kFloat && p.numel() == tokens * experts && p.is_contiguous() && p.device() == grad.device() &&
                     s.scalar_type() == at::kLong && s.numel() == tokens * top_k && s.is_contiguous() && s.device() == grad.device(),
                 "fp8_gmm_amd: a saved-tensor hook returned another tensor than was saved");

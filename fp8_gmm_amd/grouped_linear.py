@@ -237,7 +237,7 @@ class _GroupedLinear(torch.autograd.Function):
         meta = ctx.meta
         cumsums, padded_cumsums, padded = ctx.cumsums, ctx.padded_cumsums, ctx.padded
         grad_dtype = to_torch_dtype(get_fp8_te_dtype(ctx.fp8_meta["recipe"], fprop_tensor=False))
-        grad_out = grad_out.contiguous()
+        grad_out = grad_out.resolve_neg().contiguous()   # kernels see a negative view's memory alone
         dev = grad_out.device
 
         if ctx.planned and not wgrad_wants_transposed_gradient(cumsums[-1], ctx.num_groups) \

@@ -238,7 +238,7 @@ class _GroupedMlp(torch.autograd.Function):
         cumsums, padded_cumsums, padded = ctx.cumsums, ctx.padded_cumsums, ctx.padded
         t_bounds = padded_cumsums if padded else cumsums
         grad_dtype = to_torch_dtype(get_fp8_te_dtype(ctx.fp8_meta["recipe"], fprop_tensor=False))
-        grad_out = grad_out.contiguous()
+        grad_out = grad_out.resolve_neg().contiguous()   # kernels see a negative view's memory alone
         dev = grad_out.device
         wgrad = ctx.weight_requires_grad
 

@@ -563,3 +563,42 @@ def test_kernel_timing_sees_the_calls(dev):
         backend.multi_norm([x.grad])
     names = {"layer_norm", "layer_norm_backward", "embedding", "embedding_backward", "multi_clip", "multi_norm"}
     assert names <= set(timing.summary())
+
+
+# ---- gradients and rows of other kinds -------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows, cols, t", [(40, 127, "bf16"), (24, 640, "fp32"), (6, 1, "fp32"), (3, 20001, "bf16")])
+def test_layer_norm_of_negated_gradients(dev, rows, cols, t):
+    """torch hands a gradient on with its sign in a bit beside it (``torch.complex(a, y).conj()`` sends such ones to y): contiguous, strided
+    in a single column, and what a saved-tensor hook returns."""
+    x, w, b, dy = norm_inputs(dev, rows, cols, t, t, True, rows + cols)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    want = torch.autograd.grad(pkg.layer_norm(*leaves), leaves, -dy)
+    wide = torch.empty(rows, 2 * cols, dtype=dy.dtype, device=dev)
+    wide[:, ::2] = dy
+    for up in (torch._neg_view(dy), torch._neg_view(wide)[:, ::2]):
+        assert up.is_neg()
+        for a, c in zip(torch.autograd.grad(pkg.layer_norm(*leaves), leaves, up), want):
+            assert torch.equal(a, c)
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: -v, torch._neg_view):
+        y = pkg.layer_norm(*leaves)
+    for a, c in zip(torch.autograd.grad(y, leaves, -dy), want):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("tokens", [1, 50, 3000])
+def test_embedding_of_negated_gradients(dev, tokens):
+    table = torch.randn(60, 24, device=dev, requires_grad=True)
+    ids = torch.randint(0, 60, (tokens,), generator=gen(tokens)).to(dev)
+    dy = torch.randn(tokens, 24, generator=gen(tokens)).to(dev)
+    (want,) = torch.autograd.grad(pkg.embedding(ids, table, 3.0), table, -dy)
+    (got,) = torch.autograd.grad(pkg.embedding(ids, table, 3.0), table, torch._neg_view(dy))
+    assert torch.equal(got, want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: -v, torch._neg_view):
+        y = pkg.embedding(ids, table, 3.0)
+    (got,) = torch.autograd.grad(y, table, -dy)
+    assert torch.equal(got, want)
+    single = torch.randn(60, 1, device=dev, requires_grad=True)
+    up = torch.complex(torch.randn(tokens, 1, device=dev), torch.randn(tokens, 1, device=dev))
+    (got,) = torch.autograd.grad(torch.complex(torch.zeros(tokens, 1, device=dev), pkg.embedding(ids, single)).conj(), single, up)
+    (want,) = torch.autograd.grad(pkg.embedding(ids, single), single, (-up.imag).clone())
+    assert torch.equal(got, want)

@@ -1191,3 +1191,25 @@ def test_a_timed_backward_pass_keeps_the_policy_of_its_forward_pass(dev, kind):
             out.sum().backward()
         forms = timing.summary()["grouped_gemm"]["forms"]
         assert forms and all(("128 x 128 tiles" in f) == (tile == "128") for f in forms), forms
+
+
+@pytest.mark.parametrize("kind", ["linear", "mlp"])
+@pytest.mark.parametrize("planned", [True, False])
+def test_negated_gradients_keep_their_sign(dev, kind, planned):
+    """A gradient whose sign is a bit beside it (torch's negative views) is that of its values."""
+    pkg = _pkg()
+    e, h, f, sizes = 3, 160, 336, [70, 0, 45]
+    g = gen(99)
+    x = randn_bf16((sum(sizes), h), g).to(dev)
+    dy = randn_bf16((sum(sizes), f if kind == "linear" else h), g, 1e-2).to(dev)
+    make = pkg.GroupedLinear if kind == "linear" else pkg.GroupedMlp
+    state, res = None, []
+    for up in (-dy, torch._neg_view(dy)):
+        module = make(h, f, e, torch.bfloat16, device=dev, planned_passes=planned)
+        state = module.state_dict() if state is None else state
+        module.load_state_dict(state)
+        xi = x.clone().requires_grad_()
+        module(xi, torch.tensor(sizes)).backward(up)
+        res.append([xi.grad] + [p.grad for p in module.parameters()])
+    for a, b in zip(*res):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))

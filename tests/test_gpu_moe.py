@@ -784,3 +784,36 @@ def test_native_gating_differentiates_twice_and_is_timed(dev):
             out.backward(dy)
         grads.append([x.grad.clone()] + [p.grad.clone() for p in module.parameters()])
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_negated_gradients_keep_their_sign(dev, native):
+    """Gating, routing, gather and scatter take a gradient whose sign is a bit beside it (torch's negative views) for its values."""
+    ops = _ops()
+    tokens, hidden, experts, top_k = 130, 64, 8, 2
+    gen = torch.Generator().manual_seed(17)
+    x, rows = (torch.randn(n, hidden, generator=gen).to(torch.bfloat16).to(dev).requires_grad_() for n in (tokens, tokens * top_k))
+    linear = torch.nn.Linear(hidden, experts, bias=False, dtype=torch.bfloat16, device=dev)
+    scores = torch.randn(tokens, experts, generator=gen).to(dev).requires_grad_()
+    share = torch.rand(tokens * top_k, generator=gen).to(dev).requires_grad_()
+    top_expert = torch.randint(0, experts, (tokens * top_k,), generator=gen).int().to(dev)
+    indices, bin_ids, bins, _ = ops.indices_and_bins(top_expert, 3, experts)
+    up = [torch.randn(s, generator=gen).to(dev) for s in ((tokens, experts), (tokens, hidden), (tokens, top_k), (tokens * top_k, hidden))]
+    up = [up[0].to(torch.bfloat16), up[1].to(torch.bfloat16), up[2], up[3].to(torch.bfloat16)]
+    hooks = contextlib.nullcontext() if native else torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)
+
+    def gradients(sign):
+        with hooks:
+            logits, again = ops.gating(linear, x)
+            got = torch.autograd.grad((logits, again), (x, linear.weight), (sign(up[0]), sign(up[1])))
+            got += torch.autograd.grad(ops.topk(scores, top_k)[0], scores, sign(up[2]))
+            if native:
+                from fp8_gmm_amd import native as host
+
+                weights = host.route(scores, top_k)[0]
+                got += torch.autograd.grad(weights, scores, sign(up[2]).view(weights.shape))
+            got += torch.autograd.grad(ops.gather(x, indices, bin_ids, bins, top_k), x, sign(up[3]))
+            return got + torch.autograd.grad(ops.scatter(rows, indices, bin_ids, share, bins, top_k), (rows, share), sign(up[1]))
+
+    for a, c in zip(gradients(torch._neg_view), gradients(torch.neg)):
+        assert torch.equal(a, c)
