@@ -423,7 +423,8 @@ __global__ __launch_bounds__(kNormLongThreads) void layer_norm_long_dx_kernel(
       pw.get(fw);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float z = (fx[i] - mean) * rstd, g = fy[i] * fw[i];
+        // behind the row's end x is a zero, whose z is minus the mean times rstd, be that infinite
+        const float z = i < n ? (fx[i] - mean) * rstd : 0.f, g = fy[i] * fw[i];
         s1 += g;
         s2 = __builtin_fmaf(g, z, s2);
         fx[i] = rstd * (g - m1 - z * m2);

@@ -602,3 +602,22 @@ def test_embedding_of_negated_gradients(dev, tokens):
     (got,) = torch.autograd.grad(torch.complex(torch.zeros(tokens, 1, device=dev), pkg.embedding(ids, single)).conj(), single, up)
     (want,) = torch.autograd.grad(pkg.embedding(ids, single), single, (-up.imag).clone())
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("t, cols", [("bf16", 20001), ("fp32", 20001), ("fp32", 20000)])
+def test_layer_norm_of_long_rows_of_equal_values(dev, t, cols):
+    """z is 0 although the mean times rstd is infinite, behind a row's end too.  Powers of two: the sum of a row is exact."""
+    x = torch.full((3, cols), 2.0 ** 112, dtype=TYPES[t], device=dev)
+    eps = 1e-12
+    g = gen(cols)
+    w, b = (torch.randn(cols, generator=g).to(TYPES[t]).to(dev) for _ in range(2))
+    dy = torch.randn(3, cols, generator=g).to(TYPES[t]).to(dev)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    y = pkg.layer_norm(*leaves, eps)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    assert torch.equal(y, b.expand(3, -1)) and not dw.any()
+    h = dy.double() * w.double()
+    want = (h - h.mean(1, keepdim=True)) / math.sqrt(eps)
+    bound = 2 * (64 + cols / 1024) * U * (h.abs() + h.abs().mean(1, keepdim=True)) / math.sqrt(eps)
+    assert_within(dx, want, half_step(dx.dtype) * (want.abs() + bound) + bound, "dx")
+    assert_within(db, dy.double().sum(0), half_step(db.dtype) * dy.double().sum(0).abs() + 8 * U * dy.double().abs().sum(0) + smallest(db.dtype), "db")
