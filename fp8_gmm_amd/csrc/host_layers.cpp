@@ -269,6 +269,7 @@ int64_t bytes_of(const std::vector<Tensor>& tensors) {
 Tensor multi_norm(const std::vector<Tensor>& tensors) {
   py::gil_scoped_release no_gil;
   check_list(tensors, "multi_norm");
+  check_no_tangent(tensors, "multi_norm does");
   at::AutoGradMode no_grad(false);
   const at::Device device = tensors[0].device();
   const c10::OptionalDeviceGuard guard(device);
@@ -348,6 +349,8 @@ Tensor multi_clip(const std::vector<Tensor>& tensors, const std::vector<Tensor>&
   check_list(tensors, "multi_clip");
   TORCH_CHECK(outs.size() == tensors.size(), "fp8_gmm_amd: multi_clip needs a result for every tensor");
   check_list(outs, "multi_clip");
+  check_no_tangent(tensors, "multi_clip does");
+  check_no_tangent(outs, "multi_clip does");
   TORCH_CHECK(outs[0].device() == tensors[0].device(), "fp8_gmm_amd: all tensors of one call must live on the same device");
   TORCH_CHECK(max_norm >= 0, "fp8_gmm_amd: max_norm must be a number, not negative");
   for (size_t i = 0; i < tensors.size(); ++i) {

@@ -15,13 +15,7 @@ forward-mode differentiation, ``torch.func`` transforms and tracing are refused.
 import torch
 
 from . import native
-from .backend import _fail
-
-
-def _check_unwrapped(name):
-    """The kernels follow addresses: what a transform or a tracer puts in a tensor's place has none."""
-    if torch._C._functorch.peek_interpreter_stack() is not None or torch.jit.is_tracing():
-        _fail(f"fp8_gmm_amd: {name} does not run under torch.func transforms or tracing")
+from .backend import _check_unwrapped
 
 
 def layer_norm(x, weight, bias=None, eps=1e-5):

@@ -288,3 +288,27 @@ def test_refusals(dev):
     with pytest.raises(RuntimeError, match="at least one"):
         backend.multi_norm([])
     assert (a == 1).all() and (b == 1).all() and (flat == 1).all()
+
+
+def test_transforms_tangents_and_tracing_are_refused(dev):
+    """A result without its derivative would be a wrong one."""
+    t, out = torch.ones(16, device=dev), torch.empty(16, device=dev)
+    calls = {"multi_norm": lambda v: backend.multi_norm([out, v]), "multi_clip": lambda v: backend.multi_clip([out, v], [out, v], 1.0),
+             "into another": lambda v: backend.multi_clip([out, v], [out, t], 1.0)}
+    for name, call in calls.items():
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.func.vmap(call)(torch.ones(3, 16, device=dev))
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.func.grad(lambda v: call(v).sum())(t)
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.jit.trace(call, (t,), check_trace=False)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with torch.autograd.forward_ad.dual_level(), mode():
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t)))
+    leaf = torch.nn.Parameter(torch.ones(16, device=dev))
+    with torch.autograd.forward_ad.dual_level():
+        leaf.grad = torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            pkg.clip_grad_norm_([leaf], 1.0)
+    assert (t == 1).all()
