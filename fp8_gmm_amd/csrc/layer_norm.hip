@@ -597,6 +597,7 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
     return std::min(groups, groups > kForwardTurns * all ? kForwardMore * all : all);
   };
   const int mode = mode_of(cols, type, shape.lanes, whole(x, ldx, cols, type) && whole(y, cols, cols, type), streaming);
+  bool known = true;   // a row's share of the registers that no launch below is for would leave y unwritten
   with_types(type, param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
 #define FP8GMM_LAUNCH(LANES, C, MOST)                                                                                         \
@@ -611,12 +612,13 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
     FP8GMM_LAUNCH(16, 2, 256)
     FP8GMM_LAUNCH(16, 3, 256)
     FP8GMM_LAUNCH(16, 4, 256)
-    FP8GMM_LAUNCH(64, 1, 256)
-    FP8GMM_LAUNCH(64, 2, 512)
+    FP8GMM_LAUNCH(64, 2, 512)   // (one piece to each of 64 lanes is 16 lanes' share)
     FP8GMM_LAUNCH(64, 3, 512)
     FP8GMM_LAUNCH(64, 4, 512)
     if constexpr (T == FP8GMM_TYPE_FP32) {
-      FP8GMM_LAUNCH(64, 4, 1024) {}
+      FP8GMM_LAUNCH(64, 4, 1024) known = shape.lanes == 0;
+    } else {
+      known = shape.lanes == 0;
     }
 #undef FP8GMM_LAUNCH
     for (int64_t r0 = 0; shape.lanes == 0 && r0 < rows; r0 += kNormSlab) {
@@ -627,6 +629,7 @@ int fp8gmm_layer_norm(const void* x, int64_t ldx, const void* weight, const void
                          rstd != nullptr ? rstd + r0 : nullptr, cols, eps);
     }
   });
+  if (!known) return FP8GMM_ERR_LAUNCH;
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
@@ -659,13 +662,15 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
   const bool streaming = streams(rows, cols, type);
   // of a 16-bit type, edges are written without the hint (16384 x 4093, bf16: 76 us, with it 80; 60001 x 2047, fp32: 286 and 267)
   const int mode = mode_of(cols, type, shape.lanes, aligned, streaming && type == FP8GMM_TYPE_FP32);
+  bool known = true;
   with_types(type, param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
+    constexpr int kStreamed = T == FP8GMM_TYPE_FP32 ? kEdgeStream : kEdge;
     if (rows > 0) {
 #define FP8GMM_LAUNCH(LANES, C)                                                                                               \
   if (shape.lanes == LANES && shape.pieces == C) {                                                                            \
     auto* kernel = mode == kEdge         ? &layer_norm_backward_kernel<T, P, LANES, C, kEdge>                                 \
-                   : mode == kEdgeStream ? &layer_norm_backward_kernel<T, P, LANES, C, kEdgeStream>                           \
+                   : mode == kEdgeStream ? &layer_norm_backward_kernel<T, P, LANES, C, kStreamed>                             \
                                          : &layer_norm_backward_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge>; \
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBackwardThreads / shape.threads() * shape.threads()), 0, s, dy, ldy, x, ldx, \
                        weight, mean, rstd, dx, part, dweight, dbias, (int)rows, cols, shape.waves, streaming);                 \
@@ -675,7 +680,9 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
       FP8GMM_LAUNCH(64, 1)
       FP8GMM_LAUNCH(64, 2)
       if constexpr (T == FP8GMM_TYPE_FP32) {
-        FP8GMM_LAUNCH(64, 4) {}
+        FP8GMM_LAUNCH(64, 4) known = shape.lanes == 0;
+      } else {
+        known = shape.lanes == 0;
       }
 #undef FP8GMM_LAUNCH
       if (shape.lanes == 0) {
@@ -695,6 +702,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
       hipLaunchKernelGGL((layer_norm_params_kernel<P>), dim3(ceil_div(cols, 64), dbias != nullptr ? 2 : 1), dim3(1024), 0, s,
                          part, blocks, cols, dweight, dbias);
   });
+  if (!known) return FP8GMM_ERR_LAUNCH;
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 

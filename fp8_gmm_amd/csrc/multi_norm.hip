@@ -42,6 +42,7 @@ constexpr int kWiderParts = 2;
 // 52 us, without 58).  Results are written with it where whoever reads them does not find them there (290 MB clipped: 151 us,
 // without 182).
 constexpr int64_t kStreamTwice = (int64_t)512 << 20, kStreamOnce = (int64_t)32 << 20, kStreamOut = (int64_t)64 << 20;
+static_assert(kStreamTwice >= kStreamOut, "results are no fewer bytes than what is read: the hint on the reads means both");
 
 struct Entry {
   const void* in;
@@ -605,10 +606,10 @@ int multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float*
   if (finished != nullptr) launch_finish(list, max_norm, norm, finished, workspace, s);
   const auto launch = [&](auto parts) {
     constexpr int PARTS = decltype(parts)::value;
-    auto* kernel = list.direct() ? in ? out ? &multi_clip_kernel<true, true, true, PARTS> : &multi_clip_kernel<true, true, false, PARTS>
+    auto* kernel = list.direct() ? in    ? &multi_clip_kernel<true, true, true, PARTS>
                                    : out ? &multi_clip_kernel<true, false, true, PARTS>
                                          : &multi_clip_kernel<true, false, false, PARTS>
-                   : in ? out ? &multi_clip_kernel<false, true, true, PARTS> : &multi_clip_kernel<false, true, false, PARTS>
+                   : in  ? &multi_clip_kernel<false, true, true, PARTS>
                    : out ? &multi_clip_kernel<false, false, true, PARTS>
                          : &multi_clip_kernel<false, false, false, PARTS>;
     hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(list.chunks, kClipBlocks / PARTS) * PARTS), dim3(kThreads), 0, s, part,
