@@ -30,7 +30,7 @@ namespace {
 constexpr int kBackwardThreads = 1024;   // of a workgroup of the backward pass: as many rows at a time as fit, since every workgroup
 constexpr int kBackwardBlocks = 256;     // leaves one partial sum of the parameters' gradients in memory; one per compute unit
 constexpr int kNormLongThreads = 1024;
-constexpr int kNormSlab = 1 << 21;   // rows of a launch with a workgroup to a row: a grid has fewer than 2^32 threads
+constexpr int kNormSlab = 1 << 16;   // rows of a launch with a workgroup to a row, 2 GB at least: a grid has fewer than 2^32 threads
 
 // So many turns of one workgroup take less than a second launch for the sums of several: 32 x 1024, bf16, 2 turns: 8.6 us, by two
 // workgroups 10.9; 64 x 1024, 4 turns: 12.0 and 11.0; 16 x 4096, 4 turns: 14.5 and 11.3.

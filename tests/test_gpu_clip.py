@@ -312,3 +312,29 @@ def test_transforms_tangents_and_tracing_are_refused(dev):
         with pytest.raises(RuntimeError, match="forward-mode"):
             pkg.clip_grad_norm_([leaf], 1.0)
     assert (t == 1).all()
+
+
+@pytest.mark.parametrize("wider", [False, True], ids=["in place", "into fp32"])
+def test_workgroups_with_several_chunks_cross_the_tensors_borders(dev, wider):
+    """More chunks of 16 KB than the scaling has workgroups (2^20, or 2^19 by halves into fp32): some walk back over several, and over
+    short tensors between long ones.  Every tensor holds one value, so its results are all the same bits."""
+    long = 8192 * (((1 << 20) + (1 << 18)) // (16 if wider else 8)) + 4321
+    sizes = [n for k in range(8) for n in [long + k] + [1 + (977 * (11 * k + j)) % 20000 for j in range(11)]]
+    flat = torch.empty(sum(sizes), dtype=BF16, device=dev)
+    grads = list(flat.split(sizes))
+    values = [2.0 ** -12 * (1 + i % 7) for i in range(len(sizes))]
+    for t, v in zip(grads, values):
+        t.fill_(v)
+    assert sum((2 * n + 16383) // 16384 for n in sizes) > ((1 << 20) if not wider else 1 << 19)
+    outs = list(torch.full((sum(sizes),), 7.0, device=dev).split(sizes)) if wider else grads
+    norm = math.sqrt(math.fsum(n * v * v for n, v in zip(sizes, values)))
+    got = backend.multi_clip(grads, outs, 0.3 * norm)
+    assert abs(got.item() - norm) <= 1.01 * U * norm
+    factor = 0.3 * norm / (norm + 1e-6)
+    for t, v in zip(outs, values):
+        check_scaled([t[:1]], [torch.tensor([v], device=dev)], factor)
+        bits = t.view(torch.int32 if wider else torch.int16)
+        first = bits[0].item()
+        assert all(bool((p == first).all()) for p in bits.split(1 << 28))
+    if wider:
+        assert all(bool((p == v).all()) for t, v in zip(grads, values) for p in t.split(1 << 28)), "the tensors were written"

@@ -621,3 +621,64 @@ def test_layer_norm_of_long_rows_of_equal_values(dev, t, cols):
     bound = 2 * (64 + cols / 1024) * U * (h.abs() + h.abs().mean(1, keepdim=True)) / math.sqrt(eps)
     assert_within(dx, want, half_step(dx.dtype) * (want.abs() + bound) + bound, "dx")
     assert_within(db, dy.double().sum(0), half_step(db.dtype) * dy.double().sum(0).abs() + 8 * U * dy.double().abs().sum(0) + smallest(db.dtype), "db")
+
+
+# ---- launches that large calls alone reach ---------------------------------------------------------------------------
+@pytest.mark.parametrize("rows, cols, t, p", [(70000, 513, "fp32", "fp32"), (70000, 1027, "bf16", "fp32"), (70001, 1025, "fp16", "fp16"),
+                                              (300001, 57, "fp32", "fp32"), (140001, 129, "fp32", "fp32"), (140001, 253, "fp32", "fp32"),
+                                              (140001, 259, "bf16", "bf16"), (300001, 128, "bf16", "bf16"), (20000, 1024, "fp32", "fp32"),
+                                              (1100, 16001, "fp32", "fp32"), (2101, 16379, "bf16", "bf16"), (5000, 8196, "fp32", "fp32")])
+def test_layer_norm_of_results_that_outgrow_the_cache(dev, rows, cols, t, p):
+    """Results over 64 MB are written with another hint, by launches of their own: rows with edges of 16 and of 64 lanes, of one to 16
+    wavefronts, and aligned ones."""
+    g = torch.Generator(device=dev).manual_seed(rows + cols)
+    x = (torch.randn(rows, cols, generator=g, device=dev) * 2 + torch.randn(1, cols, generator=g, device=dev)).to(TYPES[t])
+    w = (1 + 0.2 * torch.randn(cols, generator=g, device=dev)).to(TYPES[p])
+    b = (0.3 * torch.randn(cols, generator=g, device=dev)).to(TYPES[p])
+    dy = (0.1 * torch.randn(rows, cols, generator=g, device=dev)).to(TYPES[t])
+    assert x.numel() * x.element_size() > 64 << 20
+    check_norm(x, w, b, dy, what=f"{rows} x {cols}")
+
+
+def test_layer_norm_of_long_rows_by_several_launches(dev):
+    """Rows past the registers, 2^16 of them to a launch, and more elements than 32 bits count."""
+    rows, cols = (1 << 17) + 37, 16392
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=dev).normal_()
+    dy = torch.empty_like(x).normal_()
+    w = torch.rand(cols, device=dev) + 0.5
+    xs, ws = x.requires_grad_(), w.requires_grad_()
+    y = pkg.layer_norm(xs, ws)
+    dx, dw = torch.autograd.grad(y, (xs, ws), dy)
+    total, bound, size = (torch.zeros(cols, dtype=torch.float64, device=dev) for _ in range(3))
+    for xp, dp, yp, gp in zip(*(v.detach().split(1 << 13) for v in (x, dy, y, dx))):
+        want, tol = norm_reference(xp, w.detach(), None, dp, 1e-5)
+        for a, v, e, name in ((yp, want[0], tol[0], "y"), (gp, want[1], tol[1], "dx")):
+            assert_within(a, v, e + half_step(a.dtype) * (v.abs() + e) + smallest(a.dtype), name)
+        total += want[2]
+        bound += tol[2]
+        size += tol[2] / (64 * U)   # at least the magnitudes that were added
+    # a thread adds up a 64th of the rows
+    assert_within(dw, total, bound + rows / 64 * U * size + half_step(dw.dtype) * total.abs(), "dw")
+
+
+@pytest.mark.parametrize("tokens, table, cols, t, ids", [((1 << 22) + 37, 60000, 9, "bf16", torch.int64), ((1 << 22) + 37, 900, 9, "fp16", torch.int32),
+                                                         ((1 << 23) + 5, 1000, 3, "fp32", torch.int64), ((1 << 22) + 3, 5000, 5, "fp32", torch.int32),
+                                                         (300001, 5000, 136, "bf16", torch.int32), (140001, 700, 264, "fp16", torch.int64),
+                                                         (16411, 9000, 4104, "bf16", torch.int64), (9001, 9000, 4099, "fp32", torch.int32)])
+def test_embedding_of_results_that_outgrow_the_cache(dev, tokens, table, cols, t, ids):
+    """Results over 64 MB are written with another hint; more than 2^22 tokens take several launches.  Copied rows are the same bits."""
+    g = torch.Generator(device=dev).manual_seed(tokens)
+    w = torch.randn(table, cols, generator=g, device=dev).to(TYPES[t]).requires_grad_()
+    at = torch.randint(-2, table + 2, (tokens,), generator=g, device=dev).to(ids)   # some outside the table
+    inside = (at >= 0) & (at < table)
+    rows = torch.where(inside, at, 0).long()
+    y = pkg.embedding(at, w)
+    assert y.numel() * y.element_size() > 64 << 20
+    assert torch.equal(y, w.detach()[rows].where(inside[:, None], torch.zeros((), dtype=w.dtype, device=dev)))
+    assert torch.equal(pkg.embedding(at, w.detach(), 2.0), y.detach() * 2)
+    dy = torch.randn(tokens, cols, generator=g, device=dev).to(TYPES[t])
+    (dw,) = torch.autograd.grad(y, w, dy)
+    total = torch.zeros(table, cols, dtype=torch.float64, device=dev).index_add_(0, rows[inside], dy[inside].double())
+    size = torch.zeros_like(total).index_add_(0, rows[inside], dy[inside].double().abs())
+    count = torch.bincount(rows[inside], minlength=table)[:, None]
+    assert_within(dw, total, half_step(w.dtype) * total.abs() + (count + 4) * 2 * U * size + smallest(w.dtype), "dw")
