@@ -35,12 +35,6 @@ def _fail(msg):
     raise RuntimeError(msg)
 
 
-def _check_unwrapped(name):
-    """The kernels follow addresses: what a transform or a tracer puts in a tensor's place has none."""
-    if torch._C._functorch.peek_interpreter_stack() is not None or torch.jit.is_tracing():
-        _fail(f"fp8_gmm_amd: {name} does not run under torch.func transforms or tracing")
-
-
 class _on_device:
     """``torch.cuda.device(device)``, entered only when `device` is not the current one already (every launch sits
     in such a block, and the context manager costs the host several microseconds)."""
@@ -693,7 +687,6 @@ def multi_norm(tensors):
     """The 2-norm of all elements of all ``tensors`` together, a float32 scalar on their device: bfloat16, float16 and float32 in
     any mixture and of any shapes and strides, squared and added up in float64.  The same bits from call to call.  No gradients are
     taken: the norm is a constant to autograd, of tensors that require a gradient too."""
-    _check_unwrapped("multi_norm")
     flush_uploads()   # a queued launch may write what is read here
     return native.multi_norm(list(tensors))
 
@@ -702,7 +695,6 @@ def multi_clip(tensors, outs, max_norm):
     """``outs[i] = tensors[i] * min(1, max_norm / (norm + 1e-6))`` with the norm of ``multi_norm``, which is returned.  A result has
     its tensor's shape, and its type or float32.  It may be its tensor itself (in place: not written again where the factor is
     1), but may share memory with nothing else of the call.  No gradients are taken."""
-    _check_unwrapped("multi_clip")
     flush_uploads()
     return native.multi_clip(list(tensors), list(outs), max_norm)
 

@@ -3,15 +3,18 @@
 #pragma once
 
 #include <torch/csrc/autograd/VariableTypeUtils.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/Event.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 
@@ -73,10 +76,18 @@ void timed(const char* name, int64_t bytes, Launch&& launch) {
 
 // Forward-mode differentiation has no rule here and is refused, as the Python functions refuse it: a tangent that is
 // silently dropped would be a wrong derivative.  Under no_grad too, where torch keeps tangents; where it drops them (inference mode)
-// none is seen here.
+// none is seen here.  Outside of a level of forward mode there are none to ask the tensors for, which takes a while where they are views.
 inline void check_no_tangent(at::TensorList inputs, const char* what = "the grouped modules do") {
+  if (torch::autograd::ForwardADLevel::try_get_by_idx(0) == nullptr) return;
   for (const Tensor& t : inputs)
     TORCH_CHECK(!t.defined() || !torch::autograd::isFwGradDefined(t), "fp8_gmm_amd: ", what, " not support forward-mode AD");
+}
+
+// The kernels follow addresses: what a transform or a tracer puts in a tensor's place has none.  (A transform under way shows by the
+// dispatch key of its layers.)
+inline void check_unwrapped(const char* name) {
+  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(at::DispatchKey::FuncTorchDynamicLayerFrontMode) && !torch::jit::tracer::isTracing(),
+              "fp8_gmm_amd: ", name, " does not run under torch.func transforms or tracing");
 }
 
 // What a backward pass starts from.  A node behind the pass that returned no gradient stands for zeros, as it does for a

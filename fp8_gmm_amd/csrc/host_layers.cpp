@@ -107,6 +107,7 @@ struct LayerNormBackward : public Node {
 Tensor layer_norm(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_, double eps) {
   return with_python_errors([&] {
     py::gil_scoped_release no_gil;
+    check_unwrapped("layer_norm");
     const Tensor bias = bias_.value_or(Tensor());
     check_plain(x, "the input of layer_norm");
     check_plain(weight, "weight");
@@ -200,6 +201,7 @@ struct EmbeddingBackward : public Node {
 Tensor embedding(const Tensor& ids_, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
   return with_python_errors([&] {
     py::gil_scoped_release no_gil;
+    check_unwrapped("embedding");
     check_plain(ids_, "ids");
     check_plain(weight, "weight");
     TORCH_CHECK(ids_.scalar_type() == at::kLong || ids_.scalar_type() == at::kInt, "fp8_gmm_amd: ids must be int64 or int32, got ",
@@ -268,6 +270,7 @@ int64_t bytes_of(const std::vector<Tensor>& tensors) {
 
 Tensor multi_norm(const std::vector<Tensor>& tensors) {
   py::gil_scoped_release no_gil;
+  check_unwrapped("multi_norm");
   check_list(tensors, "multi_norm");
   check_no_tangent(tensors, "multi_norm does");
   at::AutoGradMode no_grad(false);
@@ -346,6 +349,7 @@ void check_copied(const std::vector<Tensor>& tensors, const std::vector<Tensor>&
 
 Tensor multi_clip(const std::vector<Tensor>& tensors, const std::vector<Tensor>& outs, double max_norm) {
   py::gil_scoped_release no_gil;
+  check_unwrapped("multi_clip");
   check_list(tensors, "multi_clip");
   TORCH_CHECK(outs.size() == tensors.size(), "fp8_gmm_amd: multi_clip needs a result for every tensor");
   check_list(outs, "multi_clip");

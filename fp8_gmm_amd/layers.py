@@ -15,7 +15,6 @@ forward-mode differentiation, ``torch.func`` transforms and tracing are refused.
 import torch
 
 from . import native
-from .backend import _check_unwrapped
 
 
 def layer_norm(x, weight, bias=None, eps=1e-5):
@@ -24,7 +23,6 @@ def layer_norm(x, weight, bias=None, eps=1e-5):
     are neighbours; others are copied first.  Differentiable in all three; a row whose variance is zero has ``rstd = 1 /
     sqrt(eps)``, one whose sum or squares pass float32's range is no number or its bias, and the rows of an empty ``x`` leave
     gradients of zeros."""
-    _check_unwrapped("layer_norm")
     return native.layer_norm(x, weight, bias, eps)
 
 
@@ -33,7 +31,6 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     table's type.  ``ids``: int64 or int32.  An id outside the table gives a row of zeros and takes no gradient (a table that is sharded by
     rows is looked up with ``ids - first_row`` and its results added up); the row ``padding_idx`` is read like any other and
     takes no gradient.  The table's gradient is dense, summed in float32 over every row's tokens in a fixed order."""
-    _check_unwrapped("embedding")
     return native.embedding(ids, weight, scale, padding_idx)
 
 

@@ -160,3 +160,15 @@ def test_grouped_modules_refuse_tangents_whatever_the_gradient_mode(grad):
         scores = fw.make_dual(torch.empty(3, 8, device="cuda"), torch.empty(3, 8, device="cuda"))
         with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
             native.route(scores, 2)
+
+
+def test_transforms_and_tracing_are_refused():
+    x, w, ids = torch.ones(3, 8), torch.ones(8), torch.zeros(2, dtype=torch.int64)
+    for name, call in (("layer_norm", lambda t: pkg.layer_norm(t, w)), ("embedding", lambda t: pkg.embedding(ids, t[None])),
+                       ("multi_norm", lambda t: backend.multi_norm([t])), ("multi_clip", lambda t: backend.multi_clip([t], [t], 1.0))):
+        for transformed in (lambda: torch.func.vmap(call)(x), lambda: torch.func.grad(lambda t: call(t).sum())(w),
+                            lambda: torch.func.jvp(call, (w,), (w,)), lambda: torch.jit.trace(call, (w,), check_trace=False)):
+            with pytest.raises(RuntimeError, match=f"{name} does not run under torch.func transforms or tracing"):
+                transformed()
+        with pytest.raises(RuntimeError, match="GPU tensors"):   # and not afterwards
+            call(w)
