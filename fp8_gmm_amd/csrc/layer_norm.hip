@@ -9,15 +9,16 @@
 // a row lies far off zero).  The statistics are kept in fp32 for the backward pass, m and r of every row; every sum is taken in
 // fp32, and a result is rounded once.
 //
-// From call to call, with buffers that the caches do not hold, in us and TB/s of what has to pass:
+// From call to call, with so many buffers in turn that the caches hold nothing of the next call's (1.3 GB of rows or more), in us
+// and TB/s of what has to pass.  The figures below are taken in the same way.
 //                          forward        backward
-//   1 x 4096, bf16         8.0            8.4            one or two launches
-//   1024 x 4096, bf16      7.9            17             out of the caches
-//   16384 x 4096, bf16     43.7   6.1     73.4   5.5
-//   16384 x 4093, bf16     44     6.1     77     5.2     rows that begin at any element
-//   65536 x 2048, fp32     189    5.7     264    6.1
-//   8192 x 16384, bf16     94     5.7     164    4.9     the longest rows that stay in registers
-//   262144 x 256, bf16     44     6.1     72     5.6     four rows to a wavefront
+//   1 x 4096, bf16         4.4            8.0            one launch each, out of the caches
+//   1024 x 4096, bf16      5.8            17             out of the caches
+//   16384 x 4096, bf16     49     5.5     73     5.5     forward 43 where the caches hold a part of the rows
+//   16384 x 4093, bf16     51     5.3     81     4.9     rows that begin at any element
+//   65536 x 2048, fp32     185    5.8     259    6.2
+//   8192 x 16384, bf16     101    5.3     157    5.1     the longest rows of 16 bits that stay in registers
+//   262144 x 256, bf16     47     5.8     79     5.1     four rows to a wavefront
 // A large copy reaches 5.3 here.
 #include <algorithm>
 #include <type_traits>
@@ -32,14 +33,15 @@ constexpr int kBackwardBlocks = 256;     // leaves one partial sum of the parame
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormSlab = 1 << 16;   // rows of a launch with a workgroup to a row, 2 GB at least: a grid has fewer than 2^32 threads
 
-// So many turns of one workgroup take less than a second launch for the sums of several: 32 x 1024, bf16, 2 turns: 8.6 us, by two
-// workgroups 10.9; 64 x 1024, 4 turns: 12.0 and 11.0; 16 x 4096, 4 turns: 14.5 and 11.3.
+// So many turns of one workgroup take less than a second launch for the sums of several: 32 x 1024, bf16, 2 turns: 8.4 us, by two
+// workgroups 8.8; 64 x 1024, 4 turns: 11.5 and 9.0; 16 x 4096, 4 turns: 14.2 and 10.7.
 constexpr int kBackwardAlone = 2;
 constexpr int kNormWaves = 16;           // the most wavefronts that share a row
 constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, where a row needs no more
 // Threads of its launch: what the compute units hold at a time, which go on to other rows; three times that where they would go on
-// more than five times (16384 x 4096, bf16, 4 turns: 43 us, with twice as many 45, with all rows at once 49; 24576 x 4096, 6 turns: 74,
-// with three times as many 69; 65536 x 2048, 8 turns, 97.5 and 89.6, all at once 101; fp32, 16 turns, 194 and 189).
+// more than five times (24576 x 4096, bf16, 6 turns: 73 us, with three times as many 67, with all rows at once 77; 65536 x 2048, 8
+// turns, 96, 88 and 99; fp32, 16 turns, 192, 185 and 182; 24576 x 2048, 3 turns, 36 and 40).  Not everywhere: 16384 x 4096, 4 turns, 49,
+// with twice as many 46; 8192 x 16384, 8 turns, 92, with three times as many 101.
 constexpr int kForwardAll = 256 * 2048, kForwardTurns = 5, kForwardMore = 3;
 
 // The sum over the THREADS threads of a row, the same in all of them.  `slot`: THREADS / 64 floats of LDS per row that nobody
@@ -507,29 +509,29 @@ struct Shape {
 int pieces_of(int cols, int type) { return ceil_div(cols, 16 / type_bytes(type)); }
 // Up to `most` pieces to a thread, as few threads as that allows, and then as few pieces: a thread behind the row's end works for
 // nothing.  `waves`: the most of them.  A row's first 64 * waves pieces are there, so that every wavefront has some of the row.
-// `narrow`: the most pieces of a thread where 16 lanes have a row.  4 forward (262144 x 256, bf16, 75 us by 64 lanes, 44 so; 131072 x
-// 384, 44 and 35; 131072 x 512, 49 and 42), 2 backward (262144 x 256, 85 and 72; with 3, 131072 x 384, 55 and 161: spills).
+// `narrow`: the most pieces of a thread where 16 lanes have a row.  4 forward (262144 x 256, bf16, 70 us by 64 lanes, 47 so; 131072 x
+// 384, 39.5 and 35.7; 131072 x 512, 48.6 and 46.7), 2 backward (262144 x 256, 87 and 79; with 3, 131072 x 384, 55 and 161: spills).
 Shape shape_of(int pieces, int most, int waves, int narrow) {
   if (pieces <= 16 * narrow) return {16, 1, ceil_div(pieces, 16)};
   const int w = ceil_div(pieces, 64 * most);
   return w <= waves ? Shape{64, w, ceil_div(pieces, 64 * w)} : Shape{0, 0, 0};
 }
 // The longest rows that stay in registers have 4 pieces in each of 1024 threads, which fits fp32 alone: a 16-bit type has twice
-// the elements and spills (4096 x 32768, bf16: 190 and 638 us forward and backward, by the kernels for longer rows 148 and
-// 302; 4096 x 16384, fp32: 99 and 186, by those 143 and 294).
+// the elements and spills backward (4096 x 32768, bf16: 103 and 781 us forward and backward, by the kernels for longer rows 146 and
+// 296; 4096 x 16384, fp32: 92 and 174, by those 142 and 287).
 Shape widest(int cols, int type) {
   const int w = ceil_div(pieces_of(cols, type), 64 * 4);
   return type == FP8GMM_TYPE_FP32 && w <= kNormWaves ? Shape{64, w, 4} : Shape{0, 0, 0};
 }
-// Forward, 4 pieces to a thread: few barriers and many loads under way (16384 x 4096, bf16: 43.5 us, with 2 pieces 45.6; 65536 x
-// 2048, fp32: 194 and 206; 16384 x 1536, bf16: 21.6 and 24.6).
+// Forward, 4 pieces to a thread: few barriers and many loads under way (65536 x 2048, fp32: 185 us, with 2 pieces 193; 8192 x 16384,
+// bf16: 101 and 120; 16384 x 1536: 21.2 and 23.0; 16384 x 4093: 51 and 58, but 16384 x 4096 49 and 48).
 Shape forward_shape(int cols, int type) {
   const Shape s = shape_of(pieces_of(cols, type), 4, 8, 4);
   return s.lanes != 0 ? s : widest(cols, type);
 }
 // Backward, 2: the sums of the parameters' gradients take registers as well.  Of fp32 rows of whole pieces 1, where that fills the
-// workgroup (65536 x 2048: 263 us, with 2 pieces 272; 32768 x 4096: 265 and 281; but 32768 x 3000, in 12 wavefronts, 224 and 210,
-// and 60001 x 2047, with edges, 281 and 264; 16384 x 4096, bf16: 75 and 73).
+// workgroup (65536 x 2048: 259 us, with 2 pieces 273; 32768 x 4096: 261 and 272; but 32768 x 3000, in 12 wavefronts, 220 and 207,
+// and 60001 x 2047, with edges, 271 and 260; 16384 x 4096, bf16: 73 and 73).
 Shape backward_shape(int cols, int type, bool aligned) {
   const int pieces = pieces_of(cols, type);
   const Shape one = shape_of(pieces, 1, kNormWaves, 1), s = shape_of(pieces, 2, kNormWaves, 2);
@@ -542,8 +544,8 @@ bool whole(const void* p, int64_t pitch, int cols, int type) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch % pieces == 0 && cols % pieces == 0;
 }
 // Whether a result is written with the streaming hint: one that outgrows the cache is not found there by whoever reads it.  With it
-// and without: 16384 x 4096, bf16, forward 43.7 and 50.9 us, backward 73.4 and 71.5; 65536 x 2048, fp32, 194 and 197, 279 and 305;
-// 24576 x 2048, bf16, 37.0 and 38.6, 55.9 and 58.4.
+// and without: 16384 x 4096, bf16, forward 49 and 49 us, backward 73 and 78; 65536 x 2048, fp32, 185 and 191, 259 and 269; 24576 x
+// 2048, bf16, 36.4 and 37.2, 55.5 and 57.9.
 bool streams(int64_t rows, int cols, int type) { return rows * cols * type_bytes(type) > (int64_t)64 << 20; }
 // A descriptor is a wavefront's, which has four rows where 16 lanes have one: these have edges, if empty ones.
 int mode_of(int cols, int type, int lanes, bool aligned, bool stream_edges) {
@@ -660,7 +662,8 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
   const int blocks = backward_blocks((int)rows, cols, type, aligned), bias = dbias != nullptr;
   const Shape shape = backward_shape(cols, type, aligned);
   const bool streaming = streams(rows, cols, type);
-  // of a 16-bit type, edges are written without the hint (16384 x 4093, bf16: 76 us, with it 80; 60001 x 2047, fp32: 286 and 267)
+  // of a 16-bit type, edges are written without the hint (16384 x 4093, bf16: 81 us, with it 79, but 76 and 80 where the caches hold a
+  // part of the rows; 60001 x 2047, fp32: 282 and 260)
   const int mode = mode_of(cols, type, shape.lanes, aligned, streaming && type == FP8GMM_TYPE_FP32);
   bool known = true;
   with_types(type, param_type, [&](auto tc, auto pc) {

@@ -10,7 +10,7 @@ once, and gradients are the same bits from call to call.  A routed layer norms i
 (:mod:`fp8_gmm_amd.moe`).
 
 Autocast is not looked at: a call computes in the types of its tensors, as the grouped modules do.  Gradients can be taken once;
-forward-mode differentiation, ``torch.func`` transforms and tracing are refused.
+forward-mode differentiation (under ``no_grad`` too, where torch keeps tangents), ``torch.func`` transforms and tracing are refused.
 """
 import torch
 
