@@ -90,10 +90,16 @@ inline void check_unwrapped(const char* name) {
               "fp8_gmm_amd: ", name, " does not run under torch.func transforms or tracing");
 }
 
+// A gradient as the kernels read it, which see its memory alone: torch hands on such whose sign is a bit beside that, and inside of a
+// level of forward mode such with a tangent, which no result of a backward pass here would have.
+inline Tensor plain_gradient(const Tensor& grad) {
+  check_no_tangent({grad}, "the backward passes do");
+  return grad.resolve_neg();
+}
 // What a backward pass starts from.  A node behind the pass that returned no gradient stands for zeros, as it does for a
-// Python autograd function.  torch hands gradients on whose sign is a bit beside their memory, of which the kernels see the memory alone.
+// Python autograd function.
 inline Tensor gradient_of_result(const Node& node, const variable_list& grads) {
-  return grads[0].defined() ? grads[0].resolve_neg() : node.input_metadata(0).zeros_like();
+  return grads[0].defined() ? plain_gradient(grads[0]) : node.input_metadata(0).zeros_like();
 }
 
 void define_layers(py::module_& m);   // host_layers.cpp

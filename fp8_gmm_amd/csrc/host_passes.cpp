@@ -126,7 +126,7 @@ void check_route(const Route& r, int64_t rows, const Tensor& x) {
 
 // What a row mover takes: contiguous, on 16 bytes, with its sign in its elements.
 Tensor aligned(const Tensor& t) {
-  const Tensor c = t.resolve_neg().contiguous();
+  const Tensor c = plain_gradient(t).contiguous();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -776,6 +776,7 @@ PYBIND11_MODULE(_host, m) {
   py::class_<Counts>(m, "Counts").def("wait", &Counts::wait, py::call_guard<py::gil_scoped_release>());
   m.def("gating", &gating);
   m.def("route", &route);
+  m.def("plain_gradient", [](const Tensor& grad) { return plain_gradient(grad).contiguous(); });
   m.def("set_kernel_timing", [](bool on) { kernel_timing.store(on, std::memory_order_relaxed); });
   define_layers(m);
 }

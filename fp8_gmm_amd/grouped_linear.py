@@ -28,7 +28,7 @@ from . import _lib
 from .backend import (TensorBatch, batched_uploads, fp8_gmm, grouped_gemm, linear_pass, multi_cast_transpose,
                       multi_quantize, wgrad_wants_transposed_gradient)
 from .fp8 import Fp8GroupedModuleBase, Fp8WeightCache, get_fp8_te_dtype, refuse_tracing
-from .native import linear_step
+from .native import linear_step, plain_gradient
 from .utils import PAD_MULTIPLE, Fp8MetaWrapper, Fp8TensorType, MetaTensorType, cumsum_group_sizes, to_torch_dtype
 
 
@@ -237,7 +237,7 @@ class _GroupedLinear(torch.autograd.Function):
         meta = ctx.meta
         cumsums, padded_cumsums, padded = ctx.cumsums, ctx.padded_cumsums, ctx.padded
         grad_dtype = to_torch_dtype(get_fp8_te_dtype(ctx.fp8_meta["recipe"], fprop_tensor=False))
-        grad_out = grad_out.resolve_neg().contiguous()   # kernels see a negative view's memory alone
+        grad_out = plain_gradient(grad_out)
         dev = grad_out.device
 
         if ctx.planned and not wgrad_wants_transposed_gradient(cumsums[-1], ctx.num_groups) \

@@ -43,7 +43,7 @@ from .backend import (
 )
 from .fp8 import Fp8GroupedModuleBase, Fp8WeightCache, get_fp8_te_dtype, refuse_tracing
 from .grouped_linear import MODULE_PAD_MULTIPLE, alloc_transposed, row_slices, stage_weight_cast, transposed_views
-from .native import mlp_step
+from .native import mlp_step, plain_gradient
 from .utils import PAD_MULTIPLE, Fp8MetaWrapper, Fp8TensorType, MetaTensorType, cumsum_group_sizes, to_torch_dtype
 
 _T = Fp8TensorType
@@ -238,7 +238,7 @@ class _GroupedMlp(torch.autograd.Function):
         cumsums, padded_cumsums, padded = ctx.cumsums, ctx.padded_cumsums, ctx.padded
         t_bounds = padded_cumsums if padded else cumsums
         grad_dtype = to_torch_dtype(get_fp8_te_dtype(ctx.fp8_meta["recipe"], fprop_tensor=False))
-        grad_out = grad_out.resolve_neg().contiguous()   # kernels see a negative view's memory alone
+        grad_out = plain_gradient(grad_out)
         dev = grad_out.device
         wgrad = ctx.weight_requires_grad
 

@@ -113,7 +113,7 @@ MAX_GATING_EXPERTS = 128
 def _aligned(t):
     """``t``, or a copy of it that is contiguous, starts on 16 bytes and has its sign in its elements (what a saved-tensor or gradient
     hook returned may be anything)."""
-    t = t.resolve_neg().contiguous()
+    t = native.plain_gradient(t)
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -249,7 +249,7 @@ class _TopK(torch.autograd.Function):
     def backward(ctx, grad_weights, _):
         probs, selected = ctx.saved_tensors
         tokens, experts = probs.shape
-        grad_weights = grad_weights.resolve_neg().contiguous().float()
+        grad_weights = native.plain_gradient(grad_weights).float()
         grad = torch.empty(tokens, experts, dtype=ctx.dtype, device=probs.device)
         _lib.check(_lib.load().fp8gmm_route_topk_backward(probs.data_ptr(), selected.data_ptr(), grad_weights.data_ptr(),
                                                          tokens, experts, selected.shape[1], grad.data_ptr(),
@@ -330,7 +330,7 @@ class _Gather(torch.autograd.Function):
     def backward(ctx, grad):
         indices, inverse = ctx.saved_tensors
         inverse = _invert(indices) if inverse is None else inverse
-        return _scatter_rows(grad.resolve_neg().contiguous(), inverse, None, ctx.top_k), None, None, None
+        return _scatter_rows(native.plain_gradient(grad), inverse, None, ctx.top_k), None, None, None
 
 
 class _Scatter(torch.autograd.Function):
@@ -343,7 +343,7 @@ class _Scatter(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         x, indices, weights = ctx.saved_tensors
-        grad = grad.resolve_neg().contiguous()
+        grad = native.plain_gradient(grad)
         if weights is not None and ctx.needs_input_grad[0] and ctx.needs_input_grad[2]:
             # both gradients: one pass that reads every gradient row once
             rows, hidden = x.shape

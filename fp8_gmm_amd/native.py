@@ -6,10 +6,10 @@ _lib.load()   # the kernels' library, which the extension calls, with its interf
 
 try:
     from ._host import (Due, Route, Setup, cast_weights, embedding, gating, layer_norm, linear_step, mlp_step, multi_clip, multi_norm,
-                        route, set_kernel_timing)
+                        plain_gradient, route, set_kernel_timing)
 except ImportError as exc:
     raise ImportError("fp8_gmm_amd/_host.so is missing or does not load: build the extensions "
                       "(`make -C fp8_gmm_amd/csrc -j8`)") from exc
 
 __all__ = ["Due", "Route", "Setup", "cast_weights", "embedding", "gating", "layer_norm", "linear_step", "mlp_step", "multi_clip",
-           "multi_norm", "route", "set_kernel_timing"]
+           "multi_norm", "plain_gradient", "route", "set_kernel_timing"]

@@ -682,3 +682,19 @@ def test_embedding_of_results_that_outgrow_the_cache(dev, tokens, table, cols, t
     size = torch.zeros_like(total).index_add_(0, rows[inside], dy[inside].double().abs())
     count = torch.bincount(rows[inside], minlength=table)[:, None]
     assert_within(dw, total, half_step(w.dtype) * total.abs() + (count + 4) * 2 * U * size + smallest(w.dtype), "dw")
+
+
+def test_gradients_with_tangents_are_refused(dev):
+    """Forward over reverse: a backward pass that dropped its gradient's tangent would return a wrong derivative."""
+    x, w, table = (torch.randn(s, device=dev, requires_grad=True) for s in ((6, 32), (32,), (9, 32)))
+    ids = torch.randint(0, 9, (6,), device=dev)
+    dy = torch.randn(6, 32, device=dev)
+    for make, leaf in ((lambda: pkg.layer_norm(x, w), x), (lambda: pkg.embedding(ids, table), table)):
+        y = make()
+        with torch.autograd.forward_ad.dual_level():
+            up = torch.autograd.forward_ad.make_dual(dy, torch.ones_like(dy))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, up)
+            (got,) = torch.autograd.grad(make(), leaf, dy)   # one without is taken inside of a level too
+        (want,) = torch.autograd.grad(make(), leaf, dy)
+        assert torch.equal(got, want)

@@ -1213,3 +1213,19 @@ def test_negated_gradients_keep_their_sign(dev, kind, planned):
         res.append([xi.grad] + [p.grad for p in module.parameters()])
     for a, b in zip(*res):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("kind", ["linear", "mlp"])
+@pytest.mark.parametrize("planned", [True, False])
+def test_gradients_with_tangents_are_refused(dev, kind, planned):
+    """As tensors with tangents are: the backward pass has none for its results."""
+    pkg = _pkg()
+    e, h, f, sizes = 2, 160, 336, [70, 45]
+    g = gen(98)
+    x = randn_bf16((sum(sizes), h), g).to(dev).requires_grad_()
+    module = (pkg.GroupedLinear if kind == "linear" else pkg.GroupedMlp)(h, f, e, torch.bfloat16, device=dev, planned_passes=planned)
+    out = module(x, torch.tensor(sizes))
+    with torch.autograd.forward_ad.dual_level():
+        up = torch.autograd.forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            out.backward(up)

@@ -817,3 +817,27 @@ def test_negated_gradients_keep_their_sign(dev, native):
 
     for a, c in zip(gradients(torch._neg_view), gradients(torch.neg)):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_gradients_with_tangents_are_refused(dev, native):
+    """Gating, routing, gather and scatter have no tangents for their gradients."""
+    ops = _ops()
+    tokens, hidden, experts, top_k = 70, 64, 4, 2
+    x, rows = (torch.randn(n, hidden, device=dev).to(torch.bfloat16).requires_grad_() for n in (tokens, tokens * top_k))
+    linear = torch.nn.Linear(hidden, experts, bias=False, dtype=torch.bfloat16, device=dev)
+    scores, share = torch.randn(tokens, experts, device=dev, requires_grad=True), torch.rand(tokens * top_k, device=dev, requires_grad=True)
+    top_expert = torch.randint(0, experts, (tokens * top_k,), device=dev).int()
+    indices, bin_ids, bins, _ = ops.indices_and_bins(top_expert, 2, experts)
+    with contextlib.nullcontext() if native else torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t):
+        passes = [(ops.gating(linear, x)[0], linear.weight), (ops.topk(scores, top_k)[0], scores),
+                  (ops.gather(x, indices, bin_ids, bins, top_k), x), (ops.scatter(rows, indices, bin_ids, share, bins, top_k), rows)]
+        if native:
+            from fp8_gmm_amd import native as host
+
+            passes.append((host.route(scores, top_k)[0], scores))
+        for out, leaf in passes:
+            with torch.autograd.forward_ad.dual_level():
+                up = torch.autograd.forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad(out, leaf, up)
