@@ -253,6 +253,13 @@ EXPORTS = (
     "fp8gmm_moe_gather",
     "fp8gmm_moe_scatter",
     "fp8gmm_moe_scatter_wgrad",
+    "fp8gmm_rms_norm",
+    "fp8gmm_rms_norm_fp8",
+    "fp8gmm_rms_norm_workspace_bytes",
+    "fp8gmm_rms_norm_backward",
+    "fp8gmm_select_experts",
+    "fp8gmm_select_experts_backward",
+    "fp8gmm_multi_adamw",
     "fp8gmm_layer_norm",
     "fp8gmm_layer_norm_workspace_bytes",
     "fp8gmm_layer_norm_backward",
@@ -401,6 +408,14 @@ def load():
     L.fp8gmm_layer_norm_workspace_bytes.argtypes = [cl, ci, ci]
     L.fp8gmm_layer_norm_backward.restype = ci
     L.fp8gmm_layer_norm_backward.argtypes = [vp, cl, vp, cl, vp, vp, vp, vp, vp, vp, cl, ci, ci, ci, vp, sz, vp]
+    L.fp8gmm_rms_norm.restype = ci
+    L.fp8gmm_rms_norm.argtypes = [vp, cl, vp, cl, vp, vp, vp, vp, cl, ci, cf, ci, ci, vp]
+    L.fp8gmm_rms_norm_fp8.restype = ci
+    L.fp8gmm_rms_norm_fp8.argtypes = [vp, cl, vp, cl, vp, vp, vp, vp, vp, vp, cl, ci, cf, ci, ci, ci, vp]
+    L.fp8gmm_rms_norm_workspace_bytes.restype = sz
+    L.fp8gmm_rms_norm_workspace_bytes.argtypes = [cl, ci, ci]
+    L.fp8gmm_rms_norm_backward.restype = ci
+    L.fp8gmm_rms_norm_backward.argtypes = [vp, cl, vp, cl, vp, cl, vp, vp, vp, vp, cl, ci, ci, ci, vp, sz, vp]
     L.fp8gmm_embedding.restype = ci
     L.fp8gmm_embedding.argtypes = [vp, ci, cl, vp, cl, ci, cf, ci, vp, vp]
     L.fp8gmm_embedding_workspace_bytes.restype = sz
@@ -413,6 +428,12 @@ def load():
     L.fp8gmm_multi_norm.argtypes = [vp, ci, vp, vp, sz, vp]
     L.fp8gmm_multi_clip.restype = ci
     L.fp8gmm_multi_clip.argtypes = [vp, ci, ctypes.c_double, vp, vp, sz, vp]
+    L.fp8gmm_multi_adamw.restype = ci
+    L.fp8gmm_multi_adamw.argtypes = [vp, ci, vp, vp]
+    L.fp8gmm_select_experts.restype = ci
+    L.fp8gmm_select_experts.argtypes = [vp, ci, cl, vp, vp, vp, vp]
+    L.fp8gmm_select_experts_backward.restype = ci
+    L.fp8gmm_select_experts_backward.argtypes = [vp, ci, cl, vp, vp, vp, vp, vp]
     L.fp8gmm_gemm_schedule.restype = ci
     L.fp8gmm_gemm_schedule.argtypes = [vp, ci, ci, ci, ci, ci, vp, ci]
     L.fp8gmm_gemm_fixup.restype = ci

@@ -699,6 +699,28 @@ def multi_clip(tensors, outs, max_norm):
     return native.multi_clip(list(tensors), list(outs), max_norm)
 
 
+def multi_adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, scales=None,
+                masters=None, norm=None, max_norm=None):
+    """One step of AdamW over a list of ``params`` (bfloat16, float16, float32 in any mixture, dense), in place:
+
+        g = grad * min(1, max_norm / (norm + 1e-6))           the clipping of ``multi_clip``, on the way
+        m += (1 - beta1) (g - m),  v += (1 - beta2) (g^2 - v)
+        p = p - lr weight_decay p - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+
+    ``grads``: of the parameters' types or float32, in any strides.  ``exp_avgs``, ``exp_avg_sqs``: float32 and of the parameters' shapes
+    and order, or, with ``scales`` (two lists of float32 ``[ceil(elements / 128)]``), ``float8_e4m3fn`` codes of ``m`` and of ``sqrt(v)``, a
+    scale for every 128 elements in the order of memory, rounded by thresholds that run evenly through all values from step to step
+    (csrc/adamw.hip).  ``masters``: the parameters in float32, where these have 16 bits: the step is made on the masters, the
+    parameters are their rounded copies.  ``norm`` (one float32 on the device, as ``multi_norm`` returns it) and ``max_norm``: both or
+    neither.  ``step`` counts from 1; it and ``lr`` are numbers, or an int64 and a float32 of the device (one element each), which a
+    replayed graph reads anew.  What is written may share memory with nothing else of the call.  A gradient that is no number leaves
+    none in its element, an infinite one in its block of 8-bit moments."""
+    flush_uploads()   # a queued launch may write what is read here
+    native.multi_adamw(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), step, lr, betas, eps, weight_decay,
+                       None if scales is None else (list(scales[0]), list(scales[1])), None if masters is None else list(masters), norm,
+                       max_norm)
+
+
 def _fill_transpose_shapes(table, x, t):
     if np.any(t.rows != x.cols) or np.any(t.cols < x.rows):
         _fail("fp8_gmm_amd: transposed output must be [cols, M] with M >= rows")

@@ -1,0 +1,441 @@
+// A step of AdamW over many tensors, for gfx950 (backend.multi_adamw, optim.AdamW).
+//
+//   g = grad * min(1, max_norm / (norm + 1e-6))
+//   m += (1 - beta1) (g - m),  v += (1 - beta2) (g^2 - v)
+//   p = p - lr decay p - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+//
+// with p kept in fp32 (`master`) beside 16-bit weights where the caller wants that.  m and v are fp32, or in 8 bits: e4m3 codes of m
+// and of sqrt(v), each 128 elements with a scale of their own in fp32, the largest magnitude over 448.  All arithmetic is fp32.
+//
+// 8-bit moments are rounded by a threshold that runs evenly through [0, 1) from step to step and from element to element, the
+// multiples of two irrational numbers: a moment that grows by less than half a code's distance each step would stay where it is for
+// ever if it were rounded to nearest.  m is rounded so that its mean over the thresholds is m, sqrt(v) so that the mean of its square is
+// v: with beta2 near 1 a bias of a thousandth of v in each step would be all there is.  A root that is not zero never becomes zero.
+//
+// Bound by memory: everything passes once.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "elements.h"
+
+namespace fp8gmm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTensors = 44;         // of a launch's arguments
+constexpr int kBlock = FP8GMM_ADAMW_BLOCK;
+constexpr float kMost = Fp8Limits<FP8GMM_E4M3>::kMax;
+constexpr float kTiny = 0x1p-100f;   // moments below it are zeros in 8 bits
+// thresholds in units of 2^-32
+constexpr uint32_t kStep = 0x9E3779B9u, kElement = 0x6A09E667u;   // the golden ratio and the root of 2, without their whole numbers
+
+struct Entry {
+  void* param;
+  const void* grad;
+  void *m, *v;
+  float *m_scale, *v_scale, *master;
+  int64_t count;
+  uint32_t begin;   // first chunk
+  uint16_t type, grad_type;
+};
+struct Part {
+  Entry e[kTensors];
+};
+static_assert(sizeof(Part) <= 3600, "the arguments of a launch");
+
+struct Hyper {
+  float c1, c2;       // 1 - beta
+  float eps, decay;   // decay: lr * weight_decay, or weight_decay where lr is the device's
+  float rate, root;   // lr / (1 - beta1^t) and 1 / sqrt(1 - beta2^t)
+  float max_norm;
+  uint32_t dither;    // t * kStep
+  const float* norm;
+  // of a step whose number and learning rate the device has (a captured one): the logarithms of the betas, to the base 2
+  const int64_t* step;
+  const float* lr;
+  double log1, log2, lr_host;
+};
+
+// VEC elements of a type, of which the first n are there
+template <int TYPE, int VEC>
+struct Values {
+  typedef Elements<TYPE> E;
+  typedef typename E::bits bits;
+  static constexpr int kBytes = VEC * E::kBytes;
+  typedef uint32_t half_piece __attribute__((ext_vector_type(2), aligned(2)));
+  u32x4 raw[kBytes < 16 ? 1 : kBytes / 16];
+  template <bool FULL>
+  __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
+    const bits* const p = static_cast<const bits*>(base) + at;
+    if constexpr (kBytes < 16) {
+      if constexpr (FULL) {
+        const u32x2 v = *reinterpret_cast<const half_piece*>(p);
+        raw[0] = u32x4{v.x, v.y, 0u, 0u};
+      } else {
+        raw[0] = E::load(p, min(n, VEC));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) raw[i] = E::load(p + i * E::kVec, FULL ? E::kVec : n - i * E::kVec);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[VEC]) const {
+    constexpr int N = VEC < E::kVec ? VEC : E::kVec;
+#pragma unroll
+    for (int i = 0; i < VEC; i += N) {
+      float part[E::kVec];
+      E::unpack(raw[i / N], part);
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[i + j] = part[j];
+    }
+  }
+  template <bool FULL>
+  static __device__ __forceinline__ void store(void* base, int64_t at, int n, const float (&f)[VEC]) {
+    bits* const p = static_cast<bits*>(base) + at;
+    constexpr int N = VEC < E::kVec ? VEC : E::kVec;
+#pragma unroll
+    for (int i = 0; i < VEC; i += N) {
+      float part[E::kVec] = {};
+#pragma unroll
+      for (int j = 0; j < N; ++j) part[j] = f[i + j];
+      const u32x4 v = E::pack(part);
+      if constexpr (N < E::kVec) {
+        if constexpr (FULL) *reinterpret_cast<half_piece*>(p) = u32x2{v.x, v.y};
+        else E::store(p, min(n, N), v);
+      } else {
+        E::store(p + i, FULL ? E::kVec : n - i, v);
+      }
+    }
+  }
+};
+
+// Eight codes
+struct Codes {
+  u32x2 raw;
+  template <bool FULL>
+  __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
+    const uint8_t* const p = static_cast<const uint8_t*>(base) + at;
+    if constexpr (FULL) {
+      raw = *reinterpret_cast<const u32x2*>(p);
+    } else {
+      raw = u32x2{0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) raw[i / 4] |= (uint32_t)p[i] << i % 4 * 8;
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[i], true);
+      f[4 * i] = lo.x;
+      f[4 * i + 1] = lo.y;
+      f[4 * i + 2] = hi.x;
+      f[4 * i + 3] = hi.y;
+    }
+  }
+  // of numbers that are codes
+  template <bool FULL>
+  static __device__ __forceinline__ void store(void* base, int64_t at, int n, const float (&f)[8]) {
+    uint8_t* const p = static_cast<uint8_t*>(base) + at;
+    u32x2 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+      w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], lo, true);
+    }
+    if constexpr (FULL) {
+      *reinterpret_cast<u32x2*>(p) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) p[i] = (uint8_t)(w[i / 4] >> i % 4 * 8);
+    }
+  }
+};
+
+// The codes lie 2^(e-3) apart from 2^e on, from 2^-6 down 2^-9: adding 2^-6 there makes the distance that of all numbers with its
+// exponent, and the last 20 bits of the fraction what lies between two codes.
+__device__ __forceinline__ float below_normal(float magnitude) { return magnitude < 0x1p-6f ? 0x1p-6f : 0.f; }
+__device__ __forceinline__ float cut_to_most(float v) { return v > kMost ? kMost : v; }   // (a NaN stays)
+
+// y to a code, up with the probability of its way to the next one
+__device__ __forceinline__ float round_linear(float y, uint32_t h) {
+  const float a = fabsf(y), off = below_normal(a);
+  const float code = __uint_as_float((__float_as_uint(a + off) + (h >> 12)) & 0xfff00000u) - off;
+  return y == y ? __builtin_copysignf(cut_to_most(code), y) : y;
+}
+// y >= 0 to a code, up with the probability of its square's way to the next one's
+__device__ __forceinline__ float round_root(float y, uint32_t h) {
+  const float off = below_normal(y);
+  const uint32_t low = __float_as_uint(y + off) & 0xfff00000u;
+  const float lo = __uint_as_float(low) - off, hi = __uint_as_float(low + 0x00100000u) - off;
+  const float u = (float)((h ^ 0x80000000u) >> 8) * 0x1p-24f;
+  const bool up = (y - lo) * (y + lo) > u * ((hi - lo) * (hi + lo)) || (lo == 0.f && y > 0.f);
+  return y == y ? cut_to_most(up ? hi : lo) : y;
+}
+
+// The largest over a row of 16 lanes: a block of 128 elements
+__device__ __forceinline__ float block_max(float v) {
+  const auto step = [&](auto control) {
+    v = fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(control)::value, 0xf, 0xf, true)));
+  };
+  step(std::integral_constant<int, 0xb1>{});
+  step(std::integral_constant<int, 0x4e>{});
+  step(std::integral_constant<int, 0x141>{});
+  step(std::integral_constant<int, 0x140>{});
+  return v;
+}
+
+// What a step multiplies by, the same for all elements
+struct Factors {
+  float grad, rate, root, decay;
+  uint32_t dither;
+};
+__device__ __forceinline__ Factors factors_of(const Hyper& h) {
+  Factors f = {1.f, h.rate, h.root, h.decay, h.dither};
+  if (h.step != nullptr || h.lr != nullptr) {
+    const double lr = h.lr != nullptr ? (double)*h.lr : h.lr_host;
+    f.decay = (float)(lr * (double)h.decay);
+    if (h.step != nullptr) {
+      const double t = (double)*h.step;
+      f.rate = (float)(lr / (1. - exp2(t * h.log1)));
+      f.root = (float)(1. / sqrt(1. - exp2(t * h.log2)));
+      f.dither = (uint32_t)*h.step * kStep;
+    } else {
+      f.rate = (float)(lr * (double)h.rate);
+    }
+  }
+  if (h.norm != nullptr) {
+    const float ratio = h.max_norm / (*h.norm + 1e-6f);
+    f.grad = ratio > 1.f ? 1.f : ratio;   // a NaN stays one
+  }
+  return f;
+}
+
+template <int TYPE, int GRAD, bool MASTER, bool BITS8, bool FULL>
+__device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, const Hyper& h, const Factors& by) {
+  constexpr int VEC = BITS8 ? 8 : 4;
+  typedef Values<FP8GMM_TYPE_FP32, VEC> F32;
+  Values<TYPE, VEC> param;
+  Values<GRAD, VEC> grad;
+  F32 master;
+  std::conditional_t<BITS8, Codes, F32> mc, vc;
+  float m_scale = 1.f, v_scale = 1.f;
+  grad.template load<FULL>(e.grad, at, n);
+  if constexpr (MASTER) master.template load<FULL>(e.master, at, n);
+  else param.template load<FULL>(e.param, at, n);
+  mc.template load<FULL>(e.m, at, n);
+  vc.template load<FULL>(e.v, at, n);
+  if constexpr (BITS8) {
+    if (FULL || n > 0) {
+      m_scale = e.m_scale[at / kBlock];
+      v_scale = e.v_scale[at / kBlock];
+    }
+  }
+  float p[VEC], g[VEC], m[VEC], v[VEC];
+  if constexpr (MASTER) master.get(p);
+  else param.get(p);
+  grad.get(g);
+  mc.get(m);
+  vc.get(v);
+  float m_most = 0.f, v_most = 0.f;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    g[i] *= by.grad;
+    if constexpr (BITS8) {
+      m[i] *= m_scale;
+      v[i] *= v_scale;
+      v[i] *= v[i];
+    }
+    m[i] = __builtin_fmaf(h.c1, g[i] - m[i], m[i]);
+    v[i] = __builtin_fmaf(h.c2, __builtin_fmaf(g[i], g[i], -v[i]), v[i]);
+    const float root = sqrtf(v[i]);
+    p[i] = __builtin_fmaf(-by.decay, p[i], p[i]) - by.rate * (m[i] / __builtin_fmaf(root, by.root, h.eps));
+    if constexpr (BITS8) {
+      v[i] = root;
+      m_most = fmaxf(m_most, fabsf(m[i]));
+      v_most = fmaxf(v_most, root);
+    }
+  }
+  if constexpr (MASTER) F32::template store<FULL>(e.master, at, n, p);
+  Values<TYPE, VEC>::template store<FULL>(e.param, at, n, p);
+  if constexpr (BITS8) {
+    m_most = block_max(m_most);
+    v_most = block_max(v_most);
+    const float m_inv = m_most >= kTiny ? kMost / m_most : 0.f, v_inv = v_most >= kTiny ? kMost / v_most : 0.f;
+    const uint32_t first = (uint32_t)at * kElement + by.dither;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const uint32_t threshold = first + i * kElement;
+      m[i] = round_linear(m[i] * m_inv, threshold);
+      v[i] = round_root(v[i] * v_inv, threshold);
+    }
+    if (threadIdx.x % 16 == 0 && (FULL || n > 0)) {
+      e.m_scale[at / kBlock] = m_most / kMost;
+      e.v_scale[at / kBlock] = v_most / kMost;
+    }
+  }
+  decltype(mc)::template store<FULL>(e.m, at, n, m);
+  decltype(vc)::template store<FULL>(e.v, at, n, v);
+}
+
+template <bool MASTER, bool BITS8>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const Part part, int n, const Hyper h) {
+  constexpr int VEC = BITS8 ? 8 : 4, CHUNK = kThreads * VEC;
+  __shared__ int found;
+  for (int i = threadIdx.x; i < n; i += kThreads)
+    if (part.e[i].begin <= blockIdx.x && (i + 1 == n || blockIdx.x < part.e[i + 1].begin)) found = i;
+  __syncthreads();
+  const Entry e = part.e[__builtin_amdgcn_readfirstlane(found)];
+  const Factors by = factors_of(h);
+  const int64_t first = (int64_t)(blockIdx.x - e.begin) * CHUNK, at = first + threadIdx.x * VEC;
+  const int64_t left = e.count - at;
+  const int mine = (int)(left < VEC ? left : VEC);
+  const auto as = [&](auto type, auto grad) {
+    constexpr int T = decltype(type)::value, G = decltype(grad)::value;
+    if (e.count - first >= CHUNK) step_values<T, G, MASTER, BITS8, true>(e, at, VEC, h, by);
+    else step_values<T, G, MASTER, BITS8, false>(e, at, mine, h, by);
+  };
+  constexpr std::integral_constant<int, FP8GMM_TYPE_BF16> bf16{};
+  constexpr std::integral_constant<int, FP8GMM_TYPE_FP16> fp16{};
+  constexpr std::integral_constant<int, FP8GMM_TYPE_FP32> fp32{};
+  if (e.type == FP8GMM_TYPE_BF16) {
+    e.grad_type == FP8GMM_TYPE_FP32 ? as(bf16, fp32) : as(bf16, bf16);
+  } else if (e.type == FP8GMM_TYPE_FP16) {
+    e.grad_type == FP8GMM_TYPE_FP32 ? as(fp16, fp32) : as(fp16, fp16);
+  } else {
+    if constexpr (!MASTER) as(fp32, fp32);
+  }
+}
+
+int check_tensors(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_step& step) {
+  int masters = 0;
+  for (int i = 0; i < n; ++i) {
+    const fp8gmm_adamw_tensor& t = tensors[i];
+    if (!known_type(t.type) || (t.grad_type != t.type && t.grad_type != FP8GMM_TYPE_FP32)) return FP8GMM_ERR_BAD_FORMAT;
+    if (t.count < 0 || t.count > (int64_t)1 << 32) return FP8GMM_ERR_BAD_SHAPE;
+    if (t.count == 0) continue;
+    if (t.param == nullptr || t.grad == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr ||
+        (step.bits == 8 && (t.exp_avg_scale == nullptr || t.exp_avg_sq_scale == nullptr)))
+      return FP8GMM_ERR_NULL_POINTER;
+    if (t.master != nullptr && t.type == FP8GMM_TYPE_FP32) return FP8GMM_ERR_BAD_ARGUMENT;
+    masters |= t.master != nullptr ? 1 : 2;
+    const auto off = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; };
+    if (off(t.param, type_bytes(t.type)) || off(t.grad, type_bytes(t.grad_type)) || off(t.master, 4) ||
+        off(t.exp_avg, step.bits == 8 ? 8 : 4) || off(t.exp_avg_sq, step.bits == 8 ? 8 : 4) || off(t.exp_avg_scale, 4) || off(t.exp_avg_sq_scale, 4))
+      return FP8GMM_ERR_ALIGNMENT;
+  }
+  return masters == 3 ? FP8GMM_ERR_BAD_ARGUMENT : FP8GMM_OK;
+}
+
+// Nothing is written that another tensor of the call reads or writes.
+int check_apart(const fp8gmm_adamw_tensor* tensors, int n, int bits) {
+  struct Range {
+    uintptr_t begin, end;
+    bool writes;
+  };
+  std::vector<Range> ranges;
+  ranges.reserve(7 * (size_t)n);
+  const auto add = [&](const void* p, int64_t bytes, bool writes) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(p);
+    if (p != nullptr) ranges.push_back({begin, begin + (uintptr_t)bytes, writes});
+  };
+  for (int i = 0; i < n; ++i) {
+    const fp8gmm_adamw_tensor& t = tensors[i];
+    if (t.count == 0) continue;
+    const int64_t moments = t.count * (bits / 8), scales = (t.count + kBlock - 1) / kBlock * 4;
+    add(t.param, t.count * type_bytes(t.type), true);
+    add(t.grad, t.count * type_bytes(t.grad_type), false);
+    add(t.exp_avg, moments, true);
+    add(t.exp_avg_sq, moments, true);
+    add(t.master, t.count * 4, true);
+    if (bits == 8) {
+      add(t.exp_avg_scale, scales, true);
+      add(t.exp_avg_sq_scale, scales, true);
+    }
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  uintptr_t written = 0, read = 0;   // ends of what the ranges so far write and read
+  for (const Range& r : ranges) {
+    if (r.begin < written || (r.writes && r.begin < read)) return FP8GMM_ERR_BAD_ARGUMENT;
+    (r.writes ? written : read) = std::max(r.writes ? written : read, r.end);
+  }
+  return FP8GMM_OK;
+}
+
+int multi_adamw(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_step* step, hipStream_t s) {
+  if (n < 0) return FP8GMM_ERR_BAD_ARGUMENT;
+  if (step == nullptr || (n > 0 && tensors == nullptr)) return FP8GMM_ERR_NULL_POINTER;
+  const fp8gmm_adamw_step& a = *step;
+  if ((a.bits != 32 && a.bits != 8) || !(a.beta1 >= 0. && a.beta1 < 1.) || !(a.beta2 >= 0. && a.beta2 < 1.) || !(a.eps >= 0.) ||
+      !(a.weight_decay >= 0.) || (a.step_dev == nullptr && a.step < 1) || (a.norm != nullptr && !(a.max_norm >= 0.)) ||
+      (a.lr_dev == nullptr && !(a.lr >= 0.)))
+    return FP8GMM_ERR_BAD_ARGUMENT;
+  int rc = check_tensors(tensors, n, a);
+  if (rc == FP8GMM_OK) rc = check_apart(tensors, n, a.bits);
+  if (rc != FP8GMM_OK) return rc;
+  Hyper h = {};
+  h.c1 = (float)(1. - a.beta1);
+  h.c2 = (float)(1. - a.beta2);
+  h.eps = (float)a.eps;
+  h.max_norm = (float)a.max_norm;
+  h.norm = a.norm;
+  h.step = a.step_dev;
+  h.lr = a.lr_dev;
+  const bool device = h.step != nullptr || h.lr != nullptr;
+  const double t = (double)a.step, lr = h.lr != nullptr ? 1. : a.lr;
+  h.decay = (float)(device ? a.weight_decay : lr * a.weight_decay);
+  if (h.step == nullptr) {
+    h.rate = (float)((device ? 1. : lr) / (1. - std::pow(a.beta1, t)));
+    h.root = (float)(1. / std::sqrt(1. - std::pow(a.beta2, t)));
+    h.dither = (uint32_t)a.step * kStep;
+  }
+  h.log1 = std::log2(a.beta1);   // (of a beta of 0 minus infinity, whose power is 0)
+  h.log2 = std::log2(a.beta2);
+  h.lr_host = a.lr;
+  bool master = false;
+  for (int i = 0; i < n; ++i) master = master || tensors[i].master != nullptr;
+  const int64_t chunk = kThreads * (a.bits == 8 ? 8 : 4);
+  constexpr int64_t kMostChunks = 1 << 23;   // of a launch, which holds the largest tensor: a grid has fewer than 2^32 threads
+  Part part = {};
+  int used = 0;
+  int64_t chunks = 0;
+  const auto flush = [&] {
+    if (used == 0) return;
+    auto* kernel = master ? a.bits == 8 ? &adamw_kernel<true, true> : &adamw_kernel<true, false>
+                   : a.bits == 8 ? &adamw_kernel<false, true>
+                                 : &adamw_kernel<false, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(kThreads), 0, s, part, used, h);
+    used = 0;
+    chunks = 0;
+  };
+  for (int i = 0; i < n; ++i) {
+    const fp8gmm_adamw_tensor& t = tensors[i];
+    const int64_t all = (t.count + chunk - 1) / chunk;
+    if (all == 0) continue;
+    if (used == kTensors || chunks + all > kMostChunks) flush();
+    part.e[used++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.count,
+                      (uint32_t)chunks, (uint16_t)t.type, (uint16_t)t.grad_type};
+    chunks += all;
+  }
+  if (used == 0) return FP8GMM_OK;   // none has elements
+  flush();
+  return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace fp8gmm
+
+extern "C" {
+
+int fp8gmm_multi_adamw(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_step* step, void* stream) {
+  try {   // the host's list of ranges is the only thing here that can fail by an exception, which ends at this border
+    return fp8gmm::multi_adamw(tensors, n, step, static_cast<hipStream_t>(stream));
+  } catch (...) {
+    return FP8GMM_ERR_BAD_ARGUMENT;
+  }
+}
+
+}  // extern "C"

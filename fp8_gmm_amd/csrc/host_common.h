@@ -1,10 +1,11 @@
 // What the native host paths share (host_passes.cpp: the grouped modules and the routing; host_layers.cpp: the operators around
-// them).
+// them; host_routing.cpp: the choice of experts; host_adamw.cpp: the optimizer's step).
 #pragma once
 
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -102,6 +103,46 @@ inline Tensor gradient_of_result(const Node& node, const variable_list& grads) {
   return grads[0].defined() ? plain_gradient(grads[0]) : node.input_metadata(0).zeros_like();
 }
 
+inline int type_of(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return FP8GMM_TYPE_BF16;
+    case at::kHalf: return FP8GMM_TYPE_FP16;
+    case at::kFloat: return FP8GMM_TYPE_FP32;
+    default: TORCH_CHECK(false, "fp8_gmm_amd: ", what, " must be bfloat16, float16 or float32, got ", t.scalar_type());
+  }
+}
+
+inline void check_plain(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), "fp8_gmm_amd: expected GPU tensors (the HIP path has no CPU fallback)");
+  TORCH_CHECK(t.layout() == at::kStrided && !t.is_neg(), "fp8_gmm_amd: ", what, " must be a dense tensor");
+}
+
+inline bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// With create_graph the gradients would need a graph of their own, which the kernels do not have: differentiating them again
+// raises.  (Left without a node they would pass for constants.)
+inline void refuse_second_derivative(variable_list& result, const char* what, at::TensorList inputs) {
+  if (!torch::autograd::any_variable_requires_grad({inputs.begin(), inputs.end()})) return;
+  auto node = std::shared_ptr<torch::autograd::Error>(
+      new torch::autograd::Error(std::string("fp8_gmm_amd: ") + what + " can be differentiated once only",
+                                 torch::autograd::collect_next_edges(variable_list(inputs.begin(), inputs.end()))),
+      torch::autograd::deleteNode);
+  for (Tensor& t : result)
+    if (t.defined()) torch::autograd::set_history(t, node);
+}
+
+// Memory that a tensor's elements fill without gaps, in whatever order of its dimensions
+inline bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
+// The order of the elements in memory, which strides of a dimension of size 1 say nothing of
+inline bool same_order(const Tensor& a, const Tensor& b) {
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+inline bool pass_as_they_are(const Tensor& in, const Tensor& out) { return dense(in) && dense(out) && same_order(in, out); }
+
 void define_layers(py::module_& m);   // host_layers.cpp
+void define_routing(py::module_& m);  // host_routing.cpp
+void define_adamw(py::module_& m);    // host_adamw.cpp
 
 }  // namespace fp8gmm_host

@@ -1,10 +1,9 @@
-// The host path of the operators around the routed layers: layer norm and embedding with their gradients (layers.py), the norm
-// of many tensors and their scaling by it (backend.multi_norm, multi_clip).  A short call is bound by its host, so the argument
+// The host path of the operators around the routed layers: the norms of rows and embedding with their gradients (layers.py), the
+// norm of many tensors and their scaling by it (backend.multi_norm, multi_clip).  A short call is bound by its host, so the argument
 // checks, the nodes of the autograd graph and the launches' tables are native as in host_passes.cpp.
 #include "host_common.h"
 
 #include <ATen/MemoryOverlap.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <cmath>
@@ -12,34 +11,6 @@
 
 namespace fp8gmm_host {
 namespace {
-
-int type_of(const Tensor& t, const char* what) {
-  switch (t.scalar_type()) {
-    case at::kBFloat16: return FP8GMM_TYPE_BF16;
-    case at::kHalf: return FP8GMM_TYPE_FP16;
-    case at::kFloat: return FP8GMM_TYPE_FP32;
-    default: TORCH_CHECK(false, "fp8_gmm_amd: ", what, " must be bfloat16, float16 or float32, got ", t.scalar_type());
-  }
-}
-
-void check_plain(const Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda(), "fp8_gmm_amd: expected GPU tensors (the HIP path has no CPU fallback)");
-  TORCH_CHECK(t.layout() == at::kStrided && !t.is_neg(), "fp8_gmm_amd: ", what, " must be a dense tensor");
-}
-
-bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
-
-// With create_graph the gradients would need a graph of their own, which the kernels do not have: differentiating them again
-// raises.  (Left without a node they would pass for constants.)
-void refuse_second_derivative(variable_list& result, const char* what, at::TensorList inputs) {
-  if (!torch::autograd::any_variable_requires_grad({inputs.begin(), inputs.end()})) return;
-  auto node = std::shared_ptr<torch::autograd::Error>(
-      new torch::autograd::Error(std::string("fp8_gmm_amd: ") + what + " can be differentiated once only",
-                                 torch::autograd::collect_next_edges(variable_list(inputs.begin(), inputs.end()))),
-      torch::autograd::deleteNode);
-  for (Tensor& t : result)
-    if (t.defined()) torch::autograd::set_history(t, node);
-}
 
 // ---- layer norm ------------------------------------------------------------------------------------------------------
 // The rows of a tensor of any shape, and their pitch: as they are where the columns are neighbours, otherwise copied.
@@ -159,6 +130,181 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const std::optional<Ten
   });
 }
 
+// ---- root-mean-square norm -------------------------------------------------------------------------------------------
+struct RmsNormBackward : public Node {
+  SavedVariable h, weight;
+  Tensor rstd;
+  int64_t rows = 0, cols = 0;
+  int type = 0, param_type = 0;
+  bool residual = false;
+
+  std::string name() const override { return "RmsNormBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    h.reset_data();
+    weight.reset_data();
+    rstd.reset();
+  }
+  variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    const bool graph = at::GradMode::is_enabled();
+    variable_list result(residual ? 3 : 2);
+    // with a residual h is a result of this node
+    const Tensor hs = residual ? h.unpack(shared_from_this()) : h.unpack(), w = weight.unpack();
+    const Tensor grad = grads[0].defined() || !(residual && grads[1].defined()) ? gradient_of_result(*this, grads) : Tensor();
+    const Tensor grad_h = residual && grads[1].defined() ? plain_gradient(grads[1]) : Tensor();
+    const bool want_x = task_should_compute_output(0) || (residual && task_should_compute_output(2));
+    if (!grad.defined()) {   // the sum alone was used
+      if (task_should_compute_output(0)) result[0] = grads[1];
+      if (task_should_compute_output(2)) result[2] = grads[1];
+      return result;
+    }
+    const c10::OptionalDeviceGuard guard(grad.device());
+    Tensor dx;
+    {
+      at::AutoGradMode no_grad(false);
+      TORCH_CHECK(hs.device() == grad.device() && hs.numel() == rows * cols && hs.scalar_type() == grad.scalar_type() &&
+                      w.device() == grad.device() && w.numel() == cols && w.is_contiguous() && type_of(w, "weight") == param_type &&
+                      type_of(hs, "input") == type,
+                  "fp8_gmm_amd: a saved-tensor hook returned another tensor than was saved");
+      const Rows from = rows_of(hs.resolve_neg(), rows, cols), dy = rows_of(grad, rows, cols);
+      const Rows dh = grad_h.defined() ? rows_of(grad_h, rows, cols) : Rows{Tensor(), cols};
+      const Tensor params = w.resolve_neg();
+      if (want_x) dx = at::empty(hs.sizes(), hs.options());
+      if (task_should_compute_output(1)) result[1] = at::empty({cols}, w.options());
+      Tensor work;
+      size_t bytes = 0;
+      if (rows > 0 && result[1].defined()) {
+        bytes = fp8gmm_rms_norm_workspace_bytes(rows, (int)cols, type);
+        work = at::empty({(int64_t)bytes}, hs.options().dtype(at::kByte));
+      }
+      timed("rms_norm_backward", (2 + dx.defined() + grad_h.defined()) * hs.numel() * (int64_t)hs.element_size(), [&] {
+        check(fp8gmm_rms_norm_backward(ptr<void>(dy.t), dy.pitch, ptr<void>(dh.t), dh.pitch, ptr<void>(from.t), from.pitch,
+                                       ptr<void>(params), ptr<float>(rstd), ptr<void>(dx), ptr<void>(result[1]), rows, (int)cols, type,
+                                       param_type, ptr<void>(work), bytes, current_stream(grad.device())));
+      });
+    }
+    if (task_should_compute_output(0)) result[0] = dx;
+    if (residual && task_should_compute_output(2)) result[2] = dx;
+    if (graph) {
+      variable_list from = {grad, hs, w};
+      if (grad_h.defined()) from.push_back(grad_h);
+      refuse_second_derivative(result, "rms_norm", from);
+    }
+    return result;
+  }
+};
+
+// What both root-mean-square norms ask of their rows
+struct RmsRows {
+  int type, param_type;
+  int64_t rows, cols;
+};
+RmsRows check_rms(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps, const char* name, const char* does) {
+  check_unwrapped(name);
+  check_plain(x, "the input of a norm");
+  check_plain(weight, "weight");
+  const int type = type_of(x, "the input of a norm"), param_type = type_of(weight, "weight");
+  TORCH_CHECK(param_type == type || param_type == FP8GMM_TYPE_FP32, "fp8_gmm_amd: weight must have the input's type or be float32");
+  TORCH_CHECK(x.dim() >= 1 && weight.dim() == 1 && x.size(-1) == weight.size(0) && weight.size(0) >= 1,
+              "fp8_gmm_amd: weight must be 1-D with as many elements as the input has columns, at least one");
+  TORCH_CHECK(weight.device() == x.device(), "fp8_gmm_amd: all tensors of one call must live on the same device");
+  if (residual.defined()) {
+    check_plain(residual, "residual");
+    TORCH_CHECK(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type() && residual.device() == x.device(),
+                "fp8_gmm_amd: residual must have the input's shape, type and device");
+  }
+  TORCH_CHECK(eps >= 0 && std::isfinite(eps), "fp8_gmm_amd: eps must be a number, not negative");
+  check_no_tangent({x, weight, residual}, does);
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  TORCH_CHECK(cols <= 1 << 30 && rows <= INT32_MAX, "fp8_gmm_amd: at most 2^30 columns and 2^31 - 1 rows are supported");
+  return {type, param_type, rows, cols};
+}
+
+// (y, h): h the rows that are normed, undefined without a residual
+std::pair<Tensor, Tensor> rms_norm(const Tensor& x, const Tensor& weight, double eps, const std::optional<Tensor>& residual_) {
+  std::pair<Tensor, Tensor> out;
+  with_python_errors([&] {
+    py::gil_scoped_release no_gil;
+    const Tensor residual = residual_.value_or(Tensor());
+    const RmsRows r = check_rms(x, weight, residual, eps, "rms_norm", "rms_norm does");
+    const c10::OptionalDeviceGuard guard(x.device());
+    const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual));
+    Tensor y, h, rstd, w;
+    {
+      at::AutoGradMode no_grad(false);
+      const Rows from = rows_of(x, r.rows, r.cols), add = residual.defined() ? rows_of(residual, r.rows, r.cols) : Rows{Tensor(), r.cols};
+      w = weight.contiguous();
+      y = at::empty(x.sizes(), x.options());
+      if (residual.defined()) h = at::empty(x.sizes(), x.options());
+      if (grad) rstd = at::empty({r.rows}, x.options().dtype(at::kFloat));
+      timed("rms_norm", (residual.defined() ? 4 : 2) * x.numel() * (int64_t)x.element_size(), [&] {
+        check(fp8gmm_rms_norm(ptr<void>(from.t), from.pitch, ptr<void>(add.t), add.pitch, ptr<void>(w), ptr<void>(y), ptr<void>(h),
+                              ptr<float>(rstd), r.rows, (int)r.cols, (float)eps, r.type, r.param_type, current_stream(x.device())));
+      });
+    }
+    if (grad) {
+      auto node = std::shared_ptr<RmsNormBackward>(new RmsNormBackward(), torch::autograd::deleteNode);
+      if (residual.defined()) node->set_next_edges(torch::autograd::collect_next_edges(x, weight, residual));
+      else node->set_next_edges(torch::autograd::collect_next_edges(x, weight));
+      node->rstd = rstd;
+      node->rows = r.rows;
+      node->cols = r.cols;
+      node->type = r.type;
+      node->param_type = r.param_type;
+      node->residual = residual.defined();
+      torch::autograd::set_history(y, node);
+      if (residual.defined()) torch::autograd::set_history(h, node);
+      node->h = residual.defined() ? SavedVariable(h, true) : SavedVariable(x, false);
+      node->weight = SavedVariable(weight.is_contiguous() ? weight : w, false);
+    }
+    out = {y, h};
+    return Tensor();
+  });
+  return out;
+}
+
+// (q, scale_inv of the rows or undefined, h or undefined)
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, double eps, const std::optional<Tensor>& residual_,
+                                                const std::optional<Tensor>& scale_, const std::optional<Tensor>& amax_,
+                                                at::ScalarType format) {
+  py::gil_scoped_release no_gil;
+  const Tensor residual = residual_.value_or(Tensor()), scale = scale_.value_or(Tensor()), amax = amax_.value_or(Tensor());
+  const RmsRows r = check_rms(x, weight, residual, eps, "rms_norm_fp8", "rms_norm_fp8 does");
+  TORCH_CHECK(format == at::kFloat8_e4m3fn || format == at::kFloat8_e5m2,
+              "fp8_gmm_amd: dtype must be torch.float8_e4m3fn or torch.float8_e5m2");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual))),
+              "fp8_gmm_amd: rms_norm_fp8 takes no gradients: call it under torch.no_grad() or on detached tensors");
+  for (const Tensor& t : {scale, amax}) {
+    if (!t.defined()) continue;
+    check_plain(t, "scale and amax");
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == 1 && t.device() == x.device(),
+                "fp8_gmm_amd: scale and amax must be one float32 each, on the input's device");
+  }
+  TORCH_CHECK(scale.defined() || !amax.defined(), "fp8_gmm_amd: amax is recorded with a scale of the tensor");
+  if (amax.defined()) {
+    TORCH_CHECK(!amax.is_inference() || c10::InferenceMode::is_enabled(),
+                "fp8_gmm_amd: amax is an inference tensor, which is written in inference mode only");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && amax.requires_grad()), "fp8_gmm_amd: amax requires a gradient");
+    TORCH_CHECK(scale.data_ptr() != amax.data_ptr(), "fp8_gmm_amd: scale and amax must not share memory");
+  }
+  at::AutoGradMode no_grad(false);
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Rows from = rows_of(x, r.rows, r.cols), add = residual.defined() ? rows_of(residual, r.rows, r.cols) : Rows{Tensor(), r.cols};
+  const Tensor w = weight.contiguous();
+  const Tensor q = at::empty(x.sizes(), x.options().dtype(format));
+  Tensor h, scale_inv;
+  if (residual.defined()) h = at::empty(x.sizes(), x.options());
+  if (!scale.defined()) scale_inv = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  timed("rms_norm_fp8", x.numel() * ((residual.defined() ? 3 : 1) * (int64_t)x.element_size() + 1), [&] {
+    check(fp8gmm_rms_norm_fp8(ptr<void>(from.t), from.pitch, ptr<void>(add.t), add.pitch, ptr<void>(w), ptr<void>(q), ptr<void>(h),
+                              ptr<float>(scale), ptr<float>(amax), ptr<float>(scale_inv), r.rows, (int)r.cols, (float)eps, r.type,
+                              r.param_type, format == at::kFloat8_e4m3fn ? FP8GMM_E4M3 : FP8GMM_E5M2, current_stream(x.device())));
+  });
+  if (amax.defined()) torch::autograd::impl::bump_version(amax);
+  return {q, scale_inv, h};
+}
+
 // ---- embedding -------------------------------------------------------------------------------------------------------
 struct EmbeddingBackward : public Node {
   SavedVariable ids;
@@ -250,9 +396,6 @@ Tensor embedding(const Tensor& ids_, const Tensor& weight, double scale, std::op
 }
 
 // ---- norm of many tensors --------------------------------------------------------------------------------------------
-// Memory that a tensor's elements fill without gaps, in whatever order of its dimensions
-bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
-
 void check_list(const std::vector<Tensor>& tensors, const char* what) {
   TORCH_CHECK(!tensors.empty(), "fp8_gmm_amd: ", what, " needs at least one tensor");
   for (const Tensor& t : tensors) {
@@ -292,14 +435,6 @@ Tensor multi_norm(const std::vector<Tensor>& tensors) {
   });
   return norm;
 }
-
-// The order of the elements in memory, which strides of a dimension of size 1 say nothing of
-bool same_order(const Tensor& a, const Tensor& b) {
-  for (int64_t d = 0; d < a.dim(); ++d)
-    if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
-  return true;
-}
-bool pass_as_they_are(const Tensor& in, const Tensor& out) { return dense(in) && dense(out) && same_order(in, out); }
 
 // Where a tensor lies, in bytes: from its first element to behind its last one, and the rows in that where it consists of rows of
 // one pitch (0: of none, or of one).
@@ -404,6 +539,16 @@ Tensor multi_clip(const std::vector<Tensor>& tensors, const std::vector<Tensor>&
 
 void define_layers(py::module_& m) {
   m.def("layer_norm", &layer_norm);
+  m.def("rms_norm", [](const Tensor& x, const Tensor& weight, double eps, const std::optional<Tensor>& residual) -> py::object {
+    const auto out = rms_norm(x, weight, eps, residual);
+    return out.second.defined() ? py::cast(out) : py::cast(out.first);
+  });
+  m.def("rms_norm_fp8", [](const Tensor& x, const Tensor& weight, double eps, const std::optional<Tensor>& residual,
+                           const std::optional<Tensor>& scale, const std::optional<Tensor>& amax, at::ScalarType format) {
+    const auto [q, scale_inv, h] = rms_norm_fp8(x, weight, eps, residual, scale, amax, format);
+    const auto given = [](const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); };
+    return py::make_tuple(q, given(scale_inv), given(h));
+  });
   m.def("embedding", &embedding);
   m.def("multi_norm", &multi_norm);
   m.def("multi_clip", &multi_clip);

@@ -779,4 +779,6 @@ PYBIND11_MODULE(_host, m) {
   m.def("plain_gradient", [](const Tensor& grad) { return plain_gradient(grad).contiguous(); });
   m.def("set_kernel_timing", [](bool on) { kernel_timing.store(on, std::memory_order_relaxed); });
   define_layers(m);
+  define_routing(m);
+  define_adamw(m);
 }

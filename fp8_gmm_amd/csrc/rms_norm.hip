@@ -1,0 +1,321 @@
+// Root-mean-square norm over the columns of rows of bf16, fp16 or fp32, for gfx950, with the addition of a residual in front, a result
+// in 8 bits, and the backward pass: the norm in front of a routed layer (moe.py, rms_norm=True) or of a product in 8 bits.
+//
+//   h = x + residual, rounded (without a residual x itself), r = 1 / sqrt(mean(h^2) + eps), z = h r, y = z w
+//   g = dy w, dx = dh + r (g - z mean(g z)), dw = sum over rows of dy z
+//   in 8 bits: q = fp8(y s) by the tensor's scale s, with the largest |y| recorded, or by the row's, s = most / max |y|
+//
+// The norm is that of the rows as h is returned, so that the backward pass starts from what the forward pass ended with.  Bound by
+// memory: every row passes once in and once out.  Sums are taken in fp32, a result is rounded once.
+#include <algorithm>
+
+#include "norm_rows.h"
+
+namespace fp8gmm {
+namespace {
+
+// The least magnitude that a row's scale is made of: what is smaller is zero in 8 bits, and no scale is zero.
+constexpr float kLeast = 0x1p-100f;
+
+__device__ __forceinline__ float most_of(int fmt) { return fmt == FP8GMM_E4M3 ? Fp8Limits<FP8GMM_E4M3>::kMax : Fp8Limits<FP8GMM_E5M2>::kMax; }
+
+// The first n of V values in 8 bits, at any byte
+typedef uint32_t u32_any1 __attribute__((aligned(1)));
+typedef uint32_t u32x2_any1 __attribute__((ext_vector_type(2), aligned(1)));
+template <int V>
+__device__ __forceinline__ void store8(uint8_t* p, int n, const float (&f)[V], int fmt) {
+  uint32_t w[V / 4];
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i)
+    w[i] = fmt == FP8GMM_E4M3 ? cvt4_fp8<FP8GMM_E4M3>(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3])
+                              : cvt4_fp8<FP8GMM_E5M2>(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+  if (n >= V) {
+    if constexpr (V == 8) *reinterpret_cast<u32x2_any1*>(p) = u32x2{w[0], w[1]};
+    else *reinterpret_cast<u32_any1*>(p) = w[0];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V - 1; ++i)
+    if (i < n) p[i] = (uint8_t)(w[i / 4] >> i % 4 * 8);
+}
+
+// The largest over the workgroup's threads; `slot` as of row_sum
+template <int THREADS>
+__device__ __forceinline__ float row_max(float v, float* slot) {
+  v = wave_max(v);
+  if (threadIdx.x % 64 == 0) slot[threadIdx.x / 64] = v;
+  __syncthreads();
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) most = fmaxf(most, slot[i]);
+  return most;
+}
+
+// Where an 8-bit result goes, and its scales: `scale` and `amax` (may be NULL) of the tensor, or `scale_inv` of every row
+struct Bits8 {
+  uint8_t* q;
+  const float* scale;
+  float* amax;
+  float* scale_inv;
+  int fmt;
+};
+
+// A row to a workgroup, read three times, from the cache the second and third time.
+template <int TYPE, int PTYPE, bool BITS8>
+__global__ __launch_bounds__(kNormLongThreads) void rms_norm_long_kernel(
+    const void* __restrict__ x_, int64_t ldx, const void* __restrict__ residual_, int64_t ldr, const void* __restrict__ w,
+    void* __restrict__ y_, const Bits8 bits8, void* __restrict__ h_, float* __restrict__ rstd_out, int64_t first, int cols, float eps) {
+  typedef Elements<TYPE> E;
+  typedef typename E::bits bits;
+  constexpr int V = E::kVec, STEP = kNormLongThreads * V;
+  __shared__ float slots[2][kNormLongThreads / 64];
+  const int64_t row = first + blockIdx.x;
+  const int t = threadIdx.x;
+  const bits* const x = static_cast<const bits*>(x_) + row * ldx;
+  const bits* const residual = residual_ != nullptr ? static_cast<const bits*>(residual_) + row * ldr : nullptr;
+  bits* const h = residual != nullptr ? static_cast<bits*>(h_) + row * cols : nullptr;
+  float squares = 0.f;
+  for (int64_t at = t * V; at < cols; at += STEP) {
+    const int n = (int)(cols - at);
+    float f[V];
+    E::unpack(E::load(x + at, n), f);
+    if (residual != nullptr) {
+      float a[V];
+      E::unpack(E::load(residual + at, n), a);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] += a[i];
+      const u32x4 sum = E::pack(f);
+      E::store(h + at, n, sum);
+      E::unpack(sum, f);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) squares = __builtin_fmaf(f[i], f[i], squares);
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<kNormLongThreads>(squares, slots[0]) / (float)cols + eps);
+  if (rstd_out != nullptr && t == 0) rstd_out[row] = rstd;
+  const bits* const rows = residual != nullptr ? h : x;   // a thread reads what it has written
+  const auto normed = [&](int64_t at, float (&f)[V]) {
+    const int n = (int)(cols - at);
+    Parameters<TYPE, PTYPE> pw;
+    pw.load(w, (int)at, n);
+    float fw[V];
+    E::unpack(E::load(rows + at, n), f);
+    pw.get(fw);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = f[i] * rstd * fw[i];
+  };
+  if constexpr (BITS8) {
+    float scale = bits8.scale != nullptr ? *bits8.scale : 0.f;
+    if (bits8.scale == nullptr || bits8.amax != nullptr) {
+      float most = 0.f;
+      for (int64_t at = t * V; at < cols; at += STEP) {
+        float f[V];
+        normed(at, f);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i < cols - at) most = amax_step(most, f[i]);
+      }
+      most = row_max<kNormLongThreads>(most, slots[1]);
+      if (bits8.scale == nullptr) {
+        most = fmaxf(most, kLeast);
+        scale = most_of(bits8.fmt) / most;
+        if (t == 0) bits8.scale_inv[row] = most / most_of(bits8.fmt);
+      } else if (t == 0 && !(__builtin_nontemporal_load(bits8.amax) >= most)) {
+        atomic_max_nonneg(bits8.amax, most);
+      }
+    }
+    for (int64_t at = t * V; at < cols; at += STEP) {
+      float f[V];
+      normed(at, f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] *= scale;
+      store8<V>(bits8.q + row * cols + at, (int)(cols - at < V ? cols - at : V), f, bits8.fmt);
+    }
+  } else {
+    bits* const y = static_cast<bits*>(y_) + row * cols;
+    for (int64_t at = t * V; at < cols; at += STEP) {
+      float f[V];
+      normed(at, f);
+      E::store(y + at, (int)(cols - at), E::pack(f));
+    }
+  }
+}
+
+template <int TYPE, int PTYPE>
+__global__ __launch_bounds__(kNormLongThreads) void rms_norm_long_dx_kernel(
+    const void* __restrict__ dy_, int64_t ldy, const void* __restrict__ dh_, int64_t ldd, const void* __restrict__ h_, int64_t ldh,
+    const void* __restrict__ w, const float* __restrict__ rstd_in, void* __restrict__ dx_, int64_t first, int cols) {
+  typedef Elements<TYPE> E;
+  typedef typename E::bits bits;
+  constexpr int V = E::kVec, STEP = kNormLongThreads * V;
+  __shared__ float slots[kNormLongThreads / 64];
+  const int64_t row = first + blockIdx.x;
+  const int t = threadIdx.x;
+  const bits* const h = static_cast<const bits*>(h_) + row * ldh;
+  const bits* const dy = static_cast<const bits*>(dy_) + row * ldy;
+  const bits* const dh = dh_ != nullptr ? static_cast<const bits*>(dh_) + row * ldd : nullptr;
+  bits* const dx = static_cast<bits*>(dx_) + row * cols;
+  const float rstd = rstd_in[row];
+  float s = 0.f, c = 0.f;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int64_t at = t * V; at < cols; at += STEP) {
+      const int n = (int)(cols - at);
+      Parameters<TYPE, PTYPE> pw;
+      pw.load(w, (int)at, n);
+      float fh[V], fy[V], fw[V], fd[V] = {};
+      E::unpack(E::load(h + at, n), fh);
+      E::unpack(E::load(dy + at, n), fy);
+      if (pass == 1 && dh != nullptr) E::unpack(E::load(dh + at, n), fd);
+      pw.get(fw);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float z = i < n ? fh[i] * rstd : 0.f, g = fy[i] * fw[i];   // (behind the row's end an infinite rstd times zero)
+        s = __builtin_fmaf(g, z, s);
+        fd[i] = __builtin_fmaf(rstd, g - z * c, fd[i]);
+      }
+      if (pass == 1) E::store(dx + at, n, E::pack(fd));
+    }
+    if (pass == 0) c = row_sum<kNormLongThreads>(s, slots) / (float)cols;
+  }
+}
+
+// The weight's gradient: a thread keeps one piece of the columns for a slice of the rows.
+template <int TYPE>
+__global__ __launch_bounds__(256) void rms_norm_long_weight_kernel(
+    const void* __restrict__ dy_, int64_t ldy, const void* __restrict__ h_, int64_t ldh, const float* __restrict__ rstd_in,
+    float* __restrict__ part, int rows, int cols) {
+  typedef Elements<TYPE> E;
+  typedef typename E::bits bits;
+  constexpr int V = E::kVec;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+  if (at >= cols) return;
+  const int n = (int)(cols - at);
+  float dw[V] = {};
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float rstd = rstd_in[row];
+    float fh[V], fy[V];
+    E::unpack(E::load(static_cast<const bits*>(h_) + row * ldh + at, n), fh);
+    E::unpack(E::load(static_cast<const bits*>(dy_) + row * ldy + at, n), fy);
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[i] = __builtin_fmaf(fy[i], fh[i] * rstd, dw[i]);
+  }
+  float* const out = part + (int64_t)blockIdx.y * cols + at;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) out[i] = dw[i];
+}
+
+int backward_blocks(int64_t rows) { return (int)std::min<int64_t>(rows, 64); }
+
+int check_rms(int64_t rows, int cols, int type, int param_type) {
+  if (!known_type(type) || (param_type != type && param_type != FP8GMM_TYPE_FP32)) return FP8GMM_ERR_BAD_FORMAT;
+  // a row's offsets in 32 bits, with room for the last piece's
+  if (rows < 0 || rows > INT32_MAX || cols < 1 || cols > (1 << 30)) return FP8GMM_ERR_BAD_SHAPE;
+  return FP8GMM_OK;
+}
+
+struct Rows {
+  const void* x;
+  int64_t ldx;
+  const void* residual;
+  int64_t ldr;
+  const void* weight;
+  void* h;
+  int64_t rows;
+  int cols;
+  float eps;
+  int type, param_type;
+};
+
+// What both forward passes ask of their rows; 1: nothing to do
+int check_forward(const Rows& a) {
+  const int rc = check_rms(a.rows, a.cols, a.type, a.param_type);
+  if (rc != FP8GMM_OK) return rc;
+  if (a.ldx < a.cols || (a.residual != nullptr && a.ldr < a.cols)) return FP8GMM_ERR_BAD_SHAPE;
+  if (!(a.eps >= 0.f)) return FP8GMM_ERR_BAD_ARGUMENT;
+  if (a.rows == 0) return 1;
+  if (a.x == nullptr || a.weight == nullptr || (a.residual != nullptr && a.h == nullptr)) return FP8GMM_ERR_NULL_POINTER;
+  return FP8GMM_OK;
+}
+
+template <bool BITS8>
+int launch_forward(const Rows& a, void* y, const Bits8& bits8, float* rstd, hipStream_t s) {
+  with_types(a.type, a.param_type, [&](auto tc, auto pc) {
+    constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
+    for (int64_t r0 = 0; r0 < a.rows; r0 += kNormSlab)
+      hipLaunchKernelGGL((rms_norm_long_kernel<T, P, BITS8>), dim3((unsigned)std::min<int64_t>(kNormSlab, a.rows - r0)),
+                         dim3(kNormLongThreads), 0, s, a.x, a.ldx, a.residual, a.ldr, a.weight, y, bits8, a.h, rstd, r0, a.cols, a.eps);
+  });
+  return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace fp8gmm
+
+extern "C" {
+
+int fp8gmm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* y, void* h, float* rstd,
+                    int64_t rows, int cols, float eps, int type, int param_type, void* stream) {
+  using namespace fp8gmm;
+  const Rows a = {x, ldx, residual, ldr, weight, h, rows, cols, eps, type, param_type};
+  const int rc = check_forward(a);
+  if (rc != FP8GMM_OK) return rc == 1 ? FP8GMM_OK : rc;
+  if (y == nullptr) return FP8GMM_ERR_NULL_POINTER;
+  return launch_forward<false>(a, y, Bits8{}, rstd, static_cast<hipStream_t>(stream));
+}
+
+int fp8gmm_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* q, void* h,
+                        const float* scale, float* amax, float* scale_inv, int64_t rows, int cols, float eps, int type, int param_type,
+                        int fmt, void* stream) {
+  using namespace fp8gmm;
+  const Rows a = {x, ldx, residual, ldr, weight, h, rows, cols, eps, type, param_type};
+  const int rc = check_forward(a);
+  if (rc < 0) return rc;
+  if (fmt != FP8GMM_E4M3 && fmt != FP8GMM_E5M2) return FP8GMM_ERR_BAD_FORMAT;
+  if (rc == 1) return FP8GMM_OK;
+  if ((scale == nullptr) == (scale_inv == nullptr) || (scale == nullptr && amax != nullptr)) return FP8GMM_ERR_BAD_ARGUMENT;
+  if (q == nullptr) return FP8GMM_ERR_NULL_POINTER;
+  return launch_forward<true>(a, nullptr, Bits8{static_cast<uint8_t*>(q), scale, amax, scale_inv, fmt}, nullptr,
+                              static_cast<hipStream_t>(stream));
+}
+
+size_t fp8gmm_rms_norm_workspace_bytes(int64_t rows, int cols, int type) {
+  using namespace fp8gmm;
+  if (check_rms(rows, cols, type, type) != FP8GMM_OK) return 0;
+  return (size_t)backward_blocks(rows) * cols * sizeof(float);
+}
+
+int fp8gmm_rms_norm_backward(const void* dy, int64_t ldy, const void* dh, int64_t ldd, const void* h, int64_t ldh, const void* weight,
+                             const float* rstd, void* dx, void* dweight, int64_t rows, int cols, int type, int param_type,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace fp8gmm;
+  const int rc = check_rms(rows, cols, type, param_type);
+  if (rc != FP8GMM_OK) return rc;
+  if (ldy < cols || ldh < cols || (dh != nullptr && ldd < cols)) return FP8GMM_ERR_BAD_SHAPE;
+  if (rows > 0 && (dy == nullptr || h == nullptr || weight == nullptr || rstd == nullptr)) return FP8GMM_ERR_NULL_POINTER;
+  if (dweight != nullptr && rows > 0) {
+    if (workspace == nullptr) return FP8GMM_ERR_NULL_POINTER;
+    if (workspace_bytes < fp8gmm_rms_norm_workspace_bytes(rows, cols, type)) return FP8GMM_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return FP8GMM_ERR_ALIGNMENT;
+  }
+  if (dweight == nullptr && (dx == nullptr || rows == 0)) return FP8GMM_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  float* const part = static_cast<float*>(workspace);
+  const int blocks = backward_blocks(rows);
+  with_types(type, param_type, [&](auto tc, auto pc) {
+    constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
+    for (int64_t r0 = 0; dx != nullptr && r0 < rows; r0 += kNormSlab)
+      hipLaunchKernelGGL((rms_norm_long_dx_kernel<T, P>), dim3((unsigned)std::min<int64_t>(kNormSlab, rows - r0)), dim3(kNormLongThreads),
+                         0, s, dy, ldy, dh, ldd, h, ldh, weight, rstd, dx, r0, cols);
+    if (dweight == nullptr) return;
+    if (rows > 0)
+      hipLaunchKernelGGL((rms_norm_long_weight_kernel<T>), dim3(ceil_div(cols, 256 * Elements<T>::kVec), blocks), dim3(256), 0, s, dy, ldy,
+                         h, ldh, rstd, part, (int)rows, cols);
+    hipLaunchKernelGGL((norm_params_kernel<P>), dim3(ceil_div(cols, 64), 1), dim3(1024), 0, s, part, blocks, 1, cols, dweight,
+                       static_cast<void*>(nullptr));
+  });
+  return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -13,7 +13,7 @@ import torch
 from . import moe_ops
 from .grouped_linear import GroupedLinear
 from .grouped_mlp import GroupedMlp
-from .layers import LayerNorm
+from .layers import LayerNorm, RMSNorm
 from .native import Route, route
 
 
@@ -23,9 +23,10 @@ def _own(module, cls):
 
 
 class _RoutedModule(torch.nn.Module):
-    """``layer_norm``: the layer norms its rows (layers.LayerNorm) in front of the router and the experts."""
+    """``layer_norm`` / ``rms_norm``: the layer norms its rows (layers.LayerNorm, RMSNorm) in front of the router and the experts.
+    ``routing`` (moe_ops.Routing): how it chooses its experts, by default as the reference's example, the softmax's largest."""
 
-    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm=False):
+    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm=False, rms_norm=False, routing=None):
         super().__init__()
         self.n_embd = n_embd
         self.n_inner = n_inner
@@ -33,7 +34,14 @@ class _RoutedModule(torch.nn.Module):
         self.top_k = top_k
         self.sort_end_bit = max(int(np.ceil(np.log2(n_experts))), 1)
         self.gating_network = torch.nn.Linear(n_embd, n_experts, bias=False).to(dtype).to(device)
-        self.row_norm = LayerNorm(n_embd, dtype=dtype, device=device) if layer_norm else None
+        if layer_norm and rms_norm:
+            raise ValueError("a routed layer has one norm: layer_norm or rms_norm")
+        norm = LayerNorm if layer_norm else RMSNorm
+        self.row_norm = norm(n_embd, dtype=dtype, device=device) if layer_norm or rms_norm else None
+        self._routing = routing
+        if routing is not None:
+            self.tokens_per_expert = None   # of the last pass
+            self.register_buffer("expert_bias", torch.zeros(n_experts, device=device) if routing.bias else None)
         self._counts_host = None    # page-locked landing place of the per-expert counts, and the event of its copy
         self._counts_ready = None
 
@@ -92,15 +100,24 @@ class _RoutedModule(torch.nn.Module):
         # place where nothing else needs them, and without the inverse.
         own = getattr(self.compute, "__func__", None) is _RoutedModule.compute
         routing_logits, input = moe_ops.gating(self.gating_network, input) if own else (self.gating_network(input), input)
-        if own and moe_ops.router_fits(routing_logits, self.top_k, self.n_experts):
+        routing = getattr(self, "_routing", None)
+        if routing is None and own and moe_ops.router_fits(routing_logits, self.top_k, self.n_experts):
             expert_weights, indices, bin_ids, bins, tokens_per_expert, inverse, counts = route(routing_logits, self.top_k)
             return self._compute(input, tokens_per_expert, indices, bin_ids, expert_weights, bins, self.top_k, inverse, True, counts)
-        weights0, selected_experts = moe_ops.topk(routing_logits, self.top_k)
+        if routing is None:
+            weights0, selected_experts = moe_ops.topk(routing_logits, self.top_k)
+        else:
+            bias = self.expert_bias.float() if self.expert_bias is not None else None   # (a cast of the module casts it too)
+            weights0, selected_experts = moe_ops.select_experts(
+                routing_logits, self.top_k, routing.scoring, bias, routing.groups, routing.top_groups, routing.renormalize, routing.scale,
+                routing.group_best)
         expert_weights = weights0.flatten()
         top_experts = selected_experts.flatten()
         with torch.no_grad():
             indices, bin_ids, bins, tokens_per_expert, inverse = moe_ops.indices_bins_and_inverse(
                 top_experts, self.n_experts)
+        if routing is not None:
+            self.tokens_per_expert = tokens_per_expert
         if own:
             return self._compute(input, tokens_per_expert, indices, bin_ids, expert_weights, bins, self.top_k, inverse, True)
         return self.compute(input, tokens_per_expert, indices, bin_ids, expert_weights, bins, self.top_k)
@@ -110,8 +127,8 @@ class Fp8LinearModule(_RoutedModule):
     """Two ``GroupedLinear`` layers with an (erf) GELU between them (fp8_gmm/example.py:72-103)."""
 
     def __init__(self, n_embd, n_inner, n_experts, top_k, dtype=torch.bfloat16, cutlass=False, device="cuda",
-                 layer_norm=False):
-        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm)
+                 layer_norm=False, rms_norm=False, routing=None):
+        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm, rms_norm, routing)
         self.grouped_linear1 = GroupedLinear(n_embd, n_inner, n_experts, dtype=dtype, cutlass=cutlass, device=device)
         self.grouped_linear2 = GroupedLinear(n_inner, n_embd, n_experts, dtype=dtype, cutlass=cutlass, device=device)
         self.act = torch.nn.GELU()
@@ -139,8 +156,9 @@ class Fp8LinearModule(_RoutedModule):
 class Fp8MlpModule(_RoutedModule):
     """One ``GroupedMlp`` (tanh-GELU fused into the first GEMM) as the experts (fp8_gmm/example.py:106-130)."""
 
-    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype=torch.bfloat16, device="cuda", layer_norm=False):
-        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm)
+    def __init__(self, n_embd, n_inner, n_experts, top_k, dtype=torch.bfloat16, device="cuda", layer_norm=False, rms_norm=False,
+                 routing=None):
+        super().__init__(n_embd, n_inner, n_experts, top_k, dtype, device, layer_norm, rms_norm, routing)
         self.grouped_mlp = GroupedMlp(n_embd, n_inner, n_experts, dtype=dtype, device=device)
 
     def start_experts(self):

@@ -11,11 +11,14 @@ argument order and meaning, on HIP kernels of this package's library (csrc/route
     gather(x, indices, bin_ids, bins, top_k)           -> x[indices // top_k]               (autograd)
     scatter(x, indices, bin_ids, weights, bins, top_k) -> sum_k weights * rows, token order (autograd)
 
-plus ``indices_and_bins`` and ``topk`` of the example itself (example.py:15-32), the former as ONE library call.
+plus ``select_experts``, the choice of routers with more to it than a softmax (sigmoid scores, a bias for balance, groups of experts),
+and ``indices_and_bins`` and ``topk`` of the example itself (example.py:15-32), the former as ONE library call.
 Differences, stated where they matter: the weighted sum of ``scatter`` is accumulated in fp32 and rounded to bf16
 once (megablocks rounds every weighted row to the output type before adding), and ids outside ``[0, 2**end_bit)``
 are clamped into the range instead of being undefined.
 """
+from dataclasses import dataclass
+
 import torch
 
 from . import _lib, native
@@ -271,6 +274,45 @@ def topk(scores, top_k, moe_renorm=False):
     if moe_renorm:
         multiplier = multiplier / multiplier.sum(dim=-1, keepdim=True)
     return multiplier, selected_experts
+
+
+SCORINGS = ("softmax", "sigmoid")
+
+
+def select_experts(scores, top_k, scoring="softmax", bias=None, groups=1, top_groups=1, renormalize=False, scale=1.0, group_best=2):
+    """The experts of every token and their weights: ``(weights, selected)``, float32 and int64 ``[tokens, top_k]``, largest first.
+
+    With ``p`` the softmax of ``scores [tokens, experts]`` over the experts, or their sigmoid, and ``c = p + bias`` (``bias``: float32
+    ``[experts]`` or None): the experts lie in ``groups`` groups of neighbours, a group counts the sum of its ``group_best`` (1 or 2)
+    largest ``c``, the ``top_groups`` largest groups stay, and of their experts the ``top_k`` with the largest ``c`` are chosen.  The
+    weights are ``scale * p`` of these - the bias decides and weighs nothing - or, with ``renormalize``, ``scale * p / sum of the chosen
+    p``.  The choice is made as in exact arithmetic, by the scores where ``p`` alone decides and else in 64 bits: what agrees in
+    its first 40 bits counts as equal, and the lower number goes first.  A score that is a NaN goes last (but makes all of its token's
+    softmax one).
+
+    Scores: bfloat16, float16 or float32, up to 4096 experts in up to 16 groups, ``top_k`` up to 16.  Differentiable in the scores, by
+    the weights; the bias takes no gradient.  ``moe_ops.Routing`` has a routed layer choose so."""
+    if scoring not in SCORINGS:
+        _fail(f"fp8_gmm_amd: scoring must be one of {SCORINGS}, got {scoring!r}")
+    return native.select_experts(scores, top_k, scoring == "sigmoid", bias, groups, top_groups, group_best, renormalize, scale)
+
+
+@dataclass
+class Routing:
+    """How a routed layer chooses its experts (``moe``, ``routing=``): the options of ``select_experts``.  ``bias``: the layer has a bias
+    of zeros, its buffer ``expert_bias``, for the training loop to move against the load, ``layer.tokens_per_expert`` of the last pass."""
+
+    scoring: str = "softmax"
+    bias: bool = False
+    groups: int = 1
+    top_groups: int = 1
+    renormalize: bool = False
+    scale: float = 1.0
+    group_best: int = 2
+
+    def __post_init__(self):
+        if self.scoring not in SCORINGS:
+            raise ValueError(f"scoring must be one of {SCORINGS}, got {self.scoring!r}")
 
 
 def _check_rows(x, what):

@@ -1,8 +1,10 @@
-"""Between the backward pass and the optimizer: clipping of the gradients by their global norm.
+"""Behind the backward pass: clipping of the gradients by their global norm, and the optimizer's step.
 
-The operand-level calls are ``backend.multi_norm`` and ``backend.multi_clip``; this is the one on parameters, with the name and
-the arguments that torch's users know.
+The operand-level calls are ``backend.multi_norm``, ``backend.multi_clip`` and ``backend.multi_adamw``; these are the ones on
+parameters, with the names and the arguments that torch's users know.
 """
+from itertools import chain
+
 import torch
 
 from . import backend
@@ -27,3 +29,106 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         if error_if_nonfinite and not torch.isfinite(norm := backend.multi_norm(grads)):
             _fail(f"fp8_gmm_amd: the norm of the gradients is {norm.item()}")
         return backend.multi_clip(grads, grads, max_norm)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay, a launch for some dozens of parameters (``backend.multi_adamw``, which has the formulas).
+
+    ``state_bits``: 32, or 8 for moments in ``float8_e4m3fn`` with a float32 scale for every 128 elements, a quarter of the memory.
+    ``master_weights``: parameters of 16 bits are copies of float32 masters that the optimizer keeps.  ``max_norm``: every step clips
+    the gradients of all groups by their common norm on the way (they stay as they are); the norm before that is ``self.grad_norm``.
+    ``capturable``: the steps are counted on the device, a group's for all of its parameters, so that a captured step may be replayed;
+    ``lr`` may be a float32 tensor of the device then.  Run one step ahead of the capture: it makes the states.
+
+    Parameters are dense, on one device, bfloat16, float16 or float32; those without a gradient are passed over.  Without ``capturable``
+    each counts its own steps.  Checkpoints hold the states in their own types, whatever the parameters' (``state_dict``)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
+                 max_norm=None, capturable=False):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if not (isinstance(lr, torch.Tensor) or lr >= 0.0):
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("a tensor for lr needs capturable=True")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas must lie in [0, 1), got {betas}")
+        if not (eps >= 0.0 and weight_decay >= 0.0):
+            raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError(f"max_norm must not be negative, got {max_norm}")
+        self.state_bits, self.master_weights, self.max_norm, self.capturable = state_bits, master_weights, max_norm, capturable
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, steps=None))
+
+    def _init_state(self, p):
+        state = self.state[p]
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            _fail("fp8_gmm_amd: a parameter has no state yet: run a step ahead of the capture")
+        if not self.capturable:
+            state["step"] = 0
+        if self.state_bits == 8:
+            blocks = -(-p.numel() // 128)
+            for moment in ("exp_avg", "exp_avg_sq"):
+                state[moment] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
+                state[moment + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        else:
+            for moment in ("exp_avg", "exp_avg_sq"):
+                state[moment] = torch.zeros_like(p, dtype=torch.float32)
+        if self.master_weights and p.dtype != torch.float32:
+            state["master"] = p.detach().float()
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        taken = [[p for p in group["params"] if p.grad is not None] for group in self.param_groups]
+        first = next(chain.from_iterable(taken), None)
+        if not self.capturable and first is not None and first.is_cuda and torch.cuda.is_current_stream_capturing():
+            _fail("fp8_gmm_amd: a captured step needs AdamW(capturable=True): the others' number would be the same in every replay")
+        norm = None
+        if self.max_norm is not None and first is not None:
+            norm = self.grad_norm = backend.multi_norm([p.grad for p in chain.from_iterable(taken)])
+        for group, params in zip(self.param_groups, taken):
+            if not params:
+                continue
+            for p in params:
+                if not self.state[p]:
+                    self._init_state(p)
+            calls = {}   # the parameters of a call count the same step, and all have masters or none
+            if self.capturable:
+                if group["steps"] is None:
+                    group["steps"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
+                group["steps"].add_(1)
+            for p in params:
+                state = self.state[p]
+                if not self.capturable:
+                    state["step"] += 1
+                key = (group["steps"] if self.capturable else state["step"], "master" in state)
+                calls.setdefault(key, []).append(p)
+            for (step, masters), some in calls.items():
+                states = [self.state[p] for p in some]
+
+                def of(name):
+                    return [state[name] for state in states]
+
+                backend.multi_adamw(some, [p.grad for p in some], of("exp_avg"), of("exp_avg_sq"), step, group["lr"], tuple(group["betas"]),
+                                    group["eps"], group["weight_decay"],
+                                    (of("exp_avg_scale"), of("exp_avg_sq_scale")) if self.state_bits == 8 else None,
+                                    of("master") if masters else None, norm, None if norm is None else self.max_norm)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # torch has cast the states to their parameters' types
+        saved = chain.from_iterable(group["params"] for group in state_dict["param_groups"])
+        for key, p in zip(saved, chain.from_iterable(group["params"] for group in self.param_groups)):
+            for name, value in state_dict["state"].get(key, {}).items():
+                if isinstance(value, torch.Tensor):
+                    self.state[p][name] = value.detach().to(p.device, copy=True)
+        for group, old in zip(self.param_groups, state_dict["param_groups"]):
+            for name in ("steps", "lr"):
+                if isinstance(old.get(name), torch.Tensor):
+                    group[name] = old[name].detach().to(group["params"][0].device, copy=True)

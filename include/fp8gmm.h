@@ -43,7 +43,7 @@ extern "C" {
 #define FP8GMM_E5M2 1
 /* output kind of the GEMM epilogue */
 #define FP8GMM_OUT_BF16 2
-/* element types of the operators around the layers (layer norm, embedding, norm of many tensors) */
+/* element types of the operators around the layers (norms, embedding, routing, norm and steps of many tensors) */
 #define FP8GMM_TYPE_BF16 0
 #define FP8GMM_TYPE_FP16 1
 #define FP8GMM_TYPE_FP32 2
@@ -640,6 +640,31 @@ int fp8gmm_route_topk(const void* scores, int scores_bf16, int tokens, int num_e
 int fp8gmm_route_topk_backward(const float* probs, const int64_t* selected, const float* grad_weights, int tokens,
                                int num_experts, int top_k, void* grad_scores, int grad_bf16, void* stream);
 /*
+ * The choice of experts with what routers of many experts ask for beyond fp8gmm_route_topk (no counterpart in the reference).  With
+ * p = softmax(scores[t, :]) or sigmoid and c = p + bias: the experts lie in `groups` groups of neighbours, a group counts the sum of its
+ * `group_best` largest c, the `top_groups` largest groups stay, and of their experts the top_k largest c are chosen, largest first.
+ * selected[t, k]: their numbers, weights[t, k]: scale * p of each, with renormalize scale * p / (sum of the chosen p).  Compared are the scores
+ * themselves where p alone decides, else c and the sums in 64 bits; what agrees in its first 40 bits counts as equal, and the lower number
+ * goes first.  A score that is a NaN goes last.  scores: [tokens, experts] of `type` (FP8GMM_TYPE_*), contiguous; bias: fp32 [experts] or NULL.
+ * fp8gmm_select_experts_backward: the gradient of `weights` with respect to `scores`, in their type; the bias decides and takes none.
+ */
+#define FP8GMM_SCORING_SOFTMAX 0
+#define FP8GMM_SCORING_SIGMOID 1
+#define FP8GMM_MAX_CHOICES 16
+#define FP8GMM_MAX_CHOICE_EXPERTS 4096
+#define FP8GMM_MAX_CHOICE_GROUPS 16
+typedef struct fp8gmm_choice {
+  const float* bias;
+  int32_t experts, top_k;
+  int32_t scoring, groups, top_groups, group_best;
+  int32_t renormalize;
+  float scale;
+} fp8gmm_choice;          /* 40 bytes */
+int fp8gmm_select_experts(const void* scores, int type, int64_t tokens, const fp8gmm_choice* choice, float* weights, int64_t* selected,
+                          void* stream);
+int fp8gmm_select_experts_backward(const void* scores, int type, int64_t tokens, const fp8gmm_choice* choice, const int64_t* selected,
+                                   const float* grad_weights, void* grad_scores, void* stream);
+/*
  * The backward pass of a bias-free gating linear, logits = x weight^T (the gating_network of fp8_gmm/example.py:38,76,109):
  *   grad_weight = bf16(grad^T x),   grad_x = bf16(grad_in + grad weight),   products and sums in fp32, rounded once.
  * grad: bf16 [tokens, experts]; x, grad_in, grad_x: bf16 [tokens, hidden]; weight, grad_weight: bf16 [experts, hidden];
@@ -701,6 +726,30 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
                                const float* rstd, void* dx, void* dweight, void* dbias, int64_t rows, int cols, int type,
                                int param_type, void* workspace, size_t workspace_bytes, void* stream);
 /*
+ * fp8gmm_rms_norm: h = x + residual, rounded to `type` (residual NULL: h is x and not written), and
+ * y[r, :] = h[r, :] / sqrt(mean(h[r, :]^2) + eps) * weight.  x, residual: [rows, cols] of `type` with pitches of ldx, ldr >= cols
+ * elements; y, h: the same without a pitch; weight: [cols] of `param_type`, which is `type` or fp32.  rstd: fp32 [rows] for the backward
+ * pass, or NULL.  1 <= cols <= 2^30, rows < 2^31.  y, h (and q, dx below) lie apart from what is read.
+ * fp8gmm_rms_norm_fp8: the same norm in 8 bits, q: fp8 [rows, cols] of `fmt` (FP8GMM_E4M3 or _E5M2), saturating, a NaN stays one.
+ * With scale (device fp32): q = fp8(y * *scale), and *amax (may be NULL; holds a number that is not negative) is raised to max |y|.
+ * With scale_inv (fp32 [rows]) instead: scale_inv[r] = max(max |y[r, :]|, 2^-100) / the format's largest number, q = fp8(y / scale_inv).
+ */
+int fp8gmm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* y, void* h, float* rstd,
+                    int64_t rows, int cols, float eps, int type, int param_type, void* stream);
+int fp8gmm_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* q, void* h,
+                        const float* scale, float* amax, float* scale_inv, int64_t rows, int cols, float eps, int type, int param_type,
+                        int fmt, void* stream);
+/*
+ * Its gradients, from h as the forward pass returned it (x without a residual).  With z = h rstd and g = dy * weight:
+ * dx[r, :] = dh[r, :] + rstd (g - z mean(g z)), for x and the residual alike (dh NULL: zeros), dweight = sum over the rows of dy z; each
+ * may be NULL and is then not computed.  dx: [rows, cols] without a pitch.  workspace: fp8gmm_rms_norm_workspace_bytes bytes on 16 bytes
+ * where dweight is asked for and there are rows; without rows it is zeros.  The same bits from call to call.
+ */
+size_t fp8gmm_rms_norm_workspace_bytes(int64_t rows, int cols, int type);
+int fp8gmm_rms_norm_backward(const void* dy, int64_t ldy, const void* dh, int64_t ldd, const void* h, int64_t ldh, const void* weight,
+                             const float* rstd, void* dx, void* dweight, int64_t rows, int cols, int type, int param_type,
+                             void* workspace, size_t workspace_bytes, void* stream);
+/*
  * fp8gmm_embedding: y[t, :] = scale * weight[ids[t], :] for t in [0, n), a row of zeros where ids[t] is outside [0, table).
  * ids: int64 (ids64 != 0) or int32; weight: [table, cols] of `type`; n <= 2^28, table < 2^31 - 1, cols <= 2^23.
  * fp8gmm_embedding_backward: dweight[v, :] = scale * sum of dy[t, :] over the t with ids[t] == v, in a fixed order, the whole
@@ -731,6 +780,43 @@ size_t fp8gmm_multi_norm_workspace_bytes(int n);
 int fp8gmm_multi_norm(const fp8gmm_norm_tensor* tensors, int n, float* norm, void* workspace, size_t workspace_bytes, void* stream);
 int fp8gmm_multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm, float* norm, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/*
+ * fp8gmm_multi_adamw: one step of AdamW over n tensors.  With g = grad * min(1, max_norm / (norm + 1e-6)) (norm NULL: g = grad):
+ *   exp_avg += (1 - beta1) (g - exp_avg),  exp_avg_sq += (1 - beta2) (g^2 - exp_avg_sq),
+ *   p = p - lr weight_decay p - lr / (1 - beta1^t) exp_avg / (sqrt(exp_avg_sq / (1 - beta2^t)) + eps)
+ * in fp32, p being `master` (fp32) where there is one, of which param is then the rounded copy, else param itself; all tensors of a call
+ * with elements have masters or none has.  grad: of param's type or fp32.  bits 32: the moments are fp32.  bits 8: they are e4m3 codes, of
+ * exp_avg and of sqrt(exp_avg_sq), on 8 bytes, with an fp32 scale for each FP8GMM_ADAMW_BLOCK elements (the last block may be short); value
+ * = code * scale, scale = largest magnitude of the block / 448, 0 where that is below 2^-100 and the codes zeros.  Codes are rounded by
+ * thresholds u = frac((i * 0x6A09E667 + t * 0x9E3779B9) / 2^32) for element i (cut to 20 bits): exp_avg up where its way to the next
+ * code is at least 1 - u, the root, with u + 1/2 in place of u (24 bits), where its square's way to the next code's is more than that; a
+ * root that is not zero becomes no zero.
+ * t and lr: `step` (>= 1) and `lr`, or *step_dev and *lr_dev where these are given, which a replayed launch reads anew.  `tensors` is HOST
+ * memory and is read during the call only.  What is written overlaps nothing else of the call (FP8GMM_ERR_BAD_ARGUMENT).  At most 2^32
+ * elements each.
+ */
+#define FP8GMM_ADAMW_BLOCK 128
+typedef struct fp8gmm_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;      /* bits 8 */
+  float* exp_avg_sq_scale;
+  float* master;             /* or NULL */
+  int64_t count;             /* elements */
+  int32_t type, grad_type;
+} fp8gmm_adamw_tensor;       /* 72 bytes */
+typedef struct fp8gmm_adamw_step {
+  double lr, beta1, beta2, eps, weight_decay, max_norm;
+  const float* norm;         /* device, or NULL */
+  const int64_t* step_dev;   /* device, or NULL */
+  const float* lr_dev;       /* device, or NULL */
+  int64_t step;
+  int32_t bits, reserved;
+} fp8gmm_adamw_step;         /* 88 bytes */
+int fp8gmm_multi_adamw(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_step* step, void* stream);
 
 /* ---- schedule introspection (host only, no GPU needed) ------------------------------------ */
 /*
