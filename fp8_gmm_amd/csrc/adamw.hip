@@ -176,18 +176,6 @@ __device__ __forceinline__ float round_root(float y, uint32_t h) {
   return y == y ? cut_to_most(up ? hi : lo) : y;
 }
 
-// The largest over a row of 16 lanes: a block of 128 elements
-__device__ __forceinline__ float block_max(float v) {
-  const auto step = [&](auto control) {
-    v = fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(control)::value, 0xf, 0xf, true)));
-  };
-  step(std::integral_constant<int, 0xb1>{});
-  step(std::integral_constant<int, 0x4e>{});
-  step(std::integral_constant<int, 0x141>{});
-  step(std::integral_constant<int, 0x140>{});
-  return v;
-}
-
 // What a step multiplies by, the same for all elements
 struct Factors {
   float grad, rate, root, decay;
@@ -262,8 +250,8 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
   if constexpr (MASTER) F32::template store<FULL>(e.master, at, n, p);
   Values<TYPE, VEC>::template store<FULL>(e.param, at, n, p);
   if constexpr (BITS8) {
-    m_most = block_max(m_most);
-    v_most = block_max(v_most);
+    m_most = lanes_max<16>(m_most);   // of a block: 16 lanes of 8 elements
+    v_most = lanes_max<16>(v_most);
     const float m_inv = m_most >= kTiny ? kMost / m_most : 0.f, v_inv = v_most >= kTiny ? kMost / v_most : 0.f;
     const uint32_t first = (uint32_t)at * kElement + by.dither;
 #pragma unroll

@@ -1,5 +1,5 @@
-// Rows of bf16, fp16 or fp32 in pieces of 16 bytes, for the kernels that take all three (layer_norm.hip, embedding.hip,
-// multi_norm.hip).  A row may begin at any element: its pieces are loaded with the alignment of one, which the hardware
+// Rows of bf16, fp16 or fp32 in pieces of 16 bytes, for the kernels that take all three (layer_norm.hip, rms_norm.hip,
+// embedding.hip, multi_norm.hip, routing.hip, adamw.hip).  A row may begin at any element: its pieces are loaded with the alignment of one, which the hardware
 // takes as it takes aligned ones where a piece stays inside a line.
 #pragma once
 
@@ -128,6 +128,25 @@ __device__ __forceinline__ float lanes_sum(float v) {
     const int bits = __float_as_int(v);
     v = (__int_as_float(__builtin_amdgcn_readlane(bits, 0)) + __int_as_float(__builtin_amdgcn_readlane(bits, 16))) +
         (__int_as_float(__builtin_amdgcn_readlane(bits, 32)) + __int_as_float(__builtin_amdgcn_readlane(bits, 48)));
+  }
+  return v;
+}
+
+// The largest of numbers that are not negative, in the same way
+template <int WIDTH>
+__device__ __forceinline__ float lanes_max(float v) {
+  static_assert(WIDTH == 16 || WIDTH == 64, "a row of the data-parallel primitives, or a wavefront");
+  const auto step = [&](auto control) {
+    v = fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(control)::value, 0xf, 0xf, true)));
+  };
+  step(std::integral_constant<int, 0xb1>{});
+  step(std::integral_constant<int, 0x4e>{});
+  step(std::integral_constant<int, 0x141>{});
+  step(std::integral_constant<int, 0x140>{});
+  if constexpr (WIDTH == 64) {
+    const int bits = __float_as_int(v);
+    v = fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(bits, 0)), __int_as_float(__builtin_amdgcn_readlane(bits, 16))),
+              fmaxf(__int_as_float(__builtin_amdgcn_readlane(bits, 32)), __int_as_float(__builtin_amdgcn_readlane(bits, 48))));
   }
   return v;
 }

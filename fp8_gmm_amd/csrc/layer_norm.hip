@@ -407,13 +407,6 @@ __global__ __launch_bounds__(256) void layer_norm_long_params_kernel(
     }
 }
 
-// The longest rows that stay in registers have 4 pieces in each of 1024 threads, which fits fp32 alone: a 16-bit type has twice
-// the elements and spills backward (4096 x 32768, bf16: 103 and 781 us forward and backward, by the kernels for longer rows 146 and
-// 296; 4096 x 16384, fp32: 92 and 174, by those 142 and 287).
-Shape widest(int cols, int type) {
-  const int w = ceil_div(pieces_of(cols, type), 64 * 4);
-  return type == FP8GMM_TYPE_FP32 && w <= kNormWaves ? Shape{64, w, 4} : Shape{0, 0, 0};
-}
 // Forward, 4 pieces to a thread: few barriers and many loads under way (65536 x 2048, fp32: 185 us, with 2 pieces 193; 8192 x 16384,
 // bf16: 101 and 120; 16384 x 1536: 21.2 and 23.0; 16384 x 4093: 51 and 58, but 16384 x 4096 49 and 48).
 Shape forward_shape(int cols, int type) {
@@ -429,10 +422,6 @@ Shape backward_shape(int cols, int type, bool aligned) {
   if (type == FP8GMM_TYPE_FP32 && aligned && s.lanes != 16 && one.lanes != 0 && kBackwardThreads % one.threads() == 0) return one;
   return s.lanes != 0 ? s : widest(cols, type);
 }
-// Whether a result is written with the streaming hint: one that outgrows the cache is not found there by whoever reads it.  With it
-// and without: 16384 x 4096, bf16, forward 49 and 49 us, backward 73 and 78; 65536 x 2048, fp32, 185 and 191, 259 and 269; 24576 x
-// 2048, bf16, 36.4 and 37.2, 55.5 and 57.9.
-bool streams(int64_t rows, int cols, int type) { return rows * cols * type_bytes(type) > (int64_t)64 << 20; }
 // Workgroups of a backward pass: partial sums that its parameters' gradients have.  Of aligned rows no fewer than of others.
 int backward_blocks(int rows, int cols, int type, bool aligned) {
   const Shape s = backward_shape(cols, type, aligned);

@@ -118,6 +118,17 @@ struct Shape {
   const int w = ceil_div(pieces, 64 * most);
   return w <= waves ? Shape{64, w, ceil_div(pieces, 64 * w)} : Shape{0, 0, 0};
 }
+// The longest rows that stay in registers have 4 pieces in each of 1024 threads, which fits fp32 alone: a 16-bit type has twice
+// the elements and spills backward (4096 x 32768, bf16: 103 and 781 us forward and backward, by the kernels for longer rows 146 and
+// 296; 4096 x 16384, fp32: 92 and 174, by those 142 and 287).
+[[maybe_unused]] Shape widest(int cols, int type) {
+  const int w = ceil_div(pieces_of(cols, type), 64 * 4);
+  return type == FP8GMM_TYPE_FP32 && w <= kNormWaves ? Shape{64, w, 4} : Shape{0, 0, 0};
+}
+// Whether a result is written with the streaming hint: one that outgrows the cache is not found there by whoever reads it.  With it
+// and without: 16384 x 4096, bf16, forward 49 and 49 us, backward 73 and 78; 65536 x 2048, fp32, 185 and 191, 259 and 269; 24576 x
+// 2048, bf16, 36.4 and 37.2, 55.5 and 57.9.
+[[maybe_unused]] bool streams(int64_t rows, int cols, int type) { return rows * cols * type_bytes(type) > (int64_t)64 << 20; }
 // Rows of whole pieces on 16 bytes
 [[maybe_unused]] bool whole(const void* p, int64_t pitch, int cols, int type) {
   const int pieces = 16 / type_bytes(type);

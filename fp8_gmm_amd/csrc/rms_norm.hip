@@ -14,6 +14,12 @@
 namespace fp8gmm {
 namespace {
 
+constexpr int kBackwardThreads = 1024;   // of a workgroup of the backward pass: as many rows at a time as fit, since every workgroup
+constexpr int kBackwardBlocks = 256;     // leaves one partial sum of the weight's gradient in memory; one per compute unit
+constexpr int kBackwardAlone = 2;        // turns of one workgroup that take less than a second launch for the sums of several
+constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, where a row needs no more
+constexpr int kForwardAll = 256 * 2048, kForwardTurns = 5, kForwardMore = 3;
+
 // The least magnitude that a row's scale is made of: what is smaller is zero in 8 bits, and no scale is zero.
 constexpr float kLeast = 0x1p-100f;
 
@@ -60,7 +66,276 @@ struct Bits8 {
   int fmt;
 };
 
-// A row to a workgroup, read three times, from the cache the second and third time.
+// A workgroup takes ROWS rows at a time, LANES * waves threads to a row and C pieces to a thread, and goes on to other rows by the grid:
+// the next rows are loaded before the sums of the present ones are shared, and the weight stays in registers.
+template <int TYPE, int PTYPE, int LANES, int C, int MODE, int MOST, bool BITS8>
+__global__ __launch_bounds__(MOST) void rms_norm_kernel(
+    const void* __restrict__ x_, int64_t ldx, const void* __restrict__ residual_, int64_t ldr, const void* __restrict__ w,
+    void* __restrict__ y_, const Bits8 bits8, void* __restrict__ h_, float* __restrict__ rstd_out, int rows, int cols, float eps, int waves,
+    bool stream) {
+  typedef Elements<TYPE> E;
+  constexpr int V = E::kVec;
+  __shared__ float slots[2][kNormWaves][kNormWaves], tops[2][kNormWaves][kNormWaves];
+  const int THREADS = LANES * waves, ROWS = blockDim.x / THREADS;
+  int group = threadIdx.x / THREADS;
+  if constexpr (LANES == 64) group = __builtin_amdgcn_readfirstlane(group);
+  const int t = threadIdx.x - group * THREADS;
+  int at[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) at[c] = (c * THREADS + t) * V;
+  const int skip = piece_skip<MODE, V>(at[C - 1], cols);   // the pieces before the last one are there in whole
+  at[C - 1] = piece_begin<MODE, V>(at[C - 1], cols);
+  u32x4 nx[C], nr[C];
+  const auto load = [&](int64_t row) {
+    const RowAccess<TYPE, MODE> x(x_, row, rows, ldx, cols);
+#pragma unroll
+    for (int c = 0; c < C; ++c) nx[c] = x.template load<false>(at[c]);
+    if (residual_ != nullptr) {
+      const RowAccess<TYPE, MODE> residual(residual_, row, rows, ldr, cols);
+#pragma unroll
+      for (int c = 0; c < C; ++c) nr[c] = residual.template load<false>(at[c]);
+    }
+  };
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + group;
+  load(row);
+  Parameters<TYPE, PTYPE> pw[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) pw[c].load(w, at[c], cols - at[c]);
+  const int wave = LANES == 64 ? __builtin_amdgcn_readfirstlane(t / 64) : 0;
+  const int peer = threadIdx.x % 16;   // the wavefront whose share this lane takes up where they meet
+  const float count = (float)cols;
+  float top = 0.f;   // of all rows
+  const float tensor_scale = BITS8 && bits8.scale != nullptr ? *bits8.scale : 0.f;
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * ROWS; first < rows; first += stride, row += stride, turn ^= 1) {
+    u32x4 x[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] = nx[c];
+    if (residual_ != nullptr) {
+      const RowAccess<TYPE, MODE> h(h_, row, rows, cols, cols);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float f[V], a[V];
+        E::unpack(x[c], f);
+        E::unpack(nr[c], a);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] += a[i];
+        x[c] = E::pack(f);
+        h.store(at[c], x[c], stream);
+      }
+    }
+    if (first + stride < rows) load(row + stride);
+    float squares = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float f[V];
+      E::unpack(x[c], f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float v = !is_edge(MODE) || c < C - 1 || i >= skip ? f[i] : 0.f;
+        squares = __builtin_fmaf(v, v, squares);
+      }
+    }
+    squares = lanes_sum<LANES>(squares);
+    if (LANES == 64 && waves > 1) {   // the other turn's slots are read before the next barrier
+      if (threadIdx.x % 64 == 0) slots[turn][group][wave] = squares;
+      __syncthreads();
+      squares = lanes_sum<16>(peer < waves ? slots[turn][group][peer] : 0.f);
+    }
+    const float rstd = 1.0f / sqrtf(squares / count + eps);
+    if (rstd_out != nullptr && t == 0 && row < rows) rstd_out[row] = rstd;
+    const auto normed = [&](int c, float (&f)[V]) {
+      float fw[V];
+      E::unpack(x[c], f);
+      pw[c].get(fw);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = f[i] * rstd * fw[i];
+    };
+    if constexpr (BITS8) {
+      float scale = tensor_scale, most = 0.f;
+      if (bits8.scale == nullptr || bits8.amax != nullptr) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float f[V];
+          normed(c, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i)   // (a piece behind the end is zeros times the row's factor, be that infinite)
+            if (is_edge(MODE) || at[c] + i < cols) most = amax_step(most, f[i]);
+        }
+        if (bits8.scale != nullptr) top = fmaxf(top, most);
+      }
+      if (bits8.scale == nullptr) {
+        most = lanes_max<LANES>(most);
+        if (LANES == 64 && waves > 1) {
+          if (threadIdx.x % 64 == 0) tops[turn][group][wave] = most;
+          __syncthreads();
+          most = lanes_max<16>(peer < waves ? tops[turn][group][peer] : 0.f);
+        }
+        most = fmaxf(most, kLeast);
+        scale = most_of(bits8.fmt) / most;
+        if (t == 0 && row < rows) bits8.scale_inv[row] = most / most_of(bits8.fmt);
+      }
+      if (is_edge(MODE) || row < rows) {
+        uint8_t* const q = bits8.q + (row < rows ? row : rows - 1) * (int64_t)cols;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float f[V];
+          normed(c, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[i] *= scale;
+          if (is_edge(MODE) || at[c] < cols) store8<V>(q + at[c], MODE == kShort ? cols - at[c] : V, f, bits8.fmt);
+        }
+      }
+    } else {
+      const RowAccess<TYPE, MODE> y(y_, row, rows, cols, cols);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float f[V];
+        normed(c, f);
+        y.store(at[c], E::pack(f), stream);
+      }
+    }
+  }
+  if (BITS8 && bits8.amax != nullptr) {
+    __syncthreads();
+    top = lanes_max<64>(top);
+    float* const meet = &tops[0][0][0];
+    if (threadIdx.x % 64 == 0) meet[threadIdx.x / 64] = top;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < (int)(blockDim.x / 64); ++i) top = fmaxf(top, meet[i]);
+    if (!(__builtin_nontemporal_load(bits8.amax) >= top)) atomic_max_nonneg(bits8.amax, top);
+  }
+}
+
+// The backward pass in the same way, with the sums of dy z for the columns of its threads.  `part`: [workgroup][cols]; NULL where the
+// weight takes no gradient.  dx may be NULL.  A single workgroup writes the gradient itself.
+template <int TYPE, int PTYPE, int LANES, int C, int MODE>
+__global__ __launch_bounds__(kBackwardThreads) void rms_norm_backward_kernel(
+    const void* __restrict__ dy_, int64_t ldy, const void* __restrict__ dh_, int64_t ldd, const void* __restrict__ h_, int64_t ldh,
+    const void* __restrict__ w, const float* __restrict__ rstd_in, void* __restrict__ dx_, float* __restrict__ part,
+    void* __restrict__ dweight, int rows, int cols, int waves, bool stream) {
+  typedef Elements<TYPE> E;
+  constexpr int V = E::kVec;
+  __shared__ float slots[2][kNormWaves][kNormWaves];
+  __shared__ float sums[kBackwardThreads * V];
+  const int THREADS = LANES * waves, ROWS = blockDim.x / THREADS;
+  int group = threadIdx.x / THREADS;
+  if constexpr (LANES == 64) group = __builtin_amdgcn_readfirstlane(group);
+  const int t = threadIdx.x - group * THREADS;
+  const int wave = LANES == 64 ? __builtin_amdgcn_readfirstlane(t / 64) : 0, peer = threadIdx.x % 16;
+  int at[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) at[c] = (c * THREADS + t) * V;
+  const int skip = piece_skip<MODE, V>(at[C - 1], cols);   // the pieces before the last one are there in whole
+  at[C - 1] = piece_begin<MODE, V>(at[C - 1], cols);
+  Parameters<TYPE, PTYPE> pw[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) pw[c].load(w, at[c], cols - at[c]);
+  float dw[C][V] = {};
+  u32x4 nh[C], ny[C];
+  float nr;
+  const auto load = [&](int64_t row) {
+    const RowAccess<TYPE, MODE> h(h_, row, rows, ldh, cols), y(dy_, row, rows, ldy, cols);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      nh[c] = h.template load<true>(at[c]);
+      ny[c] = y.template load<true>(at[c]);
+    }
+    nr = row < rows ? rstd_in[row] : 0.f;
+  };
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + group;
+  load(row);
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * ROWS; first < rows; first += stride, row += stride, turn ^= 1) {
+    u32x4 h[C], y[C], d[C];   // d is wanted behind the sum alone: it comes with its own row, ahead of the next one's loads
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      h[c] = nh[c];
+      y[c] = ny[c];
+      d[c] = u32x4{0u, 0u, 0u, 0u};
+    }
+    if (dh_ != nullptr) {
+      const RowAccess<TYPE, MODE> from(dh_, row, rows, ldd, cols);
+#pragma unroll
+      for (int c = 0; c < C; ++c) d[c] = from.template load<true>(at[c]);
+    }
+    const float rstd = nr;
+    if (first + stride < rows) load(row + stride);
+    float s = 0.f;
+    if (!is_edge(MODE) || row < rows) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float fh[V], fy[V], fw[V];
+        E::unpack(h[c], fh);
+        E::unpack(y[c], fy);
+        pw[c].get(fw);
+        float u = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (is_edge(MODE) && c == C - 1 && i < skip) fy[i] = 0.f;   // elsewhere they are zeros
+          const float z = MODE != kShort || i < cols ? fh[i] * rstd : 0.f;
+          u = __builtin_fmaf(fy[i] * fw[i], z, u);
+          dw[c][i] = __builtin_fmaf(fy[i], z, dw[c][i]);
+        }
+        s += c < C - 1 || skip < V ? u : 0.f;   // nothing of a piece behind the end, whose zeros meet the row's factor, be that infinite
+      }
+    }
+    if (dx_ == nullptr) continue;
+    s = lanes_sum<LANES>(s);
+    if (LANES == 64 && waves > 1) {   // the other turn's slots are read before the next barrier
+      if (threadIdx.x % 64 == 0) slots[turn][group][wave] = s;
+      __syncthreads();
+      s = lanes_sum<16>(peer < waves ? slots[turn][group][peer] : 0.f);
+    }
+    if (is_edge(MODE) && row >= rows) continue;   // its sums leave no row out
+    const float mean = s / (float)cols;
+    const RowAccess<TYPE, MODE> dx(dx_, row, rows, cols, cols);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float fh[V], fy[V], fw[V], fd[V];
+      E::unpack(h[c], fh);
+      E::unpack(y[c], fy);
+      E::unpack(d[c], fd);
+      pw[c].get(fw);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        fd[i] = __builtin_fmaf(rstd, __builtin_fmaf(fy[i], fw[i], -(fh[i] * rstd) * mean), fd[i]);
+      dx.store(at[c], E::pack(fd), stream);
+    }
+  }
+  if (part == nullptr) return;
+  // the workgroup's rows together, in their order: THREADS * V columns at a time
+  float* const out = part + (int64_t)blockIdx.x * cols;
+  const auto write = [&](int64_t col, float sum) {
+    typedef Elements<PTYPE> P;
+    if (gridDim.x > 1) out[col] = sum;
+    else static_cast<typename P::bits*>(dweight)[col] = P::pack1(sum);
+  };
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (ROWS > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < V; ++i) sums[threadIdx.x * V + i] = dw[c][i];
+      __syncthreads();
+      for (int k = threadIdx.x; k < THREADS * V; k += blockDim.x) {
+        float sum = 0.f;
+        for (int r = 0; r < ROWS; ++r) sum += sums[r * THREADS * V + k];
+        const int piece = (c * THREADS + k / V) * V;
+        if (own<MODE>(k % V, piece_skip<MODE, V>(piece, cols), cols)) write(piece_begin<MODE, V>(piece, cols) + k % V, sum);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c < C - 1 || own<MODE>(i, skip, cols)) write(at[c] + i, dw[c][i]);
+    }
+  }
+}
+
+// Rows that no workgroup's registers hold are read up to three times, from the cache the second and third time.
 template <int TYPE, int PTYPE, bool BITS8>
 __global__ __launch_bounds__(kNormLongThreads) void rms_norm_long_kernel(
     const void* __restrict__ x_, int64_t ldx, const void* __restrict__ residual_, int64_t ldr, const void* __restrict__ w,
@@ -206,7 +481,21 @@ __global__ __launch_bounds__(256) void rms_norm_long_weight_kernel(
     if (i < n) out[i] = dw[i];
 }
 
-int backward_blocks(int64_t rows) { return (int)std::min<int64_t>(rows, 64); }
+Shape forward_shape(int cols, int type) {
+  const Shape s = shape_of(pieces_of(cols, type), 4, 8, 4);
+  return s.lanes != 0 ? s : widest(cols, type);
+}
+Shape backward_shape(int cols, int type) {
+  const Shape s = shape_of(pieces_of(cols, type), 2, kNormWaves, 2);
+  return s.lanes != 0 ? s : widest(cols, type);
+}
+// Workgroups of a backward pass: partial sums that its weight's gradient has.
+int backward_blocks(int64_t rows, int cols, int type) {
+  const Shape s = backward_shape(cols, type);
+  if (s.lanes == 0) return (int)std::min<int64_t>(rows, 64);
+  const int blocks = ceil_div(rows, kBackwardThreads / s.threads());
+  return blocks <= kBackwardAlone ? std::min(blocks, 1) : std::min(blocks, kBackwardBlocks);
+}
 
 int check_rms(int64_t rows, int cols, int type, int param_type) {
   if (!known_type(type) || (param_type != type && param_type != FP8GMM_TYPE_FP32)) return FP8GMM_ERR_BAD_FORMAT;
@@ -241,12 +530,45 @@ int check_forward(const Rows& a) {
 
 template <bool BITS8>
 int launch_forward(const Rows& a, void* y, const Bits8& bits8, float* rstd, hipStream_t s) {
+  const Shape shape = forward_shape(a.cols, a.type);
+  const int threads = shape.lanes == 0 ? 0 : std::max(shape.threads(), kForwardThreads / shape.threads() * shape.threads());
+  const bool streaming = streams(a.rows, a.cols, a.type);
+  const auto blocks = [&] {
+    const int groups = ceil_div(a.rows, threads / shape.threads()), all = kForwardAll / threads;   // rows that a workgroup takes at a time
+    return std::min(groups, groups > kForwardTurns * all ? kForwardMore * all : all);
+  };
+  const bool aligned = whole(a.x, a.ldx, a.cols, a.type) && (a.residual == nullptr || (whole(a.residual, a.ldr, a.cols, a.type) &&
+                       whole(a.h, a.cols, a.cols, a.type))) && (BITS8 || whole(y, a.cols, a.cols, a.type));
+  const int mode = mode_of(a.cols, a.type, shape.lanes, aligned, streaming);
+  bool known = true;   // a row's share of the registers that no launch below is for would leave the results unwritten
   with_types(a.type, a.param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
-    for (int64_t r0 = 0; r0 < a.rows; r0 += kNormSlab)
+#define FP8GMM_LAUNCH(LANES, C, MOST)                                                                                                \
+  if (shape.lanes == LANES && shape.pieces == C && threads <= MOST) {                                                                \
+    auto* kernel = mode == kEdge         ? &rms_norm_kernel<T, P, LANES, C, kEdge, MOST, BITS8>                                      \
+                   : mode == kEdgeStream ? &rms_norm_kernel<T, P, LANES, C, kEdgeStream, MOST, BITS8>                                \
+                                         : &rms_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge, MOST, BITS8>; \
+    hipLaunchKernelGGL(kernel, dim3(blocks()), dim3(threads), 0, s, a.x, a.ldx, a.residual, a.ldr, a.weight, y, bits8, a.h, rstd,     \
+                       (int)a.rows, a.cols, a.eps, shape.waves, streaming);                                                          \
+  } else
+    FP8GMM_LAUNCH(16, 1, 256)
+    FP8GMM_LAUNCH(16, 2, 256)
+    FP8GMM_LAUNCH(16, 3, 256)
+    FP8GMM_LAUNCH(16, 4, 256)
+    FP8GMM_LAUNCH(64, 2, 512)   // (one piece to each of 64 lanes is 16 lanes' share)
+    FP8GMM_LAUNCH(64, 3, 512)
+    FP8GMM_LAUNCH(64, 4, 512)
+    if constexpr (T == FP8GMM_TYPE_FP32) {
+      FP8GMM_LAUNCH(64, 4, 1024) known = shape.lanes == 0;
+    } else {
+      known = shape.lanes == 0;
+    }
+#undef FP8GMM_LAUNCH
+    for (int64_t r0 = 0; shape.lanes == 0 && r0 < a.rows; r0 += kNormSlab)
       hipLaunchKernelGGL((rms_norm_long_kernel<T, P, BITS8>), dim3((unsigned)std::min<int64_t>(kNormSlab, a.rows - r0)),
                          dim3(kNormLongThreads), 0, s, a.x, a.ldx, a.residual, a.ldr, a.weight, y, bits8, a.h, rstd, r0, a.cols, a.eps);
   });
+  if (!known) return FP8GMM_ERR_LAUNCH;
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
@@ -283,7 +605,7 @@ int fp8gmm_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_
 size_t fp8gmm_rms_norm_workspace_bytes(int64_t rows, int cols, int type) {
   using namespace fp8gmm;
   if (check_rms(rows, cols, type, type) != FP8GMM_OK) return 0;
-  return (size_t)backward_blocks(rows) * cols * sizeof(float);
+  return (size_t)backward_blocks(rows, cols, type) * cols * sizeof(float);
 }
 
 int fp8gmm_rms_norm_backward(const void* dy, int64_t ldy, const void* dh, int64_t ldd, const void* h, int64_t ldh, const void* weight,
@@ -301,20 +623,50 @@ int fp8gmm_rms_norm_backward(const void* dy, int64_t ldy, const void* dh, int64_
   }
   if (dweight == nullptr && (dx == nullptr || rows == 0)) return FP8GMM_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  float* const part = static_cast<float*>(workspace);
-  const int blocks = backward_blocks(rows);
+  float* const part = dweight != nullptr ? static_cast<float*>(workspace) : nullptr;
+  const int blocks = backward_blocks(rows, cols, type);
+  const Shape shape = backward_shape(cols, type);
+  const bool aligned = whole(h, ldh, cols, type) && whole(dy, ldy, cols, type) && (dh == nullptr || whole(dh, ldd, cols, type)) &&
+                       (dx == nullptr || whole(dx, cols, cols, type));
+  const bool streaming = streams(rows, cols, type);
+  const int mode = mode_of(cols, type, shape.lanes, aligned, streaming && type == FP8GMM_TYPE_FP32);
+  bool known = true;
   with_types(type, param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
-    for (int64_t r0 = 0; dx != nullptr && r0 < rows; r0 += kNormSlab)
-      hipLaunchKernelGGL((rms_norm_long_dx_kernel<T, P>), dim3((unsigned)std::min<int64_t>(kNormSlab, rows - r0)), dim3(kNormLongThreads),
-                         0, s, dy, ldy, dh, ldd, h, ldh, weight, rstd, dx, r0, cols);
-    if (dweight == nullptr) return;
-    if (rows > 0)
-      hipLaunchKernelGGL((rms_norm_long_weight_kernel<T>), dim3(ceil_div(cols, 256 * Elements<T>::kVec), blocks), dim3(256), 0, s, dy, ldy,
-                         h, ldh, rstd, part, (int)rows, cols);
-    hipLaunchKernelGGL((norm_params_kernel<P>), dim3(ceil_div(cols, 64), 1), dim3(1024), 0, s, part, blocks, 1, cols, dweight,
-                       static_cast<void*>(nullptr));
+    constexpr int kStreamed = T == FP8GMM_TYPE_FP32 ? kEdgeStream : kEdge;
+    if (rows > 0) {
+#define FP8GMM_LAUNCH(LANES, C)                                                                                                      \
+  if (shape.lanes == LANES && shape.pieces == C) {                                                                                   \
+    auto* kernel = mode == kEdge         ? &rms_norm_backward_kernel<T, P, LANES, C, kEdge>                                          \
+                   : mode == kEdgeStream ? &rms_norm_backward_kernel<T, P, LANES, C, kStreamed>                                      \
+                                         : &rms_norm_backward_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge>; \
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBackwardThreads / shape.threads() * shape.threads()), 0, s, dy, ldy, dh, ldd, h, ldh, \
+                       weight, rstd, dx, part, dweight, (int)rows, cols, shape.waves, streaming);                                    \
+  } else
+      FP8GMM_LAUNCH(16, 1)
+      FP8GMM_LAUNCH(16, 2)
+      FP8GMM_LAUNCH(64, 1)
+      FP8GMM_LAUNCH(64, 2)
+      if constexpr (T == FP8GMM_TYPE_FP32) {
+        FP8GMM_LAUNCH(64, 4) known = shape.lanes == 0;
+      } else {
+        known = shape.lanes == 0;
+      }
+#undef FP8GMM_LAUNCH
+      if (shape.lanes == 0) {
+        for (int64_t r0 = 0; dx != nullptr && r0 < rows; r0 += kNormSlab)
+          hipLaunchKernelGGL((rms_norm_long_dx_kernel<T, P>), dim3((unsigned)std::min<int64_t>(kNormSlab, rows - r0)),
+                             dim3(kNormLongThreads), 0, s, dy, ldy, dh, ldd, h, ldh, weight, rstd, dx, r0, cols);
+        if (dweight != nullptr)
+          hipLaunchKernelGGL((rms_norm_long_weight_kernel<T>), dim3(ceil_div(cols, 256 * Elements<T>::kVec), blocks), dim3(256), 0, s, dy,
+                             ldy, h, ldh, rstd, part, (int)rows, cols);
+      }
+    }
+    if (dweight != nullptr && (blocks != 1 || shape.lanes == 0))
+      hipLaunchKernelGGL((norm_params_kernel<P>), dim3(ceil_div(cols, 64), 1), dim3(1024), 0, s, part, blocks, 1, cols, dweight,
+                         static_cast<void*>(nullptr));
   });
+  if (!known) return FP8GMM_ERR_LAUNCH;
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 
