@@ -7,12 +7,13 @@
 //   w = scale p[chosen], with `renormalize` scale p[chosen] / sum of p[chosen]
 //
 // What is compared decides where a token goes, so it is compared exactly: the scores themselves where p alone would decide (it grows
-// with them), else c and the groups' sums in 64 bits.  A key is such a number with the last 12 bits of its fraction replaced by the
-// expert's number, so no two keys are equal, the largest key names its expert, and numbers that agree in their first 40 bits count as
-// equal.  The weights are fp32.
+// with them), else c and the groups' sums in 64 bits.  A key is such a number that holds the expert's number in its last bits, so no two
+// keys are equal and the largest names its expert: 16 bits of a score and 15 of the number, or a number in 64 bits whose last 12 bits of
+// the fraction are replaced (what agrees in its first 40 bits counts as equal).  The weights are fp32.
 //
-// LANES lanes have a token, 16 (a row of the data-parallel primitives) or 64, with PER neighbouring experts in the registers of each:
-// a round takes the largest key of every lane's own, exchanges them in log2(LANES) steps, and strikes it out.
+// LANES lanes have a token, 8 or 16 (of a row of the data-parallel primitives) or 64, with PER neighbouring experts in the registers of
+// each: a round takes the largest key of every lane's own, exchanges them in log2(LANES) steps, and strikes it out.  Bound by these
+// instructions, not by the scores' bytes.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,14 +24,13 @@ namespace {
 
 constexpr int kMaxChoices = FP8GMM_MAX_CHOICES;
 constexpr int kThreads = 256;
-constexpr double kFar = 1e300;          // nearer to zero than what is struck out; scores and sums are cut to it
-constexpr double kStruck = -1.7e308;
 
-// exp(x) for x <= 0 or moderate x, 2^-46 relative: 2^n times the series of exp to its eleventh power, on a remainder of at most
-// ln(2) / 2, whose next term is below 2^-47.
+// exp(x), 2^-46 relative: 2^n times the series of exp to its eleventh power, on a remainder of at most ln(2) / 2, whose next term is
+// below 2^-47.  Cut to e^-700 and e^700; a NaN comes out as one of these.
 __device__ __forceinline__ double exp64(double x) {
-  const double cut = fmin(fmax(x, -700.), 700.), n = rint(cut * 1.4426950408889634);
-  double f = __builtin_fma(n, -0.6931471805599453, cut);
+  x = fmin(fmax(x, -700.), 700.);
+  const double n = rint(x * 1.4426950408889634);
+  double f = __builtin_fma(n, -0.6931471805599453, x);
   f = __builtin_fma(n, -2.3190468138462996e-17, f);
   double p = 1. / 39916800.;
   p = __builtin_fma(p, f, 1. / 3628800.);
@@ -44,81 +44,167 @@ __device__ __forceinline__ double exp64(double x) {
   p = __builtin_fma(p, f, .5);
   p = __builtin_fma(p, f, 1.);
   p = __builtin_fma(p, f, 1.);
-  return x == x ? __builtin_ldexp(p, (int)n) : x;
+  return __builtin_ldexp(p, (int)n);
+}
+// 1 / d for 1 <= d <= e^701: the hardware's first guess and two of Newton's steps
+__device__ __forceinline__ double rcp64(double d) {
+  double r = __builtin_amdgcn_rcp(d);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
+  return __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
 }
 __device__ __forceinline__ float sigmoid(float s) { return 1.f / (1.f + expf(-s)); }
 
-// The key of a number: what is no number goes last.  `number` < 4096.
-__device__ __forceinline__ double key_of(double v, int number) {
+// Keys of 64 bits.  What is no number goes last, with minus infinity.
+typedef double key64;
+constexpr double kStruck64 = -1.7e308, kFar = 1e300;   // what is struck out, and what numbers and sums are cut to
+// (an instruction: fmax would look for NaN in both, which keys are not)
+__device__ __forceinline__ key64 larger(key64 a, key64 b) {
+  key64 r;
+  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ key64 smaller(key64 a, key64 b) {
+  key64 r;
+  asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+// `number` < 4096
+__device__ __forceinline__ key64 key_of(double v, int number) {
   v = fmin(fmax(v, -kFar), kFar) + 0.;   // (one zero, not two)
   const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-  return __builtin_bit_cast(double, (bits & ~0xfffull) | (uint64_t)(v < 0. ? number : 4095 - number));
+  return __builtin_bit_cast(double, (bits & ~0xfffull) | (uint64_t)((int64_t)bits < 0 ? number : 4095 - number));
 }
-__device__ __forceinline__ int number_of(double key) {
-  const int low = (int)(__builtin_bit_cast(uint64_t, key) & 0xfff);
-  return key < 0. ? low : 4095 - low;
+__device__ __forceinline__ int number_of(key64 key) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, key);
+  const int low = (int)(bits & 0xfff);
+  return (int64_t)bits < 0 ? low : 4095 - low;
 }
+__device__ __forceinline__ void strike(key64& key, bool gone) {   // the upper half does
+  const uint64_t bits = __builtin_bit_cast(uint64_t, key);
+  const uint32_t hi = gone ? (uint32_t)(__builtin_bit_cast(uint64_t, kStruck64) >> 32) : (uint32_t)(bits >> 32);
+  key = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)bits);
+}
+
+// Keys of 31 bits, of 16-bit scores
+typedef uint32_t key32;
+template <int TYPE>
+__device__ __forceinline__ key32 key_of_bits(uint32_t b, int number) {
+  constexpr uint32_t kInf = TYPE == FP8GMM_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+  if ((b & 0x7fffu) > kInf) b = 0x8000u | kInf;   // a NaN goes last, with minus infinity
+  if (b == 0x8000u) b = 0u;                       // one zero, not two
+  const uint32_t order = b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+  return order << 15 | (uint32_t)(0x7fff - number);
+}
+__device__ __forceinline__ key32 larger(key32 a, key32 b) { return max(a, b); }
+__device__ __forceinline__ int number_of(key32 key) { return 0x7fff - (int)(key & 0x7fffu); }
+__device__ __forceinline__ void strike(key32& key, bool gone) { key = gone ? 0u : key; }
 
 // v of another lane of the row of 16
 template <int CONTROL>
-__device__ __forceinline__ double lane64(double v) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CONTROL, 0xf, 0xf, true);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CONTROL, 0xf, 0xf, true);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+__device__ __forceinline__ uint32_t other_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xf, 0xf, true);
 }
 template <int CONTROL>
-__device__ __forceinline__ float lane32(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xf, 0xf, true));
+__device__ __forceinline__ float other_lane(float v) {
+  return __uint_as_float(other_lane<CONTROL>(__float_as_uint(v)));
+}
+template <int CONTROL>
+__device__ __forceinline__ double other_lane(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)other_lane<CONTROL>((uint32_t)(b >> 32)) << 32 | other_lane<CONTROL>((uint32_t)b));
+}
+// v of lane i of the wavefront, for all of them
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); }
+__device__ __forceinline__ float lane_of(float v, int i) { return __uint_as_float(lane_of(__float_as_uint(v), i)); }
+__device__ __forceinline__ double lane_of(double v, int i) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)lane_of((uint32_t)(b >> 32), i) << 32 | lane_of((uint32_t)b, i));
 }
 // f joined over the lanes of a token, the same in all of them
-template <int LANES, class F>
-__device__ __forceinline__ double over64(double v, F&& f) {
-  v = f(v, lane64<0xb1>(v));
-  v = f(v, lane64<0x4e>(v));
-  v = f(v, lane64<0x141>(v));
-  v = f(v, lane64<0x140>(v));
-  if constexpr (LANES == 64) {
-    v = f(v, __shfl_xor(v, 16, 64));
-    v = f(v, __shfl_xor(v, 32, 64));
-  }
+template <int LANES, class T, class F>
+__device__ __forceinline__ T over(T v, F&& f) {
+  v = f(v, other_lane<0xb1>(v));    // quad_perm: the neighbour
+  v = f(v, other_lane<0x4e>(v));    // quad_perm: the other pair
+  v = f(v, other_lane<0x141>(v));   // row_half_mirror: the other four
+  if constexpr (LANES > 8) v = f(v, other_lane<0x140>(v));   // row_mirror: the other eight
+  if constexpr (LANES == 64) v = f(f(lane_of(v, 0), lane_of(v, 16)), f(lane_of(v, 32), lane_of(v, 48)));
   return v;
 }
-template <int LANES, class F>
-__device__ __forceinline__ float over32(float v, F&& f) {
-  v = f(v, lane32<0xb1>(v));
-  v = f(v, lane32<0x4e>(v));
-  v = f(v, lane32<0x141>(v));
-  v = f(v, lane32<0x140>(v));
-  if constexpr (LANES == 64) {
-    v = f(v, __shfl_xor(v, 16, 64));
-    v = f(v, __shfl_xor(v, 32, 64));
-  }
-  return v;
-}
+struct LargerKey {
+  template <class K>
+  __device__ __forceinline__ K operator()(K a, K b) const { return larger(a, b); }
+};
 struct Largest {
-  __device__ double operator()(double a, double b) const { return fmax(a, b); }
-  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
 struct Sum {
-  __device__ double operator()(double a, double b) const { return a + b; }
-  __device__ float operator()(float a, float b) const { return a + b; }
+  template <class T>
+  __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
 };
 
-// A lane's experts: e0 .. e0 + PER - 1 of the row, minus infinity behind its end
+// A lane's experts, e0 .. e0 + PER - 1 of the row: pieces of V elements, one by one where the row ends
 template <int TYPE, int PER>
-__device__ __forceinline__ void load_scores(const void* scores, int64_t token, int experts, int e0, float (&s)[PER]) {
+struct Piece {
   typedef Elements<TYPE> E;
-  const typename E::bits* const row = static_cast<const typename E::bits*>(scores) + token * experts;
-  constexpr int V = E::kVec < PER ? E::kVec : PER;
+  typedef typename E::bits bits;
+  static constexpr int V = E::kVec < PER ? E::kVec : PER, kCount = PER / V, kBytes = V * E::kBytes;
+  typedef uint32_t half_piece __attribute__((ext_vector_type(2), aligned(2)));
+  typedef uint32_t quarter_piece __attribute__((aligned(2)));
+  u32x4 raw[kCount];
+  __device__ __forceinline__ void load(const void* base, int64_t first, int left) {
+    const bits* const p = static_cast<const bits*>(base) + first;
 #pragma unroll
-  for (int j = 0; j < PER; j += V) {
-    float f[E::kVec];
-    E::unpack(E::load(row + e0 + j, V < E::kVec ? min(V, experts - e0 - j) : experts - e0 - j), f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[j + i] = e0 + j + i < experts ? f[i] : -INFINITY;
+    for (int i = 0; i < kCount; ++i) {
+      if constexpr (kBytes == 16) {
+        raw[i] = E::load(p + i * V, left - i * V);
+      } else {
+        raw[i] = u32x4{0u, 0u, 0u, 0u};
+        if (left >= V) {
+          if constexpr (kBytes == 8) {
+            const u32x2 v = *reinterpret_cast<const half_piece*>(p);
+            raw[i].x = v.x;
+            raw[i].y = v.y;
+          } else if constexpr (kBytes == 4) {
+            raw[i].x = *reinterpret_cast<const quarter_piece*>(p);
+          } else {
+            raw[i].x = *p;
+          }
+        } else {
+          raw[i] = E::load(p, left);
+        }
+      }
+    }
   }
-}
+  __device__ __forceinline__ void get(float (&s)[PER], int left) const {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      float f[E::kVec];
+      E::unpack(raw[i], f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[i * V + j] = i * V + j < left ? f[j] : -INFINITY;
+    }
+  }
+  __device__ __forceinline__ uint32_t bits16(int j) const { return raw[j / V][j % V / 2] >> j % 2 * 16 & 0xffffu; }
+  static __device__ __forceinline__ void store(void* base, int64_t first, int left, const float (&s)[PER]) {
+    bits* const p = static_cast<bits*>(base) + first;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      float f[E::kVec] = {};
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = s[i * V + j];
+      const u32x4 v = E::pack(f);
+      if constexpr (kBytes == 16) {
+        E::store(p + i * V, left - i * V, v);
+      } else if (left >= V) {
+        if constexpr (kBytes == 8) *reinterpret_cast<half_piece*>(p) = u32x2{v.x, v.y};
+        else if constexpr (kBytes == 4) *reinterpret_cast<quarter_piece*>(p) = v.x;
+        else *p = (bits)v.x;
+      } else {
+        E::store(p, left, v);
+      }
+    }
+  }
+};
 template <int TYPE>
 __device__ __forceinline__ float score_of(const void* scores, int64_t token, int experts, int e) {
   typedef Elements<TYPE> E;
@@ -134,101 +220,178 @@ struct Choice {
   float scale;
 };
 
-// The two largest of what two lanes or experts have
-__device__ __forceinline__ void take_two(double& first, double& second, double v) {
-  second = fmax(second, fmin(first, v));
-  first = fmax(first, v);
+// Which experts' groups stay: strikes the others' keys out.  A group's key is its largest expert's (BEST 1), or made of the sum of its
+// two largest and the group's number.
+template <int LANES, int PER, int BEST, class K>
+__device__ __forceinline__ void keep_groups(K (&key)[PER], const Choice& c, int lane) {
+  const int size = c.experts / c.groups;
+  const auto take = [](K& first, K& second, K v) {
+    if constexpr (BEST == 2) second = larger(second, smaller(first, v));
+    first = larger(first, v);
+  };
+  const auto join = [&](K& first, K& second, K a, K b) {
+    take(first, second, a);
+    if constexpr (BEST == 2) second = larger(second, b);
+  };
+  const auto made = [&](K first, K second, int g) {
+    if constexpr (BEST == 2) return key_of(size > 1 ? first + second : first, g);
+    else return first;
+  };
+  K none = key[0];
+  strike(none, true);
+  // groups of whole lanes, a power of two of them in a row: every lane looks at its own group
+  const int span = size / PER;
+  if (c.experts == LANES * PER && size % PER == 0 && span <= (LANES > 8 ? 16 : 8) && (span & (span - 1)) == 0) {
+    K first = key[0], second = none;
+    if constexpr (BEST == 2) second = -kFar;
+#pragma unroll
+    for (int j = 1; j < PER; ++j) take(first, second, key[j]);
+    if (span > 1) join(first, second, other_lane<0xb1>(first), other_lane<0xb1>(second));
+    if (span > 2) join(first, second, other_lane<0x4e>(first), other_lane<0x4e>(second));
+    if (span > 4) join(first, second, other_lane<0x141>(first), other_lane<0x141>(second));
+    if (LANES > 8 && span > 8) join(first, second, other_lane<0x140>(first), other_lane<0x140>(second));
+    K mine = made(first, second, lane / span);
+    bool kept = false;
+    for (int i = 0; i < c.top_groups; ++i) {
+      const K best = over<LANES>(mine, LargerKey{});
+      const bool it = mine == best;
+      kept = kept || it;
+      strike(mine, it);
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) strike(key[j], !kept);
+    return;
+  }
+  // any others: one after the other, lane g keeps the key of group g (there are no more groups than lanes)
+  K mine = none;
+  for (int g = 0; g < c.groups; ++g) {
+    K first = none, second = none;
+    if constexpr (BEST == 2) first = second = -kFar;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if ((uint32_t)(lane * PER + j - g * size) < (uint32_t)size) take(first, second, key[j]);
+    const auto pair = [&](auto control) {
+      constexpr int CONTROL = decltype(control)::value;
+      const K a = other_lane<CONTROL>(first), b = other_lane<CONTROL>(second);
+      join(first, second, a, b);
+    };
+    pair(std::integral_constant<int, 0xb1>{});
+    pair(std::integral_constant<int, 0x4e>{});
+    pair(std::integral_constant<int, 0x141>{});
+    if constexpr (LANES > 8) pair(std::integral_constant<int, 0x140>{});
+    if constexpr (LANES == 64) {
+      const K a = first, b = second;
+      first = lane_of(a, 0);
+      second = lane_of(b, 0);
+#pragma unroll
+      for (int i = 16; i < 64; i += 16) join(first, second, lane_of(a, i), lane_of(b, i));
+    }
+    if (g == lane) mine = made(first, second, g);
+  }
+  uint32_t kept = 0;
+  for (int i = 0; i < c.top_groups; ++i) {
+    const K best = over<LANES>(mine, LargerKey{});
+    kept |= 1u << (BEST == 2 ? number_of(best) : number_of(best) / size);
+    strike(mine, mine == best);
+  }
+  int g = lane * PER / size, rest = lane * PER - g * size;   // of a lane's first expert
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    strike(key[j], !(kept >> (g & 31) & 1));
+    if (++rest == size) rest = 0, ++g;
+  }
 }
 
-template <int TYPE, int LANES, int PER>
+// The top_k largest keys' numbers, number k in lane k.  Keys of 31 bits stay as they are: less the last one taken, modulo 2^32, those
+// below it are the largest, in their order.
+template <int LANES, int PER, class K>
+__device__ __forceinline__ int take_largest(K (&key)[PER], int top_k, int lane) {
+  K mine = key[0], last = K();
+  if constexpr (std::is_same_v<K, key32>) last = 1u << 31;
+  for (int k = 0; k < top_k; ++k) {
+    K best;
+    if constexpr (std::is_same_v<K, key32>) {
+      best = key[0] - last;
+#pragma unroll
+      for (int j = 1; j < PER; ++j) best = larger(best, key[j] - last);
+      best = last = over<LANES>(best, LargerKey{}) + last;
+    } else {
+      best = key[0];
+#pragma unroll
+      for (int j = 1; j < PER; ++j) best = larger(best, key[j]);
+      best = over<LANES>(best, LargerKey{});
+      const int at = number_of(best) - lane * PER;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) strike(key[j], at == j);
+    }
+    if (k == lane) mine = best;
+  }
+  return number_of(mine);
+}
+
+// SCORES: the scores decide; else p in 64 bits does, with the bias or for the groups' sums
+template <int TYPE, int LANES, int PER, bool SCORES>
 __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __restrict__ scores, int tokens, const Choice c,
                                                                   float* __restrict__ weights, int64_t* __restrict__ selected) {
   const int lane = threadIdx.x % LANES;
   const int64_t token = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool live = token < tokens;   // the others' lanes are read by nobody, but go along
   const int64_t from = live ? token : tokens - 1;
-  const int e0 = lane * PER;
+  const int e0 = lane * PER, left = c.experts - e0;
+  Piece<TYPE, PER> piece;
+  piece.load(scores, from * c.experts + e0, left);
   float s[PER];
-  load_scores<TYPE, PER>(scores, from, c.experts, e0, s);
+  piece.get(s, left);
   float most = 0.f, total = 1.f;   // of the softmax
   if (!c.sigmoid) {
-    float m = -INFINITY;
+    float m = s[0];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) m = fmaxf(m, s[j]);
-    most = over32<LANES>(m, Largest{});
+    for (int j = 1; j < PER; ++j) m = fmaxf(m, s[j]);
+    most = over<LANES>(m, Largest{});
   }
-  const bool by_scores = c.bias == nullptr && (c.groups == 1 || c.group_best == 1);
-  double key[PER];
-  if (by_scores) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = e0 + j < c.experts ? key_of((double)s[j], e0 + j) : kStruck;
+  const bool grouped = c.top_groups < c.groups;
+  int chosen;
+  if constexpr (SCORES) {
     if (!c.sigmoid) {
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) sum += e0 + j < c.experts ? expf(s[j] - most) : 0.f;
-      total = over32<LANES>(sum, Sum{});
+      for (int j = 0; j < PER; ++j) sum += j < left ? expf(s[j] - most) : 0.f;
+      total = over<LANES>(sum, Sum{});
     }
+    std::conditional_t<TYPE == FP8GMM_TYPE_FP32, key64, key32> key[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if constexpr (TYPE == FP8GMM_TYPE_FP32) key[j] = key_of((double)s[j], e0 + j);
+      else key[j] = key_of_bits<TYPE>(piece.bits16(j), e0 + j);
+      strike(key[j], j >= left);
+    }
+    if (grouped) keep_groups<LANES, PER, 1>(key, c, lane);
+    chosen = take_largest<LANES>(key, c.top_k, lane);
   } else {
     double p[PER], sum = 0.;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      p[j] = c.sigmoid ? 1. / (1. + exp64(-(double)s[j])) : exp64((double)s[j] - (double)most);
-      sum += e0 + j < c.experts ? p[j] : 0.;
+      const double e = exp64(c.sigmoid ? -(double)s[j] : (double)s[j] - (double)most);
+      p[j] = c.sigmoid ? rcp64(1. + e) : e;
+      if (s[j] != s[j]) p[j] = (double)s[j];
+      sum += j < left ? p[j] : 0.;
     }
+    double inv = 1.;
     if (!c.sigmoid) {
-      sum = over64<LANES>(sum, Sum{});
+      sum = over<LANES>(sum, Sum{});
       total = (float)sum;
+      inv = 1. / sum;
     }
+    key64 key[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      if (!c.sigmoid) p[j] /= sum;
-      if (c.bias != nullptr && e0 + j < c.experts) p[j] += (double)c.bias[e0 + j];
-      key[j] = e0 + j < c.experts ? key_of(p[j], e0 + j) : kStruck;
+      p[j] *= inv;
+      if (c.bias != nullptr && j < left) p[j] += (double)c.bias[e0 + j];
+      key[j] = key_of(p[j], e0 + j);
+      strike(key[j], j >= left);
     }
-  }
-  if (c.groups > 1 && c.top_groups < c.groups) {
-    const int size = c.experts / c.groups;
-    double mine = kStruck;   // the key of the group that a lane stands for
-    uint32_t kept = 0;
-    for (int g = 0; g < c.groups; ++g) {
-      double first = -kFar, second = -kFar;
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if ((uint32_t)(e0 + j - g * size) < (uint32_t)size) take_two(first, second, key[j]);
-      const auto join = [&](double a, double b) {
-        take_two(first, second, a);
-        second = fmax(second, b);
-      };
-      join(lane64<0xb1>(first), lane64<0xb1>(second));
-      join(lane64<0x4e>(first), lane64<0x4e>(second));
-      join(lane64<0x141>(first), lane64<0x141>(second));
-      join(lane64<0x140>(first), lane64<0x140>(second));
-      if constexpr (LANES == 64) {
-        join(__shfl_xor(first, 16, 64), __shfl_xor(second, 16, 64));
-        join(__shfl_xor(first, 32, 64), __shfl_xor(second, 32, 64));
-      }
-      const double value = c.group_best == 2 && size > 1 ? first + second : first;
-      if (g == lane) mine = key_of(value, g);
-    }
-    for (int i = 0; i < c.top_groups; ++i) {
-      const double best = over64<LANES>(mine, Largest{});
-      kept |= 1u << (number_of(best) & 31);
-      if (mine == best) mine = kStruck;
-    }
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (e0 + j < c.experts && !(kept >> ((e0 + j) / size) & 1)) key[j] = kStruck;
-  }
-  int chosen = 0;
-  for (int k = 0; k < c.top_k; ++k) {
-    double best = key[0];
-#pragma unroll
-    for (int j = 1; j < PER; ++j) best = fmax(best, key[j]);
-    best = over64<LANES>(best, Largest{});
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (key[j] == best) key[j] = kStruck;
-    if (k == lane) chosen = number_of(best);
+    if (grouped) c.group_best == 2 ? keep_groups<LANES, PER, 2>(key, c, lane) : keep_groups<LANES, PER, 1>(key, c, lane);
+    chosen = take_largest<LANES>(key, c.top_k, lane);
   }
   const bool has = lane < c.top_k;
   float w = 0.f;
@@ -236,7 +399,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
     const float v = score_of<TYPE>(scores, from, c.experts, chosen);
     w = c.sigmoid ? sigmoid(v) : expf(v - most) / total;
   }
-  if (c.renormalize) w /= over32<LANES>(w, Sum{});
+  if (c.renormalize) w /= over<LANES>(w, Sum{});
   if (has && live) {
     weights[token * c.top_k + lane] = w * c.scale;
     selected[token * c.top_k + lane] = chosen;
@@ -250,26 +413,27 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
                                                                            const int64_t* __restrict__ selected,
                                                                            const float* __restrict__ grad_weights,
                                                                            void* __restrict__ grad_scores) {
-  typedef Elements<TYPE> E;
   const int lane = threadIdx.x % LANES;
   const int64_t token = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool live = token < tokens;
   const int64_t from = live ? token : tokens - 1;
-  const int e0 = lane * PER;
+  const int e0 = lane * PER, left = c.experts - e0;
   float s[PER], most = 0.f, total = 1.f;
   if (!c.sigmoid) {
-    load_scores<TYPE, PER>(scores, from, c.experts, e0, s);
-    float m = -INFINITY;
+    Piece<TYPE, PER> piece;
+    piece.load(scores, from * c.experts + e0, left);
+    piece.get(s, left);
+    float m = s[0];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) m = fmaxf(m, s[j]);
-    most = over32<LANES>(m, Largest{});
+    for (int j = 1; j < PER; ++j) m = fmaxf(m, s[j]);
+    most = over<LANES>(m, Largest{});
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      s[j] = e0 + j < c.experts ? expf(s[j] - most) : 0.f;
+      s[j] = j < left ? expf(s[j] - most) : 0.f;
       sum += s[j];
     }
-    total = over32<LANES>(sum, Sum{});
+    total = over<LANES>(sum, Sum{});
   }
   const bool has = lane < c.top_k;
   int chosen = -1;
@@ -287,10 +451,10 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
     }
   }
   if (c.renormalize) {
-    const float sum = over32<LANES>(p, Sum{}), dot = over32<LANES>(g * p, Sum{});
+    const float sum = over<LANES>(p, Sum{}), dot = over<LANES>(g * p, Sum{});
     g = has ? (g - dot / sum) / sum : 0.f;
   }
-  const float back = c.sigmoid ? 0.f : over32<LANES>(g * p, Sum{});
+  const float back = c.sigmoid ? 0.f : over<LANES>(g * p, Sum{});
   if (c.sigmoid) g *= p * rest;
   float out[PER];
 #pragma unroll
@@ -301,34 +465,37 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
 #pragma unroll
     for (int j = 0; j < PER; ++j) out[j] = at == j ? v : out[j];
   }
+  const float inv = 1.f / total;
   if (!c.sigmoid)
 #pragma unroll
-    for (int j = 0; j < PER; ++j) out[j] = s[j] / total * (out[j] - back);
+    for (int j = 0; j < PER; ++j) out[j] = s[j] * inv * (out[j] - back);
   if (!live) return;
-  typename E::bits* const row = static_cast<typename E::bits*>(grad_scores) + token * c.experts;
-  constexpr int V = E::kVec < PER ? E::kVec : PER;
-#pragma unroll
-  for (int j = 0; j < PER; j += V) {
-    float f[E::kVec] = {};
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = out[j + i];
-    E::store(row + e0 + j, V < E::kVec ? min(V, c.experts - e0 - j) : c.experts - e0 - j, E::pack(f));
-  }
+  Piece<TYPE, PER>::store(grad_scores, token * c.experts + e0, left, out);
 }
 
 // calls f(TYPE, LANES, PER): 16 lanes up to 512 experts, as few of them to each as there are sizes for
+constexpr int kFewTokens = 2048;
 template <class F>
-void with_shape(int type, int experts, F&& f) {
+void with_shape(int type, int64_t tokens, const Choice& c, F&& f) {
+  const bool few = tokens <= kFewTokens;
+  const int experts = c.experts;
   const auto shape = [&](auto t) {
     const auto as = [&](auto lanes, auto per) { f(t, lanes, per); };
+    constexpr std::integral_constant<int, 8> half{};
     constexpr std::integral_constant<int, 16> row{};
     constexpr std::integral_constant<int, 64> wave{};
-    if (experts <= 16) as(row, std::integral_constant<int, 1>{});
-    else if (experts <= 32) as(row, std::integral_constant<int, 2>{});
-    else if (experts <= 64) as(row, std::integral_constant<int, 4>{});
-    else if (experts <= 128) as(row, std::integral_constant<int, 8>{});
-    else if (experts <= 256) as(row, std::integral_constant<int, 16>{});
-    else if (experts <= 512) as(row, std::integral_constant<int, 32>{});
+    if (c.top_k <= 8 && c.groups <= 8 && experts <= 64) {
+      if (experts <= 16) as(half, std::integral_constant<int, 2>{});
+      else if (experts <= 32) as(half, std::integral_constant<int, 4>{});
+      else as(half, std::integral_constant<int, 8>{});
+    } else if (experts <= 64) {
+      if (experts <= 16) as(row, std::integral_constant<int, 1>{});
+      else if (experts <= 32) as(row, std::integral_constant<int, 2>{});
+      else as(row, std::integral_constant<int, 4>{});
+    }
+    else if (experts <= 128) few ? as(wave, std::integral_constant<int, 2>{}) : as(row, std::integral_constant<int, 8>{});
+    else if (experts <= 256) few ? as(wave, std::integral_constant<int, 4>{}) : as(row, std::integral_constant<int, 16>{});
+    else if (experts <= 512) few ? as(wave, std::integral_constant<int, 8>{}) : as(row, std::integral_constant<int, 32>{});
     else if (experts <= 1024) as(wave, std::integral_constant<int, 16>{});
     else as(wave, std::integral_constant<int, 64>{});
   };
@@ -364,10 +531,12 @@ int fp8gmm_select_experts(const void* scores, int type, int64_t tokens, const fp
   if (tokens == 0) return FP8GMM_OK;
   if (scores == nullptr || weights == nullptr || selected == nullptr) return FP8GMM_ERR_NULL_POINTER;
   const Choice c = choice_of(*choice);
-  with_shape(type, c.experts, [&](auto t, auto lanes, auto per) {
+  with_shape(type, tokens, c, [&](auto t, auto lanes, auto per) {
     constexpr int TOKENS = kThreads / decltype(lanes)::value;
-    hipLaunchKernelGGL((select_experts_kernel<decltype(t)::value, decltype(lanes)::value, decltype(per)::value>),
-                       dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
+    const bool by_scores = c.bias == nullptr && (c.top_groups == c.groups || c.group_best == 1);
+    auto* kernel = by_scores ? &select_experts_kernel<decltype(t)::value, decltype(lanes)::value, decltype(per)::value, true>
+                             : &select_experts_kernel<decltype(t)::value, decltype(lanes)::value, decltype(per)::value, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
                        (int)tokens, c, weights, selected);
   });
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
@@ -381,7 +550,7 @@ int fp8gmm_select_experts_backward(const void* scores, int type, int64_t tokens,
   if (tokens == 0) return FP8GMM_OK;
   if (scores == nullptr || selected == nullptr || grad_weights == nullptr || grad_scores == nullptr) return FP8GMM_ERR_NULL_POINTER;
   const Choice c = choice_of(*choice);
-  with_shape(type, c.experts, [&](auto t, auto lanes, auto per) {
+  with_shape(type, tokens, c, [&](auto t, auto lanes, auto per) {
     constexpr int TOKENS = kThreads / decltype(lanes)::value;
     hipLaunchKernelGGL((select_experts_backward_kernel<decltype(t)::value, decltype(lanes)::value, decltype(per)::value>),
                        dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
