@@ -23,7 +23,7 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 44;         // of a launch's arguments
+constexpr int kSweep = 4096;         // elements of a workgroup, several to a thread at a time
 constexpr int kBlock = FP8GMM_ADAMW_BLOCK;
 constexpr float kMost = Fp8Limits<FP8GMM_E4M3>::kMax;
 constexpr float kTiny = 0x1p-100f;   // moments below it are zeros in 8 bits
@@ -37,12 +37,64 @@ struct Entry {
   float *m_scale, *v_scale, *master;
   int64_t count;
   uint32_t begin;   // first chunk
-  uint16_t type, grad_type;
+  int type, grad_type;
 };
+// The tensors of a launch travel in its arguments, 48 bits of each of PTRS addresses, 40 of the count, and the types: nothing is uploaded,
+// and a captured call holds its table.
+template <int PTRS>
 struct Part {
-  Entry e[kTensors];
+  static constexpr int kWords = 3 * PTRS + 3, kTensors = 3600 / (4 + 2 * kWords);
+  uint32_t begin[kTensors];
+  uint16_t word[kTensors][kWords];
 };
-static_assert(sizeof(Part) <= 3600, "the arguments of a launch");
+constexpr int pointers(bool master, bool bits8) { return 4 + (bits8 ? 2 : 0) + (master ? 1 : 0); }
+template <bool MASTER, bool BITS8>
+using PartOf = Part<pointers(MASTER, BITS8)>;
+
+template <bool MASTER, bool BITS8>
+void pack(PartOf<MASTER, BITS8>& part, int at, const Entry& e) {
+  part.begin[at] = e.begin;
+  uint16_t* w = part.word[at];
+  const auto put = [&](uint64_t v) {
+    for (int k = 0; k < 3; ++k) *w++ = (uint16_t)(v >> 16 * k);
+  };
+  const auto address = [&](const void* p) { put(reinterpret_cast<uintptr_t>(p)); };
+  address(e.param);
+  address(e.grad);
+  address(e.m);
+  address(e.v);
+  if (BITS8) {
+    address(e.m_scale);
+    address(e.v_scale);
+  }
+  if (MASTER) address(e.master);
+  put((uint64_t)e.count | (uint64_t)e.type << 40 | (uint64_t)e.grad_type << 44);
+}
+template <bool MASTER, bool BITS8>
+__device__ __forceinline__ Entry unpack(const PartOf<MASTER, BITS8>& part, int at) {
+  Entry e = {};
+  e.begin = part.begin[at];
+  const uint16_t* w = part.word[at];
+  const auto get = [&] {
+    const uint64_t v = (uint64_t)w[0] | (uint64_t)w[1] << 16 | (uint64_t)w[2] << 32;
+    w += 3;
+    return v;
+  };
+  e.param = reinterpret_cast<void*>(get());
+  e.grad = reinterpret_cast<const void*>(get());
+  e.m = reinterpret_cast<void*>(get());
+  e.v = reinterpret_cast<void*>(get());
+  if constexpr (BITS8) {
+    e.m_scale = reinterpret_cast<float*>(get());
+    e.v_scale = reinterpret_cast<float*>(get());
+  }
+  if constexpr (MASTER) e.master = reinterpret_cast<float*>(get());
+  const uint64_t last = get();
+  e.count = (int64_t)(last & 0xffffffffffull);
+  e.type = (int)(last >> 40 & 0xf);
+  e.grad_type = (int)(last >> 44);
+  return e;
+}
 
 struct Hyper {
   float c1, c2;       // 1 - beta
@@ -135,16 +187,9 @@ struct Codes {
       f[4 * i + 3] = hi.y;
     }
   }
-  // of numbers that are codes
   template <bool FULL>
-  static __device__ __forceinline__ void store(void* base, int64_t at, int n, const float (&f)[8]) {
+  static __device__ __forceinline__ void store(void* base, int64_t at, int n, u32x2 w) {
     uint8_t* const p = static_cast<uint8_t*>(base) + at;
-    u32x2 w;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
-      w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], lo, true);
-    }
     if constexpr (FULL) {
       *reinterpret_cast<u32x2*>(p) = w;
     } else {
@@ -155,25 +200,28 @@ struct Codes {
   }
 };
 
-// The codes lie 2^(e-3) apart from 2^e on, from 2^-6 down 2^-9: adding 2^-6 there makes the distance that of all numbers with its
-// exponent, and the last 20 bits of the fraction what lies between two codes.
-__device__ __forceinline__ float below_normal(float magnitude) { return magnitude < 0x1p-6f ? 0x1p-6f : 0.f; }
-__device__ __forceinline__ float cut_to_most(float v) { return v > kMost ? kMost : v; }   // (a NaN stays)
-
-// y to a code, up with the probability of its way to the next one
-__device__ __forceinline__ float round_linear(float y, uint32_t h) {
-  const float a = fabsf(y), off = below_normal(a);
-  const float code = __uint_as_float((__float_as_uint(a + off) + (h >> 12)) & 0xfff00000u) - off;
-  return y == y ? __builtin_copysignf(cut_to_most(code), y) : y;
+// y to a code, up with the probability of its way to the next one: the hardware's rounding by a random number, of which it adds the upper
+// 20 bits to what lies between two codes.  Byte I of `old`.
+template <int I>
+__device__ __forceinline__ uint32_t round_linear(float y, uint32_t h, uint32_t old) {
+  return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(y, (int)h, (int)old, I);
 }
-// y >= 0 to a code, up with the probability of its square's way to the next one's
+// y >= 0 to a code, up with the probability of its square's way to the next one's.  The codes lie 2^(e-3) apart from 2^e on, from 2^-6
+// down 2^-9: adding 2^-6 there makes the distance that of all numbers with its exponent, and the last 20 bits of the fraction what
+// lies between two codes.  A NaN stays one: it comes from a product, so its first bit of the fraction is set.
 __device__ __forceinline__ float round_root(float y, uint32_t h) {
-  const float off = below_normal(y);
-  const uint32_t low = __float_as_uint(y + off) & 0xfff00000u;
-  const float lo = __uint_as_float(low) - off, hi = __uint_as_float(low + 0x00100000u) - off;
-  const float u = (float)((h ^ 0x80000000u) >> 8) * 0x1p-24f;
-  const bool up = (y - lo) * (y + lo) > u * ((hi - lo) * (hi + lo)) || (lo == 0.f && y > 0.f);
-  return y == y ? cut_to_most(up ? hi : lo) : y;
+  const float off = y < 0x1p-6f ? 0x1p-6f : 0.f;
+  const uint32_t bits = __float_as_uint(y + off);
+  const float lo = __uint_as_float(bits & 0xfff00000u) - off, gap = __uint_as_float(bits & 0x7f800000u) * 0.125f;
+  const float ways = gap * __builtin_fmaf(2.f, lo, gap);                                    // the squares' distance
+  const float u1 = __uint_as_float(h >> 9 ^ 0x3fc00000u);                                   // 1 + the threshold
+  const bool up = (y - lo) * (y + lo) > __builtin_fmaf(u1, ways, -ways);
+  const float code = up ? lo + gap : lo;
+  return y > 0.f ? fmaxf(code, 0x1p-9f) : code;
+}
+// 448 / most, not above it: no product with a magnitude up to `most` rounds to more than 448, whose next code is none
+__device__ __forceinline__ float to_codes(float most) {
+  return most >= kTiny ? __uint_as_float(__float_as_uint(kMost / most) - 1u) : 0.f;
 }
 
 // What a step multiplies by, the same for all elements
@@ -228,7 +276,8 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
   grad.get(g);
   mc.get(m);
   vc.get(v);
-  float m_most = 0.f, v_most = 0.f;
+  float m_most = 0.f, v_most = 0.f, root[VEC];
+  bool small = false;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     g[i] *= by.grad;
@@ -239,12 +288,23 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
     }
     m[i] = __builtin_fmaf(h.c1, g[i] - m[i], m[i]);
     v[i] = __builtin_fmaf(h.c2, __builtin_fmaf(g[i], g[i], -v[i]), v[i]);
-    const float root = sqrtf(v[i]);
-    p[i] = __builtin_fmaf(-by.decay, p[i], p[i]) - by.rate * (m[i] / __builtin_fmaf(root, by.root, h.eps));
+    root[i] = __builtin_amdgcn_sqrtf(v[i]);   // good to 2 roundings, and 0 of a subnormal number
+    small = small || __builtin_isfpclass(v[i], 0x90);
+  }
+  if (__builtin_expect(small, 0)) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) root[i] = sqrtf(v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const float d = __builtin_fmaf(root[i], by.root, h.eps);
+    float r = __builtin_amdgcn_rcpf(d);   // and a step of Newton's: 4 instructions for a division's 10
+    r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
+    p[i] = __builtin_fmaf(-by.rate, m[i] * r, __builtin_fmaf(-by.decay, p[i], p[i]));
+    if constexpr (MASTER) asm("" : "+v"(p[i]));   // fp32 first, then 16 bits: the weight is the master's rounded copy
     if constexpr (BITS8) {
-      v[i] = root;
       m_most = fmaxf(m_most, fabsf(m[i]));
-      v_most = fmaxf(v_most, root);
+      v_most = fmaxf(v_most, root[i]);
     }
   }
   if constexpr (MASTER) F32::template store<FULL>(e.master, at, n, p);
@@ -252,39 +312,53 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
   if constexpr (BITS8) {
     m_most = lanes_max<16>(m_most);   // of a block: 16 lanes of 8 elements
     v_most = lanes_max<16>(v_most);
-    const float m_inv = m_most >= kTiny ? kMost / m_most : 0.f, v_inv = v_most >= kTiny ? kMost / v_most : 0.f;
+    const float m_inv = to_codes(m_most), v_inv = to_codes(v_most);
     const uint32_t first = (uint32_t)at * kElement + by.dither;
+    u32x2 mw = {0u, 0u}, vw;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const uint32_t threshold = first + i * kElement;
-      m[i] = round_linear(m[i] * m_inv, threshold);
-      v[i] = round_root(v[i] * v_inv, threshold);
+    for (int i = 0; i < 2; ++i) {
+      const int j = 4 * i;
+      mw[i] = round_linear<0>(m[j] * m_inv, first + j * kElement, mw[i]);
+      mw[i] = round_linear<1>(m[j + 1] * m_inv, first + (j + 1) * kElement, mw[i]);
+      mw[i] = round_linear<2>(m[j + 2] * m_inv, first + (j + 2) * kElement, mw[i]);
+      mw[i] = round_linear<3>(m[j + 3] * m_inv, first + (j + 3) * kElement, mw[i]);
+      float c[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) c[k] = round_root(root[j + k] * v_inv, first + (j + k) * kElement);
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+      vw[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
     }
     if (threadIdx.x % 16 == 0 && (FULL || n > 0)) {
       e.m_scale[at / kBlock] = m_most / kMost;
       e.v_scale[at / kBlock] = v_most / kMost;
     }
+    Codes::store<FULL>(e.m, at, n, mw);
+    Codes::store<FULL>(e.v, at, n, vw);
+  } else {
+    F32::template store<FULL>(e.m, at, n, m);
+    F32::template store<FULL>(e.v, at, n, v);
   }
-  decltype(mc)::template store<FULL>(e.m, at, n, m);
-  decltype(vc)::template store<FULL>(e.v, at, n, v);
 }
 
 template <bool MASTER, bool BITS8>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const Part part, int n, const Hyper h) {
-  constexpr int VEC = BITS8 ? 8 : 4, CHUNK = kThreads * VEC;
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const PartOf<MASTER, BITS8> part, int n, const Hyper h) {
+  constexpr int VEC = BITS8 ? 8 : 4, STEP = kThreads * VEC;
   __shared__ int found;
   for (int i = threadIdx.x; i < n; i += kThreads)
-    if (part.e[i].begin <= blockIdx.x && (i + 1 == n || blockIdx.x < part.e[i + 1].begin)) found = i;
+    if (part.begin[i] <= blockIdx.x && (i + 1 == n || blockIdx.x < part.begin[i + 1])) found = i;
   __syncthreads();
-  const Entry e = part.e[__builtin_amdgcn_readfirstlane(found)];
+  const Entry e = unpack<MASTER, BITS8>(part, __builtin_amdgcn_readfirstlane(found));
   const Factors by = factors_of(h);
-  const int64_t first = (int64_t)(blockIdx.x - e.begin) * CHUNK, at = first + threadIdx.x * VEC;
-  const int64_t left = e.count - at;
-  const int mine = (int)(left < VEC ? left : VEC);
+  const int64_t first = (int64_t)(blockIdx.x - e.begin) * kSweep, end = first + kSweep < e.count ? first + kSweep : e.count;
   const auto as = [&](auto type, auto grad) {
     constexpr int T = decltype(type)::value, G = decltype(grad)::value;
-    if (e.count - first >= CHUNK) step_values<T, G, MASTER, BITS8, true>(e, at, VEC, h, by);
-    else step_values<T, G, MASTER, BITS8, false>(e, at, mine, h, by);
+    int64_t at = first;
+#pragma unroll 1
+    for (; at + STEP <= end; at += STEP) step_values<T, G, MASTER, BITS8, true>(e, at + threadIdx.x * VEC, VEC, h, by);
+    if (at < end) {
+      const int64_t mine = at + threadIdx.x * VEC, left = end - mine;
+      step_values<T, G, MASTER, BITS8, false>(e, mine, (int)(left < VEC ? left : VEC), h, by);
+    }
   };
   constexpr std::integral_constant<int, FP8GMM_TYPE_BF16> bf16{};
   constexpr std::integral_constant<int, FP8GMM_TYPE_FP16> fp16{};
@@ -296,6 +370,30 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Part part, int n,
   } else {
     if constexpr (!MASTER) as(fp32, fp32);
   }
+}
+
+// A launch for as many tensors as its arguments hold
+template <bool MASTER, bool BITS8>
+void launch(const fp8gmm_adamw_tensor* tensors, int n, const Hyper& h, hipStream_t s) {
+  constexpr int64_t kMostChunks = 1 << 23;   // of a launch, which holds the largest tensor: a grid has fewer than 2^32 threads
+  PartOf<MASTER, BITS8> part = {};
+  int used = 0;
+  int64_t chunks = 0;
+  const auto flush = [&] {
+    if (used > 0) hipLaunchKernelGGL((adamw_kernel<MASTER, BITS8>), dim3((unsigned)chunks), dim3(kThreads), 0, s, part, used, h);
+    used = 0;
+    chunks = 0;
+  };
+  for (int i = 0; i < n; ++i) {
+    const fp8gmm_adamw_tensor& t = tensors[i];
+    const int64_t all = (t.count + kSweep - 1) / kSweep;
+    if (all == 0) continue;
+    if (used == part.kTensors || chunks + all > kMostChunks) flush();
+    pack<MASTER, BITS8>(part, used++, {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.count,
+                                       (uint32_t)chunks, t.type, t.grad_type});
+    chunks += all;
+  }
+  flush();
 }
 
 int check_tensors(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_step& step) {
@@ -314,6 +412,9 @@ int check_tensors(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_
     if (off(t.param, type_bytes(t.type)) || off(t.grad, type_bytes(t.grad_type)) || off(t.master, 4) ||
         off(t.exp_avg, step.bits == 8 ? 8 : 4) || off(t.exp_avg_sq, step.bits == 8 ? 8 : 4) || off(t.exp_avg_scale, 4) || off(t.exp_avg_sq_scale, 4))
       return FP8GMM_ERR_ALIGNMENT;
+    for (const void* p : {(const void*)t.param, t.grad, (const void*)t.exp_avg, (const void*)t.exp_avg_sq, (const void*)t.exp_avg_scale,
+                          (const void*)t.exp_avg_sq_scale, (const void*)t.master})
+      if (reinterpret_cast<uintptr_t>(p) >> 48) return FP8GMM_ERR_BAD_ARGUMENT;
   }
   return masters == 3 ? FP8GMM_ERR_BAD_ARGUMENT : FP8GMM_OK;
 }
@@ -383,33 +484,14 @@ int multi_adamw(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_st
   h.log1 = std::log2(a.beta1);   // (of a beta of 0 minus infinity, whose power is 0)
   h.log2 = std::log2(a.beta2);
   h.lr_host = a.lr;
-  bool master = false;
-  for (int i = 0; i < n; ++i) master = master || tensors[i].master != nullptr;
-  const int64_t chunk = kThreads * (a.bits == 8 ? 8 : 4);
-  constexpr int64_t kMostChunks = 1 << 23;   // of a launch, which holds the largest tensor: a grid has fewer than 2^32 threads
-  Part part = {};
-  int used = 0;
-  int64_t chunks = 0;
-  const auto flush = [&] {
-    if (used == 0) return;
-    auto* kernel = master ? a.bits == 8 ? &adamw_kernel<true, true> : &adamw_kernel<true, false>
-                   : a.bits == 8 ? &adamw_kernel<false, true>
-                                 : &adamw_kernel<false, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(kThreads), 0, s, part, used, h);
-    used = 0;
-    chunks = 0;
-  };
+  bool master = false, any = false;
   for (int i = 0; i < n; ++i) {
-    const fp8gmm_adamw_tensor& t = tensors[i];
-    const int64_t all = (t.count + chunk - 1) / chunk;
-    if (all == 0) continue;
-    if (used == kTensors || chunks + all > kMostChunks) flush();
-    part.e[used++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.count,
-                      (uint32_t)chunks, (uint16_t)t.type, (uint16_t)t.grad_type};
-    chunks += all;
+    master = master || (tensors[i].count > 0 && tensors[i].master != nullptr);
+    any = any || tensors[i].count > 0;
   }
-  if (used == 0) return FP8GMM_OK;   // none has elements
-  flush();
+  if (!any) return FP8GMM_OK;
+  if (a.bits == 8) master ? launch<true, true>(tensors, n, h, s) : launch<false, true>(tensors, n, h, s);
+  else master ? launch<true, false>(tensors, n, h, s) : launch<false, false>(tensors, n, h, s);
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
 

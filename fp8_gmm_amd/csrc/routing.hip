@@ -473,8 +473,12 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
   Piece<TYPE, PER>::store(grad_scores, token * c.experts + e0, left, out);
 }
 
-// calls f(TYPE, LANES, PER): 16 lanes up to 512 experts, as few of them to each as there are sizes for
-constexpr int kFewTokens = 2048;
+// calls f(TYPE, LANES, PER).  Few tokens have a wavefront each, whose lanes hold few experts (us, forward by p in 64 bits / backward:
+// 1 token, 256 experts in 8 groups, 4.6 / 2.8, by 16 lanes 7.6 / 3.0; 2048 tokens 5.8 / 3.2 and 8.0 / 3.4; 4096 8.2 / 3.8 and 8.0 / 3.6; 1024
+// tokens of 512 experts 6.2 / 3.3 and 12.5 / 4.3).  Many tokens of few experts have 8 lanes each, as long as every choice and group has a
+// lane of its own (131072 tokens, 64 experts, 6 choices by their scores, 13.2 / 13.4, by 16 lanes 15.4 / 16.5; 8 experts 5.7 / 6.3 and 7.7
+// / 9.3; 16384 tokens, 64 experts, 3.6 / 3.8 and 3.9 / 4.1, 4096 tokens 3.0 / 3.4 and 2.8 / 3.2).
+constexpr int kFewTokens = 2048, kManyTokens = 8192;
 template <class F>
 void with_shape(int type, int64_t tokens, const Choice& c, F&& f) {
   const bool few = tokens <= kFewTokens;
@@ -484,7 +488,7 @@ void with_shape(int type, int64_t tokens, const Choice& c, F&& f) {
     constexpr std::integral_constant<int, 8> half{};
     constexpr std::integral_constant<int, 16> row{};
     constexpr std::integral_constant<int, 64> wave{};
-    if (c.top_k <= 8 && c.groups <= 8 && experts <= 64) {
+    if (tokens > kManyTokens && c.top_k <= 8 && c.groups <= 8 && experts <= 64) {
       if (experts <= 16) as(half, std::integral_constant<int, 2>{});
       else if (experts <= 32) as(half, std::integral_constant<int, 4>{});
       else as(half, std::integral_constant<int, 8>{});
