@@ -704,7 +704,7 @@ def multi_adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.99
     """One step of AdamW over a list of ``params`` (bfloat16, float16, float32 in any mixture, dense), in place:
 
         g = grad * min(1, max_norm / (norm + 1e-6))           the clipping of ``multi_clip``, on the way
-        m += (1 - beta1) (g - m),  v += (1 - beta2) (g^2 - v)
+        m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
         p = p - lr weight_decay p - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
 
     ``grads``: of the parameters' types or float32, in any strides.  ``exp_avgs``, ``exp_avg_sqs``: float32 and of the parameters' shapes
@@ -714,7 +714,7 @@ def multi_adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.99
     parameters are their rounded copies.  ``norm`` (one float32 on the device, as ``multi_norm`` returns it) and ``max_norm``: both or
     neither.  ``step`` counts from 1; it and ``lr`` are numbers, or an int64 and a float32 of the device (one element each), which a
     replayed graph reads anew.  What is written may share memory with nothing else of the call.  A gradient that is no number leaves
-    none in its element, an infinite one in its block of 8-bit moments."""
+    none in its element, with 8-bit moments in the moments of its block."""
     flush_uploads()   # a queued launch may write what is read here
     native.multi_adamw(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), step, lr, betas, eps, weight_decay,
                        None if scales is None else (list(scales[0]), list(scales[1])), None if masters is None else list(masters), norm,

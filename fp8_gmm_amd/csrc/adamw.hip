@@ -1,11 +1,12 @@
 // A step of AdamW over many tensors, for gfx950 (backend.multi_adamw, optim.AdamW).
 //
 //   g = grad * min(1, max_norm / (norm + 1e-6))
-//   m += (1 - beta1) (g - m),  v += (1 - beta2) (g^2 - v)
+//   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
 //   p = p - lr decay p - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
 //
 // with p kept in fp32 (`master`) beside 16-bit weights where the caller wants that.  m and v are fp32, or in 8 bits: e4m3 codes of m
-// and of sqrt(v), each 128 elements with a scale of their own in fp32, the largest magnitude over 448.  All arithmetic is fp32.
+// and of sqrt(v), each 128 elements with a scale of their own in fp32, the largest magnitude over 448.  All arithmetic is fp32; what decides the codes is a fixed sequence of correctly rounded operations (but for
+// the root, off in one of a million), so that who follows it gets the same codes.
 //
 // 8-bit moments are rounded by a threshold that runs evenly through [0, 1) from step to step and from element to element, the
 // multiples of two irrational numbers: a moment that grows by less than half a code's distance each step would stay where it is for
@@ -23,7 +24,13 @@ namespace fp8gmm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSweep = 4096;         // elements of a workgroup, several to a thread at a time
+// Elements of a workgroup, which it takes in steps of 4 (32 bits) or 8 to a thread.  Of lists that no cache holds, us: 400 tensors of bf16
+// with fp32 moments by 2048 elements 625, by 4096 668, by 8192 697; 96 tensors with 8-bit moments by 2048 317, by 4096 286, by 8192 288.
+constexpr int sweep(bool bits8) { return bits8 ? 4096 : 2048; }
+// From so many bytes on everything is read and written with the streaming hint: nothing of it is found in the caches by the next step
+// (470 million weights with masters 2364 us, without the hint 2470, with it on the reads or the writes alone 2454 and 2470; 16 million
+// without masters 64 and 73).  Below, what the caches hold from call to call counts (8 million: 31.9 with the hint, 28.7 without).
+constexpr int64_t kStreamBytes = (int64_t)256 << 20;
 constexpr int kBlock = FP8GMM_ADAMW_BLOCK;
 constexpr float kMost = Fp8Limits<FP8GMM_E4M3>::kMax;
 constexpr float kTiny = 0x1p-100f;   // moments below it are zeros in 8 bits
@@ -97,11 +104,11 @@ __device__ __forceinline__ Entry unpack(const PartOf<MASTER, BITS8>& part, int a
 }
 
 struct Hyper {
-  float c1, c2;       // 1 - beta
-  float eps, decay;   // decay: lr * weight_decay, or weight_decay where lr is the device's
-  float rate, root;   // lr / (1 - beta1^t) and 1 / sqrt(1 - beta2^t)
+  float b1, b2, c1, c2;   // the betas, and 1 - beta
+  float eps, decay;       // decay: lr * weight_decay, or weight_decay where lr is the device's
+  float rate, root;       // lr / (1 - beta1^t) and 1 / sqrt(1 - beta2^t)
   float max_norm;
-  uint32_t dither;    // t * kStep
+  uint32_t dither;        // t * kStep
   const float* norm;
   // of a step whose number and learning rate the device has (a captured one): the logarithms of the betas, to the base 2
   const int64_t* step;
@@ -110,7 +117,7 @@ struct Hyper {
 };
 
 // VEC elements of a type, of which the first n are there
-template <int TYPE, int VEC>
+template <int TYPE, int VEC, bool STREAM>
 struct Values {
   typedef Elements<TYPE> E;
   typedef typename E::bits bits;
@@ -122,14 +129,15 @@ struct Values {
     const bits* const p = static_cast<const bits*>(base) + at;
     if constexpr (kBytes < 16) {
       if constexpr (FULL) {
-        const u32x2 v = *reinterpret_cast<const half_piece*>(p);
+        const half_piece* const from = reinterpret_cast<const half_piece*>(p);
+        const u32x2 v = STREAM ? __builtin_nontemporal_load(from) : *from;
         raw[0] = u32x4{v.x, v.y, 0u, 0u};
       } else {
         raw[0] = E::load(p, min(n, VEC));
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) raw[i] = E::load(p + i * E::kVec, FULL ? E::kVec : n - i * E::kVec);
+      for (int i = 0; i < kBytes / 16; ++i) raw[i] = E::template load<STREAM>(p + i * E::kVec, FULL ? E::kVec : n - i * E::kVec);
     }
   }
   __device__ __forceinline__ void get(float (&f)[VEC]) const {
@@ -153,23 +161,26 @@ struct Values {
       for (int j = 0; j < N; ++j) part[j] = f[i + j];
       const u32x4 v = E::pack(part);
       if constexpr (N < E::kVec) {
-        if constexpr (FULL) *reinterpret_cast<half_piece*>(p) = u32x2{v.x, v.y};
+        if constexpr (FULL && STREAM) __builtin_nontemporal_store((half_piece)u32x2{v.x, v.y}, reinterpret_cast<half_piece*>(p));
+        else if constexpr (FULL) *reinterpret_cast<half_piece*>(p) = u32x2{v.x, v.y};
         else E::store(p, min(n, N), v);
       } else {
-        E::store(p + i, FULL ? E::kVec : n - i, v);
+        E::template store<STREAM>(p + i, FULL ? E::kVec : n - i, v);
       }
     }
   }
 };
 
 // Eight codes
+template <bool STREAM>
 struct Codes {
   u32x2 raw;
   template <bool FULL>
   __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
     const uint8_t* const p = static_cast<const uint8_t*>(base) + at;
     if constexpr (FULL) {
-      raw = *reinterpret_cast<const u32x2*>(p);
+      const u32x2* const from = reinterpret_cast<const u32x2*>(p);
+      raw = STREAM ? __builtin_nontemporal_load(from) : *from;
     } else {
       raw = u32x2{0u, 0u};
 #pragma unroll
@@ -190,7 +201,9 @@ struct Codes {
   template <bool FULL>
   static __device__ __forceinline__ void store(void* base, int64_t at, int n, u32x2 w) {
     uint8_t* const p = static_cast<uint8_t*>(base) + at;
-    if constexpr (FULL) {
+    if constexpr (FULL && STREAM) {
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x2*>(p));
+    } else if constexpr (FULL) {
       *reinterpret_cast<u32x2*>(p) = w;
     } else {
 #pragma unroll
@@ -201,27 +214,42 @@ struct Codes {
 };
 
 // y to a code, up with the probability of its way to the next one: the hardware's rounding by a random number, of which it adds the upper
-// 20 bits to what lies between two codes.  Byte I of `old`.
+// 20 bits to what lies between two codes.  Byte I of `old`.  (Behind 448 there is no code: the largest's product may round to more.)
 template <int I>
 __device__ __forceinline__ uint32_t round_linear(float y, uint32_t h, uint32_t old) {
-  return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(y, (int)h, (int)old, I);
+  return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(__builtin_amdgcn_fmed3f(y, -kMost, kMost), (int)h, (int)old, I);
 }
 // y >= 0 to a code, up with the probability of its square's way to the next one's.  The codes lie 2^(e-3) apart from 2^e on, from 2^-6
 // down 2^-9: adding 2^-6 there makes the distance that of all numbers with its exponent, and the last 20 bits of the fraction what
-// lies between two codes.  A NaN stays one: it comes from a product, so its first bit of the fraction is set.
+// lies between two codes.
 __device__ __forceinline__ float round_root(float y, uint32_t h) {
+  y = fminf(y, kMost);
   const float off = y < 0x1p-6f ? 0x1p-6f : 0.f;
   const uint32_t bits = __float_as_uint(y + off);
-  const float lo = __uint_as_float(bits & 0xfff00000u) - off, gap = __uint_as_float(bits & 0x7f800000u) * 0.125f;
-  const float ways = gap * __builtin_fmaf(2.f, lo, gap);                                    // the squares' distance
-  const float u1 = __uint_as_float(h >> 9 ^ 0x3fc00000u);                                   // 1 + the threshold
-  const bool up = (y - lo) * (y + lo) > __builtin_fmaf(u1, ways, -ways);
+  const float lo = __uint_as_float(bits & 0xfff00000u) - off, eight = __uint_as_float(bits & 0x7f800000u), gap = eight * 0.125f;
+  const float ways = eight * 0x1p-27f * __builtin_fmaf(2.f, lo, gap);   // the squares' distance, in units of the threshold
+  const bool up = (y - lo) * (y + lo) > (float)((h ^ 0x80000000u) >> 8) * ways;
   const float code = up ? lo + gap : lo;
   return y > 0.f ? fmaxf(code, 0x1p-9f) : code;
 }
-// 448 / most, not above it: no product with a magnitude up to `most` rounds to more than 448, whose next code is none
-__device__ __forceinline__ float to_codes(float most) {
-  return most >= kTiny ? __uint_as_float(__float_as_uint(kMost / most) - 1u) : 0.f;
+
+// The root of a number that is zero, normal or a NaN: the hardware's guess of its inverse and a step of Newton's, correctly rounded but in
+// one of a million (8 instructions' time, sqrtf takes 17).
+__device__ __forceinline__ float root_of(float v) {
+  const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f)), s = v * y;
+  return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s);
+}
+// The largest magnitude of a block, 8 elements in each of 16 lanes; a NaN where one of them is
+__device__ __forceinline__ float block_max(float v) {
+  const auto step = [&](auto control) {
+    const float other = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(control)::value, 0xf, 0xf, true));
+    v = amax_or_nan(v, other, other);
+  };
+  step(std::integral_constant<int, 0xb1>{});
+  step(std::integral_constant<int, 0x4e>{});
+  step(std::integral_constant<int, 0x141>{});
+  step(std::integral_constant<int, 0x140>{});
+  return v;
 }
 
 // What a step multiplies by, the same for all elements
@@ -250,14 +278,14 @@ __device__ __forceinline__ Factors factors_of(const Hyper& h) {
   return f;
 }
 
-template <int TYPE, int GRAD, bool MASTER, bool BITS8, bool FULL>
+template <int TYPE, int GRAD, bool MASTER, bool BITS8, bool STREAM, bool FULL>
 __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, const Hyper& h, const Factors& by) {
   constexpr int VEC = BITS8 ? 8 : 4;
-  typedef Values<FP8GMM_TYPE_FP32, VEC> F32;
-  Values<TYPE, VEC> param;
-  Values<GRAD, VEC> grad;
+  typedef Values<FP8GMM_TYPE_FP32, VEC, STREAM> F32;
+  Values<TYPE, VEC, STREAM> param;
+  Values<GRAD, VEC, STREAM> grad;
   F32 master;
-  std::conditional_t<BITS8, Codes, F32> mc, vc;
+  std::conditional_t<BITS8, Codes<STREAM>, F32> mc, vc;
   float m_scale = 1.f, v_scale = 1.f;
   grad.template load<FULL>(e.grad, at, n);
   if constexpr (MASTER) master.template load<FULL>(e.master, at, n);
@@ -276,8 +304,8 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
   grad.get(g);
   mc.get(m);
   vc.get(v);
-  float m_most = 0.f, v_most = 0.f, root[VEC];
-  bool small = false;
+  float root[VEC];
+  bool rare = false;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     g[i] *= by.grad;
@@ -286,12 +314,12 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
       v[i] *= v_scale;
       v[i] *= v[i];
     }
-    m[i] = __builtin_fmaf(h.c1, g[i] - m[i], m[i]);
-    v[i] = __builtin_fmaf(h.c2, __builtin_fmaf(g[i], g[i], -v[i]), v[i]);
-    root[i] = __builtin_amdgcn_sqrtf(v[i]);   // good to 2 roundings, and 0 of a subnormal number
-    small = small || __builtin_isfpclass(v[i], 0x90);
+    m[i] = h.b1 * m[i] + h.c1 * g[i];
+    v[i] = h.b2 * v[i] + h.c2 * g[i] * g[i];
+    root[i] = root_of(v[i]);
+    rare = rare || __builtin_isfpclass(v[i], 0x290);   // subnormal, or infinite
   }
-  if (__builtin_expect(small, 0)) {
+  if (__builtin_expect(rare, 0)) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) root[i] = sqrtf(v[i]);
   }
@@ -302,17 +330,19 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
     r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
     p[i] = __builtin_fmaf(-by.rate, m[i] * r, __builtin_fmaf(-by.decay, p[i], p[i]));
     if constexpr (MASTER) asm("" : "+v"(p[i]));   // fp32 first, then 16 bits: the weight is the master's rounded copy
-    if constexpr (BITS8) {
-      m_most = fmaxf(m_most, fabsf(m[i]));
-      v_most = fmaxf(v_most, root[i]);
-    }
   }
   if constexpr (MASTER) F32::template store<FULL>(e.master, at, n, p);
-  Values<TYPE, VEC>::template store<FULL>(e.param, at, n, p);
+  Values<TYPE, VEC, STREAM>::template store<FULL>(e.param, at, n, p);
   if constexpr (BITS8) {
-    m_most = lanes_max<16>(m_most);   // of a block: 16 lanes of 8 elements
-    v_most = lanes_max<16>(v_most);
-    const float m_inv = to_codes(m_most), v_inv = to_codes(v_most);
+    float m_most = 0.f, v_most = 0.f;
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      m_most = amax_or_nan(m_most, m[i], m[i + 1]);
+      v_most = amax_or_nan(v_most, root[i], root[i + 1]);
+    }
+    m_most = block_max(m_most);
+    v_most = block_max(v_most);
+    const float m_inv = m_most >= kTiny ? kMost / m_most : 0.f, v_inv = v_most >= kTiny ? kMost / v_most : 0.f;
     const uint32_t first = (uint32_t)at * kElement + by.dither;
     u32x2 mw = {0u, 0u}, vw;
 #pragma unroll
@@ -332,32 +362,32 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
       e.m_scale[at / kBlock] = m_most / kMost;
       e.v_scale[at / kBlock] = v_most / kMost;
     }
-    Codes::store<FULL>(e.m, at, n, mw);
-    Codes::store<FULL>(e.v, at, n, vw);
+    Codes<STREAM>::template store<FULL>(e.m, at, n, mw);
+    Codes<STREAM>::template store<FULL>(e.v, at, n, vw);
   } else {
     F32::template store<FULL>(e.m, at, n, m);
     F32::template store<FULL>(e.v, at, n, v);
   }
 }
 
-template <bool MASTER, bool BITS8>
+template <bool MASTER, bool BITS8, bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const PartOf<MASTER, BITS8> part, int n, const Hyper h) {
-  constexpr int VEC = BITS8 ? 8 : 4, STEP = kThreads * VEC;
+  constexpr int VEC = BITS8 ? 8 : 4, STEP = kThreads * VEC, SWEEP = sweep(BITS8);
   __shared__ int found;
   for (int i = threadIdx.x; i < n; i += kThreads)
     if (part.begin[i] <= blockIdx.x && (i + 1 == n || blockIdx.x < part.begin[i + 1])) found = i;
   __syncthreads();
   const Entry e = unpack<MASTER, BITS8>(part, __builtin_amdgcn_readfirstlane(found));
   const Factors by = factors_of(h);
-  const int64_t first = (int64_t)(blockIdx.x - e.begin) * kSweep, end = first + kSweep < e.count ? first + kSweep : e.count;
+  const int64_t first = (int64_t)(blockIdx.x - e.begin) * SWEEP, end = first + SWEEP < e.count ? first + SWEEP : e.count;
   const auto as = [&](auto type, auto grad) {
     constexpr int T = decltype(type)::value, G = decltype(grad)::value;
     int64_t at = first;
 #pragma unroll 1
-    for (; at + STEP <= end; at += STEP) step_values<T, G, MASTER, BITS8, true>(e, at + threadIdx.x * VEC, VEC, h, by);
+    for (; at + STEP <= end; at += STEP) step_values<T, G, MASTER, BITS8, STREAM, true>(e, at + threadIdx.x * VEC, VEC, h, by);
     if (at < end) {
       const int64_t mine = at + threadIdx.x * VEC, left = end - mine;
-      step_values<T, G, MASTER, BITS8, false>(e, mine, (int)(left < VEC ? left : VEC), h, by);
+      step_values<T, G, MASTER, BITS8, STREAM, false>(e, mine, (int)(left < VEC ? left : VEC), h, by);
     }
   };
   constexpr std::integral_constant<int, FP8GMM_TYPE_BF16> bf16{};
@@ -375,18 +405,22 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const PartOf<MASTER, BI
 // A launch for as many tensors as its arguments hold
 template <bool MASTER, bool BITS8>
 void launch(const fp8gmm_adamw_tensor* tensors, int n, const Hyper& h, hipStream_t s) {
+  int64_t bytes = 0;
+  for (int i = 0; i < n; ++i)
+    bytes += tensors[i].count * (2 * type_bytes(tensors[i].type) + type_bytes(tensors[i].grad_type) + (BITS8 ? 4 : 16) + (MASTER ? 8 : 0));
+  auto* kernel = bytes > kStreamBytes ? &adamw_kernel<MASTER, BITS8, true> : &adamw_kernel<MASTER, BITS8, false>;
   constexpr int64_t kMostChunks = 1 << 23;   // of a launch, which holds the largest tensor: a grid has fewer than 2^32 threads
   PartOf<MASTER, BITS8> part = {};
   int used = 0;
   int64_t chunks = 0;
   const auto flush = [&] {
-    if (used > 0) hipLaunchKernelGGL((adamw_kernel<MASTER, BITS8>), dim3((unsigned)chunks), dim3(kThreads), 0, s, part, used, h);
+    if (used > 0) hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(kThreads), 0, s, part, used, h);
     used = 0;
     chunks = 0;
   };
   for (int i = 0; i < n; ++i) {
     const fp8gmm_adamw_tensor& t = tensors[i];
-    const int64_t all = (t.count + kSweep - 1) / kSweep;
+    const int64_t all = (t.count + sweep(BITS8) - 1) / sweep(BITS8);
     if (all == 0) continue;
     if (used == part.kTensors || chunks + all > kMostChunks) flush();
     pack<MASTER, BITS8>(part, used++, {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.count,
@@ -466,6 +500,8 @@ int multi_adamw(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_st
   if (rc == FP8GMM_OK) rc = check_apart(tensors, n, a.bits);
   if (rc != FP8GMM_OK) return rc;
   Hyper h = {};
+  h.b1 = (float)a.beta1;
+  h.b2 = (float)a.beta2;
   h.c1 = (float)(1. - a.beta1);
   h.c2 = (float)(1. - a.beta2);
   h.eps = (float)a.eps;

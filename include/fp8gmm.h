@@ -783,14 +783,14 @@ int fp8gmm_multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm,
 
 /*
  * fp8gmm_multi_adamw: one step of AdamW over n tensors.  With g = grad * min(1, max_norm / (norm + 1e-6)) (norm NULL: g = grad):
- *   exp_avg += (1 - beta1) (g - exp_avg),  exp_avg_sq += (1 - beta2) (g^2 - exp_avg_sq),
+ *   exp_avg = beta1 exp_avg + (1 - beta1) g,  exp_avg_sq = beta2 exp_avg_sq + (1 - beta2) g^2,
  *   p = p - lr weight_decay p - lr / (1 - beta1^t) exp_avg / (sqrt(exp_avg_sq / (1 - beta2^t)) + eps)
  * in fp32, p being `master` (fp32) where there is one, of which param is then the rounded copy, else param itself; all tensors of a call
  * with elements have masters or none has.  grad: of param's type or fp32.  bits 32: the moments are fp32.  bits 8: they are e4m3 codes, of
  * exp_avg and of sqrt(exp_avg_sq), on 8 bytes, with an fp32 scale for each FP8GMM_ADAMW_BLOCK elements (the last block may be short); value
  * = code * scale, scale = largest magnitude of the block / 448, 0 where that is below 2^-100 and the codes zeros.  Codes are rounded by
  * thresholds u = frac((i * 0x6A09E667 + t * 0x9E3779B9) / 2^32) for element i (cut to 20 bits): exp_avg up where its way to the next
- * code is at least 1 - u, the root, with u + 1/2 in place of u (cut to 23 bits), where its square's way to the next code's is more than that; a
+ * code is at least 1 - u, the root, with u + 1/2 in place of u (cut to 24 bits), where its square's way to the next code's is more than that; a
  * root that is not zero becomes no zero.
  * t and lr: `step` (>= 1) and `lr`, or *step_dev and *lr_dev where these are given, which a replayed launch reads anew.  `tensors` is HOST
  * memory and is read during the call only.  What is written overlaps nothing else of the call (FP8GMM_ERR_BAD_ARGUMENT).  At most 2^32

@@ -116,7 +116,7 @@ class Problem:
         h = (torch.arange(n, device=self.dev) * 0x6A09E667 + t * 0x9E3779B9) & 0xFFFFFFFF
         for name, codes, scale, value, tol, u in (
                 ("m", self.m[i], self.scales[0][i], m, tol_m, (h >> 12).double() * 2.0 ** -20),
-                ("v", self.v[i], self.scales[1][i], v.sqrt(), tol_v / (2 * v.sqrt()).clamp(min=1e-30), ((h ^ 0x80000000) >> 9).double() * 2.0 ** -23)):
+                ("v", self.v[i], self.scales[1][i], v.sqrt(), tol_v / (2 * v.sqrt()).clamp(min=1e-30), ((h ^ 0x80000000) >> 8).double() * 2.0 ** -24)):
             most = blocks_max(value)
             assert_within(scale, most / 448, 4 * U * most / 448 + blocks_max(tol) / 448 + 1e-44, f"scale of {name} {i}")
             y = value.abs() / spread(most, n).clamp(min=1e-37) * 448
