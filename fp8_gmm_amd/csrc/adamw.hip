@@ -87,15 +87,17 @@ __device__ __forceinline__ Entry unpack(const PartOf<MASTER, BITS8>& part, int a
     w += 3;
     return v;
   };
-  e.param = reinterpret_cast<void*>(get());
-  e.grad = reinterpret_cast<const void*>(get());
-  e.m = reinterpret_cast<void*>(get());
-  e.v = reinterpret_cast<void*>(get());
+  // global memory: an address without a space would be accessed as if it might be LDS
+  const auto address = [&] { return (void*)reinterpret_cast<__attribute__((address_space(1))) void*>(get()); };
+  e.param = address();
+  e.grad = address();
+  e.m = address();
+  e.v = address();
   if constexpr (BITS8) {
-    e.m_scale = reinterpret_cast<float*>(get());
-    e.v_scale = reinterpret_cast<float*>(get());
+    e.m_scale = static_cast<float*>(address());
+    e.v_scale = static_cast<float*>(address());
   }
-  if constexpr (MASTER) e.master = reinterpret_cast<float*>(get());
+  if constexpr (MASTER) e.master = static_cast<float*>(address());
   const uint64_t last = get();
   e.count = (int64_t)(last & 0xffffffffffull);
   e.type = (int)(last >> 40 & 0xf);
@@ -252,6 +254,19 @@ __device__ __forceinline__ float block_max(float v) {
   return v;
 }
 
+// 448 / most and most / 448, correctly rounded: a guess, and what its remainder adds to it (9 and 3 instructions' time, a division takes 13)
+__device__ __forceinline__ float codes_per(float most) {
+  if (__builtin_expect(!(most >= kTiny && most < 0x1p120f), 0)) return most >= kTiny ? kMost / most : 0.f;
+  float r = __builtin_amdgcn_rcpf(most);
+  r = __builtin_fmaf(__builtin_fmaf(-most, r, 1.f), r, r);
+  const float q = kMost * r;
+  return __builtin_fmaf(__builtin_fmaf(-q, most, kMost), r, q);
+}
+__device__ __forceinline__ float per_code(float most) {
+  const float q = most * (1.f / kMost), scale = __builtin_fmaf(__builtin_fmaf(-q, kMost, most), 1.f / kMost, q);
+  return most < kTiny ? 0.f : scale;
+}
+
 // What a step multiplies by, the same for all elements
 struct Factors {
   float grad, rate, root, decay;
@@ -342,7 +357,7 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
     }
     m_most = block_max(m_most);
     v_most = block_max(v_most);
-    const float m_inv = m_most >= kTiny ? kMost / m_most : 0.f, v_inv = v_most >= kTiny ? kMost / v_most : 0.f;
+    const float m_inv = codes_per(m_most), v_inv = codes_per(v_most);
     const uint32_t first = (uint32_t)at * kElement + by.dither;
     u32x2 mw = {0u, 0u}, vw;
 #pragma unroll
@@ -359,8 +374,8 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
       vw[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
     }
     if (threadIdx.x % 16 == 0 && (FULL || n > 0)) {
-      e.m_scale[at / kBlock] = m_most / kMost;
-      e.v_scale[at / kBlock] = v_most / kMost;
+      e.m_scale[at / kBlock] = per_code(m_most);
+      e.v_scale[at / kBlock] = per_code(v_most);
     }
     Codes<STREAM>::template store<FULL>(e.m, at, n, mw);
     Codes<STREAM>::template store<FULL>(e.v, at, n, vw);
