@@ -23,9 +23,11 @@
 namespace fp8gmm {
 namespace {
 
-constexpr int kThreads = 256;
-// Elements of a workgroup, which it takes in steps of 4 (32 bits) or 8 to a thread.  Of lists that no cache holds, us: 400 tensors of bf16
-// with fp32 moments by 2048 elements 625, by 4096 668, by 8192 697; 96 tensors with 8-bit moments by 2048 317, by 4096 286, by 8192 288.
+// Threads and elements of a workgroup, 4 (32 bits) or 8 to a thread at a time.  Of lists that no cache holds, us: 400 tensors of bf16 with
+// fp32 moments by 512 threads and 2048 elements 596, by 256 and 1024 597, and 2048 625, and 4096 670, by 128 and 2048 669; 96 tensors of fp32
+// by 512 and 2048 761, by 256 and 1024 786; 96 tensors with 8-bit moments, which take ten times the instructions, by 256 and 4096 299, and
+// 8192 294, and 2048 337, by 512 and 4096 343.
+constexpr int threads(bool bits8) { return bits8 ? 256 : 512; }
 constexpr int sweep(bool bits8) { return bits8 ? 4096 : 2048; }
 // From so many bytes on everything is read and written with the streaming hint: nothing of it is found in the caches by the next step
 // (470 million weights with masters 2364 us, without the hint 2470, with it on the reads or the writes alone 2454 and 2470; 16 million
@@ -386,10 +388,10 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
 }
 
 template <bool MASTER, bool BITS8, bool STREAM>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const PartOf<MASTER, BITS8> part, int n, const Hyper h) {
-  constexpr int VEC = BITS8 ? 8 : 4, STEP = kThreads * VEC, SWEEP = sweep(BITS8);
+__global__ __launch_bounds__(threads(BITS8)) void adamw_kernel(const PartOf<MASTER, BITS8> part, int n, const Hyper h) {
+  constexpr int VEC = BITS8 ? 8 : 4, THREADS = threads(BITS8), STEP = THREADS * VEC, SWEEP = sweep(BITS8);
   __shared__ int found;
-  for (int i = threadIdx.x; i < n; i += kThreads)
+  for (int i = threadIdx.x; i < n; i += THREADS)
     if (part.begin[i] <= blockIdx.x && (i + 1 == n || blockIdx.x < part.begin[i + 1])) found = i;
   __syncthreads();
   const Entry e = unpack<MASTER, BITS8>(part, __builtin_amdgcn_readfirstlane(found));
@@ -424,12 +426,12 @@ void launch(const fp8gmm_adamw_tensor* tensors, int n, const Hyper& h, hipStream
   for (int i = 0; i < n; ++i)
     bytes += tensors[i].count * (2 * type_bytes(tensors[i].type) + type_bytes(tensors[i].grad_type) + (BITS8 ? 4 : 16) + (MASTER ? 8 : 0));
   auto* kernel = bytes > kStreamBytes ? &adamw_kernel<MASTER, BITS8, true> : &adamw_kernel<MASTER, BITS8, false>;
-  constexpr int64_t kMostChunks = 1 << 23;   // of a launch, which holds the largest tensor: a grid has fewer than 2^32 threads
+  constexpr int64_t kMostChunks = 1 << 22;   // of a launch, which holds the largest tensor: a grid has fewer than 2^32 threads
   PartOf<MASTER, BITS8> part = {};
   int used = 0;
   int64_t chunks = 0;
   const auto flush = [&] {
-    if (used > 0) hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(kThreads), 0, s, part, used, h);
+    if (used > 0) hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(threads(BITS8)), 0, s, part, used, h);
     used = 0;
     chunks = 0;
   };
