@@ -18,7 +18,12 @@ constexpr int kBackwardThreads = 1024;   // of a workgroup of the backward pass:
 constexpr int kBackwardBlocks = 256;     // leaves one partial sum of the weight's gradient in memory; one per compute unit
 constexpr int kBackwardAlone = 2;        // turns of one workgroup that take less than a second launch for the sums of several
 constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, where a row needs no more
-constexpr int kForwardAll = 256 * 2048, kForwardTurns = 5, kForwardMore = 3;
+// What a forward pass writes: the normed rows (of x, or of the sum with a residual, which it writes as well), or these in 8 bits
+enum { kRows, kSums, kBits8 };
+// Threads of its launch, which go on to other rows.  With 8 bits what the compute units hold at a time, three times that where they would go
+// on more than five times; else four times as many (16384 x 4096, bf16, with a residual 86.8 us, what they hold alone 89.2; without one 43.5
+// and 45.1; but in 8 bits 81 and 76; 16384 x 4093 93.0 and 98.4).
+constexpr int kForwardAll = 256 * 2048, kForwardTurns = 5, kForwardMore = 3, kForwardFour = 4;
 
 // The least magnitude that a row's scale is made of: what is smaller is zero in 8 bits, and no scale is zero.
 constexpr float kLeast = 0x1p-100f;
@@ -68,13 +73,16 @@ struct Bits8 {
 
 // A workgroup takes ROWS rows at a time, LANES * waves threads to a row and C pieces to a thread, and goes on to other rows by the grid:
 // the next rows are loaded before the sums of the present ones are shared, and the weight stays in registers.
-template <int TYPE, int PTYPE, int LANES, int C, int MODE, int MOST, bool BITS8>
+template <int TYPE, int PTYPE, int LANES, int C, int MODE, int MOST, int KIND>
 __global__ __launch_bounds__(MOST) void rms_norm_kernel(
     const void* __restrict__ x_, int64_t ldx, const void* __restrict__ residual_, int64_t ldr, const void* __restrict__ w,
     void* __restrict__ y_, const Bits8 bits8, void* __restrict__ h_, float* __restrict__ rstd_out, int rows, int cols, float eps, int waves,
     bool stream) {
   typedef Elements<TYPE> E;
   constexpr int V = E::kVec;
+  // With the streaming hint, but for rows that are the residual stream themselves (16384 x 4096, bf16, with a residual 89.2 us, without the
+  // hint 93.7; in 8 bits 76 and 88; without a residual 44.7 and 45.1).
+  constexpr bool BITS8 = KIND == kBits8, STREAM = KIND != kRows;
   __shared__ float slots[2][kNormWaves][kNormWaves], tops[2][kNormWaves][kNormWaves];
   const int THREADS = LANES * waves, ROWS = blockDim.x / THREADS;
   int group = threadIdx.x / THREADS;
@@ -85,15 +93,16 @@ __global__ __launch_bounds__(MOST) void rms_norm_kernel(
   for (int c = 0; c < C; ++c) at[c] = (c * THREADS + t) * V;
   const int skip = piece_skip<MODE, V>(at[C - 1], cols);   // the pieces before the last one are there in whole
   at[C - 1] = piece_begin<MODE, V>(at[C - 1], cols);
+  const bool added = KIND == kSums || (BITS8 && residual_ != nullptr);
   u32x4 nx[C], nr[C];
   const auto load = [&](int64_t row) {
     const RowAccess<TYPE, MODE> x(x_, row, rows, ldx, cols);
 #pragma unroll
-    for (int c = 0; c < C; ++c) nx[c] = x.template load<false>(at[c]);
-    if (residual_ != nullptr) {
+    for (int c = 0; c < C; ++c) nx[c] = x.template load<STREAM>(at[c]);
+    if (added) {
       const RowAccess<TYPE, MODE> residual(residual_, row, rows, ldr, cols);
 #pragma unroll
-      for (int c = 0; c < C; ++c) nr[c] = residual.template load<false>(at[c]);
+      for (int c = 0; c < C; ++c) nr[c] = residual.template load<STREAM>(at[c]);
     }
   };
   const int64_t stride = (int64_t)gridDim.x * ROWS;
@@ -112,7 +121,7 @@ __global__ __launch_bounds__(MOST) void rms_norm_kernel(
     u32x4 x[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) x[c] = nx[c];
-    if (residual_ != nullptr) {
+    if (added) {
       const RowAccess<TYPE, MODE> h(h_, row, rows, cols, cols);
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -481,17 +490,25 @@ __global__ __launch_bounds__(256) void rms_norm_long_weight_kernel(
     if (i < n) out[i] = dw[i];
 }
 
-Shape forward_shape(int cols, int type) {
-  const Shape s = shape_of(pieces_of(cols, type), 4, 8, 4);
+// Forward, 4 pieces to a thread, as in the layer norm; 2 of aligned rows in 8 bits, whose conversions want more wavefronts (4096 x 4096, bf16,
+// 23.0 us, with 4 pieces 27.0; 256 rows 5.2 and 6.1; 16384 rows 74.9 and 76.2; but 16384 x 4093 91.8 and 80.2).
+Shape forward_shape(int cols, int type, bool two) {
+  const int pieces = pieces_of(cols, type);
+  Shape s = shape_of(pieces, two ? 2 : 4, 8, 4);
+  if (s.lanes == 0) s = shape_of(pieces, 4, 8, 4);
   return s.lanes != 0 ? s : widest(cols, type);
 }
-Shape backward_shape(int cols, int type) {
-  const Shape s = shape_of(pieces_of(cols, type), 2, kNormWaves, 2);
+// Backward, 2, or 1 of aligned rows that leave a workgroup two of them (16384 x 4096, bf16, 91.7 us, with 2 pieces 93.7; 65536 x 1024 90.7 and
+// 94.7; 256 x 4096 9.1 and 10.6; 4096 x 4096 30.2 and 29.5; 64 x 8192, one row, 10.9 and 9.9).
+Shape backward_shape(int cols, int type, bool aligned) {
+  const int pieces = pieces_of(cols, type);
+  const Shape one = shape_of(pieces, 1, kNormWaves / 2, 2), s = shape_of(pieces, 2, kNormWaves, 2);
+  if (aligned && one.lanes == 64 && kBackwardThreads % one.threads() == 0) return one;
   return s.lanes != 0 ? s : widest(cols, type);
 }
-// Workgroups of a backward pass: partial sums that its weight's gradient has.
-int backward_blocks(int64_t rows, int cols, int type) {
-  const Shape s = backward_shape(cols, type);
+// Workgroups of a backward pass: partial sums that its weight's gradient has.  Of aligned rows no fewer than of others.
+int backward_blocks(int64_t rows, int cols, int type, bool aligned) {
+  const Shape s = backward_shape(cols, type, aligned);
   if (s.lanes == 0) return (int)std::min<int64_t>(rows, 64);
   const int blocks = ceil_div(rows, kBackwardThreads / s.threads());
   return blocks <= kBackwardAlone ? std::min(blocks, 1) : std::min(blocks, kBackwardBlocks);
@@ -528,26 +545,27 @@ int check_forward(const Rows& a) {
   return FP8GMM_OK;
 }
 
-template <bool BITS8>
+template <int KIND>
 int launch_forward(const Rows& a, void* y, const Bits8& bits8, float* rstd, hipStream_t s) {
-  const Shape shape = forward_shape(a.cols, a.type);
+  constexpr bool BITS8 = KIND == kBits8;
+  const bool aligned = whole(a.x, a.ldx, a.cols, a.type) && (a.residual == nullptr || (whole(a.residual, a.ldr, a.cols, a.type) &&
+                       whole(a.h, a.cols, a.cols, a.type))) && (BITS8 || whole(y, a.cols, a.cols, a.type));
+  const Shape shape = forward_shape(a.cols, a.type, BITS8 && aligned);
   const int threads = shape.lanes == 0 ? 0 : std::max(shape.threads(), kForwardThreads / shape.threads() * shape.threads());
   const bool streaming = streams(a.rows, a.cols, a.type);
   const auto blocks = [&] {
     const int groups = ceil_div(a.rows, threads / shape.threads()), all = kForwardAll / threads;   // rows that a workgroup takes at a time
-    return std::min(groups, groups > kForwardTurns * all ? kForwardMore * all : all);
+    return std::min(groups, !BITS8 ? kForwardFour * all : groups > kForwardTurns * all ? kForwardMore * all : all);
   };
-  const bool aligned = whole(a.x, a.ldx, a.cols, a.type) && (a.residual == nullptr || (whole(a.residual, a.ldr, a.cols, a.type) &&
-                       whole(a.h, a.cols, a.cols, a.type))) && (BITS8 || whole(y, a.cols, a.cols, a.type));
   const int mode = mode_of(a.cols, a.type, shape.lanes, aligned, streaming);
   bool known = true;   // a row's share of the registers that no launch below is for would leave the results unwritten
   with_types(a.type, a.param_type, [&](auto tc, auto pc) {
     constexpr int T = decltype(tc)::value, P = decltype(pc)::value;
 #define FP8GMM_LAUNCH(LANES, C, MOST)                                                                                                \
   if (shape.lanes == LANES && shape.pieces == C && threads <= MOST) {                                                                \
-    auto* kernel = mode == kEdge         ? &rms_norm_kernel<T, P, LANES, C, kEdge, MOST, BITS8>                                      \
-                   : mode == kEdgeStream ? &rms_norm_kernel<T, P, LANES, C, kEdgeStream, MOST, BITS8>                                \
-                                         : &rms_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge, MOST, BITS8>; \
+    auto* kernel = mode == kEdge         ? &rms_norm_kernel<T, P, LANES, C, kEdge, MOST, KIND>                                      \
+                   : mode == kEdgeStream ? &rms_norm_kernel<T, P, LANES, C, kEdgeStream, MOST, KIND>                                \
+                                         : &rms_norm_kernel<T, P, LANES, C, LANES == 64 ? kWhole : C == 1 ? kShort : kEdge, MOST, KIND>; \
     hipLaunchKernelGGL(kernel, dim3(blocks()), dim3(threads), 0, s, a.x, a.ldx, a.residual, a.ldr, a.weight, y, bits8, a.h, rstd,     \
                        (int)a.rows, a.cols, a.eps, shape.waves, streaming);                                                          \
   } else
@@ -584,7 +602,8 @@ int fp8gmm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ld
   const int rc = check_forward(a);
   if (rc != FP8GMM_OK) return rc == 1 ? FP8GMM_OK : rc;
   if (y == nullptr) return FP8GMM_ERR_NULL_POINTER;
-  return launch_forward<false>(a, y, Bits8{}, rstd, static_cast<hipStream_t>(stream));
+  return residual != nullptr ? launch_forward<kSums>(a, y, Bits8{}, rstd, static_cast<hipStream_t>(stream))
+                             : launch_forward<kRows>(a, y, Bits8{}, rstd, static_cast<hipStream_t>(stream));
 }
 
 int fp8gmm_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* q, void* h,
@@ -598,14 +617,14 @@ int fp8gmm_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_
   if (rc == 1) return FP8GMM_OK;
   if ((scale == nullptr) == (scale_inv == nullptr) || (scale == nullptr && amax != nullptr)) return FP8GMM_ERR_BAD_ARGUMENT;
   if (q == nullptr) return FP8GMM_ERR_NULL_POINTER;
-  return launch_forward<true>(a, nullptr, Bits8{static_cast<uint8_t*>(q), scale, amax, scale_inv, fmt}, nullptr,
+  return launch_forward<kBits8>(a, nullptr, Bits8{static_cast<uint8_t*>(q), scale, amax, scale_inv, fmt}, nullptr,
                               static_cast<hipStream_t>(stream));
 }
 
 size_t fp8gmm_rms_norm_workspace_bytes(int64_t rows, int cols, int type) {
   using namespace fp8gmm;
   if (check_rms(rows, cols, type, type) != FP8GMM_OK) return 0;
-  return (size_t)backward_blocks(rows, cols, type) * cols * sizeof(float);
+  return (size_t)backward_blocks(rows, cols, type, true) * cols * sizeof(float);
 }
 
 int fp8gmm_rms_norm_backward(const void* dy, int64_t ldy, const void* dh, int64_t ldd, const void* h, int64_t ldh, const void* weight,
@@ -624,10 +643,10 @@ int fp8gmm_rms_norm_backward(const void* dy, int64_t ldy, const void* dh, int64_
   if (dweight == nullptr && (dx == nullptr || rows == 0)) return FP8GMM_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   float* const part = dweight != nullptr ? static_cast<float*>(workspace) : nullptr;
-  const int blocks = backward_blocks(rows, cols, type);
-  const Shape shape = backward_shape(cols, type);
   const bool aligned = whole(h, ldh, cols, type) && whole(dy, ldy, cols, type) && (dh == nullptr || whole(dh, ldd, cols, type)) &&
                        (dx == nullptr || whole(dx, cols, cols, type));
+  const int blocks = backward_blocks(rows, cols, type, aligned);
+  const Shape shape = backward_shape(cols, type, aligned);
   const bool streaming = streams(rows, cols, type);
   const int mode = mode_of(cols, type, shape.lanes, aligned, streaming && type == FP8GMM_TYPE_FP32);
   bool known = true;
