@@ -499,7 +499,8 @@ Shape forward_shape(int cols, int type, bool two) {
   return s.lanes != 0 ? s : widest(cols, type);
 }
 // Backward, 2, or 1 of aligned rows that leave a workgroup two of them (16384 x 4096, bf16, 91.7 us, with 2 pieces 93.7; 65536 x 1024 90.7 and
-// 94.7; 256 x 4096 9.1 and 10.6; 4096 x 4096 30.2 and 29.5; 64 x 8192, one row, 10.9 and 9.9).
+// 94.7; 256 x 4096 9.1 and 10.6; 4096 x 4096 30.2 and 29.5; 64 x 8192, one row, 10.9 and 9.9).  The widest rows of fp32 spill some registers
+// and are ahead all the same (4096 x 16384 208 us, by the kernels for longer rows 325; 4096 x 10000 139 and 202).
 Shape backward_shape(int cols, int type, bool aligned) {
   const int pieces = pieces_of(cols, type);
   const Shape one = shape_of(pieces, 1, kNormWaves / 2, 2), s = shape_of(pieces, 2, kNormWaves, 2);

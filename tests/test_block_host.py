@@ -4,6 +4,8 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
+from torch._subclasses import FakeTensorMode
 
 import fp8_gmm_amd as pkg
 from fp8_gmm_amd import _lib, backend, moe, moe_ops
@@ -182,3 +184,55 @@ def test_adamw_status():
     assert call(tensor(exp_avg_scale=P + 5 * step), bits=8) == ARGUMENT
     assert L.fp8gmm_multi_adamw(None, 1, ctypes.byref(AdamwStep(bits=32, step=1)), None) == NULL
     assert L.fp8gmm_multi_adamw(None, 0, None, None) == NULL and L.fp8gmm_multi_adamw(None, -1, None, None) == ARGUMENT
+
+
+def fake_gpu(*shape, dtype=torch.float32):
+    return torch.empty(shape, device="cuda", dtype=dtype)
+
+
+@pytest.mark.parametrize("rows, cols", [(1, (1 << 30) + 1), (1, (1 << 32) + 64), (3, 1 << 32), (1 << 31, 8), ((1 << 32) + 1, 8)])
+def test_sizes_are_refused_before_they_are_cut_to_32_bits(rows, cols):
+    with FakeTensorMode():
+        x, w = fake_gpu(rows, cols), fake_gpu(cols)
+        for call in (lambda: pkg.rms_norm(x, w), lambda: pkg.rms_norm(x, w, 1e-5, x), lambda: pkg.rms_norm_fp8(x, w)):
+            with pytest.raises(RuntimeError, match=r"2\^30 columns"):
+                call()
+        with pytest.raises(RuntimeError, match="experts are supported"):
+            moe_ops.select_experts(x, 1)
+        if rows * cols > 1 << 32:
+            with pytest.raises(RuntimeError, match=r"2\^32 elements"):
+                backend.multi_adamw([x], [x], [x], [x], 1, 1e-3)
+    with FakeTensorMode():
+        with pytest.raises(RuntimeError, match="top_k"):
+            moe_ops.select_experts(fake_gpu(4, 64), (1 << 32) + 1)
+        with pytest.raises(RuntimeError, match="groups"):
+            moe_ops.select_experts(fake_gpu(4, 64), 1, groups=(1 << 32) + 1)
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["with gradients", "without"])
+def test_tangents_are_refused_whatever_the_gradient_mode(grad):
+    with FakeTensorMode(), fw.dual_level():
+        x, w, one = fake_gpu(3, 16), fake_gpu(16), fake_gpu(1)
+        dx, dw, d1 = (fw.make_dual(t, torch.empty_like(t)) for t in (x, w, one))
+        calls = [lambda: pkg.rms_norm(dx, w), lambda: pkg.rms_norm(x, dw), lambda: pkg.rms_norm(x, w, 1e-5, dx),
+                 lambda: pkg.rms_norm_fp8(dx, w), lambda: pkg.rms_norm_fp8(x, w, 1e-5, dx), lambda: moe_ops.select_experts(dx, 2),
+                 lambda: moe_ops.select_experts(x, 2, bias=dw)]
+        calls += [lambda i=i: backend.multi_adamw(*[[dx if j == i else x] for j in range(4)], 1, 1e-3) for i in range(4)]
+        calls += [lambda: backend.multi_adamw([x], [x], [x], [x], 1, 1e-3, norm=d1, max_norm=1.0),
+                  lambda: backend.multi_adamw([x], [x], [x], [x], 1, d1)]
+        for call in calls:
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+def test_transforms_and_tracing_are_refused():
+    x, w = torch.ones(3, 8), torch.ones(8)
+    for name, call in (("rms_norm", lambda t: pkg.rms_norm(t, w)), ("rms_norm_fp8", lambda t: pkg.rms_norm_fp8(t, w)[0].float()),
+                       ("select_experts", lambda t: moe_ops.select_experts(t[None], 2)[0]),
+                       ("multi_adamw", lambda t: backend.multi_adamw([t], [t], [t], [t], 1, 1e-3))):
+        for transformed in (lambda: torch.func.vmap(call)(x), lambda: torch.func.grad(lambda t: call(t).sum())(w),
+                            lambda: torch.func.jvp(call, (w,), (w,)), lambda: torch.jit.trace(call, (w,), check_trace=False)):
+            with pytest.raises(RuntimeError, match=f"{name} does not run under torch.func transforms or tracing"):
+                transformed()
+        with pytest.raises(RuntimeError, match="GPU tensors"):   # and not afterwards
+            call(w)

@@ -7,6 +7,7 @@ over at most 16 wavefronts: K(cols) = 64 + cols / 1024 additions bound its error
 covers the products around it.  The squares are positive: r is off by at most k r, k = 2 K u."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import fp8_gmm_amd as pkg
 from fp8_gmm_amd import backend
@@ -345,3 +346,69 @@ def test_other_streams_and_captured_passes(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(copies, eager)) and amax.item() == most > 0
         del eager
+
+
+def test_saved_tensors_are_looked_after(dev):
+    """Hooks that move what is saved, a second pass over a freed graph, rows that were changed in place, checkpointing."""
+    x, residual, w, dy, dh = inputs(dev, 30, 500, "bf16", "bf16", 21)
+    want = check(x, residual, w, dy, dh)
+    leaves = [t.detach().requires_grad_() for t in (x, residual, w)]
+
+    def norm(a, r, b):
+        return pkg.rms_norm(a, b, 1e-5, r)
+
+    def check_grads(outs):
+        got = torch.autograd.grad(outs, leaves, (dy, dh))
+        assert torch.equal(got[0], want[1]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+    with torch.autograd.graph.save_on_cpu():
+        outs = norm(*leaves)
+    check_grads(outs)
+    with pytest.raises(RuntimeError):
+        check_grads(outs)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.float()):
+        outs = norm(*leaves)
+    with pytest.raises(RuntimeError, match="saved-tensor hook"):
+        check_grads(outs)
+    rows = leaves[0] * 1.0
+    y = pkg.rms_norm(rows, leaves[2])
+    rows.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, leaves[2], dy)
+    check_grads(torch.utils.checkpoint.checkpoint(norm, *leaves, use_reentrant=False))
+    outs = norm(*leaves)
+    check_outs = [o.clone() for o in outs]
+    del outs   # (the sum is a result of the node that keeps it)
+    assert torch.autograd.grad(check_outs, leaves, (dy, dh))[2].shape == (500,)
+
+
+def test_gradients_with_tangents_are_refused(dev):
+    x, w = (torch.randn(s, device=dev, requires_grad=True) for s in ((6, 32), (32,)))
+    dy = torch.randn(6, 32, device=dev)
+    for outs in (lambda: (pkg.rms_norm(x, w),), lambda: pkg.rms_norm(x, w, 1e-5, x.detach())):
+        for i in range(len(outs())):
+            with torch.autograd.forward_ad.dual_level():
+                up = [torch.autograd.forward_ad.make_dual(dy, torch.ones_like(dy)) if j == i else dy for j in range(len(outs()))]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad(outs(), x, up)
+
+
+@pytest.mark.parametrize("rows, cols, t", [(20000, 4096, "bf16"), (9000, 4093, "fp32"), (9000, 4096, "fp32"), (70000, 512, "fp16")])
+def test_results_that_outgrow_the_cache(dev, rows, cols, t):
+    """Written with the streaming hint, by workgroups with several turns; row by row the bits of a few rows' call."""
+    x, residual, w, dy, dh = inputs(dev, rows, cols, t, t, 3)
+    with torch.no_grad():
+        y, h = pkg.rms_norm(x, w, 1e-5, residual)
+        q, inv, _ = pkg.rms_norm_fp8(x, w, 1e-5, residual)
+        plain = pkg.rms_norm(x, w, 1e-5)
+    leaf = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(pkg.rms_norm(leaf, w, 1e-5, residual), leaf, (dy, dh))
+    for part in (slice(0, 50), slice(rows // 2, rows // 2 + 50), slice(rows - 50, rows)):
+        few = x[part].clone().requires_grad_()
+        a, b = pkg.rms_norm(few, w, 1e-5, residual[part])
+        assert torch.equal(a, y[part]) and torch.equal(b, h[part])
+        assert torch.equal(torch.autograd.grad((a, b), few, (dy[part], dh[part]))[0], dx[part])
+        with torch.no_grad():
+            assert torch.equal(pkg.rms_norm(x[part], w, 1e-5), plain[part])
+            c, d, _ = pkg.rms_norm_fp8(x[part], w, 1e-5, residual[part])
+            assert torch.equal(c.view(torch.uint8), q[part].view(torch.uint8)) and torch.equal(d, inv[part])

@@ -6,6 +6,7 @@ the row's largest score is rounded by u times its magnitude, which the exponenti
 Renormalizing divides two such: 2 k and 20 u of its sum."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import fp8_gmm_amd as pkg
 from fp8_gmm_amd import moe, moe_ops
@@ -319,3 +320,49 @@ def test_a_routed_layer_chooses_so(dev, kind):
     assert torch.allclose(xa.grad.float(), xb.grad.float(), rtol=0.02, atol=2e-3) and layer.row_norm.weight.grad is not None
     layer.bfloat16()   # the bias is cast with the rest
     assert layer.expert_bias.dtype == torch.bfloat16 and torch.isfinite(layer(x)).all()
+
+
+def test_saved_tensors_are_looked_after(dev):
+    scores = scores_of(dev, 50, 64, "bf16", 4)
+    want = check(scores, 6, "sigmoid", None, 8, 4, True)
+    leaf = scores.clone().requires_grad_()
+    dw = torch.randn(50, 6, generator=gen(5)).to(dev)
+
+    def choose(t):
+        return moe_ops.select_experts(t, 6, "sigmoid", None, 8, 4, True)[0]
+
+    with torch.autograd.graph.save_on_cpu():
+        w = choose(leaf)
+    assert torch.equal(torch.autograd.grad(w, leaf, dw)[0], want[2])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(w, leaf, dw)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.float()):
+        w = choose(leaf)
+    with pytest.raises(RuntimeError, match="saved-tensor hook"):
+        torch.autograd.grad(w, leaf, dw)
+    logits = leaf * 1.0
+    w = choose(logits)
+    logits.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(w, leaf, dw)
+    again = torch.utils.checkpoint.checkpoint(choose, leaf, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(again, leaf, dw)[0], want[2])
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(choose(leaf), leaf, torch.autograd.forward_ad.make_dual(dw, torch.ones_like(dw)))
+
+
+@pytest.mark.parametrize("experts, top_k, groups", [(16, 2, 1), (60, 8, 4), (64, 6, 8), (40, 9, 1), (128, 8, 8), (256, 8, 8), (512, 4, 1)])
+def test_many_tokens_and_few_choose_alike(dev, experts, top_k, groups):
+    """Each number of tokens shares out the lanes in its own way."""
+    for t in ("bf16", "fp32"):
+        scores = scores_of(dev, 10000, experts, t, experts)
+        bias = (torch.randn(experts, generator=gen(3)) * 0.1).to(dev)
+        for b in (None, bias):
+            w, i, ds = check(scores, top_k, "sigmoid", b, groups, (groups + 1) // 2, False)
+            for n in (1, 2000, 5000):
+                part = scores[:n].clone().requires_grad_()
+                pw, pi = moe_ops.select_experts(part, top_k, "sigmoid", b, groups, (groups + 1) // 2)
+                assert torch.equal(pw, w[:n]) and torch.equal(pi, i[:n])
+                dw = torch.randn(w.shape, generator=gen(5)).to(dev)[:n]
+                assert torch.equal(torch.autograd.grad(pw, part, dw)[0], ds[:n])
