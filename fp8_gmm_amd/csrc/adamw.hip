@@ -39,6 +39,10 @@ constexpr float kTiny = 0x1p-100f;   // moments below it are zeros in 8 bits
 // thresholds in units of 2^-32
 constexpr uint32_t kStep = 0x9E3779B9u, kElement = 0x6A09E667u;   // the golden ratio and the root of 2, without their whole numbers
 
+// LDS that nobody uses: with it two workgroups share a compute unit and not four, and the nine streams of a step with masters find their
+// memory's rows open more often (470 million weights 2256 us, without it 2335; without masters it costs: 400 tensors 622 and 590).
+constexpr unsigned kIdleLds = 55 * 1024;
+
 struct Entry {
   void* param;
   const void* grad;
@@ -290,40 +294,47 @@ __device__ __forceinline__ Factors factors_of(const Hyper& h) {
   return f;
 }
 
-template <int TYPE, int GRAD, bool MASTER, bool BITS8, bool STREAM, bool FULL>
-__device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, const Hyper& h, const Factors& by) {
-  constexpr int VEC = BITS8 ? 8 : 4;
+// What a thread takes of a tensor at a time
+template <int TYPE, int GRAD, bool MASTER, bool BITS8, bool STREAM>
+struct Share {
+  static constexpr int VEC = BITS8 ? 8 : 4;
   typedef Values<FP8GMM_TYPE_FP32, VEC, STREAM> F32;
-  Values<TYPE, VEC, STREAM> param;
+  typedef Values<TYPE, VEC, STREAM> Weights;
+  std::conditional_t<MASTER, F32, Weights> param;
   Values<GRAD, VEC, STREAM> grad;
-  F32 master;
-  std::conditional_t<BITS8, Codes<STREAM>, F32> mc, vc;
-  float m_scale = 1.f, v_scale = 1.f;
-  grad.template load<FULL>(e.grad, at, n);
-  if constexpr (MASTER) master.template load<FULL>(e.master, at, n);
-  else param.template load<FULL>(e.param, at, n);
-  mc.template load<FULL>(e.m, at, n);
-  vc.template load<FULL>(e.v, at, n);
-  if constexpr (BITS8) {
-    if (FULL || n > 0) {
-      m_scale = e.m_scale[at / kBlock];
-      v_scale = e.v_scale[at / kBlock];
+  std::conditional_t<BITS8, Codes<STREAM>, F32> m, v;
+  float m_scale, v_scale;
+  template <bool FULL>
+  __device__ __forceinline__ void load(const Entry& e, int64_t at, int n) {
+    grad.template load<FULL>(e.grad, at, n);
+    param.template load<FULL>(MASTER ? static_cast<const void*>(e.master) : e.param, at, n);
+    m.template load<FULL>(e.m, at, n);
+    v.template load<FULL>(e.v, at, n);
+    if constexpr (BITS8) {
+      m_scale = FULL || n > 0 ? e.m_scale[at / kBlock] : 0.f;
+      v_scale = FULL || n > 0 ? e.v_scale[at / kBlock] : 0.f;
     }
   }
+};
+
+template <bool FULL, int TYPE, int GRAD, bool MASTER, bool BITS8, bool STREAM>
+__device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS8, STREAM>& from, const Entry& e, int64_t at, int n,
+                                            const Hyper& h, const Factors& by) {
+  typedef Share<TYPE, GRAD, MASTER, BITS8, STREAM> S;
+  constexpr int VEC = S::VEC;
   float p[VEC], g[VEC], m[VEC], v[VEC];
-  if constexpr (MASTER) master.get(p);
-  else param.get(p);
-  grad.get(g);
-  mc.get(m);
-  vc.get(v);
+  from.param.get(p);
+  from.grad.get(g);
+  from.m.get(m);
+  from.v.get(v);
   float root[VEC];
   bool rare = false;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     g[i] *= by.grad;
     if constexpr (BITS8) {
-      m[i] *= m_scale;
-      v[i] *= v_scale;
+      m[i] *= from.m_scale;
+      v[i] *= from.v_scale;
       v[i] *= v[i];
     }
     m[i] = h.b1 * m[i] + h.c1 * g[i];
@@ -343,8 +354,8 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
     p[i] = __builtin_fmaf(-by.rate, m[i] * r, __builtin_fmaf(-by.decay, p[i], p[i]));
     if constexpr (MASTER) asm("" : "+v"(p[i]));   // fp32 first, then 16 bits: the weight is the master's rounded copy
   }
-  if constexpr (MASTER) F32::template store<FULL>(e.master, at, n, p);
-  Values<TYPE, VEC, STREAM>::template store<FULL>(e.param, at, n, p);
+  if constexpr (MASTER) S::F32::template store<FULL>(e.master, at, n, p);
+  S::Weights::template store<FULL>(e.param, at, n, p);
   if constexpr (BITS8) {
     float m_most = 0.f, v_most = 0.f;
 #pragma unroll
@@ -377,8 +388,8 @@ __device__ __forceinline__ void step_values(const Entry& e, int64_t at, int n, c
     Codes<STREAM>::template store<FULL>(e.m, at, n, mw);
     Codes<STREAM>::template store<FULL>(e.v, at, n, vw);
   } else {
-    F32::template store<FULL>(e.m, at, n, m);
-    F32::template store<FULL>(e.v, at, n, v);
+    S::F32::template store<FULL>(e.m, at, n, m);
+    S::F32::template store<FULL>(e.v, at, n, v);
   }
 }
 
@@ -393,14 +404,26 @@ __global__ __launch_bounds__(threads(BITS8)) void adamw_kernel(const PartOf<MAST
   const Factors by = factors_of(h);
   const int64_t first = (int64_t)(blockIdx.x - e.begin) * SWEEP, end = first + SWEEP < e.count ? first + SWEEP : e.count;
   const auto as = [&](auto type, auto grad) {
-    constexpr int T = decltype(type)::value, G = decltype(grad)::value;
-    int64_t at = first;
+    Share<decltype(type)::value, decltype(grad)::value, MASTER, BITS8, STREAM> share;
+    int64_t at = first + threadIdx.x * VEC;
+    int left = (int)(end - first);
+    if constexpr (SWEEP == STEP) {
+      if (left >= STEP) {
+        share.template load<true>(e, at, VEC);
+        step_values<true>(share, e, at, VEC, h, by);
+        return;
+      }
+    } else {
 #pragma unroll 1
-    for (; at + STEP <= end; at += STEP) step_values<T, G, MASTER, BITS8, STREAM, true>(e, at + threadIdx.x * VEC, VEC, h, by);
-    if (at < end) {
-      const int64_t mine = at + threadIdx.x * VEC, left = end - mine;
-      step_values<T, G, MASTER, BITS8, STREAM, false>(e, mine, (int)(left < VEC ? left : VEC), h, by);
+      for (; left >= STEP; at += STEP, left -= STEP) {
+        share.template load<true>(e, at, VEC);
+        step_values<true>(share, e, at, VEC, h, by);
+      }
+      if (left == 0) return;
     }
+    const int mine = min(left - (int)threadIdx.x * VEC, VEC);
+    share.template load<false>(e, at, mine);
+    step_values<false>(share, e, at, mine, h, by);
   };
   constexpr std::integral_constant<int, FP8GMM_TYPE_BF16> bf16{};
   constexpr std::integral_constant<int, FP8GMM_TYPE_FP16> fp16{};
@@ -420,13 +443,15 @@ void launch(const fp8gmm_adamw_tensor* tensors, int n, const Hyper& h, hipStream
   int64_t bytes = 0;
   for (int i = 0; i < n; ++i)
     bytes += tensors[i].count * (2 * type_bytes(tensors[i].type) + type_bytes(tensors[i].grad_type) + (BITS8 ? 4 : 16) + (MASTER ? 8 : 0));
-  auto* kernel = bytes > kStreamBytes ? &adamw_kernel<MASTER, BITS8, true> : &adamw_kernel<MASTER, BITS8, false>;
+  const bool stream = bytes > kStreamBytes;
+  const unsigned lds = stream && MASTER && !BITS8 ? kIdleLds : 0;
+  auto* kernel = stream ? &adamw_kernel<MASTER, BITS8, true> : &adamw_kernel<MASTER, BITS8, false>;
   constexpr int64_t kMostChunks = 1 << 22;   // of a launch, which holds the largest tensor: a grid has fewer than 2^32 threads
   PartOf<MASTER, BITS8> part = {};
   int used = 0;
   int64_t chunks = 0;
   const auto flush = [&] {
-    if (used > 0) hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(threads(BITS8)), 0, s, part, used, h);
+    if (used > 0) hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(threads(BITS8)), lds, s, part, used, h);
     used = 0;
     chunks = 0;
   };
