@@ -263,6 +263,27 @@ def test_zero_moments_and_gradients(dev):
         assert torch.allclose(p.masters[0], before * (1 - 1e-4), rtol=1e-6)
 
 
+def test_squares_that_fp32_does_not_hold(dev):
+    """A second moment that is infinite leaves the decay alone; without eps, one that is zero sends a parameter to infinity."""
+    for bits in (32, 8):
+        p = Problem(dev, [500], "fp32", "fp32", bits, False, 3)
+        p.grads[0][100], p.grads[0][101] = 1e25, -1e25
+        before = p.params[0].clone()
+        p.step(1)
+        assert torch.isfinite(p.params[0]).all()
+        decayed = before.double() * (1 - 1e-4)
+        assert_within(p.params[0][100:102], decayed[100:102], 4 * U * decayed.abs()[100:102], "params")
+        if bits == 32:
+            assert p.v[0][100:102].isinf().all() and torch.isfinite(p.m[0]).all()
+        q = Problem(dev, [500], "fp32", "fp32", bits, False, 3)
+        for t in q.m + q.v:
+            t.zero_()
+        q.grads[0][1:4] = torch.tensor([0.0, 1e-25, -1e-25], device=dev)
+        q.step(1, eps=0.0)
+        assert q.params[0][1].isnan() and q.params[0][2] == -math.inf and q.params[0][3] == math.inf
+        assert torch.isfinite(q.params[0][4:]).all()
+
+
 def test_past_32_bits(dev):
     n = (1 << 31) + 12345
     tail = 4096 + 12345
