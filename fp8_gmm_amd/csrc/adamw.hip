@@ -487,6 +487,8 @@ void launch(const fp8gmm_adamw_tensor* tensors, int n, const Hyper& h, hipStream
 
 int check_tensors(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_step& step) {
   int masters = 0;
+  const auto off = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; };
+  if (off(step.norm, 4) || off(step.step_dev, 8) || off(step.lr_dev, 4)) return FP8GMM_ERR_ALIGNMENT;
   for (int i = 0; i < n; ++i) {
     const fp8gmm_adamw_tensor& t = tensors[i];
     if (!known_type(t.type) || (t.grad_type != t.type && t.grad_type != FP8GMM_TYPE_FP32)) return FP8GMM_ERR_BAD_FORMAT;
@@ -497,7 +499,6 @@ int check_tensors(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_
       return FP8GMM_ERR_NULL_POINTER;
     if (t.master != nullptr && t.type == FP8GMM_TYPE_FP32) return FP8GMM_ERR_BAD_ARGUMENT;
     masters |= t.master != nullptr ? 1 : 2;
-    const auto off = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; };
     if (off(t.param, type_bytes(t.type)) || off(t.grad, type_bytes(t.grad_type)) || off(t.master, 4) ||
         off(t.exp_avg, step.bits == 8 ? 8 : 4) || off(t.exp_avg_sq, step.bits == 8 ? 8 : 4) || off(t.exp_avg_scale, 4) || off(t.exp_avg_sq_scale, 4))
       return FP8GMM_ERR_ALIGNMENT;
@@ -508,33 +509,45 @@ int check_tensors(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_
   return masters == 3 ? FP8GMM_ERR_BAD_ARGUMENT : FP8GMM_OK;
 }
 
-// Nothing is written that another tensor of the call reads or writes.
-int check_apart(const fp8gmm_adamw_tensor* tensors, int n, int bits) {
+// Nothing is written that something else of the call reads or writes.  The ranges are sorted list by list and merged: the tensors of a list
+// mostly come in the order of their addresses.
+int check_apart(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_step& step) {
   struct Range {
     uintptr_t begin, end;
     bool writes;
   };
   std::vector<Range> ranges;
-  ranges.reserve(7 * (size_t)n);
+  ranges.reserve(7 * (size_t)n + 3);
+  const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
   const auto add = [&](const void* p, int64_t bytes, bool writes) {
     const uintptr_t begin = reinterpret_cast<uintptr_t>(p);
-    if (p != nullptr) ranges.push_back({begin, begin + (uintptr_t)bytes, writes});
+    if (p != nullptr && bytes > 0) ranges.push_back({begin, begin + (uintptr_t)bytes, writes});
   };
-  for (int i = 0; i < n; ++i) {
-    const fp8gmm_adamw_tensor& t = tensors[i];
-    if (t.count == 0) continue;
-    const int64_t moments = t.count * (bits / 8), scales = (t.count + kBlock - 1) / kBlock * 4;
-    add(t.param, t.count * type_bytes(t.type), true);
-    add(t.grad, t.count * type_bytes(t.grad_type), false);
-    add(t.exp_avg, moments, true);
-    add(t.exp_avg_sq, moments, true);
-    add(t.master, t.count * 4, true);
-    if (bits == 8) {
-      add(t.exp_avg_scale, scales, true);
-      add(t.exp_avg_sq_scale, scales, true);
-    }
-  }
-  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  const auto merge = [&](size_t from) {
+    const auto middle = ranges.begin() + (ptrdiff_t)from;
+    if (!std::is_sorted(middle, ranges.end(), before)) std::sort(middle, ranges.end(), before);
+    std::inplace_merge(ranges.begin(), middle, ranges.end(), before);
+  };
+  const auto list = [&](auto address, auto bytes, bool writes) {
+    const size_t from = ranges.size();
+    for (int i = 0; i < n; ++i) add(tensors[i].*address, bytes(tensors[i]), writes);
+    merge(from);
+  };
+  typedef fp8gmm_adamw_tensor T;
+  const auto moments = [&](const T& t) { return t.count * (step.bits / 8); };
+  const auto scales = [&](const T& t) { return step.bits == 8 ? (t.count + kBlock - 1) / kBlock * 4 : 0; };
+  list(&T::param, [](const T& t) { return t.count * type_bytes(t.type); }, true);
+  list(&T::grad, [](const T& t) { return t.count * type_bytes(t.grad_type); }, false);
+  list(&T::exp_avg, moments, true);
+  list(&T::exp_avg_sq, moments, true);
+  list(&T::exp_avg_scale, scales, true);
+  list(&T::exp_avg_sq_scale, scales, true);
+  list(&T::master, [](const T& t) { return t.count * 4; }, true);
+  const size_t from = ranges.size();
+  add(step.norm, 4, false);
+  add(step.step_dev, 8, false);
+  add(step.lr_dev, 4, false);
+  merge(from);
   uintptr_t written = 0, read = 0;   // ends of what the ranges so far write and read
   for (const Range& r : ranges) {
     if (r.begin < written || (r.writes && r.begin < read)) return FP8GMM_ERR_BAD_ARGUMENT;
@@ -552,7 +565,7 @@ int multi_adamw(const fp8gmm_adamw_tensor* tensors, int n, const fp8gmm_adamw_st
       (a.lr_dev == nullptr && !(a.lr >= 0.)))
     return FP8GMM_ERR_BAD_ARGUMENT;
   int rc = check_tensors(tensors, n, a);
-  if (rc == FP8GMM_OK) rc = check_apart(tensors, n, a.bits);
+  if (rc == FP8GMM_OK) rc = check_apart(tensors, n, a);
   if (rc != FP8GMM_OK) return rc;
   Hyper h = {};
   h.b1 = (float)a.beta1;

@@ -41,7 +41,8 @@ class AdamW(torch.optim.Optimizer):
     ``lr`` may be a float32 tensor of the device then.  Run one step ahead of the capture: it makes the states.
 
     Parameters are dense, on one device, bfloat16, float16 or float32; those without a gradient are passed over.  Without ``capturable``
-    each counts its own steps.  Checkpoints hold the states in their own types, whatever the parameters' (``state_dict``)."""
+    each counts its own steps.  Checkpoints hold the states in their own types, whatever the parameters' (``state_dict``); loading one
+    makes new states, of which a graph captured before knows nothing."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
                  max_norm=None, capturable=False):
@@ -61,8 +62,7 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, steps=None))
 
-    def _init_state(self, p):
-        state = self.state[p]
+    def _init_state(self, p, state):
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
             _fail("fp8_gmm_amd: a parameter has no state yet: run a step ahead of the capture")
         if not self.capturable:
@@ -84,51 +84,68 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        taken = [[p for p in group["params"] if p.grad is not None] for group in self.param_groups]
-        first = next(chain.from_iterable(taken), None)
+        taken = [[(p, grad) for p in group["params"] if (grad := p.grad) is not None] for group in self.param_groups]
+        first = next(chain.from_iterable(taken), (None,))[0]
         if not self.capturable and first is not None and first.is_cuda and torch.cuda.is_current_stream_capturing():
             _fail("fp8_gmm_amd: a captured step needs AdamW(capturable=True): the others' number would be the same in every replay")
         norm = None
         if self.max_norm is not None and first is not None:
-            norm = self.grad_norm = backend.multi_norm([p.grad for p in chain.from_iterable(taken)])
-        for group, params in zip(self.param_groups, taken):
-            if not params:
+            norm = self.grad_norm = backend.multi_norm([grad for _, grad in chain.from_iterable(taken)])
+        for group, pairs in zip(self.param_groups, taken):
+            if not pairs:
                 continue
-            for p in params:
-                if not self.state[p]:
-                    self._init_state(p)
             calls = {}   # the parameters of a call count the same step, and all have masters or none
+            for p, grad in pairs:
+                state = self.state[p]
+                if not state:
+                    self._init_state(p, state)
+                calls.setdefault((None if self.capturable else state["step"] + 1, "master" in state), []).append((p, grad, state))
             if self.capturable:
                 if group["steps"] is None:
-                    group["steps"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
+                    group["steps"] = torch.zeros((), dtype=torch.int64, device=pairs[0][0].device)
                 group["steps"].add_(1)
-            for p in params:
-                state = self.state[p]
-                if not self.capturable:
-                    state["step"] += 1
-                key = (group["steps"] if self.capturable else state["step"], "master" in state)
-                calls.setdefault(key, []).append(p)
             for (step, masters), some in calls.items():
-                states = [self.state[p] for p in some]
+                params, grads, states = zip(*some)
 
                 def of(name):
                     return [state[name] for state in states]
 
-                backend.multi_adamw(some, [p.grad for p in some], of("exp_avg"), of("exp_avg_sq"), step, group["lr"], tuple(group["betas"]),
-                                    group["eps"], group["weight_decay"],
+                backend.multi_adamw(params, grads, of("exp_avg"), of("exp_avg_sq"), group["steps"] if self.capturable else step, group["lr"],
+                                    tuple(group["betas"]), group["eps"], group["weight_decay"],
                                     (of("exp_avg_scale"), of("exp_avg_sq_scale")) if self.state_bits == 8 else None,
                                     of("master") if masters else None, norm, None if norm is None else self.max_norm)
+                if not self.capturable:
+                    for state in states:
+                        state["step"] = step
         return loss
 
     def load_state_dict(self, state_dict):
+        """A checkpoint of this class and of the same ``state_bits``; its way of counting steps and its masters become this optimizer's."""
+        for group in state_dict["param_groups"]:
+            states = [state_dict["state"][key] for key in group["params"] if key in state_dict["state"]]
+            if "steps" not in group or any(("exp_avg_scale" in state) != (self.state_bits == 8) for state in states):
+                raise ValueError(f"not a checkpoint of an AdamW of {self.state_bits}-bit moments")
+            if self.capturable and len({state.get("step") for state in states}) > 1:
+                raise ValueError("the parameters of a capturable group count the same steps, the checkpoint's have different ones")
         super().load_state_dict(state_dict)
-        # torch has cast the states to their parameters' types
-        saved = chain.from_iterable(group["params"] for group in state_dict["param_groups"])
-        for key, p in zip(saved, chain.from_iterable(group["params"] for group in self.param_groups)):
-            for name, value in state_dict["state"].get(key, {}).items():
-                if isinstance(value, torch.Tensor):
-                    self.state[p][name] = value.detach().to(p.device, copy=True)
         for group, old in zip(self.param_groups, state_dict["param_groups"]):
-            for name in ("steps", "lr"):
-                if isinstance(old.get(name), torch.Tensor):
-                    group[name] = old[name].detach().to(group["params"][0].device, copy=True)
+            device = group["params"][0].device
+            if isinstance(old["lr"], torch.Tensor):
+                group["lr"] = old["lr"].detach().to(device, copy=True) if self.capturable else old["lr"].item()
+            steps = old["steps"]
+            for key, p in zip(old["params"], group["params"]):
+                if key not in state_dict["state"]:
+                    continue
+                state = self.state[p]
+                # torch has cast the tensors to their parameters' types
+                state.update((name, value.detach().to(p.device, copy=True))
+                             for name, value in state_dict["state"][key].items() if isinstance(value, torch.Tensor))
+                if self.capturable:
+                    steps = state.pop("step", steps)
+                else:
+                    state.setdefault("step", None if steps is None else int(steps))
+                if not (self.master_weights and p.dtype != torch.float32):
+                    state.pop("master", None)
+                elif "master" not in state:
+                    state["master"] = p.detach().float()
+            group["steps"] = torch.full((), int(steps), dtype=torch.int64, device=device) if self.capturable and steps is not None else None

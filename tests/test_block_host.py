@@ -73,6 +73,46 @@ def test_optimizer_state_keeps_its_types_in_a_checkpoint():
     assert torch.equal(got["master"], state["master"]) and got["master"] is not state["master"] and got["exp_avg_scale"].shape == (3,)
 
 
+def test_optimizer_takes_a_checkpoint_of_other_options():
+    def make(**options):
+        return pkg.AdamW([torch.nn.Parameter(torch.full((3,), i + 1.0, dtype=torch.bfloat16)) for i in range(2)], **options)
+
+    def stepped(*steps, **options):
+        opt = make(**options)
+        for p, step in zip(opt.param_groups[0]["params"], steps):
+            opt._init_state(p, opt.state[p])
+            if not opt.capturable:
+                opt.state[p]["step"] = step
+        if opt.capturable:
+            opt.param_groups[0]["steps"] = torch.tensor(steps[0])
+        return opt
+
+    counted = make()
+    counted.load_state_dict(stepped(7, 7, capturable=True, lr=torch.tensor(0.5)).state_dict())
+    assert all(counted.state[p]["step"] == 7 for p in counted.param_groups[0]["params"])
+    assert counted.param_groups[0]["steps"] is None and counted.param_groups[0]["lr"] == 0.5
+    on_device = make(capturable=True)
+    on_device.load_state_dict(stepped(4, 4).state_dict())
+    assert on_device.param_groups[0]["steps"].dtype == torch.int64 and on_device.param_groups[0]["steps"].item() == 4
+    assert not any("step" in on_device.state[p] for p in on_device.param_groups[0]["params"])
+    fresh = make(capturable=True)
+    fresh.load_state_dict(make().state_dict())
+    assert fresh.param_groups[0]["steps"] is None and not fresh.state
+    with pytest.raises(ValueError, match="different"):
+        make(capturable=True).load_state_dict(stepped(4, 5).state_dict())
+    masters = make(master_weights=True)
+    masters.load_state_dict(stepped(4, 4).state_dict())
+    assert all(torch.equal(masters.state[p]["master"], p.detach().float()) for p in masters.param_groups[0]["params"])
+    without = make()
+    without.load_state_dict(masters.state_dict())
+    assert not any("master" in without.state[p] for p in without.param_groups[0]["params"])
+    plain = torch.optim.AdamW([torch.nn.Parameter(torch.ones(3)) for _ in range(2)])
+    for opt, other in ((make(), stepped(1, 1, state_bits=8)), (make(state_bits=8), stepped(1, 1)), (make(), plain)):
+        with pytest.raises(ValueError, match="not a checkpoint"):
+            opt.load_state_dict(other.state_dict())
+        assert not opt.state
+
+
 def test_rms_norm_status():
     L = _lib.load()
 
@@ -182,6 +222,12 @@ def test_adamw_status():
     assert call(tensor(), tensor()) == ARGUMENT and call(tensor(grad=P)) == ARGUMENT        # shared memory
     assert call(tensor(exp_avg=P + 1998)) == ALIGN and call(tensor(exp_avg=P + 1996)) == ARGUMENT
     assert call(tensor(exp_avg_scale=P + 5 * step), bits=8) == ARGUMENT
+    for name in ("norm", "step_dev", "lr_dev"):
+        assert call(tensor(), **{name: P + 1800}) == ARGUMENT and call(tensor(), **{name: P + 2 * step + 16}) == ARGUMENT
+        assert call(tensor(), **{name: P - 2}) == ALIGN
+    # in any order of the tensors' addresses
+    assert call(tensor(3), tensor(1), tensor(2, param=P + (8 + 2) * step + 400)) == ARGUMENT
+    assert call(tensor(1), tensor(3), tensor(2), tensor(0), tensor(2)) == ARGUMENT
     assert L.fp8gmm_multi_adamw(None, 1, ctypes.byref(AdamwStep(bits=32, step=1)), None) == NULL
     assert L.fp8gmm_multi_adamw(None, 0, None, None) == NULL and L.fp8gmm_multi_adamw(None, -1, None, None) == ARGUMENT
 
