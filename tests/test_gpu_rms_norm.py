@@ -225,6 +225,15 @@ def test_without_rows_and_with_some_gradients(dev):
     a, = torch.autograd.grad(both, xs, (dy, dh))
     b, = torch.autograd.grad((y, h), xs, (dy, dh))
     assert torch.allclose(a.float(), 2 * b.float(), rtol=2 ** -7)
+    leaves = [t.clone().requires_grad_() for t in (x, residual)]   # each has a gradient of its own
+    for used in ((0, 1), (1,)):
+        for t in leaves:
+            t.grad = None
+        results = pkg.rms_norm(leaves[0], w, 1e-5, leaves[1])
+        torch.autograd.backward([results[i] for i in used], [(dy, dh)[i] for i in used])
+        kept = leaves[1].grad.clone()
+        leaves[0].grad.zero_()
+        assert torch.equal(leaves[1].grad, kept) and kept.any() and dh.any()
     one = pkg.rms_norm(x[0], w)              # a vector
     assert one.shape == (96,) and torch.equal(one, pkg.rms_norm(x[:1], w)[0])
     q, inv, _ = pkg.rms_norm_fp8(x[0], w)
