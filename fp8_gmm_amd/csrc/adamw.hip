@@ -26,8 +26,8 @@ namespace {
 
 // Threads and elements of a workgroup, 4 (32 bits) or 8 to a thread at a time.  Of lists that no cache holds, us: 400 tensors of bf16 with
 // fp32 moments by 512 threads and 2048 elements 596, by 256 and 1024 597, and 2048 625, and 4096 670, by 128 and 2048 669; 96 tensors of fp32
-// by 512 and 2048 761, by 256 and 1024 786; 96 tensors with 8-bit moments, which take ten times the instructions, by 256 and 4096 299, and
-// 8192 294, and 2048 337, by 512 and 4096 343.
+// by 512 and 2048 761, by 256 and 1024 786; 96 tensors with 8-bit moments, which take ten times the instructions, by 256 and 4096 278, and
+// 6144 279, by 512 and 8192 293, by 128 and 2048 279; the same of fp32 471, 481, 474 and 482.
 constexpr int threads(bool bits8) { return bits8 ? 256 : 512; }
 constexpr int sweep(bool bits8) { return bits8 ? 4096 : 2048; }
 // From so many bytes on everything is read and written with the streaming hint: nothing of it is found in the caches by the next step
@@ -230,17 +230,25 @@ __device__ __forceinline__ uint32_t round_linear(float y, uint32_t h, uint32_t o
 }
 // 0 <= y <= 448 to a code, up with the probability of its square's way to the next one's.  The codes lie 2^(e-3) apart from 2^e on, from
 // 2^-6 down 2^-9: adding 2^-6 there makes the distance that of all numbers with its exponent, and the last 20 bits of the fraction what
-// lies between two codes.  NORMAL: none is below 2^-6.
-template <bool NORMAL>
+// lies between two codes.
+__device__ __forceinline__ float threshold_of(uint32_t h) { return (float)((h ^ 0x80000000u) >> 8); }   // in units of 2^-24
 __device__ __forceinline__ float round_root(float y, uint32_t h) {
-  const float off = !NORMAL && y < 0x1p-6f ? 0x1p-6f : 0.f;
-  const uint32_t bits = __float_as_uint(NORMAL ? y : y + off);
-  const float cut = __uint_as_float(bits & 0xfff00000u), lo = NORMAL ? cut : cut - off;
-  const float eight = __uint_as_float(bits & 0x7f800000u), gap = eight * 0.125f;
+  const float off = y < 0x1p-6f ? 0x1p-6f : 0.f;
+  const uint32_t bits = __float_as_uint(y + off);
+  const float lo = __uint_as_float(bits & 0xfff00000u) - off, eight = __uint_as_float(bits & 0x7f800000u), gap = eight * 0.125f;
   const float ways = eight * 0x1p-27f * __builtin_fmaf(2.f, lo, gap);   // the squares' distance, in units of the threshold
-  const bool up = (y - lo) * (y + lo) > (float)((h ^ 0x80000000u) >> 8) * ways;
+  const bool up = (y - lo) * (y + lo) > threshold_of(h) * ways;
   const float code = up ? lo + gap : lo;
-  return !NORMAL && y > 0.f ? fmaxf(code, 0x1p-9f) : code;
+  return y > 0.f ? fmaxf(code, 0x1p-9f) : code;
+}
+// The same of 2^-6 <= y, with the fraction alone, as a number between 8 and 16, where the codes lie 1 apart; the hardware's rounding by a
+// random number of ones or zeros goes up (from what is no code) or down.  Byte I of `old`.
+template <int I>
+__device__ __forceinline__ uint32_t round_normal_root(float y, uint32_t h, uint32_t old) {
+  const uint32_t bits = (__float_as_uint(y) & 0x007fffffu) | 0x41000000u;
+  const float v = __uint_as_float(bits), lo = __uint_as_float(bits & 0xfff00000u);
+  const bool up = (v - lo) * (v + lo) > threshold_of(h) * __builtin_fmaf(0x1p-23f, lo, 0x1p-24f);
+  return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(y, up ? -1 : 0, (int)old, I);
 }
 
 // The root of a number that is zero, normal or a NaN: the hardware's guess of its inverse and a step of Newton's, correctly rounded but in
@@ -329,8 +337,8 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
   from.grad.get(g);
   from.m.get(m);
   from.v.get(v);
-  float root[VEC], ratio[VEC];
-  bool rare = !(h.eps >= 0x1p-120f && h.eps < 0x1p120f);
+  float root[VEC], ratio[VEC], v_most = 0.f;
+  bool rare = !(h.eps >= 0x1p-30f && h.eps < 0x1p120f);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     g[i] *= by.grad;
@@ -342,10 +350,23 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
     m[i] = h.b1 * m[i] + h.c1 * g[i];
     v[i] = h.b2 * v[i] + h.c2 * g[i] * g[i];
     root[i] = root_of(v[i]);
-    rare = rare || __builtin_isfpclass(v[i], 0x290);   // subnormal, or infinite
+    if constexpr (!BITS8) rare = rare || __builtin_isfpclass(v[i], 0x290);   // subnormal, or infinite
     const float d = __builtin_fmaf(root[i], by.root, h.eps);
-    const float r = __builtin_amdgcn_rcpf(d);   // and a step of Newton's: 4 instructions for a division's 10
-    ratio[i] = m[i] * __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
+    float r = __builtin_amdgcn_rcpf(d);   // to one in 2^23; with a step of Newton's 4 instructions for a division's 10
+    if constexpr (!BITS8) r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
+    ratio[i] = m[i] * r;
+  }
+  const auto root_max = [&] {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) most = amax_or_nan(most, root[i], root[i + 1]);
+    return block_max(most);
+  };
+  if constexpr (BITS8) {
+    // A block at a time: an infinite v leaves a NaN in its root.  A subnormal one's root is wrong, but not zero and so far below the others'
+    // that its code is the smallest one, and below eps in the quotient.
+    v_most = root_max();
+    rare = rare || !(v_most < 0x1p62f) || (v_most < 0x1p-40f && v_most != 0.f);
   }
   if (__builtin_expect(rare, 0)) {   // what the guesses do not reach
 #pragma unroll
@@ -353,6 +374,7 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
       root[i] = sqrtf(v[i]);
       ratio[i] = m[i] / __builtin_fmaf(root[i], by.root, h.eps);
     }
+    if constexpr (BITS8) v_most = root_max();
   }
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
@@ -362,35 +384,38 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
   if constexpr (MASTER) S::F32::template store<FULL>(e.master, at, n, p);
   S::Weights::template store<FULL>(e.param, at, n, p);
   if constexpr (BITS8) {
-    float m_most = 0.f, v_most = 0.f;
+    float m_most = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; i += 2) {
-      m_most = amax_or_nan(m_most, m[i], m[i + 1]);
-      v_most = amax_or_nan(v_most, root[i], root[i + 1]);
-    }
+    for (int i = 0; i < VEC; i += 2) m_most = amax_or_nan(m_most, m[i], m[i + 1]);
     m_most = block_max(m_most);
-    v_most = block_max(v_most);
     const float m_inv = codes_per(m_most), v_inv = codes_per(v_most);
     const uint32_t first = (uint32_t)at * kElement + by.dither;
-    u32x2 mw = {0u, 0u}, vw;
+    u32x2 mw = {0u, 0u}, vw = {0u, 0u};
     float least = kMost;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       root[i] = fminf(root[i] * v_inv, kMost);   // (the largest's product may round to more)
       least = fminf(least, root[i]);
     }
-    const auto codes = [&](auto normal) {
+    if (__any(least < 0x1p-6f)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float c[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) c[k] = round_root<decltype(normal)::value>(root[4 * i + k], first + (4 * i + k) * kElement);
+        for (int k = 0; k < 4; ++k) c[k] = round_root(root[4 * i + k], first + (4 * i + k) * kElement);
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
         vw[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
       }
-    };
-    // A wavefront without the small ones takes a fifth fewer instructions (96 tensors of bf16 294 us, 301 by the longer form alone).
-    __any(least < 0x1p-6f) ? codes(std::false_type{}) : codes(std::true_type{});
+    } else {   // a fifth fewer instructions (96 tensors of bf16 287 us, by the longer form alone 301)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = 4 * i;
+        vw[i] = round_normal_root<0>(root[j], first + j * kElement, vw[i]);
+        vw[i] = round_normal_root<1>(root[j + 1], first + (j + 1) * kElement, vw[i]);
+        vw[i] = round_normal_root<2>(root[j + 2], first + (j + 2) * kElement, vw[i]);
+        vw[i] = round_normal_root<3>(root[j + 3], first + (j + 3) * kElement, vw[i]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int j = 4 * i;
@@ -418,24 +443,44 @@ __global__ __launch_bounds__(threads(BITS8)) void adamw_kernel(const PartOf<MAST
   for (int i = threadIdx.x; i < n; i += THREADS)
     if (part.begin[i] <= blockIdx.x && (i + 1 == n || blockIdx.x < part.begin[i + 1])) found = i;
   __syncthreads();
-  const Entry e = unpack<MASTER, BITS8>(part, __builtin_amdgcn_readfirstlane(found));
-  const Factors by = factors_of(h);
+  Entry e = unpack<MASTER, BITS8>(part, __builtin_amdgcn_readfirstlane(found));
+  Factors by = factors_of(h);
   const int64_t first = (int64_t)(blockIdx.x - e.begin) * SWEEP, end = first + SWEEP < e.count ? first + SWEEP : e.count;
   const auto as = [&](auto type, auto grad) {
-    Share<decltype(type)::value, decltype(grad)::value, MASTER, BITS8, STREAM> share;
-    int64_t at = first + threadIdx.x * VEC;
+    constexpr int TYPE = decltype(type)::value, GRAD = decltype(grad)::value;
+    Share<TYPE, GRAD, MASTER, BITS8, STREAM> share;
     int left = (int)(end - first);
+    int64_t at = threadIdx.x * VEC;
     if constexpr (SWEEP == STEP) {
+      at += first;
       if (left >= STEP) {
         share.template load<true>(e, at, VEC);
         step_values<true>(share, e, at, VEC, h, by);
         return;
       }
     } else {
+      // Where the workgroup is stays in scalar registers: without the threads' places there is room for 6 wavefronts (96 tensors 280 us, with
+      // 5 of them 287).
+      const auto go_on = [&](int64_t elements) {
+        const auto go = [&](auto*& p, int64_t bytes) {
+          typedef std::remove_pointer_t<std::remove_reference_t<decltype(p)>> T;
+          p = reinterpret_cast<T*>(reinterpret_cast<std::conditional_t<std::is_const_v<T>, const char*, char*>>(p) + bytes);
+        };
+        go(e.param, elements * Elements<TYPE>::kBytes);
+        go(e.grad, elements * Elements<GRAD>::kBytes);
+        go(e.m, elements);
+        go(e.v, elements);
+        go(e.m_scale, elements / kBlock * 4);
+        go(e.v_scale, elements / kBlock * 4);
+        if constexpr (MASTER) go(e.master, elements * 4);
+        by.dither += (uint32_t)elements * kElement;
+      };
+      go_on(first);
 #pragma unroll 1
-      for (; left >= STEP; at += STEP, left -= STEP) {
+      for (; left >= STEP; left -= STEP) {
         share.template load<true>(e, at, VEC);
         step_values<true>(share, e, at, VEC, h, by);
+        go_on(STEP);
       }
       if (left == 0) return;
     }
