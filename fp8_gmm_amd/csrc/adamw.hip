@@ -338,7 +338,7 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
   from.m.get(m);
   from.v.get(v);
   float root[VEC], ratio[VEC], v_most = 0.f;
-  bool rare = !(h.eps >= 0x1p-30f && h.eps < 0x1p120f);
+  bool rare = !(h.eps >= (BITS8 ? 0x1p-30f : 0x1p-120f) && h.eps < 0x1p120f);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     g[i] *= by.grad;
@@ -364,7 +364,7 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
   };
   if constexpr (BITS8) {
     // A block at a time: an infinite v leaves a NaN in its root.  A subnormal one's root is wrong, but not zero and so far below the others'
-    // that its code is the smallest one, and below eps in the quotient.
+    // that its code is the smallest one, and 2^-33 of eps in the quotient (below an eps of 2^-30 all take the longer way).
     v_most = root_max();
     rare = rare || !(v_most < 0x1p62f) || (v_most < 0x1p-40f && v_most != 0.f);
   }
