@@ -716,9 +716,7 @@ def multi_adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.99
     replayed graph reads anew.  What is written may share memory with nothing else of the call.  A gradient that is no number leaves
     none in its element, with 8-bit moments in the moments of its block."""
     flush_uploads()   # a queued launch may write what is read here
-    native.multi_adamw(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), step, lr, betas, eps, weight_decay,
-                       None if scales is None else (list(scales[0]), list(scales[1])), None if masters is None else list(masters), norm,
-                       max_norm)
+    native.multi_adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, scales, masters, norm, max_norm)
 
 
 def _fill_transpose_shapes(table, x, t):

@@ -23,6 +23,21 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_lists_of_what_is_no_tensor_are_refused():
+    x = torch.ones(8)
+    for bad in (5, None, [x, None], [x, 1.0], ["x"], [[x]]):
+        for i in range(4):
+            with pytest.raises(TypeError):
+                backend.multi_adamw(*[bad if j == i else [x] for j in range(4)], 1, 1e-3)
+        with pytest.raises(TypeError):
+            backend.multi_adamw([x], [x], [x], [x], 1, 1e-3, scales=([x], bad))
+        with pytest.raises(RuntimeError if bad is None else TypeError):   # None: without masters
+            backend.multi_adamw([x], [x], [x], [x], 1, 1e-3, masters=bad)
+    for given in ((x,), iter([x]), (t for t in [x])):   # anything that iterates over tensors
+        with pytest.raises(RuntimeError, match="GPU tensors"):
+            backend.multi_adamw(given, [x], [x], [x], 1, 1e-3)
+
+
 def test_modules_hold_their_parameters():
     norm = pkg.RMSNorm(16, eps=1e-6, dtype=torch.float32, device="cpu")
     assert list(norm.state_dict()) == ["weight"] and (norm.weight == 1).all() and "1e-06" in repr(norm)
