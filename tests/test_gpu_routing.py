@@ -155,6 +155,30 @@ def test_masked_scores(dev):
             assert ((i < 8) | (i >= 48)).all() and torch.isfinite(ds).all() and not ds[:, 5:50].any()
 
 
+@pytest.mark.parametrize("tokens", [40, 5000, 20000])
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float32])
+def test_tokens_with_few_experts_left(dev, tokens, t):
+    scores = scores_of(dev, tokens, 32, "fp32", 5).to(t)
+    scores[1::4, :29] = -float("inf")   # three are left
+    scores[2::4] = -float("inf")        # none
+    for kind in (dict(), dict(bias=torch.zeros(32, device=dev)), dict(groups=4, top_groups=3)):
+        for scoring in ("softmax", "sigmoid"):
+            s = scores.clone().requires_grad_()
+            w, i = moe_ops.select_experts(s, 8, scoring, **kind)
+            ds, = torch.autograd.grad(w, s, torch.ones_like(w))
+            assert (i[1::4, :3] >= 29).all() and i[2::4].tolist() == [list(range(8))] * len(i[2::4])
+            assert i[1::4, 3:].tolist() == [[0, 1, 2, 3, 4]] * len(i[1::4])
+            assert (w[1::4, :3] > 0).all() and not w[1::4, 3:].any() and not ds[1::4, :29].any()
+            assert w[2::4].isnan().all() if scoring == "softmax" else not w[2::4].any()
+            for kept in (w, ds):
+                assert torch.isfinite(kept[0::4]).all() and torch.isfinite(kept[1::4]).all() and torch.isfinite(kept[3::4]).all()
+    bias = torch.zeros(32, device=dev)
+    bias[4:20] = -float("inf")
+    for scoring in ("softmax", "sigmoid"):
+        w, i = moe_ops.select_experts(scores[0::4].contiguous(), 8, scoring, bias)
+        assert ((i < 4) | (i >= 20)).all() and torch.isfinite(w).all()
+
+
 def test_what_is_no_number(dev):
     scores = scores_of(dev, 4, 32, "fp32", 3)
     scores[0, 3] = float("nan")
