@@ -52,6 +52,15 @@ __device__ __forceinline__ double rcp64(double d) {
   r = __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
   return __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
 }
+// exp(x) of x <= 0, 2 units in the last place: the hardware's power of 2 of the rounded product, and what the rounding left of it to the
+// first order.  A NaN stays one, what is below e^-200 is zero (expf takes half as many instructions again).
+__device__ __forceinline__ float exp_of(float x) {
+  x = __builtin_elementwise_maximum(x, -200.f);
+  const float t = x * 0x1.715476p+0f;
+  const float rest = __builtin_fmaf(x, 0x1.4ae0bep-26f, __builtin_fmaf(x, 0x1.715476p+0f, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, rest * 0x1.62e43p-1f, e);
+}
 __device__ __forceinline__ float sigmoid(float s) { return 1.f / (1.f + expf(-s)); }
 
 // Keys of 64 bits.  What is no number goes last, with minus infinity.
@@ -87,13 +96,21 @@ __device__ __forceinline__ void strike(key64& key, bool gone) {   // the upper h
 
 // Keys of 31 bits, of 16-bit scores
 typedef uint32_t key32;
+// Two scores as numbers without a sign in their order: 2^15 and their magnitude more or less (so there is one zero), and so much on top
+// that NaN above infinity pass 2^16, to where those below minus infinity are; all of these become minus infinity.
 template <int TYPE>
-__device__ __forceinline__ key32 key_of_bits(uint32_t b, int number) {
-  constexpr uint32_t kInf = TYPE == FP8GMM_TYPE_BF16 ? 0x7f80u : 0x7c00u;
-  if ((b & 0x7fffu) > kInf) b = 0x8000u | kInf;   // a NaN goes last, with minus infinity
-  if (b == 0x8000u) b = 0u;                       // one zero, not two
-  const uint32_t order = b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
-  return order << 15 | (uint32_t)(0x7fff - number);
+__device__ __forceinline__ uint32_t order_of(uint32_t two) {
+  typedef uint16_t pair __attribute__((ext_vector_type(2)));
+  typedef int16_t signed_pair __attribute__((ext_vector_type(2)));
+  constexpr int kInf = TYPE == FP8GMM_TYPE_BF16 ? 0x7f80 : 0x7c00, kTop = 0x7fff - kInf, kLast = 0x8000 - kInf + kTop;
+  const signed_pair sign = __builtin_bit_cast(signed_pair, two) >> (int16_t)15;
+  const signed_pair v = (__builtin_bit_cast(signed_pair, two & 0x7fff7fffu) ^ sign) - sign;
+  const pair order = __builtin_bit_cast(pair, v) + (uint16_t)(0x8000 + kTop);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(order, pair{kLast, kLast}));
+}
+// of the pair's first or second
+__device__ __forceinline__ key32 key_of_order(uint32_t two, bool second, int number) {
+  return ((second ? two >> 1 : two << 15) & 0x7fff8000u) | (uint32_t)(0x7fff - number);
 }
 __device__ __forceinline__ key32 larger(key32 a, key32 b) { return max(a, b); }
 __device__ __forceinline__ int number_of(key32 key) { return 0x7fff - (int)(key & 0x7fffu); }
@@ -129,6 +146,26 @@ __device__ __forceinline__ T over(T v, F&& f) {
   if constexpr (LANES > 8) v = f(v, other_lane<0x140>(v));   // row_mirror: the other eight
   if constexpr (LANES == 64) v = f(f(lane_of(v, 0), lane_of(v, 16)), f(lane_of(v, 32), lane_of(v, 48)));
   return v;
+}
+// v of lane K of a token
+template <int LANES, int K, class T>
+__device__ __forceinline__ T from_lane(T v) {
+  if constexpr (LANES == 64) {
+    return lane_of(v, K);
+  } else {
+    const T first = other_lane<0x150 + K>(v);   // row_newbcast
+    if constexpr (LANES == 16) return first;
+    else return threadIdx.x & 8 ? other_lane<0x158 + K>(v) : first;
+  }
+}
+// calls f(k) for the choices k < top_k, as integral constants
+template <int LANES, int K = 0, class F>
+__device__ __forceinline__ void each_choice(int top_k, F&& f) {
+  if constexpr (K < kMaxChoices && K < LANES) {
+    if (K >= top_k) return;
+    f(std::integral_constant<int, K>{});
+    each_choice<LANES, K + 1>(top_k, f);
+  }
 }
 struct LargerKey {
   template <class K>
@@ -184,7 +221,7 @@ struct Piece {
       for (int j = 0; j < V; ++j) s[i * V + j] = i * V + j < left ? f[j] : -INFINITY;
     }
   }
-  __device__ __forceinline__ uint32_t bits16(int j) const { return raw[j / V][j % V / 2] >> j % 2 * 16 & 0xffffu; }
+  __device__ __forceinline__ uint32_t two(int j) const { return raw[j / V][j % V / 2]; }   // elements j and j + 1, of 16 bits
   static __device__ __forceinline__ void store(void* base, int64_t first, int left, const float (&s)[PER]) {
     bits* const p = static_cast<bits*>(base) + first;
 #pragma unroll
@@ -329,15 +366,15 @@ __device__ __forceinline__ int take_largest(K (&key)[PER], int top_k, int lane) 
   return number_of(mine);
 }
 
-// SCORES: the scores decide; else p in 64 bits does, with the bias or for the groups' sums
-template <int TYPE, int LANES, int PER, bool SCORES>
+// SCORES: the scores decide; else p in 64 bits does, with the bias or for the groups' sums.  WHOLE: as many experts as the lanes hold.
+template <int TYPE, int LANES, int PER, bool SCORES, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __restrict__ scores, int tokens, const Choice c,
                                                                   float* __restrict__ weights, int64_t* __restrict__ selected) {
   const int lane = threadIdx.x % LANES;
   const int64_t token = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool live = token < tokens;   // the others' lanes are read by nobody, but go along
   const int64_t from = live ? token : tokens - 1;
-  const int e0 = lane * PER, left = c.experts - e0;
+  const int e0 = lane * PER, left = WHOLE ? PER : c.experts - e0;
   Piece<TYPE, PER> piece;
   piece.load(scores, from * c.experts + e0, left);
   float s[PER];
@@ -355,14 +392,19 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
     if (!c.sigmoid) {
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) sum += j < left ? expf(s[j] - most) : 0.f;
+      for (int j = 0; j < PER; ++j) sum += j < left ? exp_of(s[j] - most) : 0.f;
       total = over<LANES>(sum, Sum{});
     }
     std::conditional_t<TYPE == FP8GMM_TYPE_FP32, key64, key32> key[PER];
+    uint32_t two = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      if constexpr (TYPE == FP8GMM_TYPE_FP32) key[j] = key_of((double)s[j], e0 + j);
-      else key[j] = key_of_bits<TYPE>(piece.bits16(j), e0 + j);
+      if constexpr (TYPE == FP8GMM_TYPE_FP32) {
+        key[j] = key_of((double)s[j], e0 + j);
+      } else {
+        if (j % 2 == 0) two = order_of<TYPE>(piece.two(j));
+        key[j] = key_of_order(two, j % 2, e0 + j);
+      }
       strike(key[j], j >= left);
     }
     if (grouped) keep_groups<LANES, PER, 1>(key, c, lane);
@@ -397,7 +439,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
   float w = 0.f;
   if (has) {
     const float v = score_of<TYPE>(scores, from, c.experts, chosen);
-    w = c.sigmoid ? sigmoid(v) : expf(v - most) / total;
+    w = c.sigmoid ? sigmoid(v) : exp_of(v - most) / total;
   }
   if (c.renormalize) w /= over<LANES>(w, Sum{});
   if (has && live) {
@@ -408,7 +450,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
 
 // Of the weights' gradients: with v = p[chosen] and renormalized weights dv = (dw - (sum of dw v) / (sum of v)) scale / (sum of v),
 // otherwise dv = scale dw; through the sigmoid ds = dv p (1 - p), through the softmax ds = p (dv - sum of dv v).
-template <int TYPE, int LANES, int PER>
+template <int TYPE, int LANES, int PER, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const void* __restrict__ scores, int tokens, const Choice c,
                                                                            const int64_t* __restrict__ selected,
                                                                            const float* __restrict__ grad_weights,
@@ -417,7 +459,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
   const int64_t token = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool live = token < tokens;
   const int64_t from = live ? token : tokens - 1;
-  const int e0 = lane * PER, left = c.experts - e0;
+  const int e0 = lane * PER, left = WHOLE ? PER : c.experts - e0;
   float s[PER], most = 0.f, total = 1.f;
   if (!c.sigmoid) {
     Piece<TYPE, PER> piece;
@@ -430,7 +472,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      s[j] = j < left ? expf(s[j] - most) : 0.f;
+      s[j] = j < left ? exp_of(s[j] - most) : 0.f;
       sum += s[j];
     }
     total = over<LANES>(sum, Sum{});
@@ -444,7 +486,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
     if ((uint64_t)e < (uint64_t)c.experts) {   // not an expert: no gradient
       chosen = (int)e;
       const float v = score_of<TYPE>(scores, from, c.experts, chosen);
-      p = c.sigmoid ? sigmoid(v) : expf(v - most) / total;
+      p = c.sigmoid ? sigmoid(v) : exp_of(v - most) / total;
       rest = c.sigmoid ? 1.f / (1.f + expf(v)) : 0.f;
     } else {
       g = 0.f;
@@ -459,12 +501,12 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
   float out[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) out[j] = 0.f;
-  for (int k = 0; k < c.top_k; ++k) {
-    const int at = __shfl(chosen, k, LANES) - e0;
-    const float v = __shfl(g, k, LANES);
+  each_choice<LANES>(c.top_k, [&](auto k) {   // (by exchanges through LDS 3 % slower, single tokens 6 %)
+    const int at = (int)from_lane<LANES, decltype(k)::value>((uint32_t)chosen) - e0;
+    const float v = from_lane<LANES, decltype(k)::value>(g);
 #pragma unroll
     for (int j = 0; j < PER; ++j) out[j] = at == j ? v : out[j];
-  }
+  });
   const float inv = 1.f / total;
   if (!c.sigmoid)
 #pragma unroll
@@ -537,9 +579,11 @@ int fp8gmm_select_experts(const void* scores, int type, int64_t tokens, const fp
   const Choice c = choice_of(*choice);
   with_shape(type, tokens, c, [&](auto t, auto lanes, auto per) {
     constexpr int TOKENS = kThreads / decltype(lanes)::value;
-    const bool by_scores = c.bias == nullptr && (c.top_groups == c.groups || c.group_best == 1);
-    auto* kernel = by_scores ? &select_experts_kernel<decltype(t)::value, decltype(lanes)::value, decltype(per)::value, true>
-                             : &select_experts_kernel<decltype(t)::value, decltype(lanes)::value, decltype(per)::value, false>;
+    constexpr int TYPE = decltype(t)::value, LANES = decltype(lanes)::value, PER = decltype(per)::value;
+    const bool by_scores = c.bias == nullptr && (c.top_groups == c.groups || c.group_best == 1), whole = c.experts == LANES * PER;
+    auto* kernel = by_scores ? whole ? &select_experts_kernel<TYPE, LANES, PER, true, true> : &select_experts_kernel<TYPE, LANES, PER, true, false>
+                   : whole   ? &select_experts_kernel<TYPE, LANES, PER, false, true>
+                             : &select_experts_kernel<TYPE, LANES, PER, false, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
                        (int)tokens, c, weights, selected);
   });
@@ -556,8 +600,10 @@ int fp8gmm_select_experts_backward(const void* scores, int type, int64_t tokens,
   const Choice c = choice_of(*choice);
   with_shape(type, tokens, c, [&](auto t, auto lanes, auto per) {
     constexpr int TOKENS = kThreads / decltype(lanes)::value;
-    hipLaunchKernelGGL((select_experts_backward_kernel<decltype(t)::value, decltype(lanes)::value, decltype(per)::value>),
-                       dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
+    constexpr int TYPE = decltype(t)::value, LANES = decltype(lanes)::value, PER = decltype(per)::value;
+    auto* kernel = c.experts == LANES * PER ? &select_experts_backward_kernel<TYPE, LANES, PER, true>
+                                            : &select_experts_backward_kernel<TYPE, LANES, PER, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
                        (int)tokens, c, selected, grad_weights, grad_scores);
   });
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;

@@ -155,6 +155,20 @@ def test_masked_scores(dev):
             assert ((i < 8) | (i >= 48)).all() and torch.isfinite(ds).all() and not ds[:, 5:50].any()
 
 
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("experts, times", [(64, 1), (64, 20), (256, 1), (256, 20)])
+def test_every_score_of_16_bits(dev, t, experts, times):
+    """All bit patterns in any company: zeros are equal, NaN and minus infinity are equal and last."""
+    g = gen(7)
+    bits = torch.cat([torch.randperm(1 << 16, generator=g) for _ in range(times)])
+    bits[::97] = torch.tensor([0, 0x8000, 0x7f80, 0xff80, 0x7c00, 0xfc00, 0x7fff, 0xffff])[torch.randint(0, 8, bits[::97].shape, generator=g)]
+    scores = (bits - (bits >> 15 << 16)).to(torch.int16).view(t).view(-1, experts).to(dev)
+    _, selected = moe_ops.select_experts(scores, 8)
+    order = scores.double().nan_to_num(nan=-float("inf"), posinf=float("inf"), neginf=-float("inf"))
+    want = order.sort(dim=1, descending=True, stable=True).indices[:, :8]
+    assert torch.equal(selected, want)
+
+
 @pytest.mark.parametrize("tokens", [40, 5000, 20000])
 @pytest.mark.parametrize("t", [torch.bfloat16, torch.float32])
 def test_tokens_with_few_experts_left(dev, tokens, t):
