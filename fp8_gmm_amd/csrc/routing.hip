@@ -25,11 +25,11 @@ namespace {
 constexpr int kMaxChoices = FP8GMM_MAX_CHOICES;
 constexpr int kThreads = 256;
 
-// exp(x), 2^-46 relative: 2^n times the series of exp to its eleventh power, on a remainder of at most ln(2) / 2, whose next term is
-// below 2^-47.  Cut to e^-700 and e^700; a NaN comes out as one of these.
+// exp(x) of -700 <= x <= 700, 2^-46 relative: 2^n times the series of exp to its eleventh power, on a remainder of at most ln(2) / 2, whose
+// next term is below 2^-47.  n is what a large number's last bits hold, and goes into the exponent as it is.
 __device__ __forceinline__ double exp64(double x) {
-  x = fmin(fmax(x, -700.), 700.);
-  const double n = rint(x * 1.4426950408889634);
+  constexpr double kWhole = 0x1.8p52;
+  const double large = __builtin_fma(x, 1.4426950408889634, kWhole), n = large - kWhole;
   double f = __builtin_fma(n, -0.6931471805599453, x);
   f = __builtin_fma(n, -2.3190468138462996e-17, f);
   double p = 1. / 39916800.;
@@ -44,12 +44,11 @@ __device__ __forceinline__ double exp64(double x) {
   p = __builtin_fma(p, f, .5);
   p = __builtin_fma(p, f, 1.);
   p = __builtin_fma(p, f, 1.);
-  return __builtin_ldexp(p, (int)n);
+  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + (__builtin_bit_cast(uint64_t, large) << 52));
 }
-// 1 / d for 1 <= d <= e^701: the hardware's first guess and two of Newton's steps
+// 1 / d for 1 <= d <= e^701: the hardware's first guess, 2^-23, and one of Newton's steps
 __device__ __forceinline__ double rcp64(double d) {
-  double r = __builtin_amdgcn_rcp(d);
-  r = __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
+  const double r = __builtin_amdgcn_rcp(d);
   return __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
 }
 // exp(x) of x <= 0, 2 units in the last place: the hardware's power of 2 of the rounded product, and what the rounding left of it to the
@@ -77,12 +76,15 @@ __device__ __forceinline__ key64 smaller(key64 a, key64 b) {
   asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
   return r;
 }
-// `number` < 4096
-__device__ __forceinline__ key64 key_of(double v, int number) {
-  v = fmin(fmax(v, -kFar), kFar) + 0.;   // (one zero, not two)
+// `number` < 4096; of a number between -kFar and kFar, not the zero below zero
+__device__ __forceinline__ key64 key_of_plain(double v, int number) {
   const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-  return __builtin_bit_cast(double, (bits & ~0xfffull) | (uint64_t)((int64_t)bits < 0 ? number : 4095 - number));
+  int32_t below = (int32_t)(bits >> 32) >> 31;
+  asm("" : "+v"(below));   // (a comparison in 64 bits and a selection otherwise)
+  return __builtin_bit_cast(double, (bits & ~0xfffull) | (((uint32_t)below & 0xfffu) ^ (uint32_t)(4095 - number)));
 }
+__device__ __forceinline__ double within(double v) { return fmin(fmax(v, -kFar), kFar) + 0.; }   // (one zero, not two)
+__device__ __forceinline__ key64 key_of(double v, int number) { return key_of_plain(within(v), number); }
 __device__ __forceinline__ int number_of(key64 key) {
   const uint64_t bits = __builtin_bit_cast(uint64_t, key);
   const int low = (int)(bits & 0xfff);
@@ -410,26 +412,46 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
     if (grouped) keep_groups<LANES, PER, 1>(key, c, lane);
     chosen = take_largest<LANES>(key, c.top_k, lane);
   } else {
-    double p[PER], sum = 0.;
+    double p[PER];
+    float odd = 0.f;   // a NaN where one of a lane's scores or biases is (or is infinite, which takes the longer way as well)
+    if (c.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const double e = exp64(c.sigmoid ? -(double)s[j] : (double)s[j] - (double)most);
-      p[j] = c.sigmoid ? rcp64(1. + e) : e;
-      if (s[j] != s[j]) p[j] = (double)s[j];
-      sum += j < left ? p[j] : 0.;
-    }
-    double inv = 1.;
-    if (!c.sigmoid) {
+      for (int j = 0; j < PER; ++j) {
+        p[j] = rcp64(1. + exp64((double)__builtin_amdgcn_fmed3f(-s[j], -700.f, 700.f)));
+        odd = __builtin_fmaf(s[j], 0.f, odd);
+      }
+    } else {
+      double sum = 0.;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        p[j] = exp64(fmax((double)s[j] - (double)most, -700.));   // (a NaN comes out as one of these numbers)
+        sum += j < left ? p[j] : 0.;
+        odd = __builtin_elementwise_maximum(odd, s[j]);
+      }
+      if (odd != odd) sum = (double)odd;
       sum = over<LANES>(sum, Sum{});
+      odd = (float)sum;
       total = (float)sum;
-      inv = 1. / sum;
+      const double inv = 1. / sum;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) p[j] *= inv;
+    }
+    if (c.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const float b = j < left ? c.bias[e0 + j] : 0.f;
+        p[j] += (double)b;
+        odd = __builtin_fmaf(b, 0.f, odd);
+      }
+    }
+    if (__builtin_expect(odd != odd, 0)) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) p[j] = within(s[j] != s[j] ? -kFar : p[j]);
     }
     key64 key[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      p[j] *= inv;
-      if (c.bias != nullptr && j < left) p[j] += (double)c.bias[e0 + j];
-      key[j] = key_of(p[j], e0 + j);
+      key[j] = key_of_plain(p[j], e0 + j);
       strike(key[j], j >= left);
     }
     if (grouped) c.group_best == 2 ? keep_groups<LANES, PER, 2>(key, c, lane) : keep_groups<LANES, PER, 1>(key, c, lane);
