@@ -341,11 +341,54 @@ __device__ __forceinline__ void keep_groups(K (&key)[PER], const Choice& c, int 
   }
 }
 
+template <int PER>
+__device__ __forceinline__ void in_order(key64 (&key)[PER], int i, int j) {
+  const key64 a = key[i], b = key[j];
+  key[i] = larger(a, b);
+  key[j] = smaller(a, b);
+}
+// Sorts keys at .. at + 7, the largest first, by merges of sorted pairs and fours
+template <int PER>
+__device__ __forceinline__ void sort8(key64 (&key)[PER], int at) {
+  constexpr int kSteps[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6},
+                                 {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+#pragma unroll
+  for (int i = 0; i < 19; ++i) in_order(key, at + kSteps[i][0], at + kSteps[i][1]);
+}
+
 // The top_k largest keys' numbers, number k in lane k.  Keys of 31 bits stay as they are: less the last one taken, modulo 2^32, those
 // below it are the largest, in their order.
 template <int LANES, int PER, class K>
 __device__ __forceinline__ int take_largest(K (&key)[PER], int top_k, int lane) {
   K mine = key[0], last = K();
+  if constexpr (std::is_same_v<K, key64> && PER >= 16) {
+    // A lane's 8 largest in their order: a round looks at the first ones, and the lane that has the largest moves up (us of 16384 tokens of 256
+    // experts, 8 choices, 10.0, by a look at all keys in every round 10.8; 4 choices 8.6 and 8.8, but 2 choices 8.0 and 7.8; 2000 tokens of 4096
+    // experts 20.9 and 28.6).
+    if (top_k > 2 && top_k <= 8) {
+      sort8(key, 0);
+#pragma unroll
+      for (int at = 8; at < PER; at += 8) {   // the larger of opposite ones are the 8 largest, and fall and rise
+        sort8(key, at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) key[i] = larger(key[i], key[at + 7 - i]);
+#pragma unroll
+        for (int step = 4; step > 0; step /= 2)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if ((i & step) == 0) in_order(key, i, i + step);
+      }
+      for (int k = 0; k < top_k; ++k) {
+        const K best = over<LANES>(key[0], LargerKey{});
+        const bool it = key[0] == best;
+#pragma unroll
+        for (int j = 0; j < 7; ++j) key[j] = it ? key[j + 1] : key[j];
+        strike(key[7], it);
+        if (k == lane) mine = best;
+      }
+      return number_of(mine);
+    }
+  }
   if constexpr (std::is_same_v<K, key32>) last = 1u << 31;
   for (int k = 0; k < top_k; ++k) {
     K best;
@@ -538,10 +581,10 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
 }
 
 // calls f(TYPE, LANES, PER).  Few tokens have a wavefront each, whose lanes hold few experts (us, forward by p in 64 bits / backward:
-// 1 token, 256 experts in 8 groups, 4.6 / 2.8, by 16 lanes 7.6 / 3.0; 2048 tokens 5.8 / 3.2 and 8.0 / 3.4; 4096 8.2 / 3.8 and 8.0 / 3.6; 1024
-// tokens of 512 experts 6.2 / 3.3 and 12.5 / 4.3).  Many tokens of few experts have 8 lanes each, as long as every choice and group has a
-// lane of its own (131072 tokens, 64 experts, 6 choices by their scores, 13.2 / 13.4, by 16 lanes 15.4 / 16.5; 8 experts 5.7 / 6.3 and 7.7
-// / 9.3; 16384 tokens, 64 experts, 3.6 / 3.8 and 3.9 / 4.1, 4096 tokens 3.0 / 3.4 and 2.8 / 3.2).
+// 1 token, 256 experts in 8 groups, 4.2 / 2.5, by 16 lanes 4.5 / 2.9; 1024 tokens 4.7 / 2.8 and 5.2 / 3.4; 2048 5.4 / 3.0 and 4.9 / 3.5; 4096
+// 7.6 / 3.6 and 5.1 / 3.7; 2048 tokens of 512 experts 6.3 / 3.3 and 7.5 / 4.9).  Many tokens of few experts have 8 lanes each, as long as
+// every choice and group has a lane of its own (131072 tokens, 64 experts, 6 choices by their scores, 11.3 / 12.3, by 16 lanes 13.2 / 15.0;
+// 8 experts 5.1 / 6.1 and 7.4 / 8.9; 16384 tokens, 64 experts, 3.1 / 3.5 and 3.4 / 3.7, 4096 tokens 2.7 / 3.1 and 2.6 / 2.8).
 constexpr int kFewTokens = 2048, kManyTokens = 8192;
 template <class F>
 void with_shape(int type, int64_t tokens, const Choice& c, F&& f) {
