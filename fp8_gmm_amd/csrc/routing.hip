@@ -12,7 +12,7 @@
 // the fraction are replaced (what agrees in its first 40 bits counts as equal).  The weights are fp32.
 //
 // LANES lanes have a token, 8 or 16 (of a row of the data-parallel primitives) or 64, with PER neighbouring experts in the registers of
-// each: a round takes the largest key of every lane's own, exchanges them in log2(LANES) steps, and strikes it out.  Bound by these
+// each: a round takes the largest key of every lane's own, exchanges them in log2(LANES) steps, and leaves it out of the next.  Bound by these
 // instructions, not by the scores' bytes.
 #include <algorithm>
 #include <type_traits>
