@@ -259,6 +259,20 @@ struct Choice {
   float scale;
 };
 
+// p[chosen] / sum of p[chosen], of the chosen score v of every lane that `has` one.  p itself may be too small for a number, of all of
+// them where a bias or the groups keep the largest scores out: these are shares by the largest of the chosen ones, m.  Softmax: e^(v - m).
+// Sigmoid: p, where m is above zero; below, with e^m left out of all, e^(v - m) / (1 + e^v).
+template <int LANES>
+__device__ __forceinline__ float share_of(const Choice& c, bool has, float v) {
+  const float m = over<LANES>(has ? v : -INFINITY, Largest{});
+  float part = 0.f;
+  if (has) {
+    part = exp_of(v - m);
+    if (c.sigmoid) part = m > 0.f ? sigmoid(v) : part / (1.f + expf(v));
+  }
+  return part / over<LANES>(part, Sum{});
+}
+
 // Which experts' groups stay: strikes the others' keys out.  A group's key is its largest expert's (BEST 1), or made of the sum of its
 // two largest and the group's number.
 template <int LANES, int PER, int BEST, class K>
@@ -474,7 +488,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
       if (odd != odd) sum = (double)odd;
       sum = over<LANES>(sum, Sum{});
       odd = (float)sum;
-      total = (float)sum;
+      total = (float)sum + (most - most);   // (no number where the largest score is none)
       const double inv = 1. / sum;
 #pragma unroll
       for (int j = 0; j < PER; ++j) p[j] *= inv;
@@ -501,20 +515,18 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
     chosen = take_largest<LANES>(key, c.top_k, lane);
   }
   const bool has = lane < c.top_k;
-  float w = 0.f;
-  if (has) {
-    const float v = score_of<TYPE>(scores, from, c.experts, chosen);
-    w = c.sigmoid ? sigmoid(v) : exp_of(v - most) / total;
-  }
-  if (c.renormalize) w /= over<LANES>(w, Sum{});
+  float w = has ? score_of<TYPE>(scores, from, c.experts, chosen) : 0.f;
+  if (c.renormalize) w = __builtin_fmaf(total, 0.f, share_of<LANES>(c, has, w));   // (a total that is no number leaves none)
+  else w = c.sigmoid ? sigmoid(w) : exp_of(w - most) / total;
   if (has && live) {
     weights[token * c.top_k + lane] = w * c.scale;
     selected[token * c.top_k + lane] = chosen;
   }
 }
 
-// Of the weights' gradients: with v = p[chosen] and renormalized weights dv = (dw - (sum of dw v) / (sum of v)) scale / (sum of v),
-// otherwise dv = scale dw; through the sigmoid ds = dv p (1 - p), through the softmax ds = p (dv - sum of dv v).
+// Of the weights' gradients, with v = p[chosen] and dv = scale dw: through the sigmoid ds = dv v (1 - v) of the chosen scores, through the
+// softmax ds = p (dv - sum of dv v) of all.  Of renormalized weights, u = v / sum of v: ds = u (dv - sum of dv u) of the chosen scores, by the
+// sigmoid times 1 - v.
 template <int TYPE, int LANES, int PER, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const void* __restrict__ scores, int tokens, const Choice c,
                                                                            const int64_t* __restrict__ selected,
@@ -542,27 +554,26 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
     }
     total = over<LANES>(sum, Sum{});
   }
-  const bool has = lane < c.top_k;
   int chosen = -1;
-  float g = 0.f, p = 0.f, rest = 0.f;
-  if (has) {
+  float g = 0.f, v = 0.f, back = 0.f;
+  if (lane < c.top_k) {
     const int64_t e = selected[from * c.top_k + lane];
-    g = grad_weights[from * c.top_k + lane] * c.scale;
     if ((uint64_t)e < (uint64_t)c.experts) {   // not an expert: no gradient
       chosen = (int)e;
-      const float v = score_of<TYPE>(scores, from, c.experts, chosen);
-      p = c.sigmoid ? sigmoid(v) : exp_of(v - most) / total;
-      rest = c.sigmoid ? 1.f / (1.f + expf(v)) : 0.f;
-    } else {
-      g = 0.f;
+      g = grad_weights[from * c.top_k + lane] * c.scale;
+      v = score_of<TYPE>(scores, from, c.experts, chosen);
     }
   }
+  const bool has = chosen >= 0;
   if (c.renormalize) {
-    const float sum = over<LANES>(p, Sum{}), dot = over<LANES>(g * p, Sum{});
-    g = has ? (g - dot / sum) / sum : 0.f;
+    const float share = share_of<LANES>(c, has, v);
+    g = share * (g - over<LANES>(g * share, Sum{}));
+  } else if (c.sigmoid) {
+    g *= sigmoid(v);
+  } else {
+    back = over<LANES>(has ? g * (exp_of(v - most) / total) : 0.f, Sum{});
   }
-  const float back = c.sigmoid ? 0.f : over<LANES>(g * p, Sum{});
-  if (c.sigmoid) g *= p * rest;
+  if (c.sigmoid) g *= 1.f / (1.f + expf(v));
   float out[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) out[j] = 0.f;
@@ -575,7 +586,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
   const float inv = 1.f / total;
   if (!c.sigmoid)
 #pragma unroll
-    for (int j = 0; j < PER; ++j) out[j] = s[j] * inv * (out[j] - back);
+    for (int j = 0; j < PER; ++j) out[j] = c.renormalize ? __builtin_fmaf(total, 0.f, out[j]) : s[j] * inv * (out[j] - back);
   if (!live) return;
   Piece<TYPE, PER>::store(grad_scores, token * c.experts + e0, left, out);
 }

@@ -1,0 +1,84 @@
+"""The choice of experts where scores, biases or groups leave few experts or small probabilities, on the GPU."""
+import pytest
+import torch
+
+from fp8_gmm_amd import moe_ops
+
+from helpers import gen
+from test_gpu_routing import TYPES, U, reference, scores_of
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+def check_shares(scores, top_k, scoring, bias, groups=1, top_groups=1, scale=1.0):
+    """Renormalized weights and their gradient, against shares that are formed from logarithms in 64 bits: the probabilities themselves
+    are too small for those as well.  Tolerances are those of test_gpu_routing.check: k of the weights and 4 k of what a gradient is the
+    difference of."""
+    s = scores.clone().requires_grad_()
+    w, chosen = moe_ops.select_experts(s, top_k, scoring, bias, groups, top_groups, True, scale)
+    _, want = reference(scores, top_k, scoring, bias, groups, top_groups, False, scale, 2)
+    assert torch.equal(chosen.cpu(), want)
+    x = scores.double().cpu().gather(1, want)
+    share = torch.softmax(torch.nn.functional.logsigmoid(x) if scoring == "sigmoid" else x, 1)
+    k = 2 * (80 + 2 * scores.float().abs().max().item()) * U + 20 * U
+    off = (w.detach().double().cpu() - share * scale).abs()
+    assert (off <= k * share * scale + 1e-38).all(), (off / share).max().item() / k
+    dw = torch.randn(w.shape, generator=gen(5)).to(scores.device)
+    ds, = torch.autograd.grad(w, s, dw)
+    rest = torch.sigmoid(-x) if scoring == "sigmoid" else torch.ones_like(x)
+    g = dw.double().cpu() * scale
+    zeros = torch.zeros(scores.shape, dtype=torch.float64)
+    wanted = zeros.scatter(1, want, rest * share * (g - (g * share).sum(1, keepdim=True)))
+    bound = zeros.scatter(1, want, rest * share * (g.abs() + (g * share).abs().sum(1, keepdim=True)))
+    h, tiny = torch.finfo(scores.dtype).eps / 2, torch.finfo(scores.dtype).smallest_normal
+    off = (ds.double().cpu() - wanted).abs()
+    assert (off <= 4 * k * bound + h * (wanted.abs() + 4 * k * bound) + tiny).all()
+    return w.detach(), chosen, ds
+
+
+@pytest.mark.parametrize("tokens, experts", [(9, 16), (40, 64), (20000, 64), (40, 256), (5000, 256), (300, 600), (30, 1500)])
+@pytest.mark.parametrize("t", ["bf16", "fp32"])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_renormalized_weights_of_small_probabilities(dev, tokens, experts, t, scoring):
+    """The chosen weights are shares of one another, however small their probabilities: 100 and 600 below the row's largest score,
+    which a bias of minus infinity or the choice of groups removes, or far below zero."""
+    for far in (100.0, 600.0):
+        scores = scores_of(dev, tokens, experts, "fp32", experts)
+        scores[:, 5:] -= far
+        scores[1::2] -= far if scoring == "sigmoid" else 0.0
+        scores = scores.to(TYPES[t])
+        bias = torch.zeros(experts, device=dev)
+        bias[:5] = -INF
+        w, chosen, ds = check_shares(scores, 8, scoring, bias, scale=2.5)
+        assert (chosen >= 5).all() and torch.isfinite(w).all() and torch.isfinite(ds).all() and ds[:, 5:].any()
+    scores = scores_of(dev, tokens, experts, "fp32", experts) - 100.0   # by sigmoid all far below zero
+    check_shares(scores.to(TYPES[t]), 6, scoring, None, 2, 1)
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float32])
+def test_renormalized_weights_behind_a_bias(dev, t):
+    """The row's largest score goes by a bias against it, and groups stay by the others, whose probabilities are all but nothing."""
+    scores = scores_of(dev, 50, 64, "fp32", 4).to(t)
+    scores[:, 3] = 120.0
+    bias = torch.zeros(64, device=dev)
+    bias[3] = -2.0
+    w, chosen, ds = check_shares(scores, 4, "softmax", bias, 8, 2)
+    assert (chosen != 3).all() and torch.isfinite(w).all() and torch.isfinite(ds).all()
+    total = w.double().sum(1)
+    assert ((total - 1).abs() <= 8 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_renormalized_weights_of_what_is_no_number(dev, scoring):
+    """A NaN makes all of its token's softmax one, of a sigmoid only what is chosen; chosen weights that are all zeros are no numbers."""
+    scores = scores_of(dev, 4, 32, "fp32", 3)
+    scores[0, 3] = float("nan")
+    scores[1, 3] = INF
+    scores[2] = -INF
+    for bias in (None, torch.zeros(32, device=dev)):
+        w, chosen = moe_ops.select_experts(scores, 8, scoring, bias, renormalize=True)
+        assert (w[:2].isnan().all() if scoring == "softmax" else torch.isfinite(w[:2]).all())
+        assert w[2].isnan().all() and torch.isfinite(w[3]).all()
+        assert ((chosen >= 0) & (chosen < 32)).all()
