@@ -9,7 +9,8 @@
 // What is compared decides where a token goes, so it is compared exactly: the scores themselves where p alone would decide (it grows
 // with them), else c and the groups' sums in 64 bits.  A key is such a number that holds the expert's number in its last bits, so no two
 // keys are equal and the largest names its expert: 16 bits of a score and 15 of the number, or a number in 64 bits whose last 12 bits of
-// the fraction are replaced (what agrees in its first 40 bits counts as equal).  The weights are fp32.
+// the fraction are replaced (what agrees in its first 40 bits counts as equal).  An expert whose score or bias is minus infinity is switched
+// off: it goes last, whatever the other one is.  The weights are fp32.
 //
 // LANES lanes have a token, 8 or 16 (of a row of the data-parallel primitives) or 64, with PER neighbouring experts in the registers of
 // each: a round takes the largest key of every lane's own, exchanges them in log2(LANES) steps, and leaves it out of the next.  Bound by these
@@ -65,6 +66,7 @@ __device__ __forceinline__ float sigmoid(float s) { return 1.f / (1.f + expf(-s)
 // Keys of 64 bits.  What is no number goes last, with minus infinity.
 typedef double key64;
 constexpr double kStruck64 = -1.7e308, kFar = 1e300;   // what is struck out, and what numbers and sums are cut to
+constexpr double kOff = -1e299;   // below it, experts that are switched off and groups of none but such
 // (an instruction: fmax would look for NaN in both, which keys are not)
 __device__ __forceinline__ key64 larger(key64 a, key64 b) {
   key64 r;
@@ -274,7 +276,7 @@ __device__ __forceinline__ float share_of(const Choice& c, bool has, float v) {
 }
 
 // Which experts' groups stay: strikes the others' keys out.  A group's key is its largest expert's (BEST 1), or made of the sum of its
-// two largest and the group's number.
+// two largest, of which one that is switched off adds nothing, and the group's number.
 template <int LANES, int PER, int BEST, class K>
 __device__ __forceinline__ void keep_groups(K (&key)[PER], const Choice& c, int lane) {
   const int size = c.experts / c.groups;
@@ -287,7 +289,7 @@ __device__ __forceinline__ void keep_groups(K (&key)[PER], const Choice& c, int 
     if constexpr (BEST == 2) second = larger(second, b);
   };
   const auto made = [&](K first, K second, int g) {
-    if constexpr (BEST == 2) return key_of(size > 1 ? first + second : first, g);
+    if constexpr (BEST == 2) return key_of(second > kOff ? first + second : first, g);
     else return first;
   };
   K none = key[0];
@@ -470,7 +472,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
     chosen = take_largest<LANES>(key, c.top_k, lane);
   } else {
     double p[PER];
-    float odd = 0.f;   // a NaN where one of a lane's scores or biases is (or is infinite, which takes the longer way as well)
+    float odd = 0.f;   // a NaN where one of a lane's scores or biases is one or infinite
     if (c.sigmoid) {
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
@@ -479,15 +481,17 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
       }
     } else {
       double sum = 0.;
+      float none = 0.f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         p[j] = exp64(fmax((double)s[j] - (double)most, -700.));   // (a NaN comes out as one of these numbers)
         sum += j < left ? p[j] : 0.;
-        odd = __builtin_elementwise_maximum(odd, s[j]);
+        odd = __builtin_fmaf(j < left ? s[j] : 0.f, 0.f, odd);
+        none = __builtin_elementwise_maximum(none, s[j]);
       }
-      if (odd != odd) sum = (double)odd;
+      if (none != none) sum = (double)none;
       sum = over<LANES>(sum, Sum{});
-      odd = (float)sum;
+      if (sum != sum) odd = (float)sum;
       total = (float)sum + (most - most);   // (no number where the largest score is none)
       const double inv = 1. / sum;
 #pragma unroll
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
     }
     if (__builtin_expect(odd != odd, 0)) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) p[j] = within(s[j] != s[j] ? -kFar : p[j]);
+      for (int j = 0; j < PER; ++j) p[j] = within(s[j] > -INFINITY ? p[j] : -kFar);   // switched off, or no number
     }
     key64 key[PER];
 #pragma unroll

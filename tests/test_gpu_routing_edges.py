@@ -82,3 +82,65 @@ def test_renormalized_weights_of_what_is_no_number(dev, scoring):
         assert (w[:2].isnan().all() if scoring == "softmax" else torch.isfinite(w[:2]).all())
         assert w[2].isnan().all() and torch.isfinite(w[3]).all()
         assert ((chosen >= 0) & (chosen < 32)).all()
+
+
+def chosen_of(scores, top_k, scoring, bias, groups, top_groups, best):
+    """The choice in 64 bits, on the CPU.  Off is an expert whose score is a NaN or minus infinity, or whose bias is one: it goes last
+    and adds nothing to its group."""
+    s = scores.double().cpu()
+    tokens, experts = s.shape
+    far = s.masked_fill(s.isnan(), -INF)
+    p = torch.sigmoid(s) if scoring == "sigmoid" else torch.softmax(far, 1).nan_to_num(0.0).masked_fill(far == INF, INF)
+    c = p if bias is None else p + bias.double().cpu()
+    off = (far == -INF) | c.isnan() | (c == -INF)
+    c = c.masked_fill(off, -INF)
+    order = c.sort(dim=1, descending=True, stable=True).indices
+    if groups > 1:
+        two = c.view(tokens, groups, -1).sort(dim=2, descending=True).values[:, :, :best]
+        value = two.masked_fill(two == -INF, 0.0).sum(2).masked_fill((two == -INF).all(2), -INF)
+        kept = value.sort(dim=1, descending=True, stable=True).indices[:, :top_groups]
+        stays = torch.zeros(tokens, groups, dtype=torch.long).scatter_(1, kept, 1).repeat_interleave(experts // groups, 1)
+        order = order.gather(1, stays.gather(1, order).sort(dim=1, descending=True, stable=True).indices)
+    return order[:, :top_k]
+
+
+LAYOUTS = [(40, 16, 1, 1), (40, 64, 8, 3), (20000, 64, 8, 3), (20000, 30, 5, 2), (40, 256, 8, 4), (5000, 256, 8, 4), (5000, 240, 6, 3),
+           (300, 600, 4, 2), (30, 1500, 3, 2)]
+
+
+@pytest.mark.parametrize("tokens, experts, groups, top_groups", LAYOUTS)
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_experts_that_are_switched_off_stay_off(dev, tokens, experts, groups, top_groups, t, scoring):
+    """By a score of minus infinity whatever their bias is, which balancing raises for an expert without load."""
+    scores = scores_of(dev, tokens, experts, "fp32", experts).to(t)
+    off = torch.rand(tokens, experts, generator=gen(1)) < torch.tensor([0.0, 0.3, 0.8, 0.97])[torch.arange(tokens) % 4, None]
+    scores[off.to(dev)] = -INF
+    bias = (torch.randn(experts, generator=gen(2)) * 0.1).to(dev)
+    bias[::3] += 0.9
+    for best in (1, 2):
+        for kind in ((1, 1), (groups, top_groups)):
+            _, got = moe_ops.select_experts(scores, 6, scoring, bias, *kind, group_best=best)
+            assert torch.equal(got.cpu(), chosen_of(scores, 6, scoring, bias, *kind, best)), (best, kind)
+    bias[1::5] = -INF   # and by a bias of minus infinity
+    for best in (1, 2):
+        for kind in ((1, 1), (groups, top_groups)):
+            _, got = moe_ops.select_experts(scores, 6, scoring, bias, *kind, group_best=best)
+            assert torch.equal(got.cpu(), chosen_of(scores, 6, scoring, bias, *kind, best)), (best, kind)
+
+
+def test_a_group_of_one_that_is_left_stays(dev):
+    """A group with one expert that is not off is ahead of a group without any, and counts that one."""
+    for scoring in ("softmax", "sigmoid"):
+        for by_bias in (True, False):
+            scores = torch.zeros(3, 32, device=dev)
+            scores[:, 21] = 1.0
+            bias = torch.zeros(32, device=dev)
+            if by_bias:
+                bias[:21] = -INF
+                bias[22:] = -INF
+            else:
+                scores[:, :21] = -INF
+                scores[:, 22:] = -INF
+            w, chosen = moe_ops.select_experts(scores, 2, scoring, bias, 4, 1)
+            assert chosen.tolist() == [[21, 16]] * 3 and (w[:, 0] > 0).all()
