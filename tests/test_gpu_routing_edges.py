@@ -144,3 +144,28 @@ def test_a_group_of_one_that_is_left_stays(dev):
                 scores[:, 22:] = -INF
             w, chosen = moe_ops.select_experts(scores, 2, scoring, bias, 4, 1)
             assert chosen.tolist() == [[21, 16]] * 3 and (w[:, 0] > 0).all()
+
+
+@pytest.mark.parametrize("tokens, experts, groups", [(2000, 8, 4), (2000, 32, 16), (20000, 32, 8), (2000, 64, 8), (20000, 64, 8), (1500, 256, 8),
+                                                     (5000, 256, 8), (5000, 240, 6), (1000, 1024, 16), (500, 3000, 12)])
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float32])
+def test_groups_of_equal_sums_stay_in_their_order(dev, tokens, experts, groups, t):
+    """The sigmoids of x and -x add up to 1, whatever x is, and with a bias of -1/4 each to 1/2: the first groups stay.  2^-30 more of one
+    of them decides."""
+    size = experts // groups
+    x = (torch.rand(tokens, groups, generator=gen(experts)) * 8).to(t).float()
+    scores = torch.full((tokens, groups, size), -30.0)
+    scores[:, :, 0], scores[:, :, size - 1] = x, -x
+    turned = torch.rand(tokens, groups, generator=gen(1)) < 0.5
+    scores[turned] = scores[turned].flip(1)
+    scores = scores.view(tokens, experts).to(t).to(dev)
+    zeros, less = torch.zeros(experts, device=dev), torch.full((experts,), -0.25, device=dev)
+    for bias in (None, zeros, less):
+        for kept in (1, 2, min(groups - 1, 8)):
+            _, chosen = moe_ops.select_experts(scores, 2 * kept, "sigmoid", bias, groups, kept)
+            stays = torch.zeros(tokens, groups, dtype=torch.bool, device=dev).scatter_(1, chosen // size, True)
+            assert stays[:, :kept].all() and not stays[:, kept:].any(), (kept, int(stays[:, kept:].any(1).sum()))
+    last = zeros.clone()
+    last[-size] = last[-1] = 2.0 ** -30
+    _, chosen = moe_ops.select_experts(scores, 2, "sigmoid", last, groups, 1)
+    assert (chosen // size == groups - 1).all()
