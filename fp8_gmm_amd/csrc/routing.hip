@@ -65,8 +65,8 @@ __device__ __forceinline__ float sigmoid(float s) { return 1.f / (1.f + expf(-s)
 
 // Keys of 64 bits.  What is no number goes last, with minus infinity.
 typedef double key64;
-constexpr double kStruck64 = -1.7e308, kFar = 1e300;   // what is struck out, and what numbers and sums are cut to
-constexpr double kOff = -1e299;   // below it, experts that are switched off and groups of none but such
+constexpr double kStruck64 = -1.7e308, kFar = 0x1p996;   // what is struck out, and what numbers and sums are cut to
+constexpr double kOff = -0x1p995;   // below it, experts that are switched off and groups of none but such
 // (an instruction: fmax would look for NaN in both, which keys are not)
 __device__ __forceinline__ key64 larger(key64 a, key64 b) {
   key64 r;
@@ -490,19 +490,21 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
       }
     } else {
       double sum = 0.;
-      float none = 0.f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         p[j] = exp64(fmax((double)s[j] - (double)most, -700.));   // (a NaN comes out as one of these numbers)
         sum += j < left ? p[j] : 0.;
         odd = __builtin_fmaf(j < left ? s[j] : 0.f, 0.f, odd);
-        none = __builtin_elementwise_maximum(none, s[j]);
       }
-      if (none != none) sum = (double)none;
+      const double numbers = sum;
+      if (__builtin_expect(odd != odd, 0)) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sum = s[j] != s[j] ? (double)s[j] : sum;
+      }
       sum = over<LANES>(sum, Sum{});
-      if (sum != sum) odd = (float)sum;
       total = (float)sum + (most - most);   // (no number where the largest score is none)
-      const double inv = 1. / sum;
+      if (__builtin_expect(sum != sum, 0)) sum = over<LANES>(numbers, Sum{});   // a NaN leaves the others' order as it is
+      const double inv = most < INFINITY ? 1. / sum : 0.;
 #pragma unroll
       for (int j = 0; j < PER; ++j) p[j] *= inv;
     }
@@ -516,7 +518,10 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
     }
     if (__builtin_expect(odd != odd, 0)) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) p[j] = within(s[j] > -INFINITY ? p[j] : -kFar);   // switched off, or no number
+      for (int j = 0; j < PER; ++j) {
+        const double first = !c.sigmoid && s[j] == INFINITY && p[j] > -kFar ? kFar : p[j];
+        p[j] = within(s[j] > -INFINITY ? first : -kFar);   // switched off, or no number
+      }
     }
     key64 key[PER];
 #pragma unroll

@@ -288,10 +288,11 @@ def select_experts(scores, top_k, scoring="softmax", bias=None, groups=1, top_gr
     weights are ``scale * p`` of these - the bias decides and weighs nothing - or, with ``renormalize``, ``scale * p / sum of the chosen
     p``.  The choice is made by the scores where ``p`` alone decides, and else in 64 bits, with ``p`` to 2^-46: what agrees in its first
     40 bits counts as equal, sums of groups what agrees to 2^-36 of the larger part, and the lower number goes first.  A score that is a
-    NaN goes last (but makes all of its token's softmax one).  A score of minus infinity switches an expert off, whatever its bias is, and
-    so does a bias of minus infinity: it goes last and adds nothing to its group, and a group of none but such goes last.  Where fewer
-    than ``top_k`` are left the lowest of the others are chosen, by scores of minus infinity with weights of zeros, but of a token without
-    any finite score the softmax, and renormalized weights that are all zeros, are no numbers, as in torch.
+    NaN goes last and leaves the others' order as it is (but makes all of its token's softmax one, as plus infinity does, which goes
+    first).  A score of minus infinity switches an expert off, whatever its bias is, and so does a bias of minus infinity: it goes last
+    and adds nothing to its group, and a group of none but such goes last.  Where fewer than ``top_k`` are left the lowest of the others
+    are chosen, by scores of minus infinity with weights of zeros, but of a token without any finite score the softmax, and renormalized
+    weights that are all zeros, are no numbers, as in torch.
 
     Scores: bfloat16, float16 or float32, up to 4096 experts in up to 16 groups, ``top_k`` up to 16.  Differentiable in the scores, by
     the weights; the bias takes no gradient.  ``moe_ops.Routing`` has a routed layer choose so."""

@@ -91,7 +91,7 @@ def chosen_of(scores, top_k, scoring, bias, groups, top_groups, best):
     tokens, experts = s.shape
     far = s.masked_fill(s.isnan(), -INF)
     p = torch.sigmoid(s) if scoring == "sigmoid" else torch.softmax(far, 1).nan_to_num(0.0).masked_fill(far == INF, INF)
-    c = p if bias is None else p + bias.double().cpu()
+    c = far if bias is None and (groups == 1 or best == 1) else p if bias is None else p + bias.double().cpu()
     off = (far == -INF) | c.isnan() | (c == -INF)
     c = c.masked_fill(off, -INF)
     order = c.sort(dim=1, descending=True, stable=True).indices
@@ -169,3 +169,25 @@ def test_groups_of_equal_sums_stay_in_their_order(dev, tokens, experts, groups, 
     last[-size] = last[-1] = 2.0 ** -30
     _, chosen = moe_ops.select_experts(scores, 2, "sigmoid", last, groups, 1)
     assert (chosen // size == groups - 1).all()
+
+
+@pytest.mark.parametrize("tokens, experts, groups, top_groups", LAYOUTS)
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_scores_that_are_no_numbers_go_last(dev, tokens, experts, groups, top_groups, t, scoring):
+    """And leave the others' order as it is, by the scores alone as with a bias; beside plus infinity, which goes first, all other
+    probabilities are zero."""
+    scores = scores_of(dev, tokens, experts, "fp32", experts).to(t)
+    r = torch.rand(tokens, experts, generator=gen(1)).to(dev)
+    share = torch.tensor([0.0, 1 / experts, 0.5, 1.0], device=dev)[torch.arange(tokens, device=dev) % 4, None]
+    scores[r < share] = float("nan")
+    scores[(r > 1 - 1 / experts) & (torch.arange(tokens, device=dev) % 3 == 0)[:, None]] = INF
+    zeros = torch.zeros(experts, device=dev)
+    bias = (torch.randn(experts, generator=gen(2)) * 0.1).to(dev)
+    for best in (1, 2):
+        for kind in ((1, 1), (groups, top_groups)):
+            for b in (None, zeros, bias):
+                w, got = moe_ops.select_experts(scores, 6, scoring, b, *kind, group_best=best)
+                assert torch.equal(got.cpu(), chosen_of(scores, 6, scoring, b, *kind, best)), (best, kind)
+                if scoring == "softmax":
+                    assert torch.equal(w.isnan().any(1), ~torch.isfinite(scores).all(1))
