@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kMaxChoices = FP8GMM_MAX_CHOICES;
 constexpr int kThreads = 256;
+constexpr int64_t kSlab = 1 << 23;   // workgroups of a launch: a grid has fewer than 2^32 threads
 
 // exp(x) of -700 <= x <= 700, 2^-46 relative: 2^n times the series of exp to its eleventh power, on a remainder of at most ln(2) / 2, whose
 // next term is below 2^-47.  n is what a large number's last bits hold, and goes into the exponent as it is.
@@ -644,6 +645,15 @@ void with_shape(int type, int64_t tokens, const Choice& c, F&& f) {
   else shape(std::integral_constant<int, FP8GMM_TYPE_FP32>{});
 }
 
+// calls f(first token, tokens, workgroups) for each launch
+template <class F>
+void each_slab(int64_t tokens, int per_group, F&& f) {
+  for (int64_t first = 0; first < tokens; first += kSlab * per_group) {
+    const int64_t some = std::min(tokens - first, kSlab * per_group);
+    f(first, (int)some, (int)((some + per_group - 1) / per_group));
+  }
+}
+
 int check_choice(int type, int64_t tokens, const fp8gmm_choice* c) {
   if (c == nullptr) return FP8GMM_ERR_NULL_POINTER;
   if (!known_type(type)) return FP8GMM_ERR_BAD_FORMAT;
@@ -678,8 +688,11 @@ int fp8gmm_select_experts(const void* scores, int type, int64_t tokens, const fp
     auto* kernel = by_scores ? whole ? &select_experts_kernel<TYPE, LANES, PER, true, true> : &select_experts_kernel<TYPE, LANES, PER, true, false>
                    : whole   ? &select_experts_kernel<TYPE, LANES, PER, false, true>
                              : &select_experts_kernel<TYPE, LANES, PER, false, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
-                       (int)tokens, c, weights, selected);
+    each_slab(tokens, TOKENS, [&](int64_t first, int some, int groups) {
+      hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
+                         static_cast<const char*>(scores) + first * c.experts * type_bytes(type), some, c, weights + first * c.top_k,
+                         selected + first * c.top_k);
+    });
   });
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }
@@ -697,8 +710,11 @@ int fp8gmm_select_experts_backward(const void* scores, int type, int64_t tokens,
     constexpr int TYPE = decltype(t)::value, LANES = decltype(lanes)::value, PER = decltype(per)::value;
     auto* kernel = c.experts == LANES * PER ? &select_experts_backward_kernel<TYPE, LANES, PER, true>
                                             : &select_experts_backward_kernel<TYPE, LANES, PER, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), scores,
-                       (int)tokens, c, selected, grad_weights, grad_scores);
+    each_slab(tokens, TOKENS, [&](int64_t first, int some, int groups) {
+      const int64_t at = first * c.experts * type_bytes(type);
+      hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const char*>(scores) + at,
+                         some, c, selected + first * c.top_k, grad_weights + first * c.top_k, static_cast<char*>(grad_scores) + at);
+    });
   });
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;
 }

@@ -191,3 +191,27 @@ def test_scores_that_are_no_numbers_go_last(dev, tokens, experts, groups, top_gr
                 assert torch.equal(got.cpu(), chosen_of(scores, 6, scoring, b, *kind, best)), (best, kind)
                 if scoring == "softmax":
                     assert torch.equal(w.isnan().any(1), ~torch.isfinite(scores).all(1))
+
+
+@pytest.mark.parametrize("tokens, experts, top_k", [((1 << 29) + 5, 2, 1), ((1 << 28) + 5, 9, 9)])
+def test_more_tokens_than_a_grid_has_threads_for(dev, tokens, experts, top_k):
+    """By 8 lanes to a token and by 16: the same rows again and again have the same results."""
+    block = 1 << 20
+    rows = torch.randn(block, experts, generator=gen(1)).to(torch.bfloat16).to(dev)
+    dw = torch.randn(block, top_k, generator=gen(2)).to(dev)
+    scores = torch.empty(tokens, experts, dtype=rows.dtype, device=dev)
+    grads = torch.empty(tokens, top_k, device=dev)
+    for at in range(0, tokens, block):
+        n = min(block, tokens - at)
+        scores[at: at + n], grads[at: at + n] = rows[:n], dw[:n]
+    part = rows.requires_grad_()
+    want = moe_ops.select_experts(part, top_k, "softmax", renormalize=top_k > 1)
+    scores.requires_grad_()
+    w, chosen = moe_ops.select_experts(scores, top_k, "softmax", renormalize=top_k > 1)
+    ds, = torch.autograd.grad(w, scores, grads)
+    wanted = (*(t.detach() for t in want), *torch.autograd.grad(want[0], part, dw))
+    del grads, scores
+    for at in range(0, tokens, block):
+        n = min(block, tokens - at)
+        for got, one in zip((w.detach(), chosen, ds), wanted):
+            assert torch.equal(got[at: at + n], one[:n]), at
