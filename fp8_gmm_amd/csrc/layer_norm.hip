@@ -562,8 +562,7 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
       }
     }
     if (params && (blocks != 1 || shape.lanes == 0))
-      hipLaunchKernelGGL((norm_params_kernel<P>), dim3(ceil_div(cols, 64), dbias != nullptr ? 2 : 1), dim3(1024), 0, s, part,
-                         blocks, 2, cols, dweight, dbias);
+      launch_norm_params<P>(part, blocks, 2, cols, dweight, dbias, s);
   });
   if (!known) return FP8GMM_ERR_LAUNCH;
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;

@@ -11,6 +11,7 @@ namespace {
 
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormSlab = 1 << 16;   // rows of a launch with a workgroup to a row, 2 GB at least: a grid has fewer than 2^32 threads
+constexpr int kNormColumns = 1 << 27;   // of a launch that adds up parameters' gradients, 16 threads to a column
 constexpr int kNormWaves = 16;       // the most wavefronts that share a row
 
 // The sum over the THREADS threads of a row, the same in all of them.  `slot`: THREADS / 64 floats of LDS per row that nobody
@@ -75,14 +76,14 @@ struct RowAccess {
 };
 
 // The workgroups' partial sums, [workgroup][outputs][cols], in their order: 64 columns a workgroup, a sixteenth of the sums a wavefront.  Without any
-// (no rows) the gradients are zeros.
+// (no rows) the gradients are zeros.  From column `first` on.
 template <int PTYPE>
-__global__ __launch_bounds__(1024) void norm_params_kernel(const float* __restrict__ part, int blocks, int outputs, int cols,
+__global__ __launch_bounds__(1024) void norm_params_kernel(const float* __restrict__ part, int blocks, int outputs, int first, int cols,
                                                           void* __restrict__ dweight, void* __restrict__ dbias) {
   typedef Elements<PTYPE> P;
   __shared__ float sums[16][64];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, which = blockIdx.y;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t col = first + (int64_t)blockIdx.x * 64 + lane;
   void* const out = which == 0 ? dweight : dbias;
   float sum = 0.f;
   if (col < cols) {
@@ -101,6 +102,13 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(const float* __restri
 }
 
 [[maybe_unused]] int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+template <int PTYPE>
+void launch_norm_params(const float* part, int blocks, int outputs, int cols, void* dweight, void* dbias, hipStream_t s) {
+  for (int64_t first = 0; first < cols; first += kNormColumns)
+    hipLaunchKernelGGL((norm_params_kernel<PTYPE>), dim3(ceil_div(std::min<int64_t>(cols - first, kNormColumns), 64), dbias != nullptr ? 2 : 1),
+                       dim3(1024), 0, s, part, blocks, outputs, (int)first, cols, dweight, dbias);
+}
 
 // How a row is shared out: `lanes` * `waves` threads, `pieces` 16-byte pieces to each.  No lanes: longer than the registers of a
 // workgroup hold.

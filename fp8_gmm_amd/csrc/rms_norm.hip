@@ -683,8 +683,7 @@ int fp8gmm_rms_norm_backward(const void* dy, int64_t ldy, const void* dh, int64_
       }
     }
     if (dweight != nullptr && (blocks != 1 || shape.lanes == 0))
-      hipLaunchKernelGGL((norm_params_kernel<P>), dim3(ceil_div(cols, 64), 1), dim3(1024), 0, s, part, blocks, 1, cols, dweight,
-                         static_cast<void*>(nullptr));
+      launch_norm_params<P>(part, blocks, 1, cols, dweight, nullptr, s);
   });
   if (!known) return FP8GMM_ERR_LAUNCH;
   return hipGetLastError() == hipSuccess ? FP8GMM_OK : FP8GMM_ERR_LAUNCH;

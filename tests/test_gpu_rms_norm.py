@@ -421,3 +421,18 @@ def test_results_that_outgrow_the_cache(dev, rows, cols, t):
             assert torch.equal(pkg.rms_norm(x[part], w, 1e-5), plain[part])
             c, d, _ = pkg.rms_norm_fp8(x[part], w, 1e-5, residual[part])
             assert torch.equal(c.view(torch.uint8), q[part].view(torch.uint8)) and torch.equal(d, inv[part])
+
+
+def test_more_columns_than_a_grid_has_threads_for(dev):
+    """Weights' gradients of rows of more than 2^28 columns.  Rows of 1 and -1: their squares and their sum are exact, the factor is 1 to
+    a few 2^-24, and the gradients are dy and its negative, rounded to bfloat16."""
+    cols = (1 << 28) + 70
+    x = torch.ones(1, cols, dtype=torch.bfloat16, device=dev)
+    x[:, 1::2] = -1
+    dy = torch.randn(1, 1 << 20, generator=gen(1)).to(torch.bfloat16).to(dev).repeat(1, 257)[:, :cols].contiguous()
+    w, b = (torch.ones(cols, dtype=torch.bfloat16, device=dev).requires_grad_() for _ in range(2))
+    for norm, bias in ((pkg.rms_norm(x, w, 0.0), None), (pkg.layer_norm(x, w, b, 0.0), b)):
+        grads = torch.autograd.grad(norm, (w,) if bias is None else (w, b), dy)
+        assert torch.equal(grads[0], (dy * x)[0])
+        assert bias is None or torch.equal(grads[1], dy[0])
+        del norm, grads
