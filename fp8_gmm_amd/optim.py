@@ -121,13 +121,31 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """A checkpoint of this class and of the same ``state_bits``; its way of counting steps and its masters become this optimizer's."""
+        # torch casts the states to their parameters' types: what is loaded, as the caller's hooks ahead of it leave it, is kept to undo
+        # that ahead of the hooks behind it.
+        loaded = []
+
+        def look(_, state_dict):
+            self._check_checkpoint(state_dict)
+            loaded.append(state_dict)
+
+        hooks = (self.register_load_state_dict_pre_hook(look),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_checkpoint(loaded[0]), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _check_checkpoint(self, state_dict):
         for group in state_dict["param_groups"]:
             states = [state_dict["state"][key] for key in group["params"] if key in state_dict["state"]]
             if "steps" not in group or any(("exp_avg_scale" in state) != (self.state_bits == 8) for state in states):
                 raise ValueError(f"not a checkpoint of an AdamW of {self.state_bits}-bit moments")
             if self.capturable and len({state.get("step") for state in states}) > 1:
                 raise ValueError("the parameters of a capturable group count the same steps, the checkpoint's have different ones")
-        super().load_state_dict(state_dict)
+
+    def _take_checkpoint(self, state_dict):
         for group, old in zip(self.param_groups, state_dict["param_groups"]):
             device = group["params"][0].device
             if isinstance(old["lr"], torch.Tensor):

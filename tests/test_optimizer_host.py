@@ -1,0 +1,74 @@
+"""The optimizer without a GPU: checkpoints, copies and refused steps.  The step itself is the kernel's and is replaced or refused here."""
+
+import pytest
+import torch
+
+import fp8_gmm_amd as pkg
+
+
+def make(n=2, **options):
+    return pkg.AdamW([torch.nn.Parameter(torch.full((3,), i + 1.0, dtype=torch.bfloat16)) for i in range(n)], **options)
+
+
+def stepped(value=7.0, **options):
+    """An optimizer whose states are there, as a step on the GPU leaves them."""
+    opt = make(**options)
+    for p in opt.param_groups[0]["params"]:
+        opt._init_state(p, opt.state[p])
+        opt.state[p]["exp_avg"].fill_(value)
+        if not opt.capturable:
+            opt.state[p]["step"] = 5
+    if opt.capturable:
+        opt.param_groups[0]["steps"] = torch.tensor(5)
+    return opt
+
+
+@pytest.mark.parametrize("options", [dict(), dict(state_bits=8, master_weights=True), dict(capturable=True)])
+def test_hooks_of_a_load_have_their_way(options):
+    saved = stepped(**options).state_dict()
+
+    def zeroed(_, state_dict):
+        return {**state_dict, "state": {k: {**v, "exp_avg": torch.zeros_like(v["exp_avg"])} for k, v in state_dict["state"].items()}}
+
+    opt = make(**options)
+    opt.register_load_state_dict_pre_hook(zeroed)
+    opt.load_state_dict(saved)
+    for p in opt.param_groups[0]["params"]:
+        assert not opt.state[p]["exp_avg"].float().any() and opt.state[p]["exp_avg"].dtype == saved["state"][0]["exp_avg"].dtype
+        assert opt.state[p]["exp_avg"] is not saved["state"][0]["exp_avg"]
+
+    opt = make(**options)
+    opt.register_load_state_dict_pre_hook(lambda _, state_dict: {**state_dict, "state": {}})
+    opt.load_state_dict(saved)
+    assert not opt.state
+
+    def renamed(_, state_dict):   # a checkpoint of another layout, put right by its hook
+        return {"state": state_dict["moments"], "param_groups": state_dict["groups"]}
+
+    opt = make(**options)
+    opt.register_load_state_dict_pre_hook(renamed)
+    opt.load_state_dict({"moments": saved["state"], "groups": saved["param_groups"]})
+    assert all((opt.state[p]["exp_avg"].float() == 7).all() for p in opt.param_groups[0]["params"])
+
+    def behind(optimizer):
+        for p in optimizer.param_groups[0]["params"]:
+            assert optimizer.state[p]["exp_avg"].dtype == saved["state"][0]["exp_avg"].dtype
+            optimizer.state[p]["exp_avg"].fill_(2.0)
+
+    opt = make(**options)
+    opt.register_load_state_dict_post_hook(behind)
+    opt.load_state_dict(saved)
+    assert all((opt.state[p]["exp_avg"].float() == 2).all() for p in opt.param_groups[0]["params"])
+
+
+def test_a_load_leaves_no_hook_behind():
+    opt = make()
+    opt.load_state_dict(stepped().state_dict())
+    for other in (stepped(state_bits=8), stepped()):
+        hooks = [len(h) for h in (opt._optimizer_load_state_dict_pre_hooks, opt._optimizer_load_state_dict_post_hooks)]
+        assert hooks == [0, 0]
+        before = {p: dict(opt.state[p]) for p in opt.param_groups[0]["params"]}
+        if other.state_bits == 8:
+            with pytest.raises(ValueError, match="not a checkpoint"):
+                opt.load_state_dict(other.state_dict())
+            assert all(opt.state[p][k] is v for p, s in before.items() for k, v in s.items())
