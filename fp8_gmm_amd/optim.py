@@ -62,6 +62,10 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, steps=None))
 
+    def __getstate__(self):   # of a copy or a pickle: the options too, which torch leaves out
+        options = ("state_bits", "master_weights", "max_norm", "capturable", "grad_norm")
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in options}}
+
     def _init_state(self, p, state):
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
             _fail("fp8_gmm_amd: a parameter has no state yet: run a step ahead of the capture")

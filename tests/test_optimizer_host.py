@@ -1,9 +1,14 @@
 """The optimizer without a GPU: checkpoints, copies and refused steps.  The step itself is the kernel's and is replaced or refused here."""
 
+import copy
+import io
+import pickle
+
 import pytest
 import torch
 
 import fp8_gmm_amd as pkg
+from fp8_gmm_amd import backend
 
 
 def make(n=2, **options):
@@ -72,3 +77,29 @@ def test_a_load_leaves_no_hook_behind():
             with pytest.raises(ValueError, match="not a checkpoint"):
                 opt.load_state_dict(other.state_dict())
             assert all(opt.state[p][k] is v for p, s in before.items() for k, v in s.items())
+
+
+@pytest.mark.parametrize("options", [dict(), dict(state_bits=8, master_weights=True, max_norm=0.5), dict(capturable=True, lr=torch.tensor(0.5))])
+def test_copies_step_as_their_original_does(options, monkeypatch):
+    opt = stepped(**options)
+    calls = []
+    monkeypatch.setattr(backend, "multi_adamw", lambda *args: calls.append(args))
+    monkeypatch.setattr(backend, "multi_norm", lambda grads: torch.tensor(2.0))
+    file = io.BytesIO()
+    torch.save(opt, file)
+    file.seek(0)
+    copies = [copy.deepcopy(opt), copy.copy(opt), torch.load(file, weights_only=False)]
+    if opt.state_bits == 32:   # (pickle alone takes no tensor of 8-bit floats, whoever holds it)
+        copies.append(pickle.loads(pickle.dumps(opt)))
+    for copied in copies:
+        for name in ("state_bits", "master_weights", "max_norm", "capturable", "grad_norm"):
+            assert getattr(copied, name) == getattr(opt, name)
+        for p, q in zip(opt.param_groups[0]["params"], copied.param_groups[0]["params"]):
+            assert {k: getattr(v, "dtype", v) for k, v in opt.state[p].items()} == {k: getattr(v, "dtype", v) for k, v in copied.state[q].items()}
+            q.grad = torch.ones_like(q)
+        copied.step()
+        assert len(calls.pop()[0]) == 2 and not calls
+        again = make(**options)
+        again.load_state_dict(copied.state_dict())
+        if "max_norm" in options:
+            assert copied.grad_norm == 2.0
