@@ -108,16 +108,23 @@ class AdamW(torch.optim.Optimizer):
                 if group["steps"] is None:
                     group["steps"] = torch.zeros((), dtype=torch.int64, device=pairs[0][0].device)
                 group["steps"].add_(1)
+            moved = False
             for (step, masters), some in calls.items():
                 params, grads, states = zip(*some)
 
                 def of(name):
                     return [state[name] for state in states]
 
-                backend.multi_adamw(params, grads, of("exp_avg"), of("exp_avg_sq"), group["steps"] if self.capturable else step, group["lr"],
-                                    tuple(group["betas"]), group["eps"], group["weight_decay"],
-                                    (of("exp_avg_scale"), of("exp_avg_sq_scale")) if self.state_bits == 8 else None,
-                                    of("master") if masters else None, norm, None if norm is None else self.max_norm)
+                try:
+                    backend.multi_adamw(params, grads, of("exp_avg"), of("exp_avg_sq"), group["steps"] if self.capturable else step,
+                                        group["lr"], tuple(group["betas"]), group["eps"], group["weight_decay"],
+                                        (of("exp_avg_scale"), of("exp_avg_sq_scale")) if self.state_bits == 8 else None,
+                                        of("master") if masters else None, norm, None if norm is None else self.max_norm)
+                except Exception:
+                    if self.capturable and not moved:   # a step that is refused does not count
+                        group["steps"].sub_(1)
+                    raise
+                moved = True
                 if not self.capturable:
                     for state in states:
                         state["step"] = step

@@ -104,3 +104,39 @@ def test_copies_step_as_their_original_does(options, monkeypatch):
         again.load_state_dict(copied.state_dict())
         if "max_norm" in options:
             assert copied.grad_norm == 2.0
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+def test_a_refused_step_does_not_count(capturable, monkeypatch):
+    opt = stepped(capturable=capturable)
+    group = opt.param_groups[0]
+
+    def steps():
+        return [int(group["steps"])] if capturable else [opt.state[p]["step"] for p in group["params"]]
+
+    for p in group["params"]:
+        p.grad = torch.ones_like(p)
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="GPU tensors"):
+            opt.step()
+    assert set(steps()) == {5}
+    monkeypatch.setattr(backend, "multi_adamw", lambda *args: None)
+    opt.step()
+    assert set(steps()) == {6}
+
+    calls = []
+
+    def second_refused(*args):   # of a group whose parameters have masters and have none
+        calls.append(args)
+        if len(calls) == 2:
+            raise RuntimeError("refused")
+
+    mixed = pkg.AdamW([torch.nn.Parameter(torch.ones(3, dtype=t)) for t in (torch.bfloat16, torch.float32)], master_weights=True,
+                      capturable=capturable)
+    for p in mixed.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    monkeypatch.setattr(backend, "multi_adamw", second_refused)
+    with pytest.raises(RuntimeError, match="refused"):
+        mixed.step()
+    assert len(calls) == 2 and (int(mixed.param_groups[0]["steps"]) == 1 if capturable else
+                                [mixed.state[p]["step"] for p in mixed.param_groups[0]["params"]] == [1, 0])
