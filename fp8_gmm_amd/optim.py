@@ -158,7 +158,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _take_checkpoint(self, state_dict):
         for group, old in zip(self.param_groups, state_dict["param_groups"]):
-            device = group["params"][0].device
+            device = group["params"][0].device if group["params"] else None
             if isinstance(old["lr"], torch.Tensor):
                 group["lr"] = old["lr"].detach().to(device, copy=True) if self.capturable else old["lr"].item()
             steps = old["steps"]

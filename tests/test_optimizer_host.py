@@ -140,3 +140,20 @@ def test_a_refused_step_does_not_count(capturable, monkeypatch):
         mixed.step()
     assert len(calls) == 2 and (int(mixed.param_groups[0]["steps"]) == 1 if capturable else
                                 [mixed.state[p]["step"] for p in mixed.param_groups[0]["params"]] == [1, 0])
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+def test_groups_without_parameters_load(capturable):
+    lr = torch.tensor(0.25) if capturable else 0.25
+
+    def with_empty(params):
+        return pkg.AdamW([{"params": params}, {"params": [], "lr": lr}], capturable=capturable)
+
+    opt = with_empty([torch.nn.Parameter(torch.ones(3))])
+    p, = opt.param_groups[0]["params"]
+    opt._init_state(p, opt.state[p])
+    opt.step()   # nothing to do
+    other = with_empty([torch.nn.Parameter(torch.ones(3))])
+    other.load_state_dict(opt.state_dict())
+    assert other.param_groups[1]["params"] == [] and float(other.param_groups[1]["lr"]) == 0.25
+    assert set(other.state[other.param_groups[0]["params"][0]]) == set(opt.state[p])
