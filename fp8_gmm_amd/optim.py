@@ -31,6 +31,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         return backend.multi_clip(grads, grads, max_norm)
 
 
+def _refuse(options):
+    for name in ("amsgrad", "maximize", "differentiable"):
+        if options.get(name):
+            raise ValueError(f"{name} is not supported")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay, a launch for some dozens of parameters (``backend.multi_adamw``, which has the formulas).
 
@@ -38,14 +44,16 @@ class AdamW(torch.optim.Optimizer):
     ``master_weights``: parameters of 16 bits are copies of float32 masters that the optimizer keeps.  ``max_norm``: every step clips
     the gradients of all groups by their common norm on the way (they stay as they are); the norm before that is ``self.grad_norm``.
     ``capturable``: the steps are counted on the device, a group's for all of its parameters, so that a captured step may be replayed;
-    ``lr`` may be a float32 tensor of the device then.  Run one step ahead of the capture: it makes the states.
+    ``lr`` may be a float32 tensor of the device then.  Run one step ahead of the capture: it makes the states.  ``foreach`` and ``fused``,
+    which choose one of torch's implementations, choose nothing here; ``amsgrad``, ``maximize`` and ``differentiable`` are refused.
 
     Parameters are dense, on one device, bfloat16, float16 or float32; those without a gradient are passed over.  Without ``capturable``
     each counts its own steps.  Checkpoints hold the states in their own types, whatever the parameters' (``state_dict``); loading one
     makes new states, of which a graph captured before knows nothing."""
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
-                 max_norm=None, capturable=False):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, *, maximize=False, foreach=None,
+                 capturable=False, differentiable=False, fused=None, state_bits=32, master_weights=False, max_norm=None):
+        _refuse(dict(amsgrad=amsgrad, maximize=maximize, differentiable=differentiable))
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
         if not (isinstance(lr, torch.Tensor) or lr >= 0.0):
@@ -61,6 +69,10 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.max_norm, self.capturable = state_bits, master_weights, max_norm, capturable
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, steps=None))
+
+    def add_param_group(self, param_group):
+        _refuse(param_group)
+        super().add_param_group(param_group)
 
     def __getstate__(self):   # of a copy or a pickle: the options too, which torch leaves out
         options = ("state_bits", "master_weights", "max_norm", "capturable", "grad_norm")

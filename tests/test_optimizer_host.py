@@ -157,3 +157,19 @@ def test_groups_without_parameters_load(capturable):
     other.load_state_dict(opt.state_dict())
     assert other.param_groups[1]["params"] == [] and float(other.param_groups[1]["lr"]) == 0.25
     assert set(other.state[other.param_groups[0]["params"][0]]) == set(opt.state[p])
+
+
+def test_arguments_that_torchs_users_give():
+    p = [torch.nn.Parameter(torch.ones(3))]
+    theirs = dict(lr=1e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1, amsgrad=False, maximize=False, foreach=None, capturable=False,
+                  differentiable=False, fused=None)
+    torch.optim.AdamW(p, **theirs)
+    for options in (theirs, {**theirs, "foreach": True}, {**theirs, "fused": True}):
+        assert pkg.AdamW(p, **options).param_groups[0]["betas"] == (0.9, 0.99)
+    for name in ("amsgrad", "maximize", "differentiable"):
+        with pytest.raises(ValueError, match=name):
+            pkg.AdamW(p, **{**theirs, name: True})
+        with pytest.raises(ValueError, match=name):
+            pkg.AdamW([{"params": p, name: True}])
+    with pytest.raises(ValueError, match="amsgrad"):
+        pkg.AdamW(p, 1e-3, (0.9, 0.99), 1e-8, 0.1, True)
