@@ -270,7 +270,8 @@ __device__ __forceinline__ float block_max(float v) {
   return v;
 }
 
-// 448 times the inverse of `most`, a guess and a step of Newton's (a division takes three times as long); and its share of a code
+// 448 times the inverse of `most`, a guess and a step of Newton's, which is correctly rounded as the guess is off by one at most (a division
+// takes three times as long); and its share of a code
 __device__ __forceinline__ float codes_per(float most) {
   if (__builtin_expect(!(most >= kTiny && most < 0x1p120f), 0)) return most >= kTiny ? kMost * (1.f / most) : 0.f;
   const float r = __builtin_amdgcn_rcpf(most);
@@ -352,9 +353,8 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
     root[i] = root_of(v[i]);
     if constexpr (!BITS8) rare = rare || __builtin_isfpclass(v[i], 0x290);   // subnormal, or infinite
     const float d = __builtin_fmaf(root[i], by.root, h.eps);
-    float r = __builtin_amdgcn_rcpf(d);   // to one in 2^23; with a step of Newton's 4 instructions for a division's 10
-    if constexpr (!BITS8) r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
-    ratio[i] = m[i] * r;
+    const float r = __builtin_amdgcn_rcpf(d);   // and a step of Newton's: 4 instructions for a division's 10
+    ratio[i] = m[i] * __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
   }
   const auto root_max = [&] {
     float most = 0.f;
