@@ -48,13 +48,16 @@ __device__ __forceinline__ double exp64(double x) {
   p = __builtin_fma(p, f, 1.);
   return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + (__builtin_bit_cast(uint64_t, large) << 52));
 }
-// 1 / d for 1 <= d <= e^701: the hardware's first guess, 2^-23, and one of Newton's steps
+// 1 / d for 1 <= d <= e^701: the hardware's first guess, 2^-23, and two of Newton's steps (with one, 2^-46 more on p, 131072 tokens of 64 experts
+// by sigmoid and bias 18.3 us, with two 18.8)
 __device__ __forceinline__ double rcp64(double d) {
-  const double r = __builtin_amdgcn_rcp(d);
+  double r = __builtin_amdgcn_rcp(d);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
   return __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
 }
-// exp(x) of x <= 0, 2 units in the last place: the hardware's power of 2 of the rounded product, and what the rounding left of it to the
-// first order.  A NaN stays one, what is below e^-200 is zero (expf takes half as many instructions again).
+// exp(x) of x <= 0, for sums whose largest part is 1 and gradients: the hardware's power of 2 of the rounded product, and what the rounding
+// left of it to the first order, 2 units in the last place.  A NaN stays one, a result below 2^-126 is zero.  (131072 tokens of 64 experts,
+// softmax, us forward and backward: 10.8 and 11.8, with expf, one unit and subnormal numbers, 11.8 and 12.8.  The weights are expf's.)
 __device__ __forceinline__ float exp_of(float x) {
   x = __builtin_elementwise_maximum(x, -200.f);
   const float t = x * 0x1.715476p+0f;
@@ -279,7 +282,7 @@ __device__ __forceinline__ float share_of(const Choice& c, bool has, float v) {
   const float m = over<LANES>(has ? v : -INFINITY, Largest{});
   float part = 0.f;
   if (has) {
-    part = exp_of(v - m);
+    part = expf(v - m);
     if (c.sigmoid) part = m > 0.f ? sigmoid(v) : part / (1.f + expf(v));
   }
   return part / over<LANES>(part, Sum{});
@@ -536,7 +539,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_kernel(const void* __
   const bool has = lane < c.top_k;
   float w = has ? score_of<TYPE>(scores, from, c.experts, chosen) : 0.f;
   if (c.renormalize) w = __builtin_fmaf(total, 0.f, share_of<LANES>(c, has, w));   // (a total that is no number leaves none)
-  else w = c.sigmoid ? sigmoid(w) : exp_of(w - most) / total;
+  else w = c.sigmoid ? sigmoid(w) : expf(w - most) / total;
   if (has && live) {
     weights[token * c.top_k + lane] = w * c.scale;
     selected[token * c.top_k + lane] = chosen;
@@ -590,7 +593,7 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
   } else if (c.sigmoid) {
     g *= sigmoid(v);
   } else {
-    back = over<LANES>(has ? g * (exp_of(v - most) / total) : 0.f, Sum{});
+    back = over<LANES>(has ? g * (expf(v - most) / total) : 0.f, Sum{});
   }
   if (c.sigmoid) g *= 1.f / (1.f + expf(v));
   float out[PER];

@@ -215,3 +215,16 @@ def test_more_tokens_than_a_grid_has_threads_for(dev, tokens, experts, top_k):
         n = min(block, tokens - at)
         for got, one in zip((w.detach(), chosen, ds), wanted):
             assert torch.equal(got[at: at + n], one[:n]), at
+
+
+@pytest.mark.parametrize("tokens, experts", [(5, 16), (10000, 64), (300, 256), (9000, 256), (40, 1500)])
+def test_small_softmax_weights_have_their_values(dev, tokens, experts):
+    """Down to fp32's subnormal numbers: e^-88 to e^-100 of the row's largest score, which is alone above them.  Tolerance: the sum of
+    expf's unit, the division's and the last rounding (2 + 1 + 1 units of 2^-24, and of the difference, up to 100, 100 units), and
+    half of 2^-149 for each of the three that may be subnormal."""
+    scores = -88.0 - 12.0 * torch.rand(tokens, experts, generator=gen(experts))
+    scores[:, 0] = 0.0
+    w, chosen = moe_ops.select_experts(scores.to(dev), 6)
+    want = torch.softmax(scores.double(), 1).gather(1, chosen.cpu())
+    off = (w.double().cpu() - want).abs()
+    assert (off <= 104 * U * want + 1.5 * 2.0 ** -149).all() and (w > 0).all()
