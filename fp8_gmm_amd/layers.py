@@ -42,10 +42,11 @@ def rms_norm_fp8(x, weight, eps=1e-5, residual=None, scale=None, amax=None, dtyp
     """The norm of ``rms_norm`` in 8 bits, rounded once, for a product in 8 bits: ``(q, scale_inv, h)``.  With ``scale`` (one float32
     on the device, of delayed scaling as the grouped modules use it: a slot of ``fp8_meta``) ``q = y * scale``, saturating, and ``amax``
     (one float32, may be None) is raised to ``max |y|``; ``scale_inv`` is None, the caller's.  Without, every row has its own scale:
-    ``scale_inv [...]`` (float32, without the columns) is ``max |y| / largest``, the largest number of ``dtype`` (``float8_e4m3fn`` or
-    ``float8_e5m2``), at least ``2^-100 / largest``, and ``q = y / scale_inv``.  ``h`` is None without a residual.  A NaN stays one and
-    leaves the maximum as it is; a row with an infinite ``y`` has an infinite scale.  No gradients are taken: tensors that require one
-    are refused outside of ``torch.no_grad()``."""
+    by ``most``, its largest ``|y|`` or 2^-100, and ``largest``, the largest number of ``dtype`` (``float8_e4m3fn`` or ``float8_e5m2``),
+    ``q = y * (largest / most)``, saturating, and ``scale_inv [...] = most / largest`` (float32, without the columns), for a product of the
+    caller's: the package's own take one scale for a tensor.  ``h`` is None without a residual.  A NaN stays one and leaves the maximum as
+    it is; a row with an infinite ``y`` has an infinite scale.  No gradients are taken: tensors that require one are refused outside of
+    ``torch.no_grad()``."""
     return native.rms_norm_fp8(x, weight, eps, residual, scale, amax, dtype)
 
 

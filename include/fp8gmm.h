@@ -735,7 +735,8 @@ int fp8gmm_layer_norm_backward(const void* dy, int64_t ldy, const void* x, int64
  * pass, or NULL.  1 <= cols <= 2^30, rows < 2^31.  y, h (and q, dx below) lie apart from what is read.
  * fp8gmm_rms_norm_fp8: the same norm in 8 bits, q: fp8 [rows, cols] of `fmt` (FP8GMM_E4M3 or _E5M2), saturating, a NaN stays one.
  * With scale (device fp32): q = fp8(y * *scale), and *amax (may be NULL; holds a number that is not negative) is raised to max |y|.
- * With scale_inv (fp32 [rows]) instead: scale_inv[r] = max(max |y[r, :]|, 2^-100) / the format's largest number, q = fp8(y / scale_inv).
+ * With scale_inv (fp32 [rows]) instead: by the row's largest magnitude, most = max(max |y[r, :]|, 2^-100), and the format's largest number,
+ * scale_inv[r] = most / largest and q = fp8(y * (largest / most)), each operation rounded to fp32.
  */
 int fp8gmm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* y, void* h, float* rstd,
                     int64_t rows, int cols, float eps, int type, int param_type, void* stream);

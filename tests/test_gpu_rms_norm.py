@@ -436,3 +436,20 @@ def test_more_columns_than_a_grid_has_threads_for(dev):
         assert torch.equal(grads[0], (dy * x)[0])
         assert bias is None or torch.equal(grads[1], dy[0])
         del norm, grads
+
+
+@pytest.mark.parametrize("cols", [64, 1000, 16384, 100001, 1 << 20])
+@pytest.mark.parametrize("fmt", [torch.float8_e4m3fn, torch.float8_e5m2])
+def test_codes_by_rows_follow_the_stated_operations(dev, cols, fmt):
+    """Rows of 1 and -1 have a factor of 1, so y is the weight, in fp32: q = fp8(y (largest / most)), scale_inv = most / largest, bit by bit."""
+    x = torch.ones(3, cols, device=dev)
+    x[:, ::2] = -1
+    largest = torch.finfo(fmt).max
+    for seed in range(4):
+        w = torch.randn(cols, generator=gen(seed)).to(dev)
+        q, scale_inv, _ = pkg.rms_norm_fp8(x, w, 0.0, dtype=fmt)
+        most = w.abs().max().cpu()
+        by = torch.tensor(largest) / most   # (of the CPU, whose division is correctly rounded)
+        want = ((x * w).cpu() * by).clamp(-largest, largest).to(fmt)
+        assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8))
+        assert (scale_inv.cpu() == most / torch.tensor(largest)).all()
