@@ -714,7 +714,8 @@ def multi_adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.99
     parameters are their rounded copies.  ``norm`` (one float32 on the device, as ``multi_norm`` returns it) and ``max_norm``: both or
     neither.  ``step`` counts from 1; it and ``lr`` are numbers, or an int64 and a float32 of the device (one element each), which a
     replayed graph reads anew.  What is written may share memory with nothing else of the call.  A gradient that is no number leaves
-    none in its element, with 8-bit moments in the moments of its block."""
+    none in its element, with 8-bit moments in the moments of its block; one whose square passes float32's range stops its parameter but
+    for the decay (8-bit moments keep it as the largest square that float32 has)."""
     flush_uploads()   # a queued launch may write what is read here
     native.multi_adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, scales, masters, norm, max_norm)
 

@@ -356,16 +356,16 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
     const float r = __builtin_amdgcn_rcpf(d);   // and a step of Newton's: 4 instructions for a division's 10
     ratio[i] = m[i] * __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
   }
-  const auto root_max = [&] {
+  const auto most_of = [](const float (&f)[VEC]) {
     float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; i += 2) most = amax_or_nan(most, root[i], root[i + 1]);
+    for (int i = 0; i < VEC; i += 2) most = amax_or_nan(most, f[i], f[i + 1]);
     return block_max(most);
   };
   if constexpr (BITS8) {
     // A block at a time: an infinite v leaves a NaN in its root.  A subnormal one's root is wrong, but not zero and so far below the others'
     // that its code is the smallest one, and 2^-33 of eps in the quotient (below an eps of 2^-30 all take the longer way, 365 us and not 289).
-    v_most = root_max();
+    v_most = most_of(root);
     rare = rare || !(v_most < 0x1p62f) || (v_most < 0x1p-40f && v_most != 0.f);
   }
   if (__builtin_expect(rare, 0)) {   // what the guesses do not reach
@@ -374,7 +374,8 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
       root[i] = sqrtf(v[i]);
       ratio[i] = m[i] / __builtin_fmaf(root[i], by.root, h.eps);
     }
-    if constexpr (BITS8) v_most = root_max();
+    // The square of a finite gradient may be infinite: its root is the largest that fp32 has, since an infinite scale would take the block along.
+    if constexpr (BITS8) v_most = most_of(root);
   }
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
@@ -384,10 +385,10 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
   if constexpr (MASTER) S::F32::template store<FULL>(e.master, at, n, p);
   S::Weights::template store<FULL>(e.param, at, n, p);
   if constexpr (BITS8) {
-    float m_most = 0.f;
-#pragma unroll
-    for (int i = 0; i < VEC; i += 2) m_most = amax_or_nan(m_most, m[i], m[i + 1]);
-    m_most = block_max(m_most);
+    const float m_most = most_of(m);
+    // The square of a finite gradient may be infinite: its root is the largest that fp32 has, since an infinite scale would take the block along.
+    constexpr float kRoot = 0x1.fffffep63f;
+    if (__builtin_expect(v_most > kRoot, 0) && m_most < INFINITY) v_most = kRoot;
     const float m_inv = codes_per(m_most), v_inv = codes_per(v_most);
     const uint32_t first = (uint32_t)at * kElement + by.dither;
     u32x2 mw = {0u, 0u}, vw = {0u, 0u};

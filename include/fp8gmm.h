@@ -795,7 +795,7 @@ int fp8gmm_multi_clip(const fp8gmm_norm_tensor* tensors, int n, double max_norm,
  * = code * scale, scale = largest magnitude of the block / 448, 0 where that is below 2^-100 and the codes zeros.  Codes are rounded by
  * thresholds u = frac((i * 0x6A09E667 + t * 0x9E3779B9) / 2^32) for element i (cut to 20 bits): exp_avg up where its way to the next
  * code is at least 1 - u, the root, with u + 1/2 in place of u (cut to 24 bits), where its square's way to the next code's is more than that; a
- * root that is not zero becomes no zero.
+ * root that is not zero becomes no zero; an infinite exp_avg_sq of finite gradients is kept as the largest root of fp32.
  * t and lr: `step` (>= 1) and `lr`, or *step_dev and *lr_dev where these are given, which a replayed launch reads anew.  `tensors` is HOST
  * memory and is read during the call only.  What is written overlaps nothing else of the call (FP8GMM_ERR_BAD_ARGUMENT).  At most 2^32
  * elements each, addresses below 2^48.

@@ -47,3 +47,23 @@ def test_parameters_move_as_beside_moments_in_32_bits(dev, masters):
         backend.multi_adamw([p], [g], [m], [v], 1, 1e-3, scales=scales, masters=master)
         moved.append((p, *(master or ())))
     assert all(torch.equal(a, b) for a, b in zip(*moved))
+
+
+def test_a_square_that_fp32_does_not_hold_leaves_its_block_alone(dev):
+    """A finite gradient whose second moment is infinite: its own parameter stands still but for the decay, as beside moments in 32 bits,
+    and the others of its block go on, in this step and in the next ones."""
+    n = 1000
+    r = torch.Generator(device=dev).manual_seed(1)
+    grads = [torch.randn(n, generator=r, device=dev) for _ in range(4)]
+    grads[0][300], grads[0][301] = 1e25, -1e30
+    p = torch.ones(n, device=dev)
+    codes = [torch.zeros(n, dtype=torch.float8_e4m3fn, device=dev) for _ in range(2)]
+    scales = [torch.zeros(8, device=dev) for _ in range(2)]
+    for t, g in enumerate(grads, 1):
+        before = p.clone()
+        backend.multi_adamw([p], [g], [codes[0]], [codes[1]], t, 1e-3, weight_decay=0.0, scales=([scales[0]], [scales[1]]))
+        assert torch.isfinite(p).all() and all(torch.isfinite(s).all() for s in scales)
+        assert all(torch.isfinite(c.float()).all() for c in codes)
+        assert t > 1 or torch.equal(p[300:302], before[300:302])
+        others = torch.cat([p[:256] != before[:256], p[384:] != before[384:]])
+        assert others.all()
