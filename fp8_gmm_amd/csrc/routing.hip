@@ -6,10 +6,10 @@
 //   `top_groups` largest groups stay; of their experts the `top_k` largest c are chosen, the lower number first where two are equal
 //   w = scale p[chosen], with `renormalize` scale p[chosen] / sum of p[chosen]
 //
-// What is compared decides where a token goes, so it is compared exactly: the scores themselves where p alone would decide (it grows
-// with them), else c and the groups' sums in 64 bits.  A key is such a number that holds the expert's number in its last bits, so no two
-// keys are equal and the largest names its expert: 16 bits of a score and 15 of the number, or a number in 64 bits whose last 12 bits of
-// the fraction are replaced (what agrees in its first 40 bits counts as equal, and groups' sums to 2^-36 of their larger part).  An expert whose score or bias is minus infinity is switched
+// What is compared decides where a token goes: the scores themselves where p alone would decide (it grows with them), else c and the groups'
+// sums in 64 bits, p to 2^-46.  A key is such a number that holds the expert's number in its last bits, so no two keys are equal and the
+// largest names its expert: 16 bits of a score and 15 of the number, or a number in 64 bits whose last 12 bits of the fraction are replaced
+// (what agrees in its first 40 bits counts as equal, of groups' sums in 36).  An expert whose score or bias is minus infinity is switched
 // off: it goes last, whatever the other one is.  The weights are fp32.
 //
 // LANES lanes have a token, 8 or 16 (of a row of the data-parallel primitives) or 64, with PER neighbouring experts in the registers of
@@ -96,14 +96,12 @@ __device__ __forceinline__ int number_of(key64 key) {
   const int low = (int)(bits & 0xfff);
   return (int64_t)bits < 0 ? low : 4095 - low;
 }
-// The sum of two keys' numbers, to the nearest multiple of 2^-36 of the larger one's power of two: sums that are equal, as that of the
-// sigmoids of x and -x is for every x, come out equal, where the keys are cut off 2^-40 below their numbers.
+// The sum of two keys' numbers, rounded to its first 36 bits: sums that are equal, as that of the sigmoids of x and -x is for every x, come
+// out equal, where the keys are cut off 2^-40 below their numbers.
 __device__ __forceinline__ double sum_of(key64 a, key64 b) {
   const auto plain = [](key64 k) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) & ~0xfffull); };
-  const auto upper = [](key64 k) { return (uint32_t)(__builtin_bit_cast(uint64_t, k) >> 32) & 0x7fffffffu; };
-  const uint32_t whole = ((max(upper(a), upper(b)) & 0x7ff00000u) + (16u << 20)) | 0x80000u;   // 1.5 * 2^16 powers of two
-  const double large = __builtin_bit_cast(double, (uint64_t)whole << 32);
-  return plain(a) + plain(b) + large - large;
+  const double sum = smaller(plain(a) + plain(b), kFar);
+  return __builtin_bit_cast(double, (__builtin_bit_cast(uint64_t, sum) + 0x8000) & ~0xffffull);
 }
 __device__ __forceinline__ void strike(key64& key, bool gone) {   // the upper half does
   const uint64_t bits = __builtin_bit_cast(uint64_t, key);
@@ -276,15 +274,17 @@ struct Choice {
 
 // p[chosen] / sum of p[chosen], of the chosen score v of every lane that `has` one.  p itself may be too small for a number, of all of
 // them where a bias or the groups keep the largest scores out: these are shares by the largest of the chosen ones, m.  Softmax: e^(v - m).
-// Sigmoid: p, where m is above zero; below, with e^m left out of all, e^(v - m) / (1 + e^v).
+// Sigmoid: p, where the sum is no small number; else, with e^m left out of all, e^(v - m) / (1 + e^v).
 template <int LANES>
 __device__ __forceinline__ float share_of(const Choice& c, bool has, float v) {
-  const float m = over<LANES>(has ? v : -INFINITY, Largest{});
   float part = 0.f;
-  if (has) {
-    part = expf(v - m);
-    if (c.sigmoid) part = m > 0.f ? sigmoid(v) : part / (1.f + expf(v));
+  if (c.sigmoid) {
+    part = has ? sigmoid(v) : 0.f;
+    const float sum = over<LANES>(part, Sum{});
+    if (__builtin_expect(!(sum < 0.5f), 1)) return part / sum;
   }
+  const float m = over<LANES>(has ? v : -INFINITY, Largest{});
+  if (has) part = c.sigmoid ? expf(v - m) / (1.f + expf(v)) : expf(v - m);
   return part / over<LANES>(part, Sum{});
 }
 
@@ -302,7 +302,7 @@ __device__ __forceinline__ void keep_groups(K (&key)[PER], const Choice& c, int 
     if constexpr (BEST == 2) second = larger(second, b);
   };
   const auto made = [&](K first, K second, int g) {
-    if constexpr (BEST == 2) return key_of(sum_of(first, second > kOff ? second : 0.), g);
+    if constexpr (BEST == 2) return key_of_plain(sum_of(first, second > kOff ? second : 0.), g);
     else return first;
   };
   K none = key[0];

@@ -287,7 +287,7 @@ def select_experts(scores, top_k, scoring="softmax", bias=None, groups=1, top_gr
     largest ``c``, the ``top_groups`` largest groups stay, and of their experts the ``top_k`` with the largest ``c`` are chosen.  The
     weights are ``scale * p`` of these - the bias decides and weighs nothing - or, with ``renormalize``, ``scale * p / sum of the chosen
     p``.  The choice is made by the scores where ``p`` alone decides, and else in 64 bits, with ``p`` to 2^-46: what agrees in its first
-    40 bits counts as equal, sums of groups what agrees to 2^-36 of the larger part, and the lower number goes first.  A score that is a
+    40 bits counts as equal, of sums of groups in 36 bits, and the lower number goes first.  A score that is a
     NaN goes last and leaves the others' order as it is (but makes all of its token's softmax one, as plus infinity does, which goes
     first).  A score of minus infinity switches an expert off, whatever its bias is, and so does a bias of minus infinity: it goes last
     and adds nothing to its group, and a group of none but such goes last.  Where fewer than ``top_k`` are left the lowest of the others

@@ -644,8 +644,8 @@ int fp8gmm_route_topk_backward(const float* probs, const int64_t* selected, cons
  * p = softmax(scores[t, :]) or sigmoid and c = p + bias: the experts lie in `groups` groups of neighbours, a group counts the sum of its
  * `group_best` largest c, the `top_groups` largest groups stay, and of their experts the top_k largest c are chosen, largest first.
  * selected[t, k]: their numbers, weights[t, k]: scale * p of each, with renormalize scale * p / (sum of the chosen p).  Compared are the scores
- * themselves where p alone decides, else c and the sums in 64 bits, p to 2^-46: what agrees in its first 40 bits counts as equal, sums what
- * agrees to 2^-36 of the larger part, and the lower number goes first.  A score that is a NaN goes last and leaves the others' order as it
+ * themselves where p alone decides, else c and the sums in 64 bits, p to 2^-46: what agrees in its first 40 bits counts as equal, of sums
+ * in 36 bits, and the lower number goes first.  A score that is a NaN goes last and leaves the others' order as it
  * is.  An expert whose score is minus infinity, whatever its bias, or whose bias is, goes last too and adds nothing to its group's sum; a
  * group of none but such goes last.
  * scores: [tokens, experts] of `type` (FP8GMM_TYPE_*), contiguous; bias: fp32 [experts] or NULL.
