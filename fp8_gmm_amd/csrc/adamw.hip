@@ -26,8 +26,8 @@ namespace {
 
 // Threads and elements of a workgroup, 4 (32 bits) or 8 to a thread at a time.  Of lists that no cache holds, us: 400 tensors of bf16 with
 // fp32 moments by 512 threads and 2048 elements 596, by 256 and 1024 597, and 2048 625, and 4096 670, by 128 and 2048 669; 96 tensors of fp32
-// by 512 and 2048 761, by 256 and 1024 786; 96 tensors with 8-bit moments, which take ten times the instructions, by 256 and 4096 278, and
-// 6144 279, by 512 and 8192 293, by 128 and 2048 279; the same of fp32 471, 481, 474 and 482.
+// by 512 and 2048 761, by 256 and 1024 786; 96 tensors with 8-bit moments, which take ten times the instructions, by 256 and 4096 287, and
+// 6144 287, by 512 and 8192 300, by 128 and 2048 284; the same with masters 463, 478, 460 and 469, of fp32 472, 483, 475 and 482.
 constexpr int threads(bool bits8) { return bits8 ? 256 : 512; }
 constexpr int sweep(bool bits8) { return bits8 ? 4096 : 2048; }
 // From so many bytes on everything is read and written with the streaming hint: nothing of it is found in the caches by the next step
@@ -364,7 +364,7 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
   };
   if constexpr (BITS8) {
     // A block at a time: an infinite v leaves a NaN in its root.  A subnormal one's root is wrong, but not zero and so far below the others'
-    // that its code is the smallest one, and 2^-33 of eps in the quotient (below an eps of 2^-30 all take the longer way, 365 us and not 289).
+    // that its code is the smallest one, and 2^-33 of eps in the quotient (below an eps of 2^-30 all take the longer way, 356 us and not 287).
     v_most = most_of(root);
     rare = rare || !(v_most < 0x1p62f) || (v_most < 0x1p-40f && v_most != 0.f);
   }
@@ -407,7 +407,7 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
         vw[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
       }
-    } else {   // a fifth fewer instructions (96 tensors of bf16 287 us, by the longer form alone 301)
+    } else {   // a fifth fewer instructions (96 tensors of bf16 287 us, by the longer form alone 298)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = 4 * i;
@@ -460,8 +460,8 @@ __global__ __launch_bounds__(threads(BITS8)) void adamw_kernel(const PartOf<MAST
         return;
       }
     } else {
-      // Where the workgroup is stays in scalar registers: without the threads' places there is room for 6 wavefronts (96 tensors 280 us, with
-      // 5 of them 287).
+      // Where the workgroup is stays in scalar registers: without the threads' places there is room for 6 wavefronts where there are no masters
+      // (96 tensors 287 us, with 5 of them 302; with masters 83 registers leave 5, 463 and 468).
       const auto go_on = [&](int64_t elements) {
         const auto go = [&](auto*& p, int64_t bytes) {
           typedef std::remove_pointer_t<std::remove_reference_t<decltype(p)>> T;

@@ -21,8 +21,8 @@ constexpr int kForwardThreads = 256;     // of a workgroup of the forward pass, 
 // What a forward pass writes: the normed rows (of x, or of the sum with a residual, which it writes as well), or these in 8 bits
 enum { kRows, kSums, kBits8 };
 // Threads of its launch, which go on to other rows.  With 8 bits what the compute units hold at a time, three times that where they would go
-// on more than five times; else four times as many (16384 x 4096, bf16, with a residual 86.8 us, what they hold alone 89.2; without one 43.5
-// and 45.1; but in 8 bits 81 and 76; 16384 x 4093 93.0 and 98.4).
+// on more than five times; else four times as many (16384 x 4096, bf16, with a residual 89.5 us, what they hold alone 90.5; without one 44.3
+// and 46.7; 16384 x 4093 92.9 and 97.0; but in 8 bits 81.4 and 79.2).
 constexpr int kForwardAll = 256 * 2048, kForwardTurns = 5, kForwardMore = 3, kForwardFour = 4;
 
 // The least magnitude that a row's scale is made of: what is smaller is zero in 8 bits, and no scale is zero.
@@ -80,8 +80,8 @@ __global__ __launch_bounds__(MOST) void rms_norm_kernel(
     bool stream) {
   typedef Elements<TYPE> E;
   constexpr int V = E::kVec;
-  // With the streaming hint, but for rows that are the residual stream themselves (16384 x 4096, bf16, with a residual 89.2 us, without the
-  // hint 93.7; in 8 bits 76 and 88; without a residual 44.7 and 45.1).
+  // With the streaming hint, but for rows that are the residual stream themselves (16384 x 4096, bf16, with a residual 89.5 us, without the
+  // hint 93.0; in 8 bits 74 and 84; without a residual 45.0 and 44.3).
   constexpr bool BITS8 = KIND == kBits8, STREAM = KIND != kRows;
   __shared__ float slots[2][kNormWaves][kNormWaves], tops[2][kNormWaves][kNormWaves];
   const int THREADS = LANES * waves, ROWS = blockDim.x / THREADS;
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_weight_kernel(
 }
 
 // Forward, 4 pieces to a thread, as in the layer norm; 2 of aligned rows in 8 bits, whose conversions want more wavefronts (4096 x 4096, bf16,
-// 23.0 us, with 4 pieces 27.0; 256 rows 5.2 and 6.1; 16384 rows 74.9 and 76.2; but 16384 x 4093 91.8 and 80.2).
+// 22.8 us, with 4 pieces 26.6; 256 rows 5.2 and 6.1; 16384 rows 74.0 and 76.3; but 16384 x 4093 91.8 and 79.2).
 Shape forward_shape(int cols, int type, bool two) {
   const int pieces = pieces_of(cols, type);
   Shape s = shape_of(pieces, two ? 2 : 4, 8, 4);

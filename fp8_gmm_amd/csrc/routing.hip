@@ -14,7 +14,8 @@
 //
 // LANES lanes have a token, 8 or 16 (of a row of the data-parallel primitives) or 64, with PER neighbouring experts in the registers of
 // each: a round takes the largest key of every lane's own, exchanges them in log2(LANES) steps, and leaves it out of the next.  Bound by these
-// instructions, not by the scores' bytes.
+// instructions, not by the scores' bytes: 16384 tokens of 256 experts, sigmoid, bias and groups, 13.4 us, of which a unit issues vector
+// instructions for 8.3 at 2.4 GHz; 131072 of 64 by softmax 12.0 and 9.0, backward 12.6 and 10.7 (the former's 6.6 and 3.0: half of it waits for memory).
 #include <algorithm>
 #include <type_traits>
 
@@ -49,7 +50,7 @@ __device__ __forceinline__ double exp64(double x) {
   return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + (__builtin_bit_cast(uint64_t, large) << 52));
 }
 // 1 / d for 1 <= d <= e^701: the hardware's first guess, 2^-23, and two of Newton's steps (with one, 2^-46 more on p, 131072 tokens of 64 experts
-// by sigmoid and bias 18.3 us, with two 18.8)
+// by sigmoid and bias 18.0 us, with two 18.5)
 __device__ __forceinline__ double rcp64(double d) {
   double r = __builtin_amdgcn_rcp(d);
   r = __builtin_fma(__builtin_fma(-d, r, 1.), r, r);
@@ -57,7 +58,7 @@ __device__ __forceinline__ double rcp64(double d) {
 }
 // exp(x) of x <= 0, for sums whose largest part is 1 and gradients: the hardware's power of 2 of the rounded product, and what the rounding
 // left of it to the first order, 2 units in the last place.  A NaN stays one, a result below 2^-126 is zero.  (131072 tokens of 64 experts,
-// softmax, us forward and backward: 10.8 and 11.8, with expf, one unit and subnormal numbers, 11.8 and 12.8.  The weights are expf's.)
+// softmax, us forward and backward: 10.8 and 11.9, with expf, one unit and subnormal numbers, 11.8 and 12.8.  The weights are expf's.)
 __device__ __forceinline__ float exp_of(float x) {
   x = __builtin_elementwise_maximum(x, -200.f);
   const float t = x * 0x1.715476p+0f;
@@ -392,8 +393,8 @@ __device__ __forceinline__ int take_largest(K (&key)[PER], int top_k, int lane) 
   K mine = key[0], last = K();
   if constexpr (std::is_same_v<K, key64> && PER >= 16) {
     // A lane's 8 largest in their order: a round looks at the first ones, and the lane that has the largest moves up (us of 16384 tokens of 256
-    // experts, 8 choices, 10.0, by a look at all keys in every round 10.8; 4 choices 8.6 and 8.8, but 2 choices 8.0 and 7.8; 2000 tokens of 4096
-    // experts 20.9 and 28.6).
+    // experts, 8 choices, 10.2, by a look at all keys in every round 11.0; 4 choices 9.0 and 9.3, but 2 choices 8.3 and 8.2; 2000 tokens of 4096
+    // experts 21.2 and 28.9).
     if (top_k > 2 && top_k <= 8) {
       sort8(key, 0);
 #pragma unroll
@@ -614,10 +615,10 @@ __global__ __launch_bounds__(kThreads) void select_experts_backward_kernel(const
 }
 
 // calls f(TYPE, LANES, PER).  Few tokens have a wavefront each, whose lanes hold few experts (us, forward by p in 64 bits / backward:
-// 1 token, 256 experts in 8 groups, 4.2 / 2.5, by 16 lanes 4.5 / 2.9; 1024 tokens 4.7 / 2.8 and 5.2 / 3.4; 2048 5.4 / 3.0 and 4.9 / 3.5; 4096
-// 7.6 / 3.6 and 5.1 / 3.7; 2048 tokens of 512 experts 6.3 / 3.3 and 7.5 / 4.9).  Many tokens of few experts have 8 lanes each, as long as
-// every choice and group has a lane of its own (131072 tokens, 64 experts, 6 choices by their scores, 11.3 / 12.3, by 16 lanes 13.2 / 15.0;
-// 8 experts 5.1 / 6.1 and 7.4 / 8.9; 16384 tokens, 64 experts, 3.1 / 3.5 and 3.4 / 3.7, 4096 tokens 2.7 / 3.1 and 2.6 / 2.8).
+// 1 token, 256 experts in 8 groups, 4.2 / 2.4, by 16 lanes 4.6 / 3.0; 1024 tokens 4.8 / 2.7 and 5.3 / 3.4; 2048 5.5 / 3.0 and 5.1 / 3.5; 4096
+// 7.8 / 3.6 and 5.1 / 3.7; 2048 tokens of 512 experts 6.4 / 3.3 and 7.5 / 5.0).  Many tokens of few experts have 8 lanes each, as long as
+// every choice and group has a lane of its own (131072 tokens, 64 experts, 6 choices by their scores, 10.8 / 11.9, by 16 lanes 13.5 / 15.0;
+// 8 experts 5.3 / 6.0 and 7.9 / 8.6; 16384 tokens, 64 experts, 3.2 / 3.7 and 3.6 / 3.8, 4096 tokens 2.7 / 3.2 and 2.6 / 2.9).
 constexpr int kFewTokens = 2048, kManyTokens = 8192;
 template <class F>
 void with_shape(int type, int64_t tokens, const Choice& c, F&& f) {

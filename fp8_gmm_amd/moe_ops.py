@@ -304,7 +304,9 @@ def select_experts(scores, top_k, scoring="softmax", bias=None, groups=1, top_gr
 @dataclass
 class Routing:
     """How a routed layer chooses its experts (``moe``, ``routing=``): the options of ``select_experts``.  ``bias``: the layer has a bias
-    of zeros, its buffer ``expert_bias``, for the training loop to move against the load, ``layer.tokens_per_expert`` of the last pass."""
+    of zeros in float32, its buffer ``expert_bias``, for the training loop to move against the load, ``layer.tokens_per_expert`` of the last
+    pass.  A cast of the module (``layer.bfloat16()``) casts the buffer with the rest: in 16 bits small moves are lost, so put it back,
+    ``layer.expert_bias = layer.expert_bias.float()``."""
 
     scoring: str = "softmax"
     bias: bool = False
