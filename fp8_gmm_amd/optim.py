@@ -71,7 +71,8 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, steps=None))
 
     def add_param_group(self, param_group):
-        _refuse(param_group)
+        if isinstance(param_group, dict):   # (torch refuses others)
+            _refuse(param_group)
         super().add_param_group(param_group)
 
     def __getstate__(self):   # of a copy or a pickle: the options too, which torch leaves out

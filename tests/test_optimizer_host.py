@@ -173,3 +173,5 @@ def test_arguments_that_torchs_users_give():
             pkg.AdamW([{"params": p, name: True}])
     with pytest.raises(ValueError, match="amsgrad"):
         pkg.AdamW(p, 1e-3, (0.9, 0.99), 1e-8, 0.1, True)
+    with pytest.raises(TypeError, match="dict"):
+        pkg.AdamW(p).add_param_group(p)
