@@ -374,7 +374,6 @@ __device__ __forceinline__ void step_values(const Share<TYPE, GRAD, MASTER, BITS
       root[i] = sqrtf(v[i]);
       ratio[i] = m[i] / __builtin_fmaf(root[i], by.root, h.eps);
     }
-    // The square of a finite gradient may be infinite: its root is the largest that fp32 has, since an infinite scale would take the block along.
     if constexpr (BITS8) v_most = most_of(root);
   }
 #pragma unroll
